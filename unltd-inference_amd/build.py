@@ -2,7 +2,7 @@
 
     python unltd-inference_amd/build.py [-v] [-i]   (-i: recompile only stale objects)
 
-libuq.so: every csrc/*.hip plus uq_abi.cpp, uq_gguf.cpp, uq_ops_abi.cpp and uq_layer.cpp, compiled by hipcc for gfx950
+libuq.so: every csrc/*.hip plus uq_abi.cpp, uq_gguf.cpp, uq_ops_abi.cpp, uq_layer.cpp and uq_serve_abi.cpp, compiled by hipcc for gfx950
   only, -O3, FP contraction off (FMAs are written explicitly), f32
   denormals kept, packed-FP32 instructions disabled. Each source is
   compiled to its own object in parallel (objects under _build/), then
@@ -51,7 +51,7 @@ def _run(cmd, verbose):
 
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip"))) + [
-        os.path.join(CSRC, f) for f in ("uq_abi.cpp", "uq_gguf.cpp", "uq_ops_abi.cpp", "uq_layer.cpp")]
+        os.path.join(CSRC, f) for f in ("uq_abi.cpp", "uq_gguf.cpp", "uq_ops_abi.cpp", "uq_layer.cpp", "uq_serve_abi.cpp")]
 
 
 def _stale(src, obj):

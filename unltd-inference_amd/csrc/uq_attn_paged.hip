@@ -1,0 +1,724 @@
+// Attention of a batch's rows over a paged cache (uq_attn_paged_d).
+//
+// With scores s[p] = kq_scale q.K[p] of a query, one pass over the keys keeps
+// a reference a and the sums
+//     l = sum 2^(s[p] log2 e + a),   o = sum 2^(s[p] log2 e + a) V[p],
+// where -a follows the largest s log2 e seen so far (o and l are multiplied by
+// 2^(a' - a) when it moves), and the result is o / l. Parts over other
+// positions join the same way.
+#include <algorithm>
+#include <climits>
+
+#include "uq_device.h"
+#include "uq_internal.h"
+#include "uq_serve_internal.h"
+
+namespace uq {
+
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any float
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+constexpr int kTPB = 256;
+constexpr int kWaves = kTPB / 64;
+constexpr int kRows = 16;       // queries of a block: the columns of a 16x16 tile
+constexpr int kGroups = 512;    // workgroups: two per CU
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct AttnArgs {
+    AttnPagedArgs a;
+    PagesView kv;
+    BatchView b;
+    int group, G, prefix_blocks;
+    float *rec_o;   // records: [..][HD] sums o ...
+    float2 *rec_al; // ... with (a, l)
+    int2 *seg;      // [block][kv head]: first and last workgroup of its units, or kDone / kWhole
+};
+
+// Where a block's units lie: in one workgroup that wrote the results itself,
+// in one whose record is the row's own, or in several workgroups' records.
+constexpr int kDone = -1, kWhole = -2;
+
+// Records: two blocks of rows for each workgroup (its run's first block where
+// that began earlier, its last where that goes on), then one per row and
+// head of the shared and of the own positions.
+__device__ __forceinline__ size_t rec_part(int w, int second, int n) { return ((size_t)w * 2 + second) * kRows + n; }
+__device__ __forceinline__ size_t rec_whole(const AttnArgs &A, int own, int row, int head) {
+    return (size_t)A.G * 2 * kRows + ((size_t)own * A.b.n_rows + row) * A.a.n_head + head;
+}
+
+template <bool F16, int HD>
+struct Geo;
+// f16 cache: tiles of 32 positions, 16x16x32 products; a lane holds 8
+// consecutive values of K, 8 (HD 64: 4) of V.
+template <int HD>
+struct Geo<true, HD> {
+    static constexpr int NP = 32, PT = 2, KC = HD / 32, DL = HD == 64 ? 4 : 8, NH = HD / (16 * DL), VS = 8;
+};
+// f32 cache: tiles of 16 positions, 16x16x4 products; 4 consecutive values.
+template <int HD>
+struct Geo<false, HD> {
+    static constexpr int NP = 16, PT = 1, KC = HD / 16, DL = 4, NH = HD / 64, VS = 4;
+};
+
+// The sequence of one part of the work: s = -1 is the shared positions with
+// the rows of the whole batch.
+struct Work {
+    int lo, n, len;      // rows, length as given
+    int base, end;       // positions [base, end)
+    int units, blocks;
+};
+
+template <int U>
+__device__ __forceinline__ Work work_of(const AttnArgs &A, int s) {
+    Work w;
+    const int cap = A.b.max_pages << A.kv.map.log2_page;
+    if (s < 0) {
+        const SeqRows r = seq_rows(0, A.b.row_start[A.b.n_seqs], A.b.n_rows);
+        w = Work{r.lo, r.n, 0, 0, A.a.shared_len, 0, 0};
+    } else {
+        const SeqRows r = seq_rows(A.b.row_start[s], A.b.row_start[s + 1], A.b.n_rows);
+        const int len = A.b.len[s];
+        w = Work{r.lo, r.n, len, A.a.shared_len, seq_len(len, cap), 0, 0};
+    }
+    w.units = w.end > w.base ? (w.end - w.base + U - 1) / U : 0;
+    w.blocks = blocks_of(w.n, A.group, kRows);
+    return w;
+}
+
+__device__ __forceinline__ float row16_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+
+// A wave's part of a block: scores, running reference and sums over its
+// tiles of the positions.
+//
+// Scores are formed transposed, S^T = K Q^T (16 positions x 16 queries a
+// tile), so that a lane holds one query's scores (column n = lane & 15) of
+// positions 4 (lane >> 4) + i; with the position order of the second
+// product's depth chosen to match (slot 8 g + j of a 32-deep product is
+// position 4 g + j of tile j / 4), the weights are its right operand where
+// they are, and o^T = V^T P^T (values x queries) needs V's values of 8
+// positions a lane: rows are loaded 16 bytes a lane and paired by v_perm, one
+// a register. No value crosses lanes but the maximum and row numbers.
+//
+// f16 cache: a query is scaled by a power of two to at most 2^15 and split
+// into two f16 terms, a weight (times 2^14) likewise; products are exact and
+// summed in f32. f32 cache: the f32 matrix products.
+template <bool F16, int HD>
+struct Wave {
+    using G = Geo<F16, HD>;
+    f4 acc[G::NH][G::DL];
+    float a, l;  // reference, this lane's share of l
+
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int h = 0; h < G::NH; h++)
+#pragma unroll
+            for (int j = 0; j < G::DL; j++) acc[h][j] = f4{0.f, 0.f, 0.f, 0.f};
+        a = INFINITY;
+        l = 0.0f;
+    }
+};
+
+// The products of values that are not finite (slots `bad` of the lane's
+// sixteen columns), left out of the matrix product because a row that may not
+// see them would take 0 * NaN from them: added for the rows that see them.
+template <bool F16, int HD, class E>
+__device__ __forceinline__ void add_unfinite(Wave<F16, HD> &W, const E *V, int myrow, const float (&p)[Geo<F16, HD>::VS],
+                                             const bool (&sees)[Geo<F16, HD>::VS], unsigned bad, int lane) {
+    using G = Geo<F16, HD>;
+    const int n = lane & 15, g = lane >> 4;
+    unsigned where = 0;  // bit y: position y of the tile
+#pragma unroll
+    for (int x = 0; x < G::VS; x++) {
+        const unsigned long long m = __ballot((bad >> x) & 1);
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            if ((m >> (16 * q)) & 0xFFFF) where |= 1u << (16 * (x >> 2) + 4 * q + (x & 3));
+    }
+    while (where) {
+        const int y = __builtin_ctz(where), from = 16 * ((y >> 2) & 3) + n, slot = 4 * (y >> 4) + (y & 3);
+        where &= where - 1;
+        float pv = 0.0f;
+        bool sv = false;
+#pragma unroll
+        for (int x = 0; x < G::VS; x++)
+            if (x == slot) pv = p[x], sv = sees[x];
+        pv = __shfl(pv, from);
+        sv = __shfl((int)sv, from);
+        const E *vp = V + (size_t)__shfl(myrow, y) * HD;
+#pragma unroll
+        for (int h = 0; h < G::NH; h++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < G::DL; j++) {
+                    const float v = (float)vp[h * 16 * G::DL + (4 * g + i) * G::DL + j];
+                    if (sv) W.acc[h][j][i] += pv * v;
+                }
+    }
+}
+
+template <bool F16, int HD>
+__global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(AttnArgs A) {
+    using G = Geo<F16, HD>;
+    using E = std::conditional_t<F16, _Float16, float>;
+    constexpr int NP = G::NP, U = kWaves * NP, MS = HD + 4;
+    constexpr float kShift = F16 ? 14.0f : 0.0f;
+    extern __shared__ uint8_t lds[];       // the block's queries; the waves' sums at its end
+    __shared__ float row_c[kRows];         // score factor of a query, times log2 e
+    __shared__ int row_lim[kRows];         // its last position, -1: none
+    __shared__ float2 wave_al[kWaves][kRows];
+    __shared__ long long scan[kWaves];
+    __shared__ long long start_s;
+    __shared__ int seq_s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int nkv = A.kv.n_head_kv;
+    const PageMap &map = A.kv.map;
+
+    // ---- this workgroup's run of units: [u, u1) of T, beginning off units into
+    // sequence seq (-1: the shared positions)
+    const int parts = A.b.n_seqs + 1;
+    long long T = 0, mine = 0, before = 0;
+    for (int c = 0; c < parts; c += kTPB) {
+        const int i = c + tid;
+        mine = 0;
+        if (i < parts && (i > 0 || A.a.shared_len > 0)) {
+            const Work w = work_of<U>(A, i - 1);
+            mine = (long long)w.units * w.blocks * nkv;
+        }
+        long long inc = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const long long up = __shfl_up(inc, d);
+            if (lane >= d) inc += up;
+        }
+        __syncthreads();
+        if (lane == 63) scan[wave] = inc;
+        __syncthreads();
+        before = T + inc - mine;
+        for (int i2 = 0; i2 < kWaves; i2++) {
+            if (i2 < wave) before += scan[i2];
+            T += scan[i2];
+        }
+    }
+    const int runs = (int)min((long long)A.G, T);  // no empty runs between others
+    if ((int)blockIdx.x >= runs) return;
+    long long u = run_start(T, runs, (int)blockIdx.x);
+    const long long u1 = run_start(T, runs, (int)blockIdx.x + 1);
+    if (parts <= kTPB) {
+        if (mine > 0 && before <= u && u < before + mine) seq_s = tid - 1, start_s = u - before;
+    } else {
+        long long run = 0;
+        for (int c = 0; c < parts; c += kTPB) {
+            const int i = c + tid;
+            mine = 0;
+            if (i < parts && (i > 0 || A.a.shared_len > 0)) {
+                const Work w = work_of<U>(A, i - 1);
+                mine = (long long)w.units * w.blocks * nkv;
+            }
+            long long inc = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const long long up = __shfl_up(inc, d);
+                if (lane >= d) inc += up;
+            }
+            __syncthreads();
+            if (lane == 63) scan[wave] = inc;
+            __syncthreads();
+            before = run + inc - mine;
+            for (int i2 = 0; i2 < kWaves; i2++) {
+                if (i2 < wave) before += scan[i2];
+                run += scan[i2];
+            }
+            if (mine > 0 && before <= u && u < before + mine) seq_s = i - 1, start_s = u - before;
+        }
+    }
+    __syncthreads();
+    int seq = seq_s;
+    long long off = start_s;
+    Work w = work_of<U>(A, seq);
+
+    Wave<F16, HD> W;
+    while (u < u1) {
+        const long long per = (long long)nkv * w.units;
+        if (off >= per * w.blocks) {  // the next sequence with units (there is one: u < T)
+            if (++seq >= A.b.n_seqs) return;
+            w = work_of<U>(A, seq);
+            off = 0;
+            continue;
+        }
+        const int rb = (int)(off / per), kvh = (int)(off % per / w.units), un = (int)(off % w.units);
+        const int count = (int)min((long long)(w.units - un), u1 - u);
+        const int nq = min(kRows, w.n * A.group - rb * kRows);  // queries of the block
+
+        // ---- the block's queries into LDS, in the order of the products' right operand
+        __syncthreads();  // the waves' sums of the block before are read
+        {
+            const int r = tid >> 4, part = tid & 15, num = rb * kRows + r;
+            const bool in = r < nq;
+            const int row = w.lo + (in ? num / A.group : 0);
+            const float *q = A.a.q + ((size_t)row * A.a.n_head + (size_t)kvh * A.group + (in ? num % A.group : 0)) * HD;
+            if (seq < 0) {
+                if (part == 0) row_lim[r] = -1;
+            } else if (part == 0) {
+                row_lim[r] = in && w.len >= 0 ? max(-1, w.len - w.n + (row - w.lo)) : -1;
+            }
+            float fac = A.a.scale * kLog2e;
+            if constexpr (F16) {
+                constexpr int C = (HD / 8 + 15) / 16;
+                float v[C][8];
+                uint32_t top = 0;
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const int ch = part + 16 * c;
+                    const bool has = in && ch < HD / 8;
+#pragma unroll
+                    for (int x = 0; x < 8; x += 4) {
+                        const f4u f = has ? *(const f4u *)(q + 8 * ch + x) : f4u{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            v[c][x + e] = f[e];
+                            top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+                // |q| < 2^ex; not finite: left as it is, its terms are not finite either
+                const int ex = top > 0 && top < 0x7F800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 15;
+                fac = ldexpf(fac, ex - 15);
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const int ch = part + 16 * c;
+                    h8 hi, lo;
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        const float s = ldexpf(v[c][x], 15 - ex);
+                        hi[x] = (_Float16)s;
+                        lo[x] = (_Float16)(s - (float)hi[x]);
+                    }
+                    if (ch < HD / 8) {
+                        h8 *dst = (h8 *)lds + (ch >> 2) * 128 + (ch & 3) * 16 + r;
+                        dst[0] = hi;
+                        dst[64] = lo;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < HD / 64; c++) {
+                    const int ch = part + 16 * c;
+                    ((f4 *)lds)[(ch >> 2) * 64 + (ch & 3) * 16 + r] = in ? (f4) * (const f4u *)(q + 4 * ch) : f4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
+            if (part == 0) row_c[r] = fac;
+            if (seq < 0) {  // the block's rows are of any sequences: each row's is looked for by 16 threads
+                __syncthreads();
+                for (int i = part; in && i < A.b.n_seqs; i += 16) {
+                    const SeqRows sr = seq_rows(A.b.row_start[i], A.b.row_start[i + 1], A.b.n_rows);
+                    if (row < sr.lo || row >= sr.lo + sr.n) continue;
+                    const int len = A.b.len[i];
+                    row_lim[r] = len >= 0 ? max(-1, len - sr.n + (row - sr.lo)) : -1;
+                }
+            }
+        }
+        __syncthreads();
+        const int lim = row_lim[n];
+        const float fac = row_c[n];
+        int lim_min = n < nq ? lim : INT_MAX, lim_max = n < nq ? lim : -1;
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) {
+            lim_min = min(lim_min, __shfl_xor(lim_min, d));
+            lim_max = max(lim_max, __shfl_xor(lim_max, d));
+        }
+        const int end = lim_max < w.end ? lim_max + 1 : w.end;  // no row sees further
+        const int32_t *table = A.b.pages + (seq < 0 ? (size_t)0 : (size_t)seq * A.b.max_pages);
+        const E *K = (const E *)A.kv.k, *V = (const E *)A.kv.v;
+
+        W.reset();
+        for (int it = 0; it < count; it++) {
+            const int p0 = w.base + (un + it) * U + wave * NP;
+            if (p0 >= end) break;  // the whole wave
+            // rows of the tile's positions, position p0 + (lane & (NP - 1)) a lane
+            const int mypos = p0 + (lane & (NP - 1));
+            const int page = mypos < end ? table[mypos >> map.log2_page] : -1;
+            const bool there = page_ok(map, page);
+            const int myrow = there ? page_row(map, page, kvh, mypos) : 0;
+            const unsigned long long have = __ballot(there);
+            if (have == 0) continue;
+            const bool edge = have != ~0ull || p0 + NP - 1 > lim_min;
+
+            // scores
+            f4 s[G::PT];
+            if constexpr (F16) {
+                h8 k[G::PT][G::KC];
+#pragma unroll
+                for (int t = 0; t < G::PT; t++) {
+                    const h8 *kp = (const h8 *)(K + (size_t)__shfl(myrow, 16 * t + n) * HD) + g;
+#pragma unroll
+                    for (int c = 0; c < G::KC; c++) k[t][c] = kp[4 * c];
+                }
+#pragma unroll
+                for (int t = 0; t < G::PT; t++) s[t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < G::KC; c++) {
+                    const h8 qh = ((const h8 *)lds)[c * 128 + lane], ql = ((const h8 *)lds)[c * 128 + 64 + lane];
+#pragma unroll
+                    for (int t = 0; t < G::PT; t++) {
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][c], qh, s[t], 0, 0, 0);
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][c], ql, s[t], 0, 0, 0);
+                    }
+                }
+            } else {
+                f4 k[G::KC];
+                const f4 *kp = (const f4 *)(K + (size_t)__shfl(myrow, n) * HD) + g;
+#pragma unroll
+                for (int c = 0; c < G::KC; c++) k[c] = kp[4 * c];
+                s[0] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < G::KC; c++) {
+                    const f4 q = ((const f4 *)lds)[c * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][e], q[e], s[0], 0, 0, 0);
+                }
+            }
+
+            // weights: slot x = 4 t + i is position p0 + 16 t + 4 g + i
+            float p[4 * G::PT];
+            float top = -INFINITY;
+            bool sees[4 * G::PT];
+#pragma unroll
+            for (int t = 0; t < G::PT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int x = 16 * t + 4 * g + i;
+                    sees[4 * t + i] = !edge || (((have >> x) & 1) && p0 + x <= lim);
+                    top = fmaxf(top, sees[4 * t + i] ? s[t][i] * fac : -INFINITY);
+                }
+            top = row16_max(top);
+            float na = fminf(W.a, kShift - top);
+            const float corr = na == INFINITY ? 1.0f : exp2_hw(na - W.a);
+            W.a = na;
+            W.l *= corr;
+#pragma unroll
+            for (int t = 0; t < G::PT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float v = na == INFINITY ? 0.0f : exp2_hw(fmaf(s[t][i], fac, na));
+                    v = sees[4 * t + i] ? v : 0.0f;
+                    p[4 * t + i] = v;
+                    W.l += v;
+                }
+#pragma unroll
+            for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                for (int j = 0; j < G::DL; j++) W.acc[h][j] *= corr;
+
+            // values: slot x of a lane is position p0 + 16 (x / 4) + 4 g + x % 4
+            if constexpr (F16) {
+                using HV = std::conditional_t<G::DL == 8, u4, u2>;
+                constexpr int D2 = G::DL / 2;
+                HV v[G::VS][G::NH];
+#pragma unroll
+                for (int x = 0; x < G::VS; x++) {
+                    const E *vp = V + (size_t)__shfl(myrow, 16 * (x >> 2) + 4 * g + (x & 3)) * HD + G::DL * n;
+#pragma unroll
+                    for (int h = 0; h < G::NH; h++) v[x][h] = *(const HV *)(vp + 16 * G::DL * h);
+                }
+                unsigned bad = 0;  // slots that hold something not finite
+                if (edge) {
+#pragma unroll
+                    for (int x = 0; x < G::VS; x++) {
+                        const bool ok = (have >> (16 * (x >> 2) + 4 * g + (x & 3))) & 1;
+                        bool fin = true;
+#pragma unroll
+                        for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                            for (int d = 0; d < D2; d++) {
+                                const uint32_t z = v[x][h][d];
+                                fin = fin && (z & 0x7C00u) != 0x7C00u && (z & 0x7C000000u) != 0x7C000000u;
+                            }
+                        fin = ((__ballot(!fin) >> (16 * g)) & 0xFFFF) == 0;
+                        if (!ok || !fin) {
+#pragma unroll
+                            for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                                for (int d = 0; d < D2; d++) v[x][h][d] = 0;
+                        }
+                        bad |= ok && !fin ? 1u << x : 0u;
+                    }
+                }
+                h8 ph, pl;
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    ph[x] = (_Float16)p[x];
+                    pl[x] = (_Float16)(p[x] - (float)ph[x]);
+                }
+#pragma unroll
+                for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                    for (int j = 0; j < G::DL; j++) {
+                        u4 f;
+#pragma unroll
+                        for (int x = 0; x < 4; x++)
+                            f[x] = __builtin_amdgcn_perm(v[2 * x + 1][h][j >> 1], v[2 * x][h][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+                        const h8 vf = __builtin_bit_cast(h8, f);
+                        W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, W.acc[h][j], 0, 0, 0);
+                        W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, W.acc[h][j], 0, 0, 0);
+                    }
+                if (edge && __any(bad != 0)) add_unfinite(W, V, myrow, p, sees, bad, lane);
+            } else {
+                f4 v[G::VS][G::NH];
+#pragma unroll
+                for (int x = 0; x < G::VS; x++) {
+                    const E *vp = V + (size_t)__shfl(myrow, 4 * g + x) * HD + 4 * n;
+#pragma unroll
+                    for (int h = 0; h < G::NH; h++) v[x][h] = *(const f4 *)(vp + 64 * h);
+                }
+                unsigned bad = 0;
+                if (edge) {
+#pragma unroll
+                    for (int x = 0; x < G::VS; x++) {
+                        const bool ok = (have >> (4 * g + x)) & 1;
+                        bool fin = true;
+#pragma unroll
+                        for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                            for (int d = 0; d < 4; d++) fin = fin && finite32(v[x][h][d]);
+                        fin = ((__ballot(!fin) >> (16 * g)) & 0xFFFF) == 0;
+                        if (!ok || !fin) {
+#pragma unroll
+                            for (int h = 0; h < G::NH; h++) v[x][h] = f4{0.f, 0.f, 0.f, 0.f};
+                        }
+                        bad |= ok && !fin ? 1u << x : 0u;
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < G::VS; x++)
+#pragma unroll
+                    for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][h][j], p[x], W.acc[h][j], 0, 0, 0);
+                if (edge && __any(bad != 0)) add_unfinite(W, V, myrow, p, sees, bad, lane);
+            }
+        }
+
+        // ---- the waves' sums joined: references, then o scaled to the least of them
+        W.l = row16_sum(W.l);
+        if (lane < kRows) wave_al[wave][lane] = make_float2(W.a, W.l);
+        __syncthreads();  // also: every wave is done with the queries in LDS
+        float amin = INFINITY;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) amin = fminf(amin, wave_al[i][n].x);
+        const float to = W.a == INFINITY ? 0.0f : exp2_hw(amin - W.a);
+        float *sums = (float *)lds + (size_t)wave * kRows * MS;
+        if (n < nq) {
+#pragma unroll
+            for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < G::DL; j += 4)
+                        *(f4 *)(sums + n * MS + h * 16 * G::DL + (4 * g + i) * G::DL + j) =
+                            f4{W.acc[h][j][i], W.acc[h][j + 1][i], W.acc[h][j + 2][i], W.acc[h][j + 3][i]} * to;
+        }
+        __syncthreads();
+        const bool starts = un == 0, ends = un + count == w.units;
+        const bool whole = starts && ends, done = whole && A.a.shared_len == 0;
+        for (int x = tid; x < nq * (HD / 4); x += kTPB) {
+            const int r = x / (HD / 4), d = x % (HD / 4) * 4, num = rb * kRows + r;
+            float ar = INFINITY, lr = 0.0f;
+            f4 o = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kWaves; i++) ar = fminf(ar, wave_al[i][r].x);
+#pragma unroll
+            for (int i = 0; i < kWaves; i++) {
+                const float2 al = wave_al[i][r];
+                lr += al.x == INFINITY ? 0.0f : al.y * exp2_hw(ar - al.x);
+                o += *(const f4 *)((const float *)lds + ((size_t)i * kRows + r) * MS + d);
+            }
+            const int row = w.lo + num / A.group, head = kvh * A.group + num % A.group;
+            if (done) {
+                const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+                f4 y = o * inv;
+                if (A.a.gate) {
+                    const float *z = A.a.gate + (size_t)row * A.a.gate_row + (size_t)head * A.a.gate_head + d;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] *= sigmoid1(z[e]);
+                }
+                *(f4u *)(A.a.out + ((size_t)row * A.a.n_head + head) * HD + d) = y;
+            } else {
+                const size_t rec = whole ? rec_whole(A, seq >= 0, row, head) : rec_part((int)blockIdx.x, starts, r);
+                *(f4 *)(A.rec_o + rec * HD + d) = o;
+                if (d == 0) A.rec_al[rec] = make_float2(ar, lr);
+            }
+        }
+        if (starts && tid == 0) {
+            const int blk = seq < 0 ? rb : A.prefix_blocks + block_index(seq, w.lo, rb, A.group, kRows);
+            A.seg[(size_t)blk * nkv + kvh] =
+                done ? make_int2(kDone, 0) : whole ? make_int2(kWhole, 0)
+                                                   : make_int2((int)blockIdx.x, run_owner(T, runs, u + w.units - 1));
+        }
+        u += count;
+        off += count;
+    }
+}
+
+// Joins the records of a row and head (its part of the shared positions, then
+// its own) where the workgroups have not written the result themselves: the
+// least reference first, then the sums in the records' order.
+template <int HD, int U>
+__global__ __launch_bounds__(kTPB) void attn_join_kernel(AttnArgs A) {
+    constexpr int E = HD / 64;
+    __shared__ int seq_s;
+    __shared__ float wgt[2 * kGroups + 2];
+    __shared__ float red[kWaves], redl[kWaves];
+    __shared__ float part[kWaves][HD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nkv = A.kv.n_head_kv;
+    const int row = (int)(blockIdx.x / A.a.n_head), head = (int)(blockIdx.x % A.a.n_head);
+    if (tid == 0) seq_s = -1;
+    __syncthreads();
+    for (int i = tid; i < A.b.n_seqs; i += kTPB) {
+        const SeqRows r = seq_rows(A.b.row_start[i], A.b.row_start[i + 1], A.b.n_rows);
+        if (row >= r.lo && row < r.lo + r.n) seq_s = i;
+    }
+    __syncthreads();
+    const int seq = seq_s, kvh = head / A.group;
+    if (seq < 0) return;
+    // the two parts: records first .. first + count - 1 of workgroups, or one whole record
+    int count[2] = {0, 0}, first[2] = {0, 0}, slot[2] = {0, 0};
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+        if (c == 0 && A.a.shared_len == 0) continue;
+        const Work w = work_of<U>(A, c == 0 ? -1 : seq);
+        if (w.units == 0) continue;
+        const int num = (row - w.lo) * A.group + head % A.group, rb = num / kRows;
+        slot[c] = num % kRows;
+        const int blk = c == 0 ? rb : A.prefix_blocks + block_index(seq, w.lo, rb, A.group, kRows);
+        const int2 s = A.seg[(size_t)blk * nkv + kvh];
+        if (s.x == kDone) return;
+        first[c] = s.x;
+        count[c] = s.x == kWhole ? 1 : s.y - s.x + 1;
+    }
+    const int total = count[0] + count[1];
+    auto rec = [&](int i) {
+        const int c = i >= count[0], k = c ? i - count[0] : i;
+        return first[c] == kWhole ? rec_whole(A, c, row, head) : rec_part(first[c] + k, k == 0, slot[c]);
+    };
+    float amin = INFINITY;
+    for (int i = tid; i < total; i += kTPB) amin = fminf(amin, A.rec_al[rec(i)].x);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) amin = fminf(amin, __shfl_xor(amin, d));
+    if (lane == 0) red[wave] = amin;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) amin = fminf(amin, red[i]);
+    float l = 0.0f;
+    for (int i = tid; i < total; i += kTPB) {
+        const float2 al = A.rec_al[rec(i)];
+        const float f = al.x == INFINITY ? 0.0f : exp2_hw(amin - al.x);
+        wgt[i] = f;
+        l += f == 0.0f ? 0.0f : f * al.y;
+    }
+    l = wave_sum(l);
+    if (lane == 0) redl[wave] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; i++) l += redl[i];
+    float o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+#pragma unroll 4
+    for (int i = wave; i < total; i += kWaves) {
+        const float *src = A.rec_o + rec(i) * HD + lane;
+        const float f = wgt[i];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const float v = src[64 * e];
+            o[e] += f == 0.0f ? 0.0f : f * v;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) part[wave][64 * e + lane] = o[e];
+    __syncthreads();
+    for (int d = tid; d < HD; d += kTPB) {
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) y += part[i][d];
+        y = l == 0.0f ? 0.0f : y / l;
+        if (A.a.gate) y *= sigmoid1(A.a.gate[(size_t)row * A.a.gate_row + (size_t)head * A.a.gate_head + d]);
+        A.a.out[((size_t)row * A.a.n_head + head) * HD + d] = y;
+    }
+}
+
+// The workspace's parts.
+struct Layout {
+    size_t o, al, seg, bytes;
+    int prefix_blocks, G;
+};
+
+Layout layout(const PagesView &kv, const BatchView &b, int n_head, int shared_len) {
+    const int group = n_head / kv.n_head_kv;
+    const size_t own = (size_t)b.n_seqs + (size_t)blocks_of(b.n_rows, group, kRows);
+    const size_t shared = shared_len ? (size_t)blocks_of(b.n_rows, group, kRows) : 0;
+    const size_t recs = (size_t)kGroups * 2 * kRows + (shared_len ? (size_t)2 * b.n_rows * n_head : 0);
+    Layout l;
+    l.G = kGroups;
+    l.prefix_blocks = (int)shared;
+    l.o = 0;
+    l.al = l.o + recs * kv.head_dim * sizeof(float);
+    l.seg = l.al + recs * sizeof(float2);
+    l.bytes = l.seg + (own + shared) * kv.n_head_kv * sizeof(int2);
+    return l;
+}
+
+template <bool F16, int HD>
+hipError_t launch(AttnArgs A, hipStream_t s) {
+    constexpr size_t lds = (size_t)kWaves * kRows * (HD + 4) * 4;
+    static_assert(lds >= (size_t)HD * 64, "the queries fit where the sums go");
+    constexpr int U = kWaves * Geo<F16, HD>::NP;
+    auto *k = attn_paged_kernel<F16, HD>;
+    if (hipError_t e = allow_lds((const void *)k, lds)) return e;
+    hipLaunchKernelGGL(k, dim3((unsigned)A.G), dim3(kTPB), lds, s, A);
+    if (hipError_t e = hipGetLastError()) return e;
+    hipLaunchKernelGGL((attn_join_kernel<HD, U>), dim3((unsigned)((size_t)A.b.n_rows * A.a.n_head)), dim3(kTPB), 0, s, A);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t attn_paged_ws_bytes(const PagesView &kv, const BatchView &b, int n_head, int shared_len) {
+    return layout(kv, b, n_head, shared_len).bytes;
+}
+
+hipError_t launch_attn_paged(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a, void *ws, hipStream_t s) {
+    if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
+    const Layout l = layout(kv, b, a.n_head, a.shared_len);
+    uint8_t *p = (uint8_t *)ws;
+    const AttnArgs A{a, kv, b, a.n_head / kv.n_head_kv, l.G, l.prefix_blocks, (float *)(p + l.o), (float2 *)(p + l.al), (int2 *)(p + l.seg)};
+    switch (kv.head_dim) {
+    case 64: return kv.f16 ? launch<true, 64>(A, s) : launch<false, 64>(A, s);
+    case 128: return kv.f16 ? launch<true, 128>(A, s) : launch<false, 128>(A, s);
+    case 256: return kv.f16 ? launch<true, 256>(A, s) : launch<false, 256>(A, s);
+    case 512: return kv.f16 ? launch<true, 512>(A, s) : launch<false, 512>(A, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace uq

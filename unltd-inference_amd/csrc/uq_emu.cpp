@@ -14,6 +14,7 @@
 
 #include "uq_policies.h"
 #include "uq_q8k_tiles.h"
+#include "uq_serve_index.h"
 
 using namespace uq;
 
@@ -411,5 +412,20 @@ int uq_emu_gemm_q8k(float *y, const float *x, size_t m_rows, const uint8_t *w, s
         emu_gemm_q8k<true>(y, x, M, W.p, rb, K, N);
     return 0;
 }
+
+// The index arithmetic of the paged cache and of the attention's work list.
+void uq_emu_seq_rows(int a, int b, int n_rows, int *out) {
+    const SeqRows r = seq_rows(a, b, n_rows);
+    out[0] = r.lo, out[1] = r.n;
+}
+int uq_emu_seq_len(int len, int cap) { return seq_len(len, cap); }
+int uq_emu_page_row(int n_pages, int n_head_kv, int log2_page, int page, int j, int pos) {
+    const PageMap m{n_pages, n_head_kv, log2_page};
+    return page_ok(m, page) ? page_row(m, page, j, pos) : -1;
+}
+long long uq_emu_run_start(long long T, int G, int w) { return run_start(T, G, w); }
+int uq_emu_run_owner(long long T, int G, long long u) { return run_owner(T, G, u); }
+int uq_emu_blocks_of(int n, int group, int RB) { return blocks_of(n, group, RB); }
+int uq_emu_block_index(int b, int lo, int rb, int group, int RB) { return block_index(b, lo, rb, group, RB); }
 
 }  // extern "C"

@@ -1,0 +1,416 @@
+// Batched serving: preparation and append of a batch's heads
+// (uq_kv_append_d) and the verification of drafted tokens
+// (uq_draft_verify_d). The attention over the pages is uq_attn_paged.hip.
+#include <climits>
+
+#include "uq_device.h"
+#include "uq_serve_internal.h"
+
+namespace uq {
+
+namespace {
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any float
+
+// ---- heads of a row ---------------------------------------------------------
+
+constexpr int kAppTPB = 256;
+constexpr int kAppMaxHd = 512;
+
+// The row's sequence, position and page, found by the whole workgroup at once
+// (one round trip for the starts and lengths, one for the page) and left in
+// LDS. pos -1: the row belongs to no sequence or lies at a negative position.
+struct RowAt {
+    int seq, pos, page;
+};
+
+__device__ __forceinline__ void find_row(const BatchView &b, const PageMap &m, int row, RowAt *at) {
+    if (threadIdx.x == 0) *at = RowAt{-1, -1, -1};
+    __syncthreads();
+    for (int i = threadIdx.x; i < b.n_seqs; i += kAppTPB) {
+        const SeqRows r = seq_rows(b.row_start[i], b.row_start[i + 1], b.n_rows);
+        if (row < r.lo || row >= r.lo + r.n) continue;
+        const int cap = b.max_pages << m.log2_page, len = b.len[i];
+        const int pos = len - r.n + (row - r.lo);
+        int page = -1;
+        if (len >= 0 && pos >= 0 && pos < cap) page = b.pages[(size_t)i * b.max_pages + (pos >> m.log2_page)];
+        *at = RowAt{i, len >= 0 ? pos : -1, page};
+    }
+    __syncthreads();
+}
+
+// E consecutive floats of a row from any float on.
+template <int E>
+__device__ __forceinline__ void load_row(float (&v)[E], const float *p) {
+    if constexpr (E >= 4) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const f4u f = *(const f4u *)(p + e);
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[e + i] = f[i];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = p[e];
+    }
+}
+template <int E>
+__device__ __forceinline__ void store_row(float *p, const float (&v)[E]) {
+    if constexpr (E >= 4) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(f4u *)(p + e) = f4u{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) p[e] = v[e];
+    }
+}
+// Rounded to nearest even, as one store of 2 E bytes (rows are 2 E-byte aligned).
+template <int E>
+__device__ __forceinline__ void store_half(_Float16 *p, const float (&v)[E]) {
+    typedef _Float16 hE __attribute__((ext_vector_type(E)));
+    if constexpr (E == 1) {
+        *p = (_Float16)v[0];
+    } else {
+        hE h;
+#pragma unroll
+        for (int e = 0; e < E; e++) h[e] = (_Float16)v[e];
+        *(hE *)p = h;
+    }
+}
+
+// rms norm of a row held E values a lane (uq_rmsnorm's bits): the sequential
+// f64 sum of the f32 squares as the wave's tree with the bound of
+// seq_sum_f32 (uq_device.h), or, undecided, replayed in order with each value
+// taken from its lane.
+template <int E>
+__device__ __forceinline__ void norm_row(float (&v)[E], const float (&w)[E], float eps) {
+    constexpr int n = 64 * E;
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e++) s += (double)__fmul_rn(v[e], v[e]);
+    const double S = wave_sum_d(s), dn = (double)n, er = (double)(n + 66) * 0x1p-52 * S;
+    float mean = (float)((S - er) / dn);
+    if (__float_as_uint(mean) != __float_as_uint((float)((S + er) / dn))) {  // wave-uniform
+        double q = 0.0;
+        for (int l = 0; l < 64; l++)
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float t = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[e]), l));
+                q += (double)__fmul_rn(t, t);
+            }
+        mean = (float)(q / dn);
+    }
+    const float scale = __fdiv_rn(1.0f, sqrtf_cr(__fadd_rn(mean, eps)));
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = __fmul_rn(__fmul_rn(v[e], scale), w[e]);
+}
+
+struct AppendArgs {
+    uq_head_rows h;
+    PagesView kv;
+    BatchView b;
+};
+
+// One workgroup for a row's heads blockIdx.y, blockIdx.y + gridDim.y, ...: the
+// row's angles once (f64 sine and cosine, as the per-row rotations take
+// them; they cost as much as a head's whole norm), kept in LDS, then a wave a
+// head: E = HD / 64 values a lane, norm in registers, rotation through the
+// wave's own LDS row, one store.
+template <int HD, bool F16>
+__global__ __launch_bounds__(kAppTPB) void kv_append_kernel(AppendArgs a) {
+    constexpr int E = HD / 64, NW = kAppTPB / 64;
+    __shared__ RowAt at;
+    __shared__ double2 turn[kAppMaxHd / 2];
+    __shared__ float rowv[NW][HD];
+    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uq_head_rows &h = a.h;
+    find_row(a.b, a.kv.map, row, &at);
+    const int pos = at.pos, page = at.page;
+    if (pos < 0) return;
+    const int half = (int)h.n_rot / 2, step = h.rope == UQ_ROPE_IMROPE ? 3 : 1;
+    const int turns = h.rope == UQ_ROPE_NONE ? 0 : (half + step - 1) / step;
+    for (int t = threadIdx.x; t < turns; t += kAppTPB) {
+        double angle = (double)pos;
+        if (h.rope == UQ_ROPE_IMROPE)
+            for (int i = 0; i < 3 * t; i++) angle *= h.theta_scale;
+        else
+            angle *= (double)h.d_freqs[t];
+        double sn, cs;
+        sincos(angle, &sn, &cs);
+        turn[t] = make_double2(sn, cs);
+    }
+    __syncthreads();
+    const int nq = h.d_q ? (int)h.n_head : 0, nk = h.d_k ? a.kv.n_head_kv : 0;
+    const bool cached = page_ok(a.kv.map, page);
+    for (int u = wave + NW * (int)blockIdx.y; u < nq + 2 * nk; u += NW * (int)gridDim.y) {
+        const bool isq = u < nq, isv = u >= nq + nk;
+        const int j = isq ? u : isv ? u - nq - nk : u - nq;
+        if (!isq && !cached) continue;  // the whole wave
+        const float *src = isq ? h.d_q + (size_t)row * h.q_row + (size_t)j * h.q_head
+                         : isv ? h.d_v + (size_t)row * h.v_row + (size_t)j * HD
+                               : h.d_k + (size_t)row * h.k_row + (size_t)j * HD;
+        float v[E];
+        load_row<E>(v, src + E * lane);
+        if (!isv) {
+            const float *w = isq ? h.d_q_norm : h.d_k_norm;
+            if (w) {
+                float wv[E];
+                load_row<E>(wv, w + E * lane);
+                norm_row<E>(v, wv, h.eps);
+            }
+            if (turns) {
+                float *rv = rowv[wave];
+#pragma unroll
+                for (int e = 0; e < E; e++) rv[E * lane + e] = v[e];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                for (int t = lane; t < turns; t += 64) {
+                    const int x = h.rope == UQ_ROPE_LLAMA ? 2 * t : step * t;
+                    const int y = h.rope == UQ_ROPE_LLAMA ? x + 1 : x + half;
+                    const double2 tr = turn[t];
+                    const double x0 = (double)rv[x], x1 = (double)rv[y];
+                    rv[x] = (float)fma(tr.y, x0, -(tr.x * x1));
+                    rv[y] = (float)fma(tr.x, x0, tr.y * x1);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int e = 0; e < E; e++) v[e] = rv[E * lane + e];
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+        if (isq) {
+            store_row<E>(h.d_q_out + ((size_t)row * h.n_head + j) * HD + E * lane, v);
+        } else {
+            const size_t o = (size_t)page_row(a.kv.map, page, j, pos) * HD + E * lane;
+            if constexpr (F16)
+                store_half<E>((_Float16 *)(isv ? a.kv.v : a.kv.k) + o, v);
+            else
+                store_row<E>((float *)(isv ? a.kv.v : a.kv.k) + o, v);
+        }
+    }
+}
+
+// ---- verification -------------------------------------------------------------
+
+constexpr int kVerTPB = 256;
+constexpr int kVerTiles = 8;
+constexpr int kVerChunk = kVerTPB * kVerTiles;  // tokens a workgroup sums
+
+struct VerifyArgs {
+    int32_t *accepted, *next;
+    const float *p, *q;
+    size_t p_row, q_row;
+    const int32_t *tokens;
+    const float *u;
+    BatchView b;
+    int vocab, chunks;
+    double2 *sums;  // [n_seqs][chunks]: the chunk's weight after a refusal, and of p alone
+};
+
+// A weight that is NaN, negative or infinite counts as zero.
+__device__ __forceinline__ double weight(double w) { return w > 0.0 && w < (double)INFINITY ? w : 0.0; }
+
+struct Row {
+    size_t row;   // the row that is drawn from
+    int accepted, last;  // last: index of the sequence's last row
+    bool ended;   // every draft was accepted
+    int x;        // the refused token (certain drafts)
+};
+
+// The first refused draft of sequence s (rows r), found by the whole
+// workgroup: the products are exact in f64 (24 x 24 bits).
+__device__ __forceinline__ Row verify_row(const VerifyArgs &a, const SeqRows &r, int *first) {
+    const int k = r.n - 1;
+    if (threadIdx.x == 0) *first = k;
+    __syncthreads();
+    for (int i = threadIdx.x; i < k; i += kVerTPB) {
+        const size_t row = (size_t)r.lo + i;
+        const int x = a.tokens[row + 1];
+        bool ok = false;
+        if ((unsigned)x < (unsigned)a.vocab) {
+            const double q = a.q ? (double)a.q[row * a.q_row + x] : 1.0;
+            ok = (double)a.u[row] * q < (double)a.p[row * a.p_row + x];
+        }
+        if (!ok) atomicMin(first, i);  // integers: any order gives the least
+    }
+    __syncthreads();
+    const int i = *first;
+    Row o;
+    o.row = (size_t)r.lo + i;
+    o.accepted = i;
+    o.last = r.lo + k;
+    o.ended = i == k;
+    o.x = !o.ended && !a.q ? a.tokens[o.row + 1] : -1;
+    return o;
+}
+
+// Weights of token t: after a refusal, and of p.
+__device__ __forceinline__ double2 weights(const VerifyArgs &a, const Row &o, int t) {
+    const double p = (double)a.p[o.row * a.p_row + t];
+    double w = p;
+    if (!o.ended) w = a.q ? p - (double)a.q[o.row * a.q_row + t] : t == o.x ? 0.0 : p;
+    return make_double2(weight(w), weight(p));
+}
+
+// Sums of one chunk of one sequence's row. Each of p and q is read once here,
+// the drawn token's chunk once more by verify_draw_kernel.
+__global__ __launch_bounds__(kVerTPB) void verify_sum_kernel(VerifyArgs a) {
+    __shared__ int first;
+    __shared__ double red[kVerTPB / 64];
+    const int s = blockIdx.y, c = blockIdx.x;
+    const SeqRows r = seq_rows(a.b.row_start[s], a.b.row_start[s + 1], a.b.n_rows);
+    if (r.n == 0) return;
+    const Row o = verify_row(a, r, &first);
+    double2 w[kVerTiles];
+#pragma unroll
+    for (int j = 0; j < kVerTiles; j++) {
+        const int t = c * kVerChunk + j * kVerTPB + threadIdx.x;
+        w[j] = t < a.vocab ? weights(a, o, t) : make_double2(0.0, 0.0);
+    }
+    double x = 0.0, y = 0.0;
+#pragma unroll
+    for (int j = 0; j < kVerTiles; j++) x += w[j].x, y += w[j].y;
+    x = block_sum_d<kVerTPB>(x, red);
+    y = block_sum_d<kVerTPB>(y, red);
+    if (threadIdx.x == 0) a.sums[(size_t)s * a.chunks + c] = make_double2(x, y);
+}
+
+// Inclusive sum of v over the workgroup's threads in thread order (wave scan,
+// then the waves before); total: the last thread's. Three barriers.
+__device__ __forceinline__ double block_scan_d(double v, double *red, double *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double up = __shfl_up(v, d);
+        if (lane >= d) v += up;
+    }
+    if (lane == 63) red[wave] = v;
+    __syncthreads();
+    double before = 0.0, t = 0.0;
+    for (int i = 0; i < kVerTPB / 64; i++) {
+        if (i == wave) before = t;
+        t += red[i];
+    }
+    __syncthreads();
+    *total = t;
+    return before + v;
+}
+
+// One workgroup a sequence: the chunk that the threshold falls in, then the
+// token in it. Rounded running sums need not ascend where a weight is zero or
+// at the joints of the tree, so a token needs weight of its own to be drawn,
+// and where no sum exceeds the threshold the last one with weight is it.
+__global__ __launch_bounds__(kVerTPB) void verify_draw_kernel(VerifyArgs a) {
+    __shared__ int first, hit, last;
+    __shared__ double red[kVerTPB / 64];
+    __shared__ double base_s;
+    const int s = blockIdx.x, tid = threadIdx.x;
+    const SeqRows r = seq_rows(a.b.row_start[s], a.b.row_start[s + 1], a.b.n_rows);
+    if (r.n == 0) {
+        if (tid == 0) a.accepted[s] = 0, a.next[s] = -1;
+        return;
+    }
+    const Row o = verify_row(a, r, &first);
+    if (tid == 0) a.accepted[s] = o.accepted, hit = INT_MAX, last = -1;
+    // every thread a run of chunks
+    const double2 *sums = a.sums + (size_t)s * a.chunks;
+    const int per = (a.chunks + kVerTPB - 1) / kVerTPB, c0 = min(a.chunks, tid * per), c1 = min(a.chunks, c0 + per);
+    double2 t = make_double2(0.0, 0.0);
+    for (int c = c0; c < c1; c++) t.x += sums[c].x, t.y += sums[c].y;
+    double total, unused;
+    double inc = block_scan_d(t.x, red, &total);  // its barriers publish hit and last
+    const double incp = block_scan_d(t.y, red, &unused);
+    const bool plain = !(total > 0.0);  // no weight after the refusal: p itself
+    const double mine = plain ? t.y : t.x;
+    if (plain) inc = incp, total = unused;
+    double u = (double)a.u[o.last];
+    u = u >= 0.0 ? u : u < 0.0 ? 0.0 : 1.0;  // NaN as 1
+    const double thr = u >= 1.0 ? (double)INFINITY : u * total;
+    if (mine > 0.0) {
+        atomicMax(&last, tid);
+        if (inc > thr) atomicMin(&hit, tid);
+    }
+    __syncthreads();
+    if (last < 0) {
+        if (tid == 0) a.next[s] = -1;
+        return;
+    }
+    const int owner = hit != INT_MAX ? hit : last;
+    __syncthreads();
+    if (tid == owner) {  // the chunk in the run
+        double run = inc - mine, base = run;
+        int found = c0;
+        for (int c = c0; c < c1; c++) {
+            const double v = plain ? sums[c].y : sums[c].x;
+            if (!(v > 0.0)) continue;
+            found = c;
+            base = run;
+            run += v;
+            if (run > thr) break;
+        }
+        base_s = base;
+        first = found;
+        hit = INT_MAX;
+        last = -1;
+    }
+    __syncthreads();
+    const int c = first;
+    double base = base_s;
+    for (int j = 0; j < kVerTiles; j++) {
+        const int x = c * kVerChunk + j * kVerTPB + tid;
+        const double2 v = x < a.vocab ? weights(a, o, x) : make_double2(0.0, 0.0);
+        const double w = plain ? v.y : v.x;
+        double sum;
+        const double upto = base + block_scan_d(w, red, &sum);
+        if (w > 0.0) {
+            atomicMax(&last, x);
+            if (upto > thr) atomicMin(&hit, x);
+        }
+        __syncthreads();
+        if (hit != INT_MAX) break;  // read alike by all: the next update lies behind a barrier
+        base += sum;
+    }
+    if (tid == 0) a.next[s] = hit != INT_MAX ? hit : last;
+}
+
+}  // namespace
+
+hipError_t launch_kv_append(const PagesView &kv, const BatchView &b, const uq_head_rows &h, hipStream_t s) {
+    if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
+    const int units = (h.d_q ? (int)h.n_head : 0) + (h.d_k ? 2 * kv.n_head_kv : 0);
+    if (units == 0) return hipSuccess;
+    const int most = (units + kAppTPB / 64 - 1) / (kAppTPB / 64);
+    int split = (512 + b.n_rows - 1) / b.n_rows;
+    split = split < 1 ? 1 : split > most ? most : split;
+    const AppendArgs a{h, kv, b};
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)b.n_rows, (unsigned)split), dim3(kAppTPB), 0, s, a);
+        return hipGetLastError();
+    };
+    switch (kv.head_dim) {
+    case 64: return kv.f16 ? go(kv_append_kernel<64, true>) : go(kv_append_kernel<64, false>);
+    case 128: return kv.f16 ? go(kv_append_kernel<128, true>) : go(kv_append_kernel<128, false>);
+    case 256: return kv.f16 ? go(kv_append_kernel<256, true>) : go(kv_append_kernel<256, false>);
+    case 512: return kv.f16 ? go(kv_append_kernel<512, true>) : go(kv_append_kernel<512, false>);
+    }
+    return hipErrorInvalidValue;
+}
+
+size_t draft_verify_ws_bytes(int n_seqs, int vocab) {
+    return (size_t)n_seqs * (((size_t)vocab + kVerChunk - 1) / kVerChunk) * sizeof(double2);
+}
+
+hipError_t launch_draft_verify(int32_t *accepted, int32_t *next, const float *p, size_t p_row, const float *q,
+                               size_t q_row, const int32_t *tokens, const float *u, const BatchView &b, int vocab,
+                               void *ws, hipStream_t s) {
+    if (b.n_seqs == 0) return hipSuccess;
+    const int chunks = (vocab + kVerChunk - 1) / kVerChunk;
+    const VerifyArgs a{accepted, next, p, q, p_row, q_row, tokens, u, b, vocab, chunks, (double2 *)ws};
+    hipLaunchKernelGGL(verify_sum_kernel, dim3((unsigned)chunks, (unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace uq

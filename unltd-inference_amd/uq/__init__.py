@@ -142,6 +142,12 @@ SIGNATURES = {
     "uq_layer_prefill_ws_floats": ([_P, _P, _P, _S, _S], _S),
     "uq_gdn_layer_prefill_d": ([_P, _P, _P, _P, _S, _P, _P, _P, _S, _P], _I),
     "uq_attn_layer_prefill_d": ([_P, _P, _P, _P, _S, _S, _S, _P, _P, _P, _S, _P], _I),
+    # include/uq_serve.h (structs by address; uq.serve builds them)
+    "uq_kv_append_d": ([_P, _P, _P, _P], _I),
+    "uq_attn_paged_ws_bytes": ([_P, _P, _S, _S], _S),
+    "uq_attn_paged_d": ([_P, _P, _P, _P, _S, _S, C.c_float, _P, _S, _S, _P, _S, _P], _I),
+    "uq_draft_verify_ws_bytes": ([_P, _S], _S),
+    "uq_draft_verify_d": ([_P, _P, _P, _S, _P, _S, _P, _P, _P, _S, _P, _S, _P], _I),
 }
 
 
