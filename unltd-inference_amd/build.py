@@ -2,11 +2,11 @@
 
     python unltd-inference_amd/build.py [-v] [-i]   (-i: recompile only stale objects)
 
-libuq.so: every csrc/*.hip plus uq_abi.cpp, uq_gguf.cpp, uq_ops_abi.cpp, uq_layer.cpp and uq_serve_abi.cpp, compiled by hipcc for gfx950
-  only, -O3, FP contraction off (FMAs are written explicitly), f32
-  denormals kept, packed-FP32 instructions disabled. Each source is
-  compiled to its own object in parallel (objects under _build/), then
-  linked.
+libuq.so: every csrc/*.hip plus uq_abi.cpp, uq_gguf.cpp, uq_ops_abi.cpp,
+  uq_layer.cpp and uq_serve_abi.cpp, compiled by hipcc for gfx950 only, -O3,
+  FP contraction off (FMAs are written explicitly), f32 denormals kept,
+  packed-FP32 instructions disabled. Each source is compiled to its own
+  object in parallel (objects under _build/), then linked.
 libuq_emu.so: csrc/uq_emu.cpp with g++: the kernels' per-lane code run on
   the CPU, used by the CPU test-suite.
 """
@@ -36,6 +36,10 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
 
+# Matrix products with their sums in VGPRs: attn_many_kernel's queries then fill the accumulation registers, and the
+# vector units reach the sums without copies (with the sums there: 25 registers spilled, 230 copies a tile).
+SOURCE_FLAGS = {"uq_attn_many.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 
 def _run(cmd, verbose):
     if verbose:
@@ -51,7 +55,8 @@ def _run(cmd, verbose):
 
 def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip"))) + [
-        os.path.join(CSRC, f) for f in ("uq_abi.cpp", "uq_gguf.cpp", "uq_ops_abi.cpp", "uq_layer.cpp", "uq_serve_abi.cpp")]
+        os.path.join(CSRC, f) for f in ("uq_abi.cpp", "uq_gguf.cpp", "uq_ops_abi.cpp", "uq_layer.cpp",
+                                        "uq_serve_abi.cpp")]
 
 
 def _stale(src, obj):
@@ -70,7 +75,8 @@ def build_lib(verbose: bool = False, jobs: int | None = None, incremental: bool 
     todo = [(s, o) for s, o in zip(srcs, objs) if not incremental or _stale(s, o)]
     jobs = jobs or max(1, min(len(todo), 8, os.cpu_count() or 1))
     with ThreadPoolExecutor(jobs) as ex:
-        list(ex.map(lambda so: _run(["hipcc", *HIPCC_FLAGS, "-x", "hip", "-c", so[0], "-o", so[1]], verbose),
+        list(ex.map(lambda so: _run(["hipcc", *HIPCC_FLAGS, *SOURCE_FLAGS.get(os.path.basename(so[0]), []), "-x", "hip",
+                                     "-c", so[0], "-o", so[1]], verbose),
                     todo))
     tmp = LIB + ".tmp"
     _run(["hipcc", f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp], verbose)

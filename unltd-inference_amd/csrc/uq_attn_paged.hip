@@ -6,51 +6,17 @@
 // where -a follows the largest s log2 e seen so far (o and l are multiplied by
 // 2^(a' - a) when it moves), and the result is o / l. Parts over other
 // positions join the same way.
-#include <algorithm>
-#include <climits>
-
-#include "uq_device.h"
-#include "uq_internal.h"
-#include "uq_serve_internal.h"
+#include "uq_attn_paged.h"
 
 namespace uq {
 
 namespace {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any float
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-
 constexpr int kTPB = 256;
 constexpr int kWaves = kTPB / 64;
-constexpr int kRows = 16;       // queries of a block: the columns of a 16x16 tile
-constexpr int kGroups = 512;    // workgroups: two per CU
-constexpr float kLog2e = 1.44269504088896340736f;
-
-struct AttnArgs {
-    AttnPagedArgs a;
-    PagesView kv;
-    BatchView b;
-    int group, G, prefix_blocks;
-    float *rec_o;   // records: [..][HD] sums o ...
-    float2 *rec_al; // ... with (a, l)
-    int2 *seg;      // [block][kv head]: first and last workgroup of its units, or kDone / kWhole
-};
-
-// Where a block's units lie: in one workgroup that wrote the results itself,
-// in one whose record is the row's own, or in several workgroups' records.
-constexpr int kDone = -1, kWhole = -2;
-
-// Records: two blocks of rows for each workgroup (its run's first block where
-// that began earlier, its last where that goes on), then one per row and
-// head of the shared and of the own positions.
-__device__ __forceinline__ size_t rec_part(int w, int second, int n) { return ((size_t)w * 2 + second) * kRows + n; }
-__device__ __forceinline__ size_t rec_whole(const AttnArgs &A, int own, int row, int head) {
-    return (size_t)A.G * 2 * kRows + ((size_t)own * A.b.n_rows + row) * A.a.n_head + head;
-}
+constexpr int kRows = 16;     // queries of a block: the columns of a 16x16 tile
+constexpr int kCUs = 256;
+constexpr int kGroups = 2 * kCUs;  // workgroups: two per CU
 
 template <bool F16, int HD>
 struct Geo;
@@ -66,31 +32,6 @@ struct Geo<false, HD> {
     static constexpr int NP = 16, PT = 1, KC = HD / 16, DL = 4, NH = HD / 64, VS = 4;
 };
 
-// The sequence of one part of the work: s = -1 is the shared positions with
-// the rows of the whole batch.
-struct Work {
-    int lo, n, len;      // rows, length as given
-    int base, end;       // positions [base, end)
-    int units, blocks;
-};
-
-template <int U>
-__device__ __forceinline__ Work work_of(const AttnArgs &A, int s) {
-    Work w;
-    const int cap = A.b.max_pages << A.kv.map.log2_page;
-    if (s < 0) {
-        const SeqRows r = seq_rows(0, A.b.row_start[A.b.n_seqs], A.b.n_rows);
-        w = Work{r.lo, r.n, 0, 0, A.a.shared_len, 0, 0};
-    } else {
-        const SeqRows r = seq_rows(A.b.row_start[s], A.b.row_start[s + 1], A.b.n_rows);
-        const int len = A.b.len[s];
-        w = Work{r.lo, r.n, len, A.a.shared_len, seq_len(len, cap), 0, 0};
-    }
-    w.units = w.end > w.base ? (w.end - w.base + U - 1) / U : 0;
-    w.blocks = blocks_of(w.n, A.group, kRows);
-    return w;
-}
-
 __device__ __forceinline__ float row16_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
     v = fmaxf(v, __shfl_xor(v, 16));
     return fmaxf(v, __shfl_xor(v, 32));
@@ -99,8 +40,6 @@ __device__ __forceinline__ float row16_sum(float v) {
     v += __shfl_xor(v, 16);
     return v + __shfl_xor(v, 32);
 }
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
 __device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
 // A wave's part of a block: scores, running reference and sums over its
@@ -179,82 +118,23 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
     using E = std::conditional_t<F16, _Float16, float>;
     constexpr int NP = G::NP, U = kWaves * NP, MS = HD + 4;
     constexpr float kShift = F16 ? 14.0f : 0.0f;
-    extern __shared__ uint8_t lds[];       // the block's queries; the waves' sums at its end
+    extern __shared__ __align__(1024) uint8_t lds[];  // the block's queries; the waves' sums at its end
     __shared__ float row_c[kRows];         // score factor of a query, times log2 e
     __shared__ int row_lim[kRows];         // its last position, -1: none
     __shared__ float2 wave_al[kWaves][kRows];
-    __shared__ long long scan[kWaves];
-    __shared__ long long start_s;
-    __shared__ int seq_s;
+    __shared__ RunLds run_lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 
-    // ---- this workgroup's run of units: [u, u1) of T, beginning off units into
-    // sequence seq (-1: the shared positions)
-    const int parts = A.b.n_seqs + 1;
-    long long T = 0, mine = 0, before = 0;
-    for (int c = 0; c < parts; c += kTPB) {
-        const int i = c + tid;
-        mine = 0;
-        if (i < parts && (i > 0 || A.a.shared_len > 0)) {
-            const Work w = work_of<U>(A, i - 1);
-            mine = (long long)w.units * w.blocks * nkv;
-        }
-        long long inc = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long up = __shfl_up(inc, d);
-            if (lane >= d) inc += up;
-        }
-        __syncthreads();
-        if (lane == 63) scan[wave] = inc;
-        __syncthreads();
-        before = T + inc - mine;
-        for (int i2 = 0; i2 < kWaves; i2++) {
-            if (i2 < wave) before += scan[i2];
-            T += scan[i2];
-        }
-    }
-    const int runs = (int)min((long long)A.G, T);  // no empty runs between others
-    if ((int)blockIdx.x >= runs) return;
-    long long u = run_start(T, runs, (int)blockIdx.x);
-    const long long u1 = run_start(T, runs, (int)blockIdx.x + 1);
-    if (parts <= kTPB) {
-        if (mine > 0 && before <= u && u < before + mine) seq_s = tid - 1, start_s = u - before;
-    } else {
-        long long run = 0;
-        for (int c = 0; c < parts; c += kTPB) {
-            const int i = c + tid;
-            mine = 0;
-            if (i < parts && (i > 0 || A.a.shared_len > 0)) {
-                const Work w = work_of<U>(A, i - 1);
-                mine = (long long)w.units * w.blocks * nkv;
-            }
-            long long inc = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const long long up = __shfl_up(inc, d);
-                if (lane >= d) inc += up;
-            }
-            __syncthreads();
-            if (lane == 63) scan[wave] = inc;
-            __syncthreads();
-            before = run + inc - mine;
-            for (int i2 = 0; i2 < kWaves; i2++) {
-                if (i2 < wave) before += scan[i2];
-                run += scan[i2];
-            }
-            if (mine > 0 && before <= u && u < before + mine) seq_s = i - 1, start_s = u - before;
-        }
-    }
-    __syncthreads();
-    int seq = seq_s;
-    long long off = start_s;
-    Work w = work_of<U>(A, seq);
+    Run R;
+    if (!find_run<kTPB, U>(A, [&](int, const Work &w) { return (long long)w.units * w.blocks * nkv; }, run_lds, R)) return;
+    long long u = R.u, off = R.off;
+    int seq = R.seq;
+    Work w = R.work;
 
     Wave<F16, HD> W;
-    while (u < u1) {
+    while (u < R.u1) {
         const long long per = (long long)nkv * w.units;
         if (off >= per * w.blocks) {  // the next sequence with units (there is one: u < T)
             if (++seq >= A.b.n_seqs) return;
@@ -263,7 +143,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             continue;
         }
         const int rb = (int)(off / per), kvh = (int)(off % per / w.units), un = (int)(off % w.units);
-        const int count = (int)min((long long)(w.units - un), u1 - u);
+        const int count = (int)min((long long)(w.units - un), R.u1 - u);
         const int nq = min(kRows, w.n * A.group - rb * kRows);  // queries of the block
 
         // ---- the block's queries into LDS, in the order of the products' right operand
@@ -563,16 +443,16 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                 }
                 *(f4u *)(A.a.out + ((size_t)row * A.a.n_head + head) * HD + d) = y;
             } else {
-                const size_t rec = whole ? rec_whole(A, seq >= 0, row, head) : rec_part((int)blockIdx.x, starts, r);
+                const size_t rec = whole ? rec_whole(A, seq >= 0, row, head) : rec_part(A.part[seq >= 0], (int)blockIdx.x, starts, r);
                 *(f4 *)(A.rec_o + rec * HD + d) = o;
                 if (d == 0) A.rec_al[rec] = make_float2(ar, lr);
             }
         }
         if (starts && tid == 0) {
-            const int blk = seq < 0 ? rb : A.prefix_blocks + block_index(seq, w.lo, rb, A.group, kRows);
+            const int blk = seq < 0 ? rb : A.part[1].block0 + block_index(seq, w.lo, rb, A.group, kRows);
             A.seg[(size_t)blk * nkv + kvh] =
                 done ? make_int2(kDone, 0) : whole ? make_int2(kWhole, 0)
-                                                   : make_int2((int)blockIdx.x, run_owner(T, runs, u + w.units - 1));
+                                                   : make_int2((int)blockIdx.x, run_owner(R.T, R.runs, u + w.units - 1));
         }
         u += count;
         off += count;
@@ -582,11 +462,11 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 // Joins the records of a row and head (its part of the shared positions, then
 // its own) where the workgroups have not written the result themselves: the
 // least reference first, then the sums in the records' order.
-template <int HD, int U>
+template <int HD>
 __global__ __launch_bounds__(kTPB) void attn_join_kernel(AttnArgs A) {
     constexpr int E = HD / 64;
     __shared__ int seq_s;
-    __shared__ float wgt[2 * kGroups + 2];
+    __shared__ float wgt[2 * kGroups + 2];  // two parts' workgroups
     __shared__ float red[kWaves], redl[kWaves];
     __shared__ float part[kWaves][HD];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nkv = A.kv.n_head_kv;
@@ -605,11 +485,11 @@ __global__ __launch_bounds__(kTPB) void attn_join_kernel(AttnArgs A) {
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         if (c == 0 && A.a.shared_len == 0) continue;
-        const Work w = work_of<U>(A, c == 0 ? -1 : seq);
-        if (w.units == 0) continue;
-        const int num = (row - w.lo) * A.group + head % A.group, rb = num / kRows;
-        slot[c] = num % kRows;
-        const int blk = c == 0 ? rb : A.prefix_blocks + block_index(seq, w.lo, rb, A.group, kRows);
+        const Work w = work_of<1>(A, c == 0 ? -1 : seq);
+        const int num = (row - w.lo) * A.group + head % A.group, rb = num / A.part[c].rows;
+        if (w.units == 0 || (c == 1 && A.many && seen_units<1>(A, w, rb) == 0)) continue;
+        slot[c] = num % A.part[c].rows;
+        const int blk = c == 0 ? rb : A.part[1].block0 + block_index(seq, w.lo, rb, A.group, A.part[1].rows);
         const int2 s = A.seg[(size_t)blk * nkv + kvh];
         if (s.x == kDone) return;
         first[c] = s.x;
@@ -618,7 +498,7 @@ __global__ __launch_bounds__(kTPB) void attn_join_kernel(AttnArgs A) {
     const int total = count[0] + count[1];
     auto rec = [&](int i) {
         const int c = i >= count[0], k = c ? i - count[0] : i;
-        return first[c] == kWhole ? rec_whole(A, c, row, head) : rec_part(first[c] + k, k == 0, slot[c]);
+        return first[c] == kWhole ? rec_whole(A, c, row, head) : rec_part(A.part[c], first[c] + k, k == 0, slot[c]);
     };
     float amin = INFINITY;
     for (int i = tid; i < total; i += kTPB) amin = fminf(amin, A.rec_al[rec(i)].x);
@@ -667,58 +547,103 @@ __global__ __launch_bounds__(kTPB) void attn_join_kernel(AttnArgs A) {
     }
 }
 
-// The workspace's parts.
-struct Layout {
-    size_t o, al, seg, bytes;
-    int prefix_blocks, G;
+// The workspace's parts, and how the parts of the work are launched.
+struct Plan {
+    size_t al, seg, bytes;
+    bool apart;  // the shared positions in a launch of their own
+    AttnArgs A;
 };
 
-Layout layout(const PagesView &kv, const BatchView &b, int n_head, int shared_len) {
-    const int group = n_head / kv.n_head_kv;
-    const size_t own = (size_t)b.n_seqs + (size_t)blocks_of(b.n_rows, group, kRows);
-    const size_t shared = shared_len ? (size_t)blocks_of(b.n_rows, group, kRows) : 0;
-    const size_t recs = (size_t)kGroups * 2 * kRows + (shared_len ? (size_t)2 * b.n_rows * n_head : 0);
-    Layout l;
-    l.G = kGroups;
-    l.prefix_blocks = (int)shared;
-    l.o = 0;
-    l.al = l.o + recs * kv.head_dim * sizeof(float);
-    l.seg = l.al + recs * sizeof(float2);
-    l.bytes = l.seg + (own + shared) * kv.n_head_kv * sizeof(int2);
-    return l;
+// Queries of a block for R queries of a KV head, 0: the kernel of few.
+int many_rows(const PagesView &kv, size_t R) {
+    if (!attn_many_ok(kv) || R <= 32) return 0;
+    return (R + 127) / 128 * 128 == (R + 63) / 64 * 64 ? 128 : 64;
+}
+int many_groups(int rows) { return rows == 64 ? 2 * kCUs : kCUs; }
+
+Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
+    const int group = a.n_head / kv.n_head_kv;
+    const size_t queries = (size_t)b.n_rows * group;
+    Plan p{};
+    AttnArgs &A = p.A;
+    A.a = a, A.kv = kv, A.b = b, A.group = group;
+    const int few = kRows;
+    const int shared = a.shared_len ? many_rows(kv, queries) : 0;
+    const int own = many_rows(kv, (queries + b.n_seqs - 1) / b.n_seqs);
+    A.part[0] = shared ? Part{shared, many_groups(shared), 0, 0} : Part{few, kGroups, 0, 0};
+    A.part[1] = own ? Part{own, many_groups(own), 0, 0} : Part{few, kGroups, 0, 0};
+    A.many = own != 0;
+    p.apart = a.shared_len && (shared || own);
+    auto groups_recs = [&](const Part &x) { return (size_t)2 * x.G * x.rows; };
+    size_t recs = groups_recs(A.part[1]);
+    if (p.apart) A.part[0].base = recs, recs += groups_recs(A.part[0]);
+    A.whole = recs;
+    if (a.shared_len) recs += (size_t)2 * b.n_rows * a.n_head;
+    size_t blocks = a.shared_len ? (size_t)blocks_of(b.n_rows, group, A.part[0].rows) : 0;
+    A.part[1].block0 = (int)blocks;
+    blocks += (size_t)b.n_seqs + (size_t)blocks_of(b.n_rows, group, A.part[1].rows);
+    p.al = recs * kv.head_dim * sizeof(float);
+    p.seg = p.al + recs * sizeof(float2);
+    p.bytes = p.seg + blocks * kv.n_head_kv * sizeof(int2);
+    return p;
 }
 
 template <bool F16, int HD>
-hipError_t launch(AttnArgs A, hipStream_t s) {
+hipError_t launch(const AttnArgs &A, hipStream_t s) {
     constexpr size_t lds = (size_t)kWaves * kRows * (HD + 4) * 4;
     static_assert(lds >= (size_t)HD * 64, "the queries fit where the sums go");
-    constexpr int U = kWaves * Geo<F16, HD>::NP;
     auto *k = attn_paged_kernel<F16, HD>;
     if (hipError_t e = allow_lds((const void *)k, lds)) return e;
-    hipLaunchKernelGGL(k, dim3((unsigned)A.G), dim3(kTPB), lds, s, A);
-    if (hipError_t e = hipGetLastError()) return e;
-    hipLaunchKernelGGL((attn_join_kernel<HD, U>), dim3((unsigned)((size_t)A.b.n_rows * A.a.n_head)), dim3(kTPB), 0, s, A);
+    hipLaunchKernelGGL(k, dim3(kGroups), dim3(kTPB), lds, s, A);
+    return hipGetLastError();
+}
+
+hipError_t launch_few(const AttnArgs &A, hipStream_t s) {
+    switch (A.kv.head_dim) {
+    case 64: return A.kv.f16 ? launch<true, 64>(A, s) : launch<false, 64>(A, s);
+    case 128: return A.kv.f16 ? launch<true, 128>(A, s) : launch<false, 128>(A, s);
+    case 256: return A.kv.f16 ? launch<true, 256>(A, s) : launch<false, 256>(A, s);
+    case 512: return A.kv.f16 ? launch<true, 512>(A, s) : launch<false, 512>(A, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_join(const AttnArgs &A, hipStream_t s) {
+    const dim3 grid((unsigned)((size_t)A.b.n_rows * A.a.n_head));
+    switch (A.kv.head_dim) {
+    case 64: hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(kTPB), 0, s, A); break;
+    case 128: hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(kTPB), 0, s, A); break;
+    case 256: hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(kTPB), 0, s, A); break;
+    case 512: hipLaunchKernelGGL(attn_join_kernel<512>, grid, dim3(kTPB), 0, s, A); break;
+    default: return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
 
 }  // namespace
 
 size_t attn_paged_ws_bytes(const PagesView &kv, const BatchView &b, int n_head, int shared_len) {
-    return layout(kv, b, n_head, shared_len).bytes;
+    if (b.n_rows == 0 || b.n_seqs == 0) return 16;
+    AttnPagedArgs a{};
+    a.n_head = n_head, a.shared_len = shared_len;
+    return plan(kv, b, a).bytes;
 }
 
 hipError_t launch_attn_paged(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a, void *ws, hipStream_t s) {
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
-    const Layout l = layout(kv, b, a.n_head, a.shared_len);
-    uint8_t *p = (uint8_t *)ws;
-    const AttnArgs A{a, kv, b, a.n_head / kv.n_head_kv, l.G, l.prefix_blocks, (float *)(p + l.o), (float2 *)(p + l.al), (int2 *)(p + l.seg)};
-    switch (kv.head_dim) {
-    case 64: return kv.f16 ? launch<true, 64>(A, s) : launch<false, 64>(A, s);
-    case 128: return kv.f16 ? launch<true, 128>(A, s) : launch<false, 128>(A, s);
-    case 256: return kv.f16 ? launch<true, 256>(A, s) : launch<false, 256>(A, s);
-    case 512: return kv.f16 ? launch<true, 512>(A, s) : launch<false, 512>(A, s);
-    }
-    return hipErrorInvalidValue;
+    Plan p = plan(kv, b, a);
+    AttnArgs &A = p.A;
+    A.rec_o = (float *)ws;
+    A.rec_al = (float2 *)((uint8_t *)ws + p.al);
+    A.seg = (int2 *)((uint8_t *)ws + p.seg);
+    auto go = [&](int first, int last) {
+        A.first = first, A.last = last;
+        return A.part[first].rows == kRows ? launch_few(A, s) : launch_attn_many(A, s);
+    };
+    if (p.apart)
+        if (hipError_t e = go(0, 0)) return e;
+    if (hipError_t e = go(a.shared_len && !p.apart ? 0 : 1, 1)) return e;
+    return launch_join(A, s);
 }
 
 }  // namespace uq
