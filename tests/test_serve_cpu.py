@@ -136,7 +136,6 @@ def emu():
     E.uq_emu_run_start.argtypes, E.uq_emu_run_start.restype = [LL, I, I], LL
     E.uq_emu_run_owner.argtypes = [LL, I, LL]
     E.uq_emu_blocks_of.argtypes = [I, I, I]
-    E.uq_emu_block_index.argtypes = [I, I, I, I, I]
     return E
 
 
@@ -177,17 +176,11 @@ def test_every_unit_has_one_owner(T, G):
 
 
 @pytest.mark.parametrize("group,RB", [(1, 16), (3, 16), (4, 16), (24, 16), (4, 128), (8, 64)])
-def test_block_indexes_do_not_meet(group, RB):
-    E, rng = emu(), np.random.default_rng(group)
-    for _ in range(30):
-        rows = rng.integers(0, 40, 25)
-        lo, seen, last = 0, set(), 25 + E.uq_emu_blocks_of(int(rows.sum()), group, RB)
-        for b, n in enumerate(rows.tolist()):
-            for rb in range(E.uq_emu_blocks_of(n, group, RB)):
-                i = E.uq_emu_block_index(b, lo, rb, group, RB)
-                assert 0 <= i < last and i not in seen
-                seen.add(i)
-            lo += n
+def test_blocks_hold_every_query(group, RB):
+    E = emu()
+    for n in (0, 1, 2, 15, 16, 17, 40, 127, 128, 129, 1 << 24):
+        blocks = E.uq_emu_blocks_of(n, group, RB)
+        assert blocks * RB >= n * group > (blocks - 1) * RB or n == blocks == 0
 
 
 def test_the_model_reads_pages_as_the_layout_says():

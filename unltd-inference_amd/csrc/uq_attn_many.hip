@@ -533,11 +533,11 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
                 wave_fence();
             }
         }
-        if (starts && tid == 0) {
-            const int blk = seq < 0 ? rb : A.part[1].block0 + block_index(seq, w.lo, rb, A.group, RB);
-            A.seg[(size_t)blk * nkv + kvh] =
-                done ? make_int2(kDone, 0) : whole ? make_int2(kWhole, 0)
-                                                   : make_int2((int)blockIdx.x, run_owner(R.T, R.runs, u + cost - at - 1));
+        if (starts && tid < nq) {  // a block has half as many queries as the workgroup threads
+            const int num = rb * RB + tid;
+            put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
+                    done ? kDone : whole ? kWhole : (int)blockIdx.x,
+                    done || whole ? 0 : run_owner(R.T, R.runs, u + cost - at - 1), tid);
         }
         u += upto - at;
         off += upto - at;

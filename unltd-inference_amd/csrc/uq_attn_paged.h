@@ -20,7 +20,6 @@ struct Part {
     int rows;     // queries of a block
     int G;        // workgroups
     size_t base;  // first of the workgroups' records
-    int block0;   // first of the part's blocks in seg
 };
 
 struct AttnArgs {
@@ -34,7 +33,7 @@ struct AttnArgs {
     size_t whole;   // first of the rows' own records
     float *rec_o;   // records: [..][HD] sums o ...
     float2 *rec_al; // ... with (a, l)
-    int2 *seg;      // [block][kv head]: first and last workgroup of its units, or kDone / kWhole
+    int2 *seg;      // [part][row][head]: where the units of its block lie (put_seg)
 };
 
 // uq_attn_many.hip: part A.first (= A.last) on blocks of A.part[].rows = 64 or
@@ -65,6 +64,13 @@ __device__ __forceinline__ size_t rec_part(const Part &p, int w, int second, int
 }
 __device__ __forceinline__ size_t rec_whole(const AttnArgs &A, int part, int row, int head) {
     return A.whole + ((size_t)part * A.b.n_rows + row) * A.a.n_head + head;
+}
+
+// What the workgroup that starts a block notes for each of its queries: the
+// first workgroup with units of the block, or kDone or kWhole, the last one,
+// and the query's place among the block's records.
+__device__ __forceinline__ void put_seg(const AttnArgs &A, int part, int row, int head, int first, int last, int slot) {
+    A.seg[((size_t)part * A.b.n_rows + row) * A.a.n_head + head] = make_int2(first, last << 8 | slot);
 }
 
 // The sequence of one part of the work: s = -1 is the shared positions with

@@ -448,11 +448,10 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                 if (d == 0) A.rec_al[rec] = make_float2(ar, lr);
             }
         }
-        if (starts && tid == 0) {
-            const int blk = seq < 0 ? rb : A.part[1].block0 + block_index(seq, w.lo, rb, A.group, kRows);
-            A.seg[(size_t)blk * nkv + kvh] =
-                done ? make_int2(kDone, 0) : whole ? make_int2(kWhole, 0)
-                                                   : make_int2((int)blockIdx.x, run_owner(R.T, R.runs, u + w.units - 1));
+        if (starts && tid < nq) {
+            const int num = rb * kRows + tid;
+            put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
+                    done ? kDone : whole ? kWhole : (int)blockIdx.x, done || whole ? 0 : run_owner(R.T, R.runs, u + w.units - 1), tid);
         }
         u += count;
         off += count;
@@ -461,87 +460,113 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 
 // Joins the records of a row and head (its part of the shared positions, then
 // its own) where the workgroups have not written the result themselves: the
-// least reference first, then the sums in the records' order.
-template <int HD>
-__global__ __launch_bounds__(kTPB) void attn_join_kernel(AttnArgs A) {
-    constexpr int E = HD / 64;
-    __shared__ int seq_s;
-    __shared__ float wgt[2 * kGroups + 2];  // two parts' workgroups
-    __shared__ float red[kWaves], redl[kWaves];
-    __shared__ float part[kWaves][HD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nkv = A.kv.n_head_kv;
-    const int row = (int)(blockIdx.x / A.a.n_head), head = (int)(blockIdx.x % A.a.n_head);
-    if (tid == 0) seq_s = -1;
-    __syncthreads();
-    for (int i = tid; i < A.b.n_seqs; i += kTPB) {
-        const SeqRows r = seq_rows(A.b.row_start[i], A.b.row_start[i + 1], A.b.n_rows);
-        if (row >= r.lo && row < r.lo + r.n) seq_s = i;
+// least reference first, then the sums. What it takes is round trips (row
+// starts, lengths and seg; references; sums), so a row and head has a
+// workgroup of 16 or 4 waves that take every 16th or 4th record while there
+// are few of them, and one wave of a workgroup's four where there are many
+// with few records.
+template <int HD, int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kernel(AttnArgs A, int pairs) {
+    constexpr int E = HD / 64, PER = WAVES == 1 ? 4 : 1;  // pairs of a workgroup
+    __shared__ float red[WAVES], redl[WAVES];
+    __shared__ float part[WAVES][WAVES == 1 ? 1 : HD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int pair = (int)blockIdx.x * PER + (WAVES == 1 ? wave : 0);
+    if (pair >= pairs) return;  // a wave by itself (WAVES 1), else none
+    const int row = pair / A.a.n_head, head = pair % A.a.n_head;
+    int2 sg[2];
+#pragma unroll
+    for (int c = 0; c < 2; c++) sg[c] = A.seg[((size_t)c * A.b.n_rows + row) * A.a.n_head + head];
+    int seq = -1;
+    for (int i0 = 0; i0 < A.b.n_seqs && seq < 0; i0 += 64) {
+        const int i = i0 + lane;
+        bool mine = false;
+        if (i < A.b.n_seqs) {
+            const SeqRows r = seq_rows(A.b.row_start[i], A.b.row_start[i + 1], A.b.n_rows);
+            mine = row >= r.lo && row < r.lo + r.n;
+        }
+        const unsigned long long any = __ballot(mine);
+        if (any) seq = i0 + __builtin_ctzll(any);
     }
-    __syncthreads();
-    const int seq = seq_s, kvh = head / A.group;
     if (seq < 0) return;
     // the two parts: records first .. first + count - 1 of workgroups, or one whole record
     int count[2] = {0, 0}, first[2] = {0, 0}, slot[2] = {0, 0};
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         if (c == 0 && A.a.shared_len == 0) continue;
-        const Work w = work_of<1>(A, c == 0 ? -1 : seq);
-        const int num = (row - w.lo) * A.group + head % A.group, rb = num / A.part[c].rows;
-        if (w.units == 0 || (c == 1 && A.many && seen_units<1>(A, w, rb) == 0)) continue;
-        slot[c] = num % A.part[c].rows;
-        const int blk = c == 0 ? rb : A.part[1].block0 + block_index(seq, w.lo, rb, A.group, A.part[1].rows);
-        const int2 s = A.seg[(size_t)blk * nkv + kvh];
-        if (s.x == kDone) return;
-        first[c] = s.x;
-        count[c] = s.x == kWhole ? 1 : s.y - s.x + 1;
+        if (c == 1) {
+            const Work w = work_of<1>(A, seq);
+            const int num = (row - w.lo) * A.group + head % A.group;
+            if (w.units == 0 || (A.many && seen_units<1>(A, w, num / A.part[1].rows) == 0)) continue;
+        }
+        const int last = min(sg[c].y >> 8, A.part[c].G - 1);
+        if (sg[c].x == kDone) return;
+        first[c] = sg[c].x;
+        slot[c] = min(sg[c].y & 255, A.part[c].rows - 1);
+        count[c] = first[c] == kWhole ? 1 : first[c] < 0 ? 0 : max(0, last - first[c] + 1);
     }
     const int total = count[0] + count[1];
     auto rec = [&](int i) {
         const int c = i >= count[0], k = c ? i - count[0] : i;
         return first[c] == kWhole ? rec_whole(A, c, row, head) : rec_part(A.part[c], first[c] + k, k == 0, slot[c]);
     };
+    const int begin = WAVES == 1 ? 0 : wave;
+    // the references of 64 records of this wave at a time
     float amin = INFINITY;
-    for (int i = tid; i < total; i += kTPB) amin = fminf(amin, A.rec_al[rec(i)].x);
+    for (int i = begin + WAVES * lane; i < total; i += 64 * WAVES) amin = fminf(amin, A.rec_al[rec(i)].x);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) amin = fminf(amin, __shfl_xor(amin, d));
-    if (lane == 0) red[wave] = amin;
-    __syncthreads();
+    if constexpr (WAVES > 1) {
+        if (lane == 0) red[wave] = amin;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) amin = fminf(amin, red[i]);
-    float l = 0.0f;
-    for (int i = tid; i < total; i += kTPB) {
-        const float2 al = A.rec_al[rec(i)];
-        const float f = al.x == INFINITY ? 0.0f : exp2_hw(amin - al.x);
-        wgt[i] = f;
-        l += f == 0.0f ? 0.0f : f * al.y;
+        for (int i = 0; i < WAVES; i++) amin = fminf(amin, red[i]);
     }
-    l = wave_sum(l);
-    if (lane == 0) redl[wave] = l;
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kWaves; i++) l += redl[i];
-    float o[E];
+    float l = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = 0.0f;
-#pragma unroll 4
-    for (int i = wave; i < total; i += kWaves) {
-        const float *src = A.rec_o + rec(i) * HD + lane;
-        const float f = wgt[i];
+    for (int i0 = begin; i0 < total; i0 += 64 * WAVES) {
+        const int mine = i0 + WAVES * lane;
+        float f = 0.0f;
+        if (mine < total) {
+            const float2 al = A.rec_al[rec(mine)];
+            f = al.x == INFINITY ? 0.0f : exp2_hw(amin - al.x);
+            l += f == 0.0f ? 0.0f : f * al.y;
+        }
+        const int n = min(64, (total - i0 + WAVES - 1) / WAVES);
+#pragma unroll 8
+        for (int k = 0; k < n; k++) {
+            const float *src = A.rec_o + rec(i0 + WAVES * k) * HD + lane;
+            const float fk = __shfl(f, k);
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            const float v = src[64 * e];
-            o[e] += f == 0.0f ? 0.0f : f * v;
+            for (int e = 0; e < E; e++) {
+                const float v = src[64 * e];
+                o[e] += fk == 0.0f ? 0.0f : fk * v;
+            }
         }
     }
+    l = wave_sum(l);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) redl[wave] = l;
 #pragma unroll
-    for (int e = 0; e < E; e++) part[wave][64 * e + lane] = o[e];
-    __syncthreads();
-    for (int d = tid; d < HD; d += kTPB) {
-        float y = 0.0f;
+        for (int e = 0; e < E; e++) part[wave][64 * e + lane] = o[e];
+        __syncthreads();
+        l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kWaves; i++) y += part[i][d];
-        y = l == 0.0f ? 0.0f : y / l;
+        for (int i = 0; i < WAVES; i++) l += redl[i];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int d = 64 * e + lane;
+        if (WAVES > 1 && e % WAVES != wave) continue;  // the waves share the values
+        float y = o[e];
+        if constexpr (WAVES > 1) {
+            y = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; i++) y += part[i][d];
+        }
+        y = l == 0.0f ? 0.0f : y * inv;
         if (A.a.gate) y *= sigmoid1(A.a.gate[(size_t)row * A.a.gate_row + (size_t)head * A.a.gate_head + d]);
         A.a.out[((size_t)row * A.a.n_head + head) * HD + d] = y;
     }
@@ -570,8 +595,8 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     const int few = kRows;
     const int shared = a.shared_len ? many_rows(kv, queries) : 0;
     const int own = many_rows(kv, (queries + b.n_seqs - 1) / b.n_seqs);
-    A.part[0] = shared ? Part{shared, many_groups(shared), 0, 0} : Part{few, kGroups, 0, 0};
-    A.part[1] = own ? Part{own, many_groups(own), 0, 0} : Part{few, kGroups, 0, 0};
+    A.part[0] = shared ? Part{shared, many_groups(shared), 0} : Part{few, kGroups, 0};
+    A.part[1] = own ? Part{own, many_groups(own), 0} : Part{few, kGroups, 0};
     A.many = own != 0;
     p.apart = a.shared_len && (shared || own);
     auto groups_recs = [&](const Part &x) { return (size_t)2 * x.G * x.rows; };
@@ -579,12 +604,9 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     if (p.apart) A.part[0].base = recs, recs += groups_recs(A.part[0]);
     A.whole = recs;
     if (a.shared_len) recs += (size_t)2 * b.n_rows * a.n_head;
-    size_t blocks = a.shared_len ? (size_t)blocks_of(b.n_rows, group, A.part[0].rows) : 0;
-    A.part[1].block0 = (int)blocks;
-    blocks += (size_t)b.n_seqs + (size_t)blocks_of(b.n_rows, group, A.part[1].rows);
     p.al = recs * kv.head_dim * sizeof(float);
     p.seg = p.al + recs * sizeof(float2);
-    p.bytes = p.seg + blocks * kv.n_head_kv * sizeof(int2);
+    p.bytes = p.seg + (size_t)2 * b.n_rows * a.n_head * sizeof(int2);
     return p;
 }
 
@@ -608,16 +630,26 @@ hipError_t launch_few(const AttnArgs &A, hipStream_t s) {
     return hipErrorInvalidValue;
 }
 
-hipError_t launch_join(const AttnArgs &A, hipStream_t s) {
-    const dim3 grid((unsigned)((size_t)A.b.n_rows * A.a.n_head));
-    switch (A.kv.head_dim) {
-    case 64: hipLaunchKernelGGL(attn_join_kernel<64>, grid, dim3(kTPB), 0, s, A); break;
-    case 128: hipLaunchKernelGGL(attn_join_kernel<128>, grid, dim3(kTPB), 0, s, A); break;
-    case 256: hipLaunchKernelGGL(attn_join_kernel<256>, grid, dim3(kTPB), 0, s, A); break;
-    case 512: hipLaunchKernelGGL(attn_join_kernel<512>, grid, dim3(kTPB), 0, s, A); break;
-    default: return hipErrorInvalidValue;
-    }
+template <int HD>
+hipError_t join(const AttnArgs &A, hipStream_t s) {
+    const int pairs = A.b.n_rows * A.a.n_head;  // below 2^29
+    if (pairs > 16 * kCUs)
+        hipLaunchKernelGGL((attn_join_kernel<HD, 1>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, s, A, pairs);
+    else if (pairs > 4 * kCUs)
+        hipLaunchKernelGGL((attn_join_kernel<HD, 4>), dim3((unsigned)pairs), dim3(256), 0, s, A, pairs);
+    else
+        hipLaunchKernelGGL((attn_join_kernel<HD, 16>), dim3((unsigned)pairs), dim3(1024), 0, s, A, pairs);
     return hipGetLastError();
+}
+
+hipError_t launch_join(const AttnArgs &A, hipStream_t s) {
+    switch (A.kv.head_dim) {
+    case 64: return join<64>(A, s);
+    case 128: return join<128>(A, s);
+    case 256: return join<256>(A, s);
+    case 512: return join<512>(A, s);
+    }
+    return hipErrorInvalidValue;
 }
 
 }  // namespace

@@ -426,6 +426,5 @@ int uq_emu_page_row(int n_pages, int n_head_kv, int log2_page, int page, int j, 
 long long uq_emu_run_start(long long T, int G, int w) { return run_start(T, G, w); }
 int uq_emu_run_owner(long long T, int G, long long u) { return run_owner(T, G, u); }
 int uq_emu_blocks_of(int n, int group, int RB) { return blocks_of(n, group, RB); }
-int uq_emu_block_index(int b, int lo, int rb, int group, int RB) { return block_index(b, lo, rb, group, RB); }
 
 }  // extern "C"

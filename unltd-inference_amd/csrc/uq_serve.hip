@@ -1,6 +1,7 @@
 // Batched serving: preparation and append of a batch's heads
 // (uq_kv_append_d) and the verification of drafted tokens
 // (uq_draft_verify_d). The attention over the pages is uq_attn_paged.hip.
+#include <algorithm>
 #include <climits>
 
 #include "uq_device.h"
@@ -194,8 +195,7 @@ __global__ __launch_bounds__(kAppTPB) void kv_append_kernel(AppendArgs a) {
 // ---- verification -------------------------------------------------------------
 
 constexpr int kVerTPB = 256;
-constexpr int kVerTiles = 8;
-constexpr int kVerChunk = kVerTPB * kVerTiles;  // tokens a workgroup sums
+constexpr int kVerChunk = 512;  // tokens that a wave sums: 8 a lane
 
 struct VerifyArgs {
     int32_t *accepted, *next;
@@ -205,7 +205,9 @@ struct VerifyArgs {
     const float *u;
     BatchView b;
     int vocab, chunks;
+    int run;        // chunks of a wave
     double2 *sums;  // [n_seqs][chunks]: the chunk's weight after a refusal, and of p alone
+    int4 *heads;    // [n_seqs]: first row, rows, accepted, the bits of the number that draws
 };
 
 // A weight that is NaN, negative or infinite counts as zero.
@@ -218,62 +220,94 @@ struct Row {
     int x;        // the refused token (certain drafts)
 };
 
-// The first refused draft of sequence s (rows r), found by the whole
-// workgroup: the products are exact in f64 (24 x 24 bits).
-__device__ __forceinline__ Row verify_row(const VerifyArgs &a, const SeqRows &r, int *first) {
-    const int k = r.n - 1;
-    if (threadIdx.x == 0) *first = k;
-    __syncthreads();
-    for (int i = threadIdx.x; i < k; i += kVerTPB) {
-        const size_t row = (size_t)r.lo + i;
-        const int x = a.tokens[row + 1];
-        bool ok = false;
-        if ((unsigned)x < (unsigned)a.vocab) {
-            const double q = a.q ? (double)a.q[row * a.q_row + x] : 1.0;
-            ok = (double)a.u[row] * q < (double)a.p[row * a.p_row + x];
-        }
-        if (!ok) atomicMin(first, i);  // integers: any order gives the least
-    }
-    __syncthreads();
-    const int i = *first;
+__device__ __forceinline__ Row row_at(const VerifyArgs &a, const SeqRows &r, int accepted) {
     Row o;
-    o.row = (size_t)r.lo + i;
-    o.accepted = i;
-    o.last = r.lo + k;
-    o.ended = i == k;
+    o.row = (size_t)r.lo + accepted;
+    o.accepted = accepted;
+    o.last = r.lo + r.n - 1;
+    o.ended = accepted == r.n - 1;
     o.x = !o.ended && !a.q ? a.tokens[o.row + 1] : -1;
     return o;
 }
-
-// Weights of token t: after a refusal, and of p.
-__device__ __forceinline__ double2 weights(const VerifyArgs &a, const Row &o, int t) {
-    const double p = (double)a.p[o.row * a.p_row + t];
-    double w = p;
-    if (!o.ended) w = a.q ? p - (double)a.q[o.row * a.q_row + t] : t == o.x ? 0.0 : p;
-    return make_double2(weight(w), weight(p));
+// The first refused draft of a sequence's rows r, by one wave: the products
+// are exact in f64 (24 x 24 bits).
+__device__ __forceinline__ int first_refused(const VerifyArgs &a, const SeqRows &r) {
+    const int k = r.n - 1, lane = threadIdx.x & 63;
+    for (int i0 = 0; i0 < k; i0 += 64) {
+        const int i = i0 + lane;
+        bool ok = true;
+        if (i < k) {
+            const size_t row = (size_t)r.lo + i;
+            const int x = a.tokens[row + 1];
+            const double u = (double)a.u[row];
+            ok = false;
+            if ((unsigned)x < (unsigned)a.vocab) {
+                const double q = a.q ? (double)a.q[row * a.q_row + x] : 1.0;
+                ok = u * q < (double)a.p[row * a.p_row + x];
+            }
+        }
+        const unsigned long long no = __ballot(!ok);
+        if (no) return i0 + __builtin_ctzll(no);
+    }
+    return k;
 }
 
-// Sums of one chunk of one sequence's row. Each of p and q is read once here,
-// the drawn token's chunk once more by verify_draw_kernel.
+// Weights of token t: after a refusal, and of p.
+__device__ __forceinline__ double2 weights(const VerifyArgs &a, const Row &o, int t, float p, float q) {
+    double w = (double)p;
+    if (!o.ended) w = a.q ? (double)p - (double)q : t == o.x ? 0.0 : w;
+    return make_double2(weight(w), weight((double)p));
+}
+
+// Sums of the chunks of one sequence's row, `run` of them a wave, which finds
+// the row by itself (three round trips, so a wave takes several chunks where
+// there are many; the next chunk is under way while one is summed). p and q
+// are read once here, and the drawn token's chunk once more by
+// verify_draw_kernel. No barrier.
 __global__ __launch_bounds__(kVerTPB) void verify_sum_kernel(VerifyArgs a) {
-    __shared__ int first;
-    __shared__ double red[kVerTPB / 64];
-    const int s = blockIdx.y, c = blockIdx.x;
+    const int s = blockIdx.y, lane = threadIdx.x & 63;
+    const int c0 = (int)(blockIdx.x * (kVerTPB / 64) + (threadIdx.x >> 6)) * a.run, c1 = min(a.chunks, c0 + a.run);
     const SeqRows r = seq_rows(a.b.row_start[s], a.b.row_start[s + 1], a.b.n_rows);
-    if (r.n == 0) return;
-    const Row o = verify_row(a, r, &first);
-    double2 w[kVerTiles];
+    if (r.n == 0 && c0 == 0 && lane == 0) a.heads[s] = make_int4(r.lo, 0, 0, 0);
+    if (r.n == 0 || c0 >= c1) return;
+    const Row o = row_at(a, r, first_refused(a, r));
+    if (c0 == 0 && lane == 0) a.heads[s] = make_int4(r.lo, r.n, o.accepted, __float_as_int(a.u[r.lo + r.n - 1]));
+    const float *p = a.p + o.row * a.p_row, *q = a.q && !o.ended ? a.q + o.row * a.q_row : p;
+    f4u vp[2], vq[2];
+    auto load = [&](int c) {  // tokens 256 j + 4 lane .. of the chunk
 #pragma unroll
-    for (int j = 0; j < kVerTiles; j++) {
-        const int t = c * kVerChunk + j * kVerTPB + threadIdx.x;
-        w[j] = t < a.vocab ? weights(a, o, t) : make_double2(0.0, 0.0);
+        for (int j = 0; j < 2; j++) {
+            const int t = c * kVerChunk + 256 * j + 4 * lane;
+            if (t + 4 <= a.vocab) {
+                vp[j] = *(const f4u *)(p + t);
+                vq[j] = *(const f4u *)(q + t);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    vp[j][e] = t + e < a.vocab ? p[t + e] : 0.0f;
+                    vq[j][e] = t + e < a.vocab ? q[t + e] : 0.0f;
+                }
+            }
+        }
+    };
+    load(c0);
+    for (int c = c0; c < c1; c++) {
+        f4u p2[2], q2[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) p2[j] = vp[j], q2[j] = vq[j];
+        if (c + 1 < c1) load(c + 1);
+        double x = 0.0, y = 0.0;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double2 w = weights(a, o, c * kVerChunk + 256 * j + 4 * lane + e, p2[j][e], q2[j][e]);
+                x += w.x, y += w.y;
+            }
+        x = wave_sum_d(x);
+        y = wave_sum_d(y);
+        if (lane == 0) a.sums[(size_t)s * a.chunks + c] = make_double2(x, y);
     }
-    double x = 0.0, y = 0.0;
-#pragma unroll
-    for (int j = 0; j < kVerTiles; j++) x += w[j].x, y += w[j].y;
-    x = block_sum_d<kVerTPB>(x, red);
-    y = block_sum_d<kVerTPB>(y, red);
-    if (threadIdx.x == 0) a.sums[(size_t)s * a.chunks + c] = make_double2(x, y);
 }
 
 // Inclusive sum of v over the workgroup's threads in thread order (wave scan,
@@ -302,29 +336,30 @@ __device__ __forceinline__ double block_scan_d(double v, double *red, double *to
 // at the joints of the tree, so a token needs weight of its own to be drawn,
 // and where no sum exceeds the threshold the last one with weight is it.
 __global__ __launch_bounds__(kVerTPB) void verify_draw_kernel(VerifyArgs a) {
-    __shared__ int first, hit, last;
+    __shared__ int hit, last, chunk_s;
     __shared__ double red[kVerTPB / 64];
     __shared__ double base_s;
     const int s = blockIdx.x, tid = threadIdx.x;
-    const SeqRows r = seq_rows(a.b.row_start[s], a.b.row_start[s + 1], a.b.n_rows);
-    if (r.n == 0) {
-        if (tid == 0) a.accepted[s] = 0, a.next[s] = -1;
-        return;
-    }
-    const Row o = verify_row(a, r, &first);
-    if (tid == 0) a.accepted[s] = o.accepted, hit = INT_MAX, last = -1;
-    // every thread a run of chunks
+    // every thread a run of chunks; loads before anything waits for one
     const double2 *sums = a.sums + (size_t)s * a.chunks;
     const int per = (a.chunks + kVerTPB - 1) / kVerTPB, c0 = min(a.chunks, tid * per), c1 = min(a.chunks, c0 + per);
     double2 t = make_double2(0.0, 0.0);
-    for (int c = c0; c < c1; c++) t.x += sums[c].x, t.y += sums[c].y;
-    double total, unused;
+    for (int c = c0; c < c1; c++) t.x += sums[c].x, t.y += sums[c].y;  // a sequence without rows: of anything, not used
+    const int4 head = a.heads[s];
+    const SeqRows r{head.x, head.y};
+    const int accepted = head.z;
+    if (tid == 0) a.accepted[s] = accepted;
+    if (r.n == 0) {
+        if (tid == 0) a.next[s] = -1;
+        return;
+    }
+    double u = (double)__int_as_float(head.w);
+    if (tid == 0) hit = INT_MAX, last = -1;
+    double total;
     double inc = block_scan_d(t.x, red, &total);  // its barriers publish hit and last
-    const double incp = block_scan_d(t.y, red, &unused);
-    const bool plain = !(total > 0.0);  // no weight after the refusal: p itself
+    const bool plain = !(total > 0.0);            // no weight after the refusal: p itself
+    if (plain) inc = block_scan_d(t.y, red, &total);
     const double mine = plain ? t.y : t.x;
-    if (plain) inc = incp, total = unused;
-    double u = (double)a.u[o.last];
     u = u >= 0.0 ? u : u < 0.0 ? 0.0 : 1.0;  // NaN as 1
     const double thr = u >= 1.0 ? (double)INFINITY : u * total;
     if (mine > 0.0) {
@@ -350,27 +385,32 @@ __global__ __launch_bounds__(kVerTPB) void verify_draw_kernel(VerifyArgs a) {
             if (run > thr) break;
         }
         base_s = base;
-        first = found;
+        chunk_s = found;
         hit = INT_MAX;
         last = -1;
     }
     __syncthreads();
-    const int c = first;
-    double base = base_s;
-    for (int j = 0; j < kVerTiles; j++) {
-        const int x = c * kVerChunk + j * kVerTPB + tid;
-        const double2 v = x < a.vocab ? weights(a, o, x) : make_double2(0.0, 0.0);
-        const double w = plain ? v.y : v.x;
-        double sum;
-        const double upto = base + block_scan_d(w, red, &sum);
-        if (w > 0.0) {
-            atomicMax(&last, x);
-            if (upto > thr) atomicMin(&hit, x);
-        }
-        __syncthreads();
-        if (hit != INT_MAX) break;  // read alike by all: the next update lies behind a barrier
-        base += sum;
+    // the token in the chunk: two neighbours a thread
+    const Row o = row_at(a, r, accepted);
+    const float *p = a.p + o.row * a.p_row, *q = a.q && !o.ended ? a.q + o.row * a.q_row : p;
+    const int x0 = chunk_s * kVerChunk + 2 * tid;
+    double w[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int x = x0 + j;
+        const double2 v = x < a.vocab ? weights(a, o, x, p[x], q[x]) : make_double2(0.0, 0.0);
+        w[j] = plain ? v.y : v.x;
     }
+    const double upto = base_s + block_scan_d(w[0] + w[1], red, &total);
+    if (w[1] > 0.0) {
+        atomicMax(&last, x0 + 1);
+        if (upto > thr) atomicMin(&hit, x0 + 1);
+    }
+    if (w[0] > 0.0) {
+        atomicMax(&last, x0);
+        if (upto - w[1] > thr) atomicMin(&hit, x0);
+    }
+    __syncthreads();
     if (tid == 0) a.next[s] = hit != INT_MAX ? hit : last;
 }
 
@@ -398,7 +438,7 @@ hipError_t launch_kv_append(const PagesView &kv, const BatchView &b, const uq_he
 }
 
 size_t draft_verify_ws_bytes(int n_seqs, int vocab) {
-    return (size_t)n_seqs * (((size_t)vocab + kVerChunk - 1) / kVerChunk) * sizeof(double2);
+    return (size_t)n_seqs * ((((size_t)vocab + kVerChunk - 1) / kVerChunk) * sizeof(double2) + sizeof(int4));
 }
 
 hipError_t launch_draft_verify(int32_t *accepted, int32_t *next, const float *p, size_t p_row, const float *q,
@@ -406,8 +446,13 @@ hipError_t launch_draft_verify(int32_t *accepted, int32_t *next, const float *p,
                                void *ws, hipStream_t s) {
     if (b.n_seqs == 0) return hipSuccess;
     const int chunks = (vocab + kVerChunk - 1) / kVerChunk;
-    const VerifyArgs a{accepted, next, p, q, p_row, q_row, tokens, u, b, vocab, chunks, (double2 *)ws};
-    hipLaunchKernelGGL(verify_sum_kernel, dim3((unsigned)chunks, (unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
+    // one chunk a wave up to two rounds of 8 workgroups a CU, then up to 8
+    const long long waves = (long long)chunks * b.n_seqs;
+    const int run = (int)std::min(8LL, std::max(1LL, waves / (2 * 8 * 256 * (kVerTPB / 64))));
+    const VerifyArgs a{accepted, next, p, q, p_row, q_row, tokens, u, b, vocab, chunks, run,
+                       (double2 *)ws, (int4 *)((double2 *)ws + (size_t)b.n_seqs * chunks)};
+    const int per = kVerTPB / 64 * run;
+    hipLaunchKernelGGL(verify_sum_kernel, dim3((unsigned)((chunks + per - 1) / per), (unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
     if (hipError_t e = hipGetLastError()) return e;
     hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
     return hipGetLastError();

@@ -45,9 +45,5 @@ UQ_HD int blocks_of(int n, int group, int RB) { return (int)(((long long)n * gro
 UQ_HD long long run_start(long long T, int G, int w) { return (long long)w * T / G; }
 // The workgroup whose run holds unit u < T.
 UQ_HD int run_owner(long long T, int G, long long u) { return (int)(((u + 1) * G - 1) / T); }
-// Index of (block rb, sequence b) among all blocks: b + floor(lo * group / RB)
-// + rb is injective, as a sequence's ceil(n group / RB) blocks number at most
-// floor((lo + n) group / RB) - floor(lo group / RB) + 1.
-UQ_HD int block_index(int b, int lo, int rb, int group, int RB) { return b + (int)((long long)lo * group / RB) + rb; }
 
 }  // namespace uq
