@@ -36,9 +36,10 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
 
-# Matrix products with their sums in VGPRs: attn_many_kernel's queries then fill the accumulation registers, and the
-# vector units reach the sums without copies (with the sums there: 25 registers spilled, 230 copies a tile).
-SOURCE_FLAGS = {"uq_attn_many.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# Matrix products with their sums in VGPRs, where one wave has a SIMD's registers to itself: the accumulation registers
+# then hold queries or tiles under way, and the vector units reach the sums without copies (attn_many_kernel with the
+# sums there: 25 registers spilled, 230 copies a tile).
+SOURCE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("uq_attn_many.hip", "uq_attn_paged.hip")}
 
 
 def _run(cmd, verbose):

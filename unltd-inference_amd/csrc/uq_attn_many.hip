@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
     __shared__ int red[QW];
     __shared__ RunLds run_lds;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = uniform(tid >> 6);
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 

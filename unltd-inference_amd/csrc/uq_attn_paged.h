@@ -125,6 +125,13 @@ __device__ __forceinline__ long long seen_sum(const AttnArgs &A, const Work &w, 
     return t;
 }
 
+// A value that is the same in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long uniform(long long v) {
+    const unsigned lo = (unsigned)uniform((int)v), hi = (unsigned)uniform((int)(v >> 32));
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+
 // A workgroup's run: units [u, u1) of T, the first of them off units into
 // sequence seq (-1: the shared positions).
 struct Run {
@@ -134,8 +141,7 @@ struct Run {
 };
 struct RunLds {
     long long scan[4], off;
-    int seq;
-    Work work;
+    int seq, work[7];
 };
 // The run of this workgroup (of TPB threads), by a scan over the sequences'
 // units (count(s, work of s); every workgroup reads all row starts and lengths: one round
@@ -145,7 +151,7 @@ template <int TPB, int U, class Count>
 __device__ bool find_run(const AttnArgs &A, Count count, RunLds &lds, Run &r) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, parts = A.b.n_seqs + 1;
     // units of sequence i - 1 and of those before it, for i = c + tid; returns the total up to c + TPB
-    Work w;
+    Work w{};
     auto scan = [&](int c, long long run, long long &mine, long long &before) {
         const int i = c + tid;
         mine = 0;
@@ -169,26 +175,33 @@ __device__ bool find_run(const AttnArgs &A, Count count, RunLds &lds, Run &r) {
         }
         return run;
     };
+    auto keep = [&](int s, long long b) {
+        lds.seq = s, lds.off = r.u - b;
+        lds.work[0] = w.lo, lds.work[1] = w.n, lds.work[2] = w.len, lds.work[3] = w.base, lds.work[4] = w.end;
+        lds.work[5] = w.units, lds.work[6] = w.blocks;
+    };
     long long mine = 0, before = 0;
     r.T = 0;
     for (int c = 0; c < parts; c += TPB) r.T = scan(c, r.T, mine, before);
+    r.T = uniform(r.T);
     r.runs = (int)min((long long)A.part[A.first].G, r.T);  // no empty runs between others
     if ((int)blockIdx.x >= r.runs) return false;
     r.u = run_start(r.T, r.runs, (int)blockIdx.x);
     r.u1 = run_start(r.T, r.runs, (int)blockIdx.x + 1);
     if (parts <= TPB) {
-        if (mine > 0 && before <= r.u && r.u < before + mine) lds.seq = tid - 1, lds.off = r.u - before, lds.work = w;
+        if (mine > 0 && before <= r.u && r.u < before + mine) keep(tid - 1, before);
     } else {
         long long run = 0;
         for (int c = 0; c < parts; c += TPB) {
             run = scan(c, run, mine, before);
-            if (mine > 0 && before <= r.u && r.u < before + mine) lds.seq = c + tid - 1, lds.off = r.u - before, lds.work = w;
+            if (mine > 0 && before <= r.u && r.u < before + mine) keep(c + tid - 1, before);
         }
     }
     __syncthreads();
-    r.seq = lds.seq;
-    r.off = lds.off;
-    r.work = lds.work;
+    r.seq = uniform(lds.seq);
+    r.off = uniform(lds.off);
+    r.work = Work{uniform(lds.work[0]), uniform(lds.work[1]), uniform(lds.work[2]), uniform(lds.work[3]),
+                  uniform(lds.work[4]), uniform(lds.work[5]), uniform(lds.work[6])};
     return true;
 }
 

@@ -16,7 +16,7 @@ constexpr int kTPB = 256;
 constexpr int kWaves = kTPB / 64;
 constexpr int kRows = 16;     // queries of a block: the columns of a 16x16 tile
 constexpr int kCUs = 256;
-constexpr int kGroups = 2 * kCUs;  // workgroups: two per CU
+constexpr int kGroups = 2 * kCUs;  // workgroups of attn_paged_kernel
 
 template <bool F16, int HD>
 struct Geo;
@@ -73,44 +73,20 @@ struct Wave {
     }
 };
 
-// The products of values that are not finite (slots `bad` of the lane's
-// sixteen columns), left out of the matrix product because a row that may not
-// see them would take 0 * NaN from them: added for the rows that see them.
-template <bool F16, int HD, class E>
-__device__ __forceinline__ void add_unfinite(Wave<F16, HD> &W, const E *V, int myrow, const float (&p)[Geo<F16, HD>::VS],
-                                             const bool (&sees)[Geo<F16, HD>::VS], unsigned bad, int lane) {
+template <bool F16, int HD>
+struct Tile {
     using G = Geo<F16, HD>;
-    const int n = lane & 15, g = lane >> 4;
-    unsigned where = 0;  // bit y: position y of the tile
-#pragma unroll
-    for (int x = 0; x < G::VS; x++) {
-        const unsigned long long m = __ballot((bad >> x) & 1);
-#pragma unroll
-        for (int q = 0; q < 4; q++)
-            if ((m >> (16 * q)) & 0xFFFF) where |= 1u << (16 * (x >> 2) + 4 * q + (x & 3));
-    }
-    while (where) {
-        const int y = __builtin_ctz(where), from = 16 * ((y >> 2) & 3) + n, slot = 4 * (y >> 4) + (y & 3);
-        where &= where - 1;
-        float pv = 0.0f;
-        bool sv = false;
-#pragma unroll
-        for (int x = 0; x < G::VS; x++)
-            if (x == slot) pv = p[x], sv = sees[x];
-        pv = __shfl(pv, from);
-        sv = __shfl((int)sv, from);
-        const E *vp = V + (size_t)__shfl(myrow, y) * HD;
-#pragma unroll
-        for (int h = 0; h < G::NH; h++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < G::DL; j++) {
-                    const float v = (float)vp[h * 16 * G::DL + (4 * g + i) * G::DL + j];
-                    if (sv) W.acc[h][j][i] += pv * v;
-                }
-    }
-}
+    using KV = std::conditional_t<F16, h8, f4>;
+    using VV = std::conditional_t<!F16, f4, std::conditional_t<G::DL == 8, u4, u2>>;
+    KV k[G::PT][G::KC];
+    VV v[G::VS][G::NH];
+};
+// A tile's first position, the row of position lane & (NP - 1), the lanes
+// whose position exists.
+struct Place {
+    int p0, row;
+    unsigned long long have;
+};
 
 template <bool F16, int HD>
 __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(AttnArgs A) {
@@ -123,7 +99,8 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
     __shared__ int row_lim[kRows];         // its last position, -1: none
     __shared__ float2 wave_al[kWaves][kRows];
     __shared__ RunLds run_lds;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int wave = uniform(tid >> 6);
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 
@@ -225,33 +202,66 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             lim_min = min(lim_min, __shfl_xor(lim_min, d));
             lim_max = max(lim_max, __shfl_xor(lim_max, d));
         }
+        lim_min = uniform(lim_min), lim_max = uniform(lim_max);
         const int end = lim_max < w.end ? lim_max + 1 : w.end;  // no row sees further
         const int32_t *table = A.b.pages + (seq < 0 ? (size_t)0 : (size_t)seq * A.b.max_pages);
         const E *K = (const E *)A.kv.k, *V = (const E *)A.kv.v;
 
         W.reset();
-        for (int it = 0; it < count; it++) {
-            const int p0 = w.base + (un + it) * U + wave * NP;
-            if (p0 >= end) break;  // the whole wave
-            // rows of the tile's positions, position p0 + (lane & (NP - 1)) a lane
-            const int mypos = p0 + (lane & (NP - 1));
-            const int page = mypos < end ? table[mypos >> map.log2_page] : -1;
+        bool unfinite = false;  // values that are not finite were left out where some query may not see them
+        // A tile's keys and values in registers. The next tile's keys are on their way while this one's values are
+        // multiplied, and its values while its own keys are, in the same registers; the loads are issued without a
+        // branch (what is no position loads any row), so that they need not be waited for at one.
+        Tile<F16, HD> T;
+        auto page_of = [&](int it) {  // of position lane & (NP - 1) of the wave's tile
+            const int pos = w.base + (un + it) * U + wave * NP + (lane & (NP - 1));
+            return it < count && pos < end ? table[pos >> map.log2_page] : -1;
+        };
+        auto place = [&](Place &x, int it, int page) {
             const bool there = page_ok(map, page);
-            const int myrow = there ? page_row(map, page, kvh, mypos) : 0;
-            const unsigned long long have = __ballot(there);
-            if (have == 0) continue;
+            x.p0 = w.base + (un + it) * U + wave * NP;
+            x.row = there ? page_row(map, page, kvh, x.p0 + (lane & (NP - 1))) : 0;
+            x.have = __ballot(there);
+        };
+        auto row_at = [](const Place &x, int lane4, int more) {  // of lane lane4 / 4 + more
+            return __builtin_amdgcn_ds_bpermute(lane4 + 4 * more, x.row);
+        };
+        auto fetch_keys = [&](const Place &x) {
+            using KV = typename Tile<F16, HD>::KV;
+#pragma unroll
+            for (int t = 0; t < G::PT; t++) {
+                const KV *kp = (const KV *)(K + (size_t)row_at(x, 4 * n, 16 * t) * HD) + g;
+#pragma unroll
+                for (int c = 0; c < G::KC; c++) T.k[t][c] = kp[4 * c];
+            }
+        };
+        auto fetch_values = [&](const Place &x) {
+            using VV = typename Tile<F16, HD>::VV;
+#pragma unroll
+            for (int i = 0; i < G::VS; i++) {
+                const E *vp = V + (size_t)row_at(x, 16 * g, 16 * (i >> 2) + (i & 3)) * HD + G::DL * n;
+#pragma unroll
+                for (int h = 0; h < G::NH; h++) T.v[i][h] = *(const VV *)(vp + 16 * G::DL * h);
+            }
+        };
+        if (map.n_pages > 0) {  // else there is nothing to load from
+          Place cur, nxt;
+          place(cur, 0, page_of(0));
+          int page = page_of(1);
+          fetch_keys(cur);
+          fetch_values(cur);
+          for (int it = 0; it < count; it++) {
+            place(nxt, it + 1, page);
+            page = page_of(it + 2);
+            const unsigned long long have = cur.have;
+            const int p0 = cur.p0;
             const bool edge = have != ~0ull || p0 + NP - 1 > lim_min;
+            const uint32_t hv = (uint32_t)have >> (4 * g);  // bit 16 t + i: position 16 t + 4 g + i
+            const int room = lim - p0 - 4 * g;
 
             // scores
             f4 s[G::PT];
             if constexpr (F16) {
-                h8 k[G::PT][G::KC];
-#pragma unroll
-                for (int t = 0; t < G::PT; t++) {
-                    const h8 *kp = (const h8 *)(K + (size_t)__shfl(myrow, 16 * t + n) * HD) + g;
-#pragma unroll
-                    for (int c = 0; c < G::KC; c++) k[t][c] = kp[4 * c];
-                }
 #pragma unroll
                 for (int t = 0; t < G::PT; t++) s[t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -259,23 +269,23 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                     const h8 qh = ((const h8 *)lds)[c * 128 + lane], ql = ((const h8 *)lds)[c * 128 + 64 + lane];
 #pragma unroll
                     for (int t = 0; t < G::PT; t++) {
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][c], qh, s[t], 0, 0, 0);
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[t][c], ql, s[t], 0, 0, 0);
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.k[t][c], qh, s[t], 0, 0, 0);
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.k[t][c], ql, s[t], 0, 0, 0);
                     }
                 }
             } else {
-                f4 k[G::KC];
-                const f4 *kp = (const f4 *)(K + (size_t)__shfl(myrow, n) * HD) + g;
-#pragma unroll
-                for (int c = 0; c < G::KC; c++) k[c] = kp[4 * c];
                 s[0] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < G::KC; c++) {
                     const f4 q = ((const f4 *)lds)[c * 64 + lane];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[c][e], q[e], s[0], 0, 0, 0);
+                    for (int e = 0; e < 4; e++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(T.k[0][c][e], q[e], s[0], 0, 0, 0);
                 }
             }
+
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_keys(nxt);
+            __builtin_amdgcn_sched_barrier(0);
 
             // weights: slot x = 4 t + i is position p0 + 16 t + 4 g + i
             float p[4 * G::PT];
@@ -285,8 +295,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             for (int t = 0; t < G::PT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int x = 16 * t + 4 * g + i;
-                    sees[4 * t + i] = !edge || (((have >> x) & 1) && p0 + x <= lim);
+                    sees[4 * t + i] = !edge || (((hv >> (16 * t + i)) & 1) && 16 * t + i <= room);
                     top = fmaxf(top, sees[4 * t + i] ? s[t][i] * fac : -INFINITY);
                 }
             top = row16_max(top);
@@ -310,36 +319,23 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 
             // values: slot x of a lane is position p0 + 16 (x / 4) + 4 g + x % 4
             if constexpr (F16) {
-                using HV = std::conditional_t<G::DL == 8, u4, u2>;
                 constexpr int D2 = G::DL / 2;
-                HV v[G::VS][G::NH];
-#pragma unroll
-                for (int x = 0; x < G::VS; x++) {
-                    const E *vp = V + (size_t)__shfl(myrow, 16 * (x >> 2) + 4 * g + (x & 3)) * HD + G::DL * n;
-#pragma unroll
-                    for (int h = 0; h < G::NH; h++) v[x][h] = *(const HV *)(vp + 16 * G::DL * h);
-                }
-                unsigned bad = 0;  // slots that hold something not finite
+                auto &v = T.v;
                 if (edge) {
 #pragma unroll
                     for (int x = 0; x < G::VS; x++) {
-                        const bool ok = (have >> (16 * (x >> 2) + 4 * g + (x & 3))) & 1;
+                        const bool ok = (hv >> (16 * (x >> 2) + (x & 3))) & 1;
                         bool fin = true;
 #pragma unroll
                         for (int h = 0; h < G::NH; h++)
 #pragma unroll
                             for (int d = 0; d < D2; d++) {
                                 const uint32_t z = v[x][h][d];
-                                fin = fin && (z & 0x7C00u) != 0x7C00u && (z & 0x7C000000u) != 0x7C000000u;
+                                const bool lo = (z & 0x7C00u) != 0x7C00u, hi = (z & 0x7C000000u) != 0x7C000000u;
+                                fin = fin && lo && hi;
+                                v[x][h][d] = (ok && lo ? z & 0x0000FFFFu : 0u) | (ok && hi ? z & 0xFFFF0000u : 0u);
                             }
-                        fin = ((__ballot(!fin) >> (16 * g)) & 0xFFFF) == 0;
-                        if (!ok || !fin) {
-#pragma unroll
-                            for (int h = 0; h < G::NH; h++)
-#pragma unroll
-                                for (int d = 0; d < D2; d++) v[x][h][d] = 0;
-                        }
-                        bad |= ok && !fin ? 1u << x : 0u;
+                        unfinite = unfinite || (ok && !fin);
                     }
                 }
                 h8 ph, pl;
@@ -360,31 +356,22 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                         W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, W.acc[h][j], 0, 0, 0);
                         W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, W.acc[h][j], 0, 0, 0);
                     }
-                if (edge && __any(bad != 0)) add_unfinite(W, V, myrow, p, sees, bad, lane);
             } else {
-                f4 v[G::VS][G::NH];
-#pragma unroll
-                for (int x = 0; x < G::VS; x++) {
-                    const E *vp = V + (size_t)__shfl(myrow, 4 * g + x) * HD + 4 * n;
-#pragma unroll
-                    for (int h = 0; h < G::NH; h++) v[x][h] = *(const f4 *)(vp + 64 * h);
-                }
-                unsigned bad = 0;
+                auto &v = T.v;
                 if (edge) {
 #pragma unroll
                     for (int x = 0; x < G::VS; x++) {
-                        const bool ok = (have >> (4 * g + x)) & 1;
+                        const bool ok = (hv >> x) & 1;
                         bool fin = true;
 #pragma unroll
                         for (int h = 0; h < G::NH; h++)
 #pragma unroll
-                            for (int d = 0; d < 4; d++) fin = fin && finite32(v[x][h][d]);
-                        fin = ((__ballot(!fin) >> (16 * g)) & 0xFFFF) == 0;
-                        if (!ok || !fin) {
-#pragma unroll
-                            for (int h = 0; h < G::NH; h++) v[x][h] = f4{0.f, 0.f, 0.f, 0.f};
-                        }
-                        bad |= ok && !fin ? 1u << x : 0u;
+                            for (int d = 0; d < 4; d++) {
+                                const bool one = finite32(v[x][h][d]);
+                                fin = fin && one;
+                                v[x][h][d] = ok && one ? v[x][h][d] : 0.0f;
+                            }
+                        unfinite = unfinite || (ok && !fin);
                     }
                 }
 #pragma unroll
@@ -394,8 +381,33 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 #pragma unroll
                         for (int j = 0; j < 4; j++)
                             W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][h][j], p[x], W.acc[h][j], 0, 0, 0);
-                if (edge && __any(bad != 0)) add_unfinite(W, V, myrow, p, sees, bad, lane);
             }
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_values(nxt);
+            cur = nxt;
+          }
+          if (__any(unfinite)) {
+              // A query that may not see them would have taken 0 * NaN from them; those that do take them now (any
+              // weight: the sum is infinite or NaN all the same).
+              for (int it = 0; it < count; it++)
+                  for (int y = 0; y < NP; y++) {
+                      const int pos = w.base + (un + it) * U + wave * NP + y;
+                      const int pg = pos < end ? table[pos >> map.log2_page] : -1;
+                      if (!page_ok(map, pg)) continue;
+                      const E *vp = V + (size_t)page_row(map, pg, kvh, pos) * HD;
+#pragma unroll
+                      for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                          for (int i = 0; i < 4; i++) {
+#pragma unroll
+                              for (int j = 0; j < G::DL; j++) {
+                                  const float v = (float)vp[h * 16 * G::DL + (4 * g + i) * G::DL + j];
+                                  if (pos <= lim && !finite32(v)) W.acc[h][j][i] += v;
+                              }
+                              __builtin_amdgcn_sched_barrier(0);
+                          }
+                  }
+          }
         }
 
         // ---- the waves' sums joined: references, then o scaled to the least of them
