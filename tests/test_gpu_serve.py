@@ -322,6 +322,19 @@ def test_attention_with_a_value_not_finite_that_some_rows_see(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,lens", [([1, 1], [1, 33]), ([50, 1], [50, 129])])
+def test_attention_keeps_a_nan_that_is_all_a_tile_shows(dtype, rows, lens):
+    """The only position that a row sees, or the only one in the last tile that it sees, has a key of NaN."""
+    rng = np.random.default_rng(28)
+    c = M.Cache(rng, dtype, 1, 64, 16, rows, lens)
+    for b, pos in ((0, 0), (1, lens[1] - 1)):
+        pg, sl, _ = c.slots(b, pos + 1)
+        c.k[pg[-1], :, sl[-1]] = np.nan
+    got = attend(c, rng.standard_normal((sum(rows), 2, 64)).astype(np.float32), 2, 0.125)
+    assert np.isnan(got).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_attention_of_large_and_small_numbers(dtype):
     """Scores of thousands (one weight is all), queries of 1e-30 and 1e30, keys of zero, the largest f16."""
     rng = np.random.default_rng(23)

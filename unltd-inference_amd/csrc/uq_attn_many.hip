@@ -81,52 +81,17 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
     __shared__ int unfinite;          // some tile holds values that are not finite and that not every query sees
     __shared__ int row_lim[RB];
     __shared__ int red[QW];
-    __shared__ RunLds run_lds;
+    __shared__ WalkLds walk_lds;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
     const int wave = uniform(tid >> 6);
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 
-    auto units_of = [&](const Work &w, int seq, int rb) { return seq < 0 ? w.units : seen_units<NP>(A, w, rb); };
-    // A block of a KV head counts kOver units beside its own: what its start and end cost, so that a run with two of
-    // them has fewer tiles. They lie before the units: a run that ends among them leaves the block to the next one.
-    Run R;
-    if (!find_run<NT, NP>(A, [&](int s, const Work &w) {
-            return w.units == 0 ? 0 : nkv * (s < 0 ? (long long)(w.units + M::kOver) * w.blocks : seen_sum<NP>(A, w, M::kOver));
-        }, run_lds, R))
-        return;
-    long long u = R.u;
-    int seq = R.seq, rb = 0;
-    Work w = R.work;
-    long long off = R.off;  // into block rb
-    int units = units_of(w, seq, 0);
-    auto next_block = [&]() {  // false: none is left (the batch changed under the call)
-        if (++rb >= w.blocks) {
-            do {
-                if (++seq >= A.b.n_seqs) return false;
-                w = work_of<NP>(A, seq);
-            } while (w.blocks == 0);
-            rb = 0;
-        }
-        units = units_of(w, seq, rb);
-        return true;
-    };
-
-    while (u < R.u1) {
-        const int cost = units > 0 ? units + M::kOver : 0;
-        if (off >= (long long)nkv * cost) {
-            off -= (long long)nkv * cost;
-            if (!next_block()) return;
-            continue;
-        }
-        const int kvh = (int)(off / cost), at = (int)(off % cost);
-        const int upto = (int)min((long long)cost, at + (R.u1 - u)), un = max(0, at - M::kOver);
-        const int count = max(0, upto - M::kOver) - un;
-        if (count == 0) {
-            u += upto - at;
-            off += upto - at;
-            continue;
-        }
+    Walk<NT, NP, M::kOver> X;
+    if (!X.find(A, walk_lds)) return;
+    while (X.next(A)) {
+        const Work &w = X.w;
+        const int seq = X.seq, rb = X.rb, kvh = X.kvh, un = X.un, count = X.count;
         const int nq = min(RB, w.n * A.group - rb * RB);
         const bool active = wave * 32 < nq;
 
@@ -490,7 +455,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
 
         // ---- results
         l += __shfl_xor(l, 32);
-        const bool starts = un == 0, ends = un + count == units, whole = starts && ends;
+        const bool starts = X.starts, whole = starts && X.ends;
         const bool done = whole && A.a.shared_len == 0;
         if (active) {
             // by way of LDS, 128 values of the 32 queries at a time, to store them row by row
@@ -537,10 +502,8 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
             const int num = rb * RB + tid;
             put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
                     done ? kDone : whole ? kWhole : (int)blockIdx.x,
-                    done || whole ? 0 : run_owner(R.T, R.runs, u + cost - at - 1), tid);
+                    done || whole ? 0 : X.last(), tid);
         }
-        u += upto - at;
-        off += upto - at;
     }
 }
 

@@ -28,7 +28,6 @@ struct AttnArgs {
     BatchView b;
     int group;
     int first, last;  // the launch's parts
-    bool many;        // part 1 runs on attn_many_kernel
     Part part[2];
     size_t whole;   // first of the rows' own records
     float *rec_o;   // records: [..][HD] sums o ...
@@ -132,33 +131,39 @@ __device__ __forceinline__ long long uniform(long long v) {
     return (long long)((unsigned long long)hi << 32 | lo);
 }
 
-// A workgroup's run: units [u, u1) of T, the first of them off units into
-// sequence seq (-1: the shared positions).
-struct Run {
-    long long T, u, u1, off;
-    int runs, seq;
-    Work work;  // of seq
-};
-struct RunLds {
+// The walk of a workgroup of TPB threads over its run of the work. Every block
+// of a KV head counts OVER units beside its units of U positions: what its
+// start and end cost, so that a run with two of them has less else to do.
+// They lie before the units; a run that ends among them leaves the block to
+// the next one. What find reads are all row starts and lengths, by every
+// workgroup: one round trip to the L2, where another kernel for a plan would
+// cost a launch.
+struct WalkLds {
     long long scan[4], off;
-    int seq, work[7];
+    int index, work[7];
 };
-// The run of this workgroup (of TPB threads), by a scan over the sequences'
-// units (count(s, work of s); every workgroup reads all row starts and lengths: one round
-// trip to the L2, where another kernel for a plan would cost a launch). False:
-// none.
-template <int TPB, int U, class Count>
-__device__ bool find_run(const AttnArgs &A, Count count, RunLds &lds, Run &r) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, parts = A.b.n_seqs + 1;
-    // units of sequence i - 1 and of those before it, for i = c + tid; returns the total up to c + TPB
-    Work w{};
-    auto scan = [&](int c, long long run, long long &mine, long long &before) {
-        const int i = c + tid;
-        mine = 0;
-        if (i < parts && (i > 0 ? A.last == 1 : A.first == 0)) {
-            w = work_of<U>(A, i - 1);
-            mine = count(i - 1, w);
-        }
+template <int TPB, int U, int OVER>
+struct Walk {
+    int runs, seq, rb, units;  // runs of all workgroups; where the next block is looked for
+    long long T, u, u1, off;   // all units, the rest of this run, the next unit's place among its block's (all KV heads)
+    Work w;
+    // the block at hand
+    int kvh, un, count;  // its KV head, the first of its units here and how many
+    bool starts, ends;   // whether those begin and end it
+    long long end;       // its last unit among all
+
+    __device__ __forceinline__ int units_of(const AttnArgs &A, int b) const {
+        return seq < 0 ? w.units : seen_units<U>(A, w, b);
+    }
+    __device__ __forceinline__ static long long cost(const AttnArgs &A, int n) {
+        return n > 0 ? (long long)A.kv.n_head_kv * (n + OVER) : 0;
+    }
+    // Units before item c + tid and its own (of items c .. c + TPB - 1 with value(i) each); returns those up to c + TPB
+    template <class Value>
+    __device__ static __forceinline__ long long scan(WalkLds &lds, int c, int n, long long run, long long &mine, long long &before,
+                                                     Value value) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        mine = c + tid < n ? value(c + tid) : 0;
         long long inc = mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -169,41 +174,94 @@ __device__ bool find_run(const AttnArgs &A, Count count, RunLds &lds, Run &r) {
         if (lane == 63) lds.scan[wave] = inc;
         __syncthreads();
         before = run + inc - mine;
+#pragma unroll
         for (int k = 0; k < TPB / 64; k++) {
             if (k < wave) before += lds.scan[k];
             run += lds.scan[k];
         }
         return run;
-    };
-    auto keep = [&](int s, long long b) {
-        lds.seq = s, lds.off = r.u - b;
-        lds.work[0] = w.lo, lds.work[1] = w.n, lds.work[2] = w.len, lds.work[3] = w.base, lds.work[4] = w.end;
-        lds.work[5] = w.units, lds.work[6] = w.blocks;
-    };
-    long long mine = 0, before = 0;
-    r.T = 0;
-    for (int c = 0; c < parts; c += TPB) r.T = scan(c, r.T, mine, before);
-    r.T = uniform(r.T);
-    r.runs = (int)min((long long)A.part[A.first].G, r.T);  // no empty runs between others
-    if ((int)blockIdx.x >= r.runs) return false;
-    r.u = run_start(r.T, r.runs, (int)blockIdx.x);
-    r.u1 = run_start(r.T, r.runs, (int)blockIdx.x + 1);
-    if (parts <= TPB) {
-        if (mine > 0 && before <= r.u && r.u < before + mine) keep(tid - 1, before);
-    } else {
-        long long run = 0;
-        for (int c = 0; c < parts; c += TPB) {
-            run = scan(c, run, mine, before);
-            if (mine > 0 && before <= r.u && r.u < before + mine) keep(c + tid - 1, before);
-        }
     }
-    __syncthreads();
-    r.seq = uniform(lds.seq);
-    r.off = uniform(lds.off);
-    r.work = Work{uniform(lds.work[0]), uniform(lds.work[1]), uniform(lds.work[2]), uniform(lds.work[3]),
-                  uniform(lds.work[4]), uniform(lds.work[5]), uniform(lds.work[6])};
-    return true;
-}
+    __device__ bool find(const AttnArgs &A, WalkLds &lds) {
+        const int tid = threadIdx.x, parts = A.b.n_seqs + 1;
+        Work mine_w{};
+        auto value = [&](int i) {
+            if (i > 0 ? A.last == 0 : A.first == 1) return 0LL;
+            mine_w = work_of<U>(A, i - 1);
+            if (mine_w.units == 0) return 0LL;
+            return i == 0 ? cost(A, mine_w.units) * mine_w.blocks : A.kv.n_head_kv * seen_sum<U>(A, mine_w, OVER);
+        };
+        long long mine = 0, before = 0, run = 0;
+        T = 0;
+        for (int c = 0; c < parts; c += TPB) T = scan(lds, c, parts, T, mine, before, value);
+        T = uniform(T);
+        runs = (int)min((long long)A.part[A.first].G, T);  // no empty runs between others
+        if ((int)blockIdx.x >= runs) return false;
+        u = run_start(T, runs, (int)blockIdx.x);
+        u1 = run_start(T, runs, (int)blockIdx.x + 1);
+        auto keep = [&](int i) {
+            lds.index = i - 1, lds.off = u - before;
+            lds.work[0] = mine_w.lo, lds.work[1] = mine_w.n, lds.work[2] = mine_w.len, lds.work[3] = mine_w.base;
+            lds.work[4] = mine_w.end, lds.work[5] = mine_w.units, lds.work[6] = mine_w.blocks;
+        };
+        if (parts <= TPB) {
+            if (mine > 0 && before <= u && u < before + mine) keep(tid);
+        } else {
+            for (int c = 0; c < parts; c += TPB) {
+                run = scan(lds, c, parts, run, mine, before, value);
+                if (mine > 0 && before <= u && u < before + mine) keep(c + tid);
+            }
+        }
+        __syncthreads();
+        seq = uniform(lds.index);
+        off = uniform(lds.off);
+        w = Work{uniform(lds.work[0]), uniform(lds.work[1]), uniform(lds.work[2]), uniform(lds.work[3]),
+                 uniform(lds.work[4]), uniform(lds.work[5]), uniform(lds.work[6])};
+        rb = 0;
+        if (w.blocks > 1) {  // the block, likewise
+            run = 0;
+            for (int c = 0; c < w.blocks; c += TPB) {
+                run = scan(lds, c, w.blocks, run, mine, before, [&](int b) { return cost(A, units_of(A, b)); });
+                if (mine > 0 && before <= off && off < before + mine) lds.index = c + tid, lds.off = off - before;
+                if (off < run) break;  // the same for every thread
+            }
+            __syncthreads();
+            rb = uniform(lds.index);
+            off = uniform(lds.off);
+        }
+        units = units_of(A, rb);
+        return true;
+    }
+    // The next block with units of this run; false: none.
+    __device__ __forceinline__ bool next(const AttnArgs &A) {
+        while (u < u1) {
+            const int each = units > 0 ? units + OVER : 0;
+            if (off >= (long long)A.kv.n_head_kv * each) {
+                off -= (long long)A.kv.n_head_kv * each;
+                if (++rb >= w.blocks) {
+                    do {
+                        if (++seq >= A.b.n_seqs) return false;  // the batch changed under the call
+                        w = work_of<U>(A, seq);
+                    } while (w.blocks == 0);
+                    rb = 0;
+                }
+                units = units_of(A, rb);
+                continue;
+            }
+            kvh = off >> 31 ? (int)(off / each) : (int)off / each;
+            const int at = (int)(off - (long long)kvh * each), upto = (int)min((long long)each, at + (u1 - u));
+            un = max(0, at - OVER);
+            count = max(0, upto - OVER) - un;
+            starts = un == 0, ends = upto == each;
+            end = u + each - at - 1;
+            u += upto - at;
+            off += upto - at;
+            if (count > 0) return true;
+        }
+        return false;
+    }
+    // The workgroup that ends the block at hand.
+    __device__ __forceinline__ int last() const { return run_owner(T, runs, end); }
+};
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

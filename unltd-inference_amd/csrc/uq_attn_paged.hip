@@ -17,6 +17,7 @@ constexpr int kWaves = kTPB / 64;
 constexpr int kRows = 16;     // queries of a block: the columns of a 16x16 tile
 constexpr int kCUs = 256;
 constexpr int kGroups = 2 * kCUs;  // workgroups of attn_paged_kernel
+constexpr int kOver = 3;           // a block's start and end in tiles: 8 us against 2.7 us a tile at full load
 
 template <bool F16, int HD>
 struct Geo;
@@ -92,36 +93,35 @@ template <bool F16, int HD>
 __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(AttnArgs A) {
     using G = Geo<F16, HD>;
     using E = std::conditional_t<F16, _Float16, float>;
-    constexpr int NP = G::NP, U = kWaves * NP, MS = HD + 4;
+    constexpr int NP = G::NP, MS = HD + 4;  // a unit is a wave's tile
     constexpr float kShift = F16 ? 14.0f : 0.0f;
     extern __shared__ __align__(1024) uint8_t lds[];  // the block's queries; the waves' sums at its end
     __shared__ float row_c[kRows];         // score factor of a query, times log2 e
     __shared__ int row_lim[kRows];         // its last position, -1: none
     __shared__ float2 wave_al[kWaves][kRows];
-    __shared__ RunLds run_lds;
+    __shared__ WalkLds walk_lds;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = uniform(tid >> 6);
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 
-    Run R;
-    if (!find_run<kTPB, U>(A, [&](int, const Work &w) { return (long long)w.units * w.blocks * nkv; }, run_lds, R)) return;
-    long long u = R.u, off = R.off;
-    int seq = R.seq;
-    Work w = R.work;
-
+    Walk<kTPB, NP, kOver> X;
+    if (!X.find(A, walk_lds)) return;
     Wave<F16, HD> W;
-    while (u < R.u1) {
-        const long long per = (long long)nkv * w.units;
-        if (off >= per * w.blocks) {  // the next sequence with units (there is one: u < T)
-            if (++seq >= A.b.n_seqs) return;
-            w = work_of<U>(A, seq);
-            off = 0;
-            continue;
-        }
-        const int rb = (int)(off / per), kvh = (int)(off % per / w.units), un = (int)(off % w.units);
-        const int count = (int)min((long long)(w.units - un), R.u1 - u);
-        const int nq = min(kRows, w.n * A.group - rb * kRows);  // queries of the block
+    while (X.next(A)) {
+        const Work &w = X.w;
+        const int seq = X.seq, rb = X.rb, kvh = X.kvh, un = X.un, nq = min(kRows, w.n * A.group - rb * kRows);
+        // the last position that a query of the block sees, for all that is known without its rows
+        const int seen = seq < 0 ? INT_MAX - 1 : w.len - w.n + (rb * kRows + nq - 1) / A.group;
+        const int end = min(w.end, max(0, seen + 1));
+        const int count = min(X.count, max(0, (end - w.base + NP - 1) / NP - un));
+        const int32_t *table = A.b.pages + (seq < 0 ? (size_t)0 : (size_t)seq * A.b.max_pages);
+        const E *K = (const E *)A.kv.k, *V = (const E *)A.kv.v;
+        auto page_of = [&](int it) {  // of position lane & (NP - 1) of tile it
+            const int pos = w.base + (un + it) * NP + (lane & (NP - 1));
+            return it < count && pos < end ? table[pos >> map.log2_page] : -1;
+        };
+        int page = page_of(wave), ahead = page_of(wave + kWaves);  // on their way while the queries are
 
         // ---- the block's queries into LDS, in the order of the products' right operand
         __syncthreads();  // the waves' sums of the block before are read
@@ -196,30 +196,19 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
         __syncthreads();
         const int lim = row_lim[n];
         const float fac = row_c[n];
-        int lim_min = n < nq ? lim : INT_MAX, lim_max = n < nq ? lim : -1;
+        int lim_min = n < nq ? lim : INT_MAX;
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) {
-            lim_min = min(lim_min, __shfl_xor(lim_min, d));
-            lim_max = max(lim_max, __shfl_xor(lim_max, d));
-        }
-        lim_min = uniform(lim_min), lim_max = uniform(lim_max);
-        const int end = lim_max < w.end ? lim_max + 1 : w.end;  // no row sees further
-        const int32_t *table = A.b.pages + (seq < 0 ? (size_t)0 : (size_t)seq * A.b.max_pages);
-        const E *K = (const E *)A.kv.k, *V = (const E *)A.kv.v;
-
+        for (int d = 1; d < 16; d <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, d));
+        lim_min = uniform(lim_min);
         W.reset();
         bool unfinite = false;  // values that are not finite were left out where some query may not see them
         // A tile's keys and values in registers. The next tile's keys are on their way while this one's values are
         // multiplied, and its values while its own keys are, in the same registers; the loads are issued without a
         // branch (what is no position loads any row), so that they need not be waited for at one.
         Tile<F16, HD> T;
-        auto page_of = [&](int it) {  // of position lane & (NP - 1) of the wave's tile
-            const int pos = w.base + (un + it) * U + wave * NP + (lane & (NP - 1));
-            return it < count && pos < end ? table[pos >> map.log2_page] : -1;
-        };
         auto place = [&](Place &x, int it, int page) {
             const bool there = page_ok(map, page);
-            x.p0 = w.base + (un + it) * U + wave * NP;
+            x.p0 = w.base + (un + it) * NP;
             x.row = there ? page_row(map, page, kvh, x.p0 + (lane & (NP - 1))) : 0;
             x.have = __ballot(there);
         };
@@ -246,13 +235,12 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
         };
         if (map.n_pages > 0) {  // else there is nothing to load from
           Place cur, nxt;
-          place(cur, 0, page_of(0));
-          int page = page_of(1);
+          place(cur, wave, page);
           fetch_keys(cur);
           fetch_values(cur);
-          for (int it = 0; it < count; it++) {
-            place(nxt, it + 1, page);
-            page = page_of(it + 2);
+          for (int it = wave; it < count; it += kWaves) {
+            place(nxt, it + kWaves, ahead);
+            ahead = page_of(it + 2 * kWaves);
             const unsigned long long have = cur.have;
             const int p0 = cur.p0;
             const bool edge = have != ~0ull || p0 + NP - 1 > lim_min;
@@ -307,7 +295,8 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             for (int t = 0; t < G::PT; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    float v = na == INFINITY ? 0.0f : exp2_hw(fmaf(s[t][i], fac, na));
+                    // no score above -infinity: no weight, but a NaN stays one
+                    float v = na == INFINITY ? (s[t][i] == s[t][i] ? 0.0f : s[t][i]) : exp2_hw(fmaf(s[t][i], fac, na));
                     v = sees[4 * t + i] ? v : 0.0f;
                     p[4 * t + i] = v;
                     W.l += v;
@@ -389,9 +378,9 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
           if (__any(unfinite)) {
               // A query that may not see them would have taken 0 * NaN from them; those that do take them now (any
               // weight: the sum is infinite or NaN all the same).
-              for (int it = 0; it < count; it++)
+              for (int it = wave; it < count; it += kWaves)
                   for (int y = 0; y < NP; y++) {
-                      const int pos = w.base + (un + it) * U + wave * NP + y;
+                      const int pos = w.base + (un + it) * NP + y;
                       const int pg = pos < end ? table[pos >> map.log2_page] : -1;
                       if (!page_ok(map, pg)) continue;
                       const E *vp = V + (size_t)page_row(map, pg, kvh, pos) * HD;
@@ -430,8 +419,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                             f4{W.acc[h][j][i], W.acc[h][j + 1][i], W.acc[h][j + 2][i], W.acc[h][j + 3][i]} * to;
         }
         __syncthreads();
-        const bool starts = un == 0, ends = un + count == w.units;
-        const bool whole = starts && ends, done = whole && A.a.shared_len == 0;
+        const bool starts = X.starts, whole = starts && X.ends, done = whole && A.a.shared_len == 0;
         for (int x = tid; x < nq * (HD / 4); x += kTPB) {
             const int r = x / (HD / 4), d = x % (HD / 4) * 4, num = rb * kRows + r;
             float ar = INFINITY, lr = 0.0f;
@@ -441,7 +429,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 #pragma unroll
             for (int i = 0; i < kWaves; i++) {
                 const float2 al = wave_al[i][r];
-                lr += al.x == INFINITY ? 0.0f : al.y * exp2_hw(ar - al.x);
+                lr += al.y * (al.x == INFINITY ? 0.0f : exp2_hw(ar - al.x));  // l is NaN where it says so
                 o += *(const f4 *)((const float *)lds + ((size_t)i * kRows + r) * MS + d);
             }
             const int row = w.lo + num / A.group, head = kvh * A.group + num % A.group;
@@ -463,10 +451,8 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
         if (starts && tid < nq) {
             const int num = rb * kRows + tid;
             put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
-                    done ? kDone : whole ? kWhole : (int)blockIdx.x, done || whole ? 0 : run_owner(R.T, R.runs, u + w.units - 1), tid);
+                    done ? kDone : whole ? kWhole : (int)blockIdx.x, done || whole ? 0 : X.last(), tid);
         }
-        u += count;
-        off += count;
     }
 }
 
@@ -509,7 +495,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
         if (c == 1) {
             const Work w = work_of<1>(A, seq);
             const int num = (row - w.lo) * A.group + head % A.group;
-            if (w.units == 0 || (A.many && seen_units<1>(A, w, num / A.part[1].rows) == 0)) continue;
+            if (w.units == 0 || seen_units<1>(A, w, num / A.part[1].rows) == 0) continue;
         }
         const int last = min(sg[c].y >> 8, A.part[c].G - 1);
         if (sg[c].x == kDone) return;
@@ -543,7 +529,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
         if (mine < total) {
             const float2 al = A.rec_al[rec(mine)];
             f = al.x == INFINITY ? 0.0f : exp2_hw(amin - al.x);
-            l += f == 0.0f ? 0.0f : f * al.y;
+            l += f * al.y;
         }
         const int n = min(64, (total - i0 + WAVES - 1) / WAVES);
 #pragma unroll 8
@@ -551,10 +537,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
             const float *src = A.rec_o + rec(i0 + WAVES * k) * HD + lane;
             const float fk = __shfl(f, k);
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float v = src[64 * e];
-                o[e] += fk == 0.0f ? 0.0f : fk * v;
-            }
+            for (int e = 0; e < E; e++) o[e] += fk * src[64 * e];
         }
     }
     l = wave_sum(l);
@@ -609,7 +592,6 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     const int own = many_rows(kv, (queries + b.n_seqs - 1) / b.n_seqs);
     A.part[0] = shared ? Part{shared, many_groups(shared), 0} : Part{few, kGroups, 0};
     A.part[1] = own ? Part{own, many_groups(own), 0} : Part{few, kGroups, 0};
-    A.many = own != 0;
     p.apart = a.shared_len && (shared || own);
     auto groups_recs = [&](const Part &x) { return (size_t)2 * x.G * x.rows; };
     size_t recs = groups_recs(A.part[1]);
