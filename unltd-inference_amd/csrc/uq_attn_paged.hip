@@ -14,9 +14,9 @@ namespace {
 
 constexpr int kTPB = 256;
 constexpr int kWaves = kTPB / 64;
-constexpr int kRows = 16;     // queries of a block: the columns of a 16x16 tile
 constexpr int kCUs = 256;
-constexpr int kGroups = 2 * kCUs;  // workgroups of attn_paged_kernel
+// Workgroups of attn_paged_kernel a CU: its registers' (32 queries of 256 values: 128 for the sums alone) and LDS's limit.
+constexpr int few_per_cu(int hd, int rt) { return hd == 512 || (hd == 256 && rt == 2) ? 1 : 2; }
 constexpr int kOver = 3;           // a block's start and end in tiles: 8 us against 2.7 us a tile at full load
 
 template <bool F16, int HD>
@@ -58,19 +58,24 @@ __device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) &
 // f16 cache: a query is scaled by a power of two to at most 2^15 and split
 // into two f16 terms, a weight (times 2^14) likewise; products are exact and
 // summed in f32. f32 cache: the f32 matrix products.
-template <bool F16, int HD>
+//
+// RT is 1 or 2: of 16 or 32 queries of a KV head, columns n and n + 16.
+template <bool F16, int HD, int RT>
 struct Wave {
     using G = Geo<F16, HD>;
-    f4 acc[G::NH][G::DL];
-    float a, l;  // reference, this lane's share of l
+    f4 acc[RT][G::NH][G::DL];
+    float a[RT], l[RT];  // reference, this lane's share of l
 
     __device__ __forceinline__ void reset() {
 #pragma unroll
-        for (int h = 0; h < G::NH; h++)
+        for (int y = 0; y < RT; y++) {
 #pragma unroll
-            for (int j = 0; j < G::DL; j++) acc[h][j] = f4{0.f, 0.f, 0.f, 0.f};
-        a = INFINITY;
-        l = 0.0f;
+            for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                for (int j = 0; j < G::DL; j++) acc[y][h][j] = f4{0.f, 0.f, 0.f, 0.f};
+            a[y] = INFINITY;
+            l[y] = 0.0f;
+        }
     }
 };
 
@@ -89,16 +94,16 @@ struct Place {
     unsigned long long have;
 };
 
-template <bool F16, int HD>
-__global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(AttnArgs A) {
+template <bool F16, int HD, int RT>
+__global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(AttnArgs A) {
     using G = Geo<F16, HD>;
     using E = std::conditional_t<F16, _Float16, float>;
-    constexpr int NP = G::NP, MS = HD + 4;  // a unit is a wave's tile
+    constexpr int NP = G::NP, MS = HD + 4, ROWS = 16 * RT;  // a unit is a wave's tile
     constexpr float kShift = F16 ? 14.0f : 0.0f;
     extern __shared__ __align__(1024) uint8_t lds[];  // the block's queries; the waves' sums at its end
-    __shared__ float row_c[kRows];         // score factor of a query, times log2 e
-    __shared__ int row_lim[kRows];         // its last position, -1: none
-    __shared__ float2 wave_al[kWaves][kRows];
+    __shared__ float row_c[ROWS];         // score factor of a query, times log2 e
+    __shared__ int row_lim[ROWS];         // its last position, -1: none
+    __shared__ float2 wave_al[kWaves][ROWS];
     __shared__ WalkLds walk_lds;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int wave = uniform(tid >> 6);
@@ -107,12 +112,12 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 
     Walk<kTPB, NP, kOver> X;
     if (!X.find(A, walk_lds)) return;
-    Wave<F16, HD> W;
+    Wave<F16, HD, RT> W;
     while (X.next(A)) {
         const Work &w = X.w;
-        const int seq = X.seq, rb = X.rb, kvh = X.kvh, un = X.un, nq = min(kRows, w.n * A.group - rb * kRows);
+        const int seq = X.seq, rb = X.rb, kvh = X.kvh, un = X.un, nq = min(ROWS, w.n * A.group - rb * ROWS);
         // the last position that a query of the block sees, for all that is known without its rows
-        const int seen = seq < 0 ? INT_MAX - 1 : w.len - w.n + (rb * kRows + nq - 1) / A.group;
+        const int seen = seq < 0 ? INT_MAX - 1 : w.len - w.n + (rb * ROWS + nq - 1) / A.group;
         const int end = min(w.end, max(0, seen + 1));
         const int count = min(X.count, max(0, (end - w.base + NP - 1) / NP - un));
         const int32_t *table = A.b.pages + (seq < 0 ? (size_t)0 : (size_t)seq * A.b.max_pages);
@@ -125,8 +130,9 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 
         // ---- the block's queries into LDS, in the order of the products' right operand
         __syncthreads();  // the waves' sums of the block before are read
-        {
-            const int r = tid >> 4, part = tid & 15, num = rb * kRows + r;
+#pragma unroll
+        for (int y = 0; y < RT; y++) {
+            const int r = (tid >> 4) + 16 * y, part = tid & 15, num = rb * ROWS + r;
             const bool in = r < nq;
             const int row = w.lo + (in ? num / A.group : 0);
             const float *q = A.a.q + ((size_t)row * A.a.n_head + (size_t)kvh * A.group + (in ? num % A.group : 0)) * HD;
@@ -170,7 +176,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                         lo[x] = (_Float16)(s - (float)hi[x]);
                     }
                     if (ch < HD / 8) {
-                        h8 *dst = (h8 *)lds + (ch >> 2) * 128 + (ch & 3) * 16 + r;
+                        h8 *dst = (h8 *)lds + y * HD * 4 + (ch >> 2) * 128 + (ch & 3) * 16 + (r & 15);
                         dst[0] = hi;
                         dst[64] = lo;
                     }
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 #pragma unroll
                 for (int c = 0; c < HD / 64; c++) {
                     const int ch = part + 16 * c;
-                    ((f4 *)lds)[(ch >> 2) * 64 + (ch & 3) * 16 + r] = in ? (f4) * (const f4u *)(q + 4 * ch) : f4{0.f, 0.f, 0.f, 0.f};
+                    ((f4 *)lds)[y * HD * 4 + (ch >> 2) * 64 + (ch & 3) * 16 + (r & 15)] = in ? (f4) * (const f4u *)(q + 4 * ch) : f4{0.f, 0.f, 0.f, 0.f};
                 }
             }
             if (part == 0) row_c[r] = fac;
@@ -194,9 +200,14 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             }
         }
         __syncthreads();
-        const int lim = row_lim[n];
-        const float fac = row_c[n];
-        int lim_min = n < nq ? lim : INT_MAX;
+        int lim[RT], lim_min = INT_MAX;
+        float fac[RT];
+#pragma unroll
+        for (int y = 0; y < RT; y++) {
+            lim[y] = row_lim[n + 16 * y];
+            fac[y] = row_c[n + 16 * y];
+            if (n + 16 * y < nq) lim_min = min(lim_min, lim[y]);
+        }
 #pragma unroll
         for (int d = 1; d < 16; d <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, d));
         lim_min = uniform(lim_min);
@@ -245,66 +256,71 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             const int p0 = cur.p0;
             const bool edge = have != ~0ull || p0 + NP - 1 > lim_min;
             const uint32_t hv = (uint32_t)have >> (4 * g);  // bit 16 t + i: position 16 t + 4 g + i
-            const int room = lim - p0 - 4 * g;
 
             // scores
-            f4 s[G::PT];
-            if constexpr (F16) {
+            f4 s[RT][G::PT];
 #pragma unroll
-                for (int t = 0; t < G::PT; t++) s[t] = f4{0.f, 0.f, 0.f, 0.f};
+            for (int y = 0; y < RT; y++)
 #pragma unroll
-                for (int c = 0; c < G::KC; c++) {
-                    const h8 qh = ((const h8 *)lds)[c * 128 + lane], ql = ((const h8 *)lds)[c * 128 + 64 + lane];
+                for (int t = 0; t < G::PT; t++) s[y][t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int t = 0; t < G::PT; t++) {
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.k[t][c], qh, s[t], 0, 0, 0);
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.k[t][c], ql, s[t], 0, 0, 0);
+            for (int c = 0; c < G::KC; c++)
+#pragma unroll
+                for (int y = 0; y < RT; y++) {
+                    if constexpr (F16) {
+                        const h8 *q = (const h8 *)lds + y * HD * 4 + c * 128 + lane;
+                        const h8 qh = q[0], ql = q[64];
+#pragma unroll
+                        for (int t = 0; t < G::PT; t++) {
+                            s[y][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.k[t][c], qh, s[y][t], 0, 0, 0);
+                            s[y][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(T.k[t][c], ql, s[y][t], 0, 0, 0);
+                        }
+                    } else {
+                        const f4 q = ((const f4 *)lds)[y * HD * 4 + c * 64 + lane];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[y][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(T.k[0][c][e], q[e], s[y][0], 0, 0, 0);
                     }
                 }
-            } else {
-                s[0] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < G::KC; c++) {
-                    const f4 q = ((const f4 *)lds)[c * 64 + lane];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(T.k[0][c][e], q[e], s[0], 0, 0, 0);
-                }
-            }
 
             __builtin_amdgcn_sched_barrier(0);
             fetch_keys(nxt);
             __builtin_amdgcn_sched_barrier(0);
 
             // weights: slot x = 4 t + i is position p0 + 16 t + 4 g + i
-            float p[4 * G::PT];
-            float top = -INFINITY;
-            bool sees[4 * G::PT];
+            float p[RT][4 * G::PT];
 #pragma unroll
-            for (int t = 0; t < G::PT; t++)
+            for (int y = 0; y < RT; y++) {
+                const int room = lim[y] - p0 - 4 * g;
+                float top = -INFINITY;
+                bool sees[4 * G::PT];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    sees[4 * t + i] = !edge || (((hv >> (16 * t + i)) & 1) && 16 * t + i <= room);
-                    top = fmaxf(top, sees[4 * t + i] ? s[t][i] * fac : -INFINITY);
-                }
-            top = row16_max(top);
-            float na = fminf(W.a, kShift - top);
-            const float corr = na == INFINITY ? 1.0f : exp2_hw(na - W.a);
-            W.a = na;
-            W.l *= corr;
+                for (int t = 0; t < G::PT; t++)
 #pragma unroll
-            for (int t = 0; t < G::PT; t++)
+                    for (int i = 0; i < 4; i++) {
+                        sees[4 * t + i] = !edge || (((hv >> (16 * t + i)) & 1) && 16 * t + i <= room);
+                        top = fmaxf(top, sees[4 * t + i] ? s[y][t][i] * fac[y] : -INFINITY);
+                    }
+                top = row16_max(top);
+                const float na = fminf(W.a[y], kShift - top);
+                const float corr = na == INFINITY ? 1.0f : exp2_hw(na - W.a[y]);
+                W.a[y] = na;
+                W.l[y] *= corr;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    // no score above -infinity: no weight, but a NaN stays one
-                    float v = na == INFINITY ? (s[t][i] == s[t][i] ? 0.0f : s[t][i]) : exp2_hw(fmaf(s[t][i], fac, na));
-                    v = sees[4 * t + i] ? v : 0.0f;
-                    p[4 * t + i] = v;
-                    W.l += v;
-                }
+                for (int t = 0; t < G::PT; t++)
 #pragma unroll
-            for (int h = 0; h < G::NH; h++)
+                    for (int i = 0; i < 4; i++) {
+                        // no score above -infinity: no weight, but a NaN stays one
+                        const float z = s[y][t][i];
+                        float v = na == INFINITY ? (z == z ? 0.0f : z) : exp2_hw(fmaf(z, fac[y], na));
+                        v = sees[4 * t + i] ? v : 0.0f;
+                        p[y][4 * t + i] = v;
+                        W.l[y] += v;
+                    }
 #pragma unroll
-                for (int j = 0; j < G::DL; j++) W.acc[h][j] *= corr;
+                for (int h = 0; h < G::NH; h++)
+#pragma unroll
+                    for (int j = 0; j < G::DL; j++) W.acc[y][h][j] *= corr;
+            }
 
             // values: slot x of a lane is position p0 + 16 (x / 4) + 4 g + x % 4
             if constexpr (F16) {
@@ -327,12 +343,14 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                         unfinite = unfinite || (ok && !fin);
                     }
                 }
-                h8 ph, pl;
+                h8 ph[RT], pl[RT];
 #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    ph[x] = (_Float16)p[x];
-                    pl[x] = (_Float16)(p[x] - (float)ph[x]);
-                }
+                for (int y = 0; y < RT; y++)
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        ph[y][x] = (_Float16)p[y][x];
+                        pl[y][x] = (_Float16)(p[y][x] - (float)ph[y][x]);
+                    }
 #pragma unroll
                 for (int h = 0; h < G::NH; h++)
 #pragma unroll
@@ -342,8 +360,11 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                         for (int x = 0; x < 4; x++)
                             f[x] = __builtin_amdgcn_perm(v[2 * x + 1][h][j >> 1], v[2 * x][h][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
                         const h8 vf = __builtin_bit_cast(h8, f);
-                        W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, W.acc[h][j], 0, 0, 0);
-                        W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, W.acc[h][j], 0, 0, 0);
+#pragma unroll
+                        for (int y = 0; y < RT; y++) {
+                            W.acc[y][h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[y], W.acc[y][h][j], 0, 0, 0);
+                            W.acc[y][h][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[y], W.acc[y][h][j], 0, 0, 0);
+                        }
                     }
             } else {
                 auto &v = T.v;
@@ -369,7 +390,9 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
                     for (int h = 0; h < G::NH; h++)
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            W.acc[h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][h][j], p[x], W.acc[h][j], 0, 0, 0);
+#pragma unroll
+                            for (int y = 0; y < RT; y++)
+                                W.acc[y][h][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[x][h][j], p[y][x], W.acc[y][h][j], 0, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
             fetch_values(nxt);
@@ -391,7 +414,9 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
 #pragma unroll
                               for (int j = 0; j < G::DL; j++) {
                                   const float v = (float)vp[h * 16 * G::DL + (4 * g + i) * G::DL + j];
-                                  if (pos <= lim && !finite32(v)) W.acc[h][j][i] += v;
+#pragma unroll
+                                  for (int y = 0; y < RT; y++)
+                                      if (pos <= lim[y] && !finite32(v)) W.acc[y][h][j][i] += v;
                               }
                               __builtin_amdgcn_sched_barrier(0);
                           }
@@ -400,28 +425,37 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
         }
 
         // ---- the waves' sums joined: references, then o scaled to the least of them
-        W.l = row16_sum(W.l);
-        if (lane < kRows) wave_al[wave][lane] = make_float2(W.a, W.l);
+#pragma unroll
+        for (int y = 0; y < RT; y++) {
+            W.l[y] = row16_sum(W.l[y]);
+            if (lane < 16) wave_al[wave][lane + 16 * y] = make_float2(W.a[y], W.l[y]);
+        }
         __syncthreads();  // also: every wave is done with the queries in LDS
-        float amin = INFINITY;
+        float *sums = (float *)lds + (size_t)wave * ROWS * MS;
 #pragma unroll
-        for (int i = 0; i < kWaves; i++) amin = fminf(amin, wave_al[i][n].x);
-        const float to = W.a == INFINITY ? 0.0f : exp2_hw(amin - W.a);
-        float *sums = (float *)lds + (size_t)wave * kRows * MS;
-        if (n < nq) {
+        for (int y = 0; y < RT; y++) {
+            const int q = n + 16 * y;
+            float amin = INFINITY;
 #pragma unroll
-            for (int h = 0; h < G::NH; h++)
+            for (int i = 0; i < kWaves; i++) amin = fminf(amin, wave_al[i][q].x);
+            const float to = W.a[y] == INFINITY ? 0.0f : exp2_hw(amin - W.a[y]);
+            if (q < nq) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int h = 0; h < G::NH; h++)
 #pragma unroll
-                    for (int j = 0; j < G::DL; j += 4)
-                        *(f4 *)(sums + n * MS + h * 16 * G::DL + (4 * g + i) * G::DL + j) =
-                            f4{W.acc[h][j][i], W.acc[h][j + 1][i], W.acc[h][j + 2][i], W.acc[h][j + 3][i]} * to;
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int j = 0; j < G::DL; j += 4) {
+                            const f4 *o = W.acc[y][h];
+                            *(f4 *)(sums + q * MS + h * 16 * G::DL + (4 * g + i) * G::DL + j) =
+                                f4{o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]} * to;
+                        }
+            }
         }
         __syncthreads();
         const bool starts = X.starts, whole = starts && X.ends, done = whole && A.a.shared_len == 0;
         for (int x = tid; x < nq * (HD / 4); x += kTPB) {
-            const int r = x / (HD / 4), d = x % (HD / 4) * 4, num = rb * kRows + r;
+            const int r = x / (HD / 4), d = x % (HD / 4) * 4, num = rb * ROWS + r;
             float ar = INFINITY, lr = 0.0f;
             f4 o = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -430,7 +464,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             for (int i = 0; i < kWaves; i++) {
                 const float2 al = wave_al[i][r];
                 lr += al.y * (al.x == INFINITY ? 0.0f : exp2_hw(ar - al.x));  // l is NaN where it says so
-                o += *(const f4 *)((const float *)lds + ((size_t)i * kRows + r) * MS + d);
+                o += *(const f4 *)((const float *)lds + ((size_t)i * ROWS + r) * MS + d);
             }
             const int row = w.lo + num / A.group, head = kvh * A.group + num % A.group;
             if (done) {
@@ -449,7 +483,7 @@ __global__ __launch_bounds__(kTPB, HD <= 256 ? 2 : 1) void attn_paged_kernel(Att
             }
         }
         if (starts && tid < nq) {
-            const int num = rb * kRows + tid;
+            const int num = rb * ROWS + tid;
             put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
                     done ? kDone : whole ? kWhole : (int)blockIdx.x, done || whole ? 0 : X.last(), tid);
         }
@@ -574,12 +608,29 @@ struct Plan {
     AttnArgs A;
 };
 
-// Queries of a block for R queries of a KV head, 0: the kernel of few.
-int many_rows(const PagesView &kv, size_t R) {
-    if (!attn_many_ok(kv) || R <= 32) return 0;
-    return (R + 127) / 128 * 128 == (R + 63) / 64 * 64 ? 128 : 64;
+// Queries of a block for R queries of a KV head (all rows' of the shared part,
+// a sequence's at the mean): 64 or 128 on attn_many_kernel for more than 32,
+// the least that wastes the least; else 16 or 32 on attn_paged_kernel. 32 read
+// the cache half as often (us, 16 | 32; f16, 32 sequences of 20 queries: 79 |
+// 68; f32, of 40: 117 | 106; 509 rows of one, f32: 500 | 370; 48 rows with
+// 16384 shared, f32: 300 | 180), but
+//  - leave a CU one workgroup for 256 f32 values, which reads too slowly from
+//    memory unless the blocks are of one or two sequences (32 sequences of 64
+//    queries: 220 | 274; 8 of 256: 345 | 382; 2 of 1024: 655 | 458);
+//  - of a shared part need a launch apart from own parts in blocks of 16,
+//    10 us that few tiles a wave do not bring in (17 rows' 12 heads over 2011
+//    positions: 23 | 37; 12000: 43 | 50; 20000: 65 | 61).
+int block_rows(const PagesView &kv, size_t R, int n_seqs, int shared) {
+    if (R <= 16 || kv.head_dim == 512) return 16;
+    if (R > 32 && attn_many_ok(kv)) return (R + 127) / 128 * 128 == (R + 63) / 64 * 64 ? 128 : 64;
+    if (!kv.f16 && kv.head_dim == 256 && n_seqs > 2) return 16;
+    const size_t tiles = (R + 15) / 16 * kv.n_head_kv * ((size_t)shared / (kv.f16 ? 32 : 16));
+    return shared && tiles < 32 * 2 * kCUs ? 16 : 32;
 }
-int many_groups(int rows) { return rows == 64 ? 2 * kCUs : kCUs; }
+int block_groups(const PagesView &kv, int rows) {
+    if (rows <= 32) return kCUs * few_per_cu(kv.head_dim, rows / 16);
+    return rows == 64 ? 2 * kCUs : kCUs;  // 2 or 4 waves, a SIMD's registers each
+}
 
 Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     const int group = a.n_head / kv.n_head_kv;
@@ -587,14 +638,14 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     Plan p{};
     AttnArgs &A = p.A;
     A.a = a, A.kv = kv, A.b = b, A.group = group;
-    const int few = kRows;
-    const int shared = a.shared_len ? many_rows(kv, queries) : 0;
-    const int own = many_rows(kv, (queries + b.n_seqs - 1) / b.n_seqs);
-    A.part[0] = shared ? Part{shared, many_groups(shared), 0} : Part{few, kGroups, 0};
-    A.part[1] = own ? Part{own, many_groups(own), 0} : Part{few, kGroups, 0};
-    p.apart = a.shared_len && (shared || own);
+    A.part[1].rows = block_rows(kv, (queries + b.n_seqs - 1) / b.n_seqs, b.n_seqs, 0);
+    A.part[0].rows = a.shared_len ? block_rows(kv, queries, 1, a.shared_len) : A.part[1].rows;
+    if (A.part[0].rows == 16)  // no gain from a launch apart
+        A.part[0].rows = std::min(A.part[1].rows, 32);
+    for (Part &x : A.part) x.G = block_groups(kv, x.rows);
     auto groups_recs = [&](const Part &x) { return (size_t)2 * x.G * x.rows; };
     size_t recs = groups_recs(A.part[1]);
+    p.apart = A.part[0].rows != A.part[1].rows;
     if (p.apart) A.part[0].base = recs, recs += groups_recs(A.part[0]);
     A.whole = recs;
     if (a.shared_len) recs += (size_t)2 * b.n_rows * a.n_head;
@@ -604,22 +655,25 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     return p;
 }
 
-template <bool F16, int HD>
+template <bool F16, int HD, int RT>
 hipError_t launch(const AttnArgs &A, hipStream_t s) {
-    constexpr size_t lds = (size_t)kWaves * kRows * (HD + 4) * 4;
-    static_assert(lds >= (size_t)HD * 64, "the queries fit where the sums go");
-    auto *k = attn_paged_kernel<F16, HD>;
+    constexpr size_t lds = (size_t)kWaves * 16 * RT * (HD + 4) * 4;
+    static_assert(lds >= (size_t)HD * 64 * RT, "the queries fit where the sums go");
+    static_assert(few_per_cu(HD, RT) * (lds + 2048) <= 160 * 1024, "LDS");
+    auto *k = attn_paged_kernel<F16, HD, RT>;
     if (hipError_t e = allow_lds((const void *)k, lds)) return e;
-    hipLaunchKernelGGL(k, dim3(kGroups), dim3(kTPB), lds, s, A);
+    hipLaunchKernelGGL(k, dim3((unsigned)A.part[A.first].G), dim3(kTPB), lds, s, A);
     return hipGetLastError();
 }
 
+template <bool F16>
 hipError_t launch_few(const AttnArgs &A, hipStream_t s) {
+    const bool two = A.part[A.first].rows == 32;
     switch (A.kv.head_dim) {
-    case 64: return A.kv.f16 ? launch<true, 64>(A, s) : launch<false, 64>(A, s);
-    case 128: return A.kv.f16 ? launch<true, 128>(A, s) : launch<false, 128>(A, s);
-    case 256: return A.kv.f16 ? launch<true, 256>(A, s) : launch<false, 256>(A, s);
-    case 512: return A.kv.f16 ? launch<true, 512>(A, s) : launch<false, 512>(A, s);
+    case 64: return two ? launch<F16, 64, 2>(A, s) : launch<F16, 64, 1>(A, s);
+    case 128: return two ? launch<F16, 128, 2>(A, s) : launch<F16, 128, 1>(A, s);
+    case 256: return two ? launch<F16, 256, 2>(A, s) : launch<F16, 256, 1>(A, s);
+    case 512: return launch<F16, 512, 1>(A, s);
     }
     return hipErrorInvalidValue;
 }
@@ -664,7 +718,7 @@ hipError_t launch_attn_paged(const PagesView &kv, const BatchView &b, const Attn
     A.seg = (int2 *)((uint8_t *)ws + p.seg);
     auto go = [&](int first, int last) {
         A.first = first, A.last = last;
-        return A.part[first].rows == kRows ? launch_few(A, s) : launch_attn_many(A, s);
+        return A.part[first].rows > 32 ? launch_attn_many(A, s) : kv.f16 ? launch_few<true>(A, s) : launch_few<false>(A, s);
     };
     if (p.apart)
         if (hipError_t e = go(0, 0)) return e;
