@@ -38,7 +38,7 @@ typedef struct uq_kv_pages {
     uq_dtype dtype;
     size_t n_pages;   /* n_pages * n_head_kv * page_size below 2^31 */
     size_t page_size; /* a power of two, at most 65536 */
-    size_t n_head_kv;
+    size_t n_head_kv; /* at most 1024 */
     size_t head_dim; /* 64, 128, 256 or 512 */
 } uq_kv_pages;
 
@@ -54,7 +54,7 @@ typedef struct uq_kv_pages {
  * and a position beyond the table hold nothing: appending there writes
  * nothing, attention passes over them. */
 typedef struct uq_seq_batch {
-    size_t n_seqs, n_rows;
+    size_t n_seqs, n_rows; /* at most 65535, 2^23 */
     const int32_t *d_row_start; /* [n_seqs + 1] */
     const int32_t *d_len;       /* [n_seqs] */
     const int32_t *d_pages;     /* [n_seqs][max_pages] */
@@ -127,9 +127,9 @@ uq_status uq_kv_append_d(const uq_kv_pages *kv, const uq_seq_batch *batch, const
  *
  * The workspace (uq_attn_paged_ws_bytes, 16-byte aligned) does not depend on
  * the lengths. uq_attn_paged_ws_bytes returns 0 for arguments that the call
- * refuses. Errors: UQ_ERR_ARG (also a workspace too small or shared_len
- * beyond the table), UQ_ERR_DTYPE, UQ_ERR_LEN (n_head no multiple of
- * n_head_kv). */
+ * refuses. Errors: UQ_ERR_ARG (also a workspace too small, shared_len beyond
+ * the table, n_rows * n_head above 2^25 or kq_scale not finite), UQ_ERR_DTYPE,
+ * UQ_ERR_LEN (n_head no multiple of n_head_kv). */
 size_t uq_attn_paged_ws_bytes(const uq_kv_pages *kv, const uq_seq_batch *batch, size_t n_head, size_t shared_len);
 uq_status uq_attn_paged_d(float *d_out, const float *d_q, const uq_kv_pages *kv, const uq_seq_batch *batch,
                           size_t n_head, size_t shared_len, float kq_scale, const float *d_gate, size_t gate_row,

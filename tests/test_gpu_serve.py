@@ -50,7 +50,7 @@ def ulps(a, b):
 # ------------------------------------------------------------------------- append
 
 @pytest.mark.parametrize("dtype,heads,kv,hd,page,rows,lens,rope,n_rot,norm,pad", [
-    ("f16", 16, 4, 256, 64, [1], [3071], "imrope", 64, True, 0),
+    ("f16", 16, 4, 256, 64, [1], [2999], "imrope", 64, True, 0),
     ("f32", 16, 4, 256, 16, [3, 0, 5, 1], [3, 9, 700, 1], "imrope", 64, True, 2),
     ("f16", 6, 2, 128, 1, [4, 2], [17, 2], "neox", 128, True, 1),
     ("f32", 8, 8, 64, 4096, [2] * 70, list(range(2, 72)), "llama", 32, True, 0),
@@ -235,7 +235,13 @@ SHAPES = [
     (4, 2, 128, 16, [20] * 7, [620, 610, 650, 600, 608, 601, 640], 599, 3),
     (8, 1, 64, 1, [3] * 11, [140 + 9 * i for i in range(11)], 130, 0),
     (5, 1, 256, 32, [40, 20], [35, 64], 0, 0),  # more rows than positions
-    (16, 4, 256, 64, [1] * 20 + [70], [60 + 7 * i for i in range(21)], 50, 0)]  # shared and own on different kernels
+    (16, 4, 256, 64, [1] * 20 + [70], [60 + 7 * i for i in range(21)], 50, 0),  # shared and own on different kernels
+    # blocks of 32 queries: 17 to 32 of a KV head, more where the cache is f32
+    (20, 1, 128, 32, [1] * 3, [50, 200, 333], 0, 0),
+    (24, 1, 256, 16, [1, 1], [40, 700], 0, 1),
+    (32, 1, 64, 8, [1, 0, 1], [1, 5, 64], 0, 0),
+    (8, 1, 128, 16, [3] * 4, [64, 90, 61, 150], 60, 0),
+    (16, 8, 64, 16, [1] * 100, [2601 + i % 7 for i in range(100)], 2600, 2)]  # f32: shared on 32, own on 16
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -353,6 +359,180 @@ def test_attention_of_large_and_small_numbers(dtype):
     assert np.all(np.abs(got[1:] - want[1:]) <= bound[1:])
     one = np.abs(got[0] - want[0]) <= np.maximum(bound[0], 1e-4)
     assert one.all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30])
+def test_attention_with_any_scale(dtype, scale):
+    """Turned round, the mean of the values, nearly the mean: blocks of few and of many queries."""
+    rng = np.random.default_rng(29)
+    c = M.Cache(rng, dtype, 2, 64, 16, [1, 30], [90, 200])
+    check(c, rng.standard_normal((31, 6, 64)).astype(np.float32), 6, scale, what=f"{dtype} scale {scale}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_of_many_queries_large_and_not_finite(dtype):
+    """Queries of 1e30, 1e-30 and 0 among others, and of NaN and infinity, whose own results show it and no others."""
+    rng = np.random.default_rng(30)
+    c = M.Cache(rng, dtype, 1, 128, 16, [40], [300])
+    q = rng.standard_normal((40, 4, 128)).astype(np.float32)
+    clean = q.copy()
+    q[3] *= 1e-30
+    q[4] = 0
+    q[5, 1] *= 1e5
+    bad = [(7, 0), (8, 3), (39, 2)]
+    for (r, h), x in zip(bad, (np.nan, np.inf, -np.inf)):
+        q[r, h, 11] = x
+    got = attend(c, q, 4, 0.1)
+    clean[[3, 4, 5]] = q[[3, 4, 5]]
+    want, bound = M.attention(c, clean, 4, 0.1)
+    good = np.ones((40, 4), bool)
+    for r, h in bad:
+        good[r, h] = False
+        assert not np.isfinite(got[r, h]).any()
+    bound[5, 1] = np.maximum(bound[5, 1], 1e-3)  # scores of 1e5: which weight is all may turn on their last bits
+    good[5, 1] = False
+    assert np.all(np.abs(got - want)[good] <= bound[good])
+    assert np.isfinite(got[5, 1]).all()
+
+
+@pytest.mark.parametrize("rows", [[1, 2], [40, 30]])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_without_pages_or_rows(dtype, rows):
+    """A cache of no pages, a table of none: zeros. A batch whose rows are all none: nothing is written."""
+    n = sum(rows)
+    q = dev(np.ones((n, 4, 64), np.float32))
+    start, zero = dev(np.array([0, rows[0], n], np.int32)), dev(np.zeros(3, np.int32))
+    lens, table = dev(np.array([100, 70], np.int32)), dev(np.arange(14, dtype=np.int32))
+    some = dev(np.ones((14, 2, 16, 64), M.DTYPE[dtype][1]))
+    like = np.empty((n, 4, 64), np.float32)
+    for shared in (0, 33):
+        for kv, batch, want in [
+                (serve.KvPages(None, None, M.DTYPE[dtype][0], 0, 16, 2, 64), serve.SeqBatch(2, n, start, lens, table, 7), 0.0),
+                (serve.KvPages(some, some, M.DTYPE[dtype][0], 14, 16, 2, 64), serve.SeqBatch(2, n, zero, lens, table, 7), 7.0),
+                (serve.KvPages(some, some, M.DTYPE[dtype][0], 14, 16, 2, 64), serve.SeqBatch(2, n, start, lens), 0.0)]:
+            if shared and not batch.max_pages:
+                continue
+            out = dev(np.full(like.shape, 7.0, np.float32))
+            ws = uq.DeviceArray(serve.attn_paged_ws_bytes(kv, batch, 4, shared))
+            serve.attn_paged_d(out, q, kv, batch, 4, 0.125, ws, shared_len=shared)
+            assert np.all(host(out, like) == want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attention_in_a_pool_beyond_32_bits(dtype):
+    """Pages whose values lie 2^32 and more bytes and elements into the arrays, appended to and read, by few queries
+    and by many (a page number of them would be another page's in 32 bits)."""
+    hd, page, heads = 128, 16, 4
+    elem = 2 if dtype == "f16" else 4
+    per = page * hd  # elements of a page (one KV head)
+    n_pages = (1 << 32) // per + 64
+    rows, lens = [40, 1], [200, 150]
+    rng = np.random.default_rng(31)
+    c = M.Cache(rng, dtype, 1, hd, page, rows, lens, spare=0)
+    high = n_pages - 1 - np.arange(c.n_pages)  # page x of the small cache is this page of the large one
+    d_k, d_v = uq.DeviceArray(n_pages * per * elem), uq.DeviceArray(n_pages * per * elem)
+
+    lo = int(high[-1]) * per * elem
+    for d, a in ((d_k, c.k), (d_v, c.v)):
+        buf = np.ascontiguousarray(a[::-1])
+        uq._check(uq.lib().uq_memcpy_htod(d.ptr.value + lo, buf.ctypes.data, buf.nbytes, None))
+        uq.synchronize()
+    pages = serve.KvPages(d_k, d_v, M.DTYPE[dtype][0], n_pages, page, 1, hd)
+    table = np.where(c.table >= 0, high[c.table], -1).astype(np.int32)
+    batch = serve.SeqBatch(2, 41, dev(c.start), dev(np.array(lens, np.int32)), dev(table), c.max_pages)
+    q, k, v = (rng.standard_normal((41, w, hd)).astype(np.float32) for w in (heads, 1, 1))
+    dq, dk, dv = dev(q), dev(k), dev(v)
+    out = dev(np.zeros_like(q))
+    serve.kv_append_d(pages, batch, serve.HeadRows(d_k=dk, k_row=hd, d_v=dv, v_row=hd))
+    for r, (b, pos) in enumerate(c.row_positions()):
+        pg, sl, _ = c.slots(b, pos + 1)
+        c.k[pg[-1], :, sl[-1]], c.v[pg[-1], :, sl[-1]] = k[r], v[r]
+    ws = uq.DeviceArray(serve.attn_paged_ws_bytes(pages, batch, heads))
+    serve.attn_paged_d(out, dq, pages, batch, heads, 0.1, ws)
+    want, bound = M.attention(c, q, heads, 0.1)
+    assert np.all(np.abs(host(out, q) - want) <= bound)
+    for d in (d_k, d_v):
+        d.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,lens,shared", [([3, 1], [70, 90], 48), ([50, 40], [90, 140], 40), ([70], [150], 0)])
+def test_attention_in_place_from_any_float(dtype, rows, lens, shared):
+    """d_out = d_q, four bytes off any alignment."""
+    rng = np.random.default_rng(32)
+    c = M.Cache(rng, dtype, 2, 64, 16, rows, lens, shared=shared)
+    q = rng.standard_normal((c.n_rows, 4, 64)).astype(np.float32)
+    want = attend(c, q, 4, 0.125, shared)
+    pages, batch = c.upload()
+    buf = dev(np.concatenate([[5.0], q.ravel(), [6.0]]).astype(np.float32))
+    view = type("View", (), {})()
+    view.ptr = buf.ptr.value + 4
+    ws = uq.DeviceArray(serve.attn_paged_ws_bytes(pages, batch, 4, shared))
+    serve.attn_paged_d(view, view, pages, batch, 4, 0.125, ws, shared_len=shared)
+    got = host(buf, np.empty(q.size + 2, np.float32))
+    assert got[0] == 5.0 and got[-1] == 6.0
+    assert np.array_equal(got[1:-1].view(np.int32), want.ravel().view(np.int32))
+
+
+def test_two_calls_at_once():
+    """Two batches on two streams, each with its workspace, again and again: each call's bits are those it has alone."""
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(__file__))))
+    import bench
+    hip = bench.Hip()
+    streams = [hip.stream(), hip.stream()]
+    rng = np.random.default_rng(33)
+    work = []
+    for dtype, heads, kv, hd, rows, lens, shared in [("f16", 8, 2, 128, [1] * 5 + [60], [2000, 30, 500, 77, 900, 400], 0),
+                                                     ("f16", 16, 4, 256, [2] * 20, list(range(700, 720)), 690)]:
+        c = M.Cache(rng, dtype, kv, hd, 16, rows, lens, shared=shared)
+        q = rng.standard_normal((c.n_rows, heads, hd)).astype(np.float32)
+        want = attend(c, q, heads, 0.1, shared)
+        pages, batch = c.upload()
+        ws = uq.DeviceArray(serve.attn_paged_ws_bytes(pages, batch, heads, shared))
+        outs = [dev(np.zeros_like(q)) for _ in range(10)]
+        work.append((pages, batch, dev(q), outs, ws, heads, shared, want, c))
+    hip.sync()
+    for i in range(10):
+        for s, (pages, batch, dq, outs, ws, heads, shared, want, c) in zip(streams, work):
+            serve.attn_paged_d(outs[i], dq, pages, batch, heads, 0.1, ws, shared_len=shared, stream=s)
+    hip.sync()
+    for pages, batch, dq, outs, ws, heads, shared, want, c in work:
+        for o in outs:
+            assert np.array_equal(host(o, want).view(np.int32), want.view(np.int32))
+
+
+def test_two_graphs_share_a_workspace():
+    """Replayed in turn on one stream, with eager calls of the same workspace between: a call leaves nothing behind
+    that another needs."""
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(__file__))))
+    import bench
+    hip = bench.Hip()
+    s = hip.stream()
+    rng = np.random.default_rng(34)
+    work = []
+    for rows, lens, shared in [([1, 1, 1], [900, 33, 410], 0), ([40, 1], [300, 280], 256)]:
+        c = M.Cache(rng, "f16", 2, 128, 16, rows, lens, shared=shared)
+        q = rng.standard_normal((c.n_rows, 8, 128)).astype(np.float32)
+        want = attend(c, q, 8, 0.1, shared)
+        work.append((*c.upload(), dev(q), dev(np.zeros_like(q)), shared, want, c))
+    ws = uq.DeviceArray(max(serve.attn_paged_ws_bytes(w[0], w[1], 8, w[4]) for w in work))
+    ws.upload(np.full(ws.nbytes, 0xFF, np.uint8))
+
+    def step(w, stream):
+        serve.attn_paged_d(w[3], w[2], w[0], w[1], 8, 0.1, ws, shared_len=w[4], stream=stream)
+
+    hip.sync()
+    graphs = [hip.capture(s, lambda w=w: step(w, s)) for w in work]  # the kernels' first call for these shapes
+    for i in range(6):
+        w = work[i % 2]
+        w[3].upload(np.full(w[5].shape, 7.0, np.float32))
+        if i % 3 == 2:
+            step(work[1 - i % 2], None)
+        hip.sync()
+        hip.launch_graph(graphs[i % 2], s)
+        hip.sync()
+        assert np.array_equal(host(w[3], w[5]).view(np.int32), w[5].view(np.int32)), f"replay {i}"
 
 
 def test_attention_does_not_depend_on_the_other_sequences():
@@ -536,6 +716,35 @@ def test_verify_weights_that_are_none():
     p[4] = np.nan
     acc, nxt = run_verify(p, None, np.zeros(5), np.full(5, 0.9), [1] * 5)
     assert acc.tolist() == [0] * 5 and nxt.tolist() == [4000, 4000, -1, 4099, -1]
+
+
+def test_verify_captured():
+    """Replays follow the tokens, numbers, probabilities and row starts of the time."""
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(__file__))))
+    import bench
+    hip = bench.Hip()
+    s = hip.stream()
+    rng = np.random.default_rng(35)
+    vocab, n = 3001, 12
+    like = np.zeros(3, np.int32)
+    d_p, d_q, d_tok, d_u = (uq.DeviceArray(4 * k) for k in (n * vocab, n * vocab, n, n))
+    d_start, acc, nxt = dev(np.zeros(4, np.int32)), dev(like), dev(like)
+    batch = serve.SeqBatch(3, n, d_start)
+    ws = uq.DeviceArray(serve.draft_verify_ws_bytes(batch, vocab))
+    hip.sync()
+    g = hip.capture(s, lambda: serve.draft_verify_d(acc, nxt, d_p, d_q, d_tok, d_u, batch, vocab, ws, stream=s))
+    for rows in ([4, 4, 4], [1, 0, 8], [0, 0, 0], [12, 0, 0]):
+        p = probabilities(rng, n, vocab, 2.0)
+        q = probabilities(rng, n, vocab, 2.0) * 0.3 + p * 0.7
+        tok = np.array([rng.integers(0, vocab)] + [int(np.argmax(p[r] * rng.random(vocab))) for r in range(n - 1)], np.int32)
+        u = rng.random(n).astype(np.float32)
+        for d, a in ((d_p, p), (d_q, q), (d_tok, tok), (d_u, u), (d_start, np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))):
+            d.upload(a)
+        hip.sync()
+        hip.launch_graph(g, s)
+        hip.sync()
+        want = M.verify(p, q, tok, u, rows)
+        assert np.array_equal(host(acc, like), want[0]) and np.array_equal(host(nxt, like), want[1]), rows
 
 
 # ------------------------------------------------------------------------- together

@@ -100,6 +100,11 @@ def test_attention_refusals():
         assert need > 0
         refused("ARG", serve.attn_paged_d, A, A, p, b, 4, 1.0, At(nbytes=need - 1), shared_len=shared, text="workspace")
     refused("ARG", serve.attn_paged_d, A, A, p, batch(n_rows=1 << 24), 1 << 15, 1.0, A)
+    refused("ARG", serve.attn_paged_d, A, A, p, batch(n_rows=(1 << 23) + 2), 4, 1.0, A)  # a grid of 2^32 threads
+    assert serve.attn_paged_ws_bytes(p, batch(n_rows=1 << 15), 1 << 10) > 0
+    refused("ARG", serve.attn_paged_d, A, A, p, batch(n_rows=(1 << 15) + 1), 1 << 10, 1.0, A, text="2^25")
+    for scale in (float("nan"), float("inf"), -float("inf")):
+        refused("ARG", serve.attn_paged_d, A, A, p, b, 4, scale, A, text="kq_scale")
 
 
 def test_verification_refusals():

@@ -429,7 +429,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
         }
         wait_vm_barrier<0>();
 
-        // ---- values that are not finite, left out by store_values because a query that may not see them would take
+        // ---- values that are not finite, left out by mend_values because a query that may not see them would take
         // 0 * NaN from them: for the queries that see them (any weight: the sum is infinite or NaN all the same)
         if (unfinite && active) {
             for (int t = 0; t < count; t++) {

@@ -107,7 +107,7 @@ __device__ __forceinline__ int seen_to(const Work &w, int rows) {
 }
 template <int U>
 __device__ __forceinline__ int seen_units(const AttnArgs &A, const Work &w, int rb) {
-    return seen_to<U>(w, ((rb + 1) * A.part[1].rows - 1) / A.group + 1);  // below 2^30: n_rows n_head is below 2^29
+    return seen_to<U>(w, ((rb + 1) * A.part[1].rows - 1) / A.group + 1);  // below 2^26: n_rows n_head is at most 2^25
 }
 // Their sum over the blocks, without a division a block; `more` for each with any.
 template <int U>

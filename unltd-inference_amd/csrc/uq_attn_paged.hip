@@ -402,8 +402,8 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
               // A query that may not see them would have taken 0 * NaN from them; those that do take them now (any
               // weight: the sum is infinite or NaN all the same).
               for (int it = wave; it < count; it += kWaves)
-                  for (int y = 0; y < NP; y++) {
-                      const int pos = w.base + (un + it) * NP + y;
+                  for (int x = 0; x < NP; x++) {
+                      const int pos = w.base + (un + it) * NP + x;
                       const int pg = pos < end ? table[pos >> map.log2_page] : -1;
                       if (!page_ok(map, pg)) continue;
                       const E *vp = V + (size_t)page_row(map, pg, kvh, pos) * HD;
@@ -680,7 +680,7 @@ hipError_t launch_few(const AttnArgs &A, hipStream_t s) {
 
 template <int HD>
 hipError_t join(const AttnArgs &A, hipStream_t s) {
-    const int pairs = A.b.n_rows * A.a.n_head;  // below 2^29
+    const int pairs = A.b.n_rows * A.a.n_head;  // at most 2^25
     if (pairs > 16 * kCUs)
         hipLaunchKernelGGL((attn_join_kernel<HD, 1>), dim3((unsigned)((pairs + 3) / 4)), dim3(256), 0, s, A, pairs);
     else if (pairs > 4 * kCUs)

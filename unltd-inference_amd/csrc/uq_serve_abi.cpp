@@ -1,6 +1,7 @@
 // C ABI of batched serving (include/uq_serve.h): argument checks, then the
 // launches of uq_serve.hip and uq_attn_paged.hip.
 #include <climits>
+#include <cmath>
 #include <cstdint>
 
 #include "uq_internal.h"
@@ -18,8 +19,10 @@ namespace {
 
 uq_status hip_st(hipError_t e, const char *what) { return e == hipSuccess ? UQ_OK : uq::hip_error(e, what); }
 
-constexpr size_t kMaxRows = 1u << 24;  // rows and sequences of a call: well inside 32-bit grids and indexes
+constexpr size_t kMaxRows = 1u << 23;  // of a call: a grid of 256 threads each stays below 2^32
 constexpr size_t kMaxSeqs = 65535;     // a grid dimension of the verification
+constexpr size_t kMaxPairs = 1u << 25; // rows times heads of the attention: a grid of 64 threads each, likewise
+constexpr size_t kMaxVocab = 1u << 24;
 
 // need_len: the call reads lengths and pages as well as row starts.
 uq_status view_batch(const char *fn, const uq_seq_batch *b, bool need_len, uq::BatchView *v) {
@@ -73,8 +76,8 @@ uq_status view_attn(const char *fn, const uq_kv_pages *kv, const uq_seq_batch *b
                     uq::PagesView *pv, uq::BatchView *bv) {
     UQ_TRY(view_pages(fn, kv, b, pv, bv));
     UQ_TRY(check_heads(fn, n_head, *pv));
-    if (b->n_rows * n_head > (size_t)INT_MAX / 4)
-        return set_error(UQ_ERR_ARG, "%s: %zu rows of %zu heads above 2^29", fn, b->n_rows, n_head);
+    if (b->n_rows * n_head > kMaxPairs)
+        return set_error(UQ_ERR_ARG, "%s: %zu rows of %zu heads above 2^25", fn, b->n_rows, n_head);
     if (shared_len > b->max_pages * kv->page_size)
         return set_error(UQ_ERR_ARG, "%s: shared_len %zu beyond a table of %zu positions", fn, shared_len,
                          b->max_pages * kv->page_size);
@@ -134,6 +137,7 @@ uq_status uq_attn_paged_d(float *d_out, const float *d_q, const uq_kv_pages *kv,
     uq::PagesView pv;
     uq::BatchView bv;
     UQ_TRY(view_attn(fn, kv, batch, n_head, shared_len, &pv, &bv));
+    if (!std::isfinite(kq_scale)) return set_error(UQ_ERR_ARG, "%s: kq_scale is not finite", fn);
     if (batch->n_rows == 0 || batch->n_seqs == 0) return UQ_OK;
     if (!d_out || !d_q || !d_ws) return set_error(UQ_ERR_ARG, "%s: null device pointer", fn);
     if ((uintptr_t)d_ws % 16) return set_error(UQ_ERR_ARG, "%s: the workspace is not 16-byte aligned", fn);
@@ -145,7 +149,7 @@ uq_status uq_attn_paged_d(float *d_out, const float *d_q, const uq_kv_pages *kv,
 
 size_t uq_draft_verify_ws_bytes(const uq_seq_batch *batch, size_t vocab) {
     uq::BatchView bv;
-    if (view_batch("draft_verify_ws_bytes", batch, false, &bv) || vocab == 0 || vocab > kMaxRows) return 0;
+    if (view_batch("draft_verify_ws_bytes", batch, false, &bv) || vocab == 0 || vocab > kMaxVocab) return 0;
     return uq::draft_verify_ws_bytes(bv.n_seqs, (int)vocab);
 }
 
@@ -155,7 +159,7 @@ uq_status uq_draft_verify_d(int32_t *d_accepted, int32_t *d_next, const float *d
     const char *fn = "draft_verify_d";
     uq::BatchView bv;
     UQ_TRY(view_batch(fn, batch, false, &bv));
-    if (vocab == 0 || vocab > kMaxRows) return set_error(UQ_ERR_ARG, "%s: vocab %zu outside 1 .. 2^24", fn, vocab);
+    if (vocab == 0 || vocab > kMaxVocab) return set_error(UQ_ERR_ARG, "%s: vocab %zu outside 1 .. 2^24", fn, vocab);
     if (p_row < vocab || (d_q && q_row < vocab))
         return set_error(UQ_ERR_LEN, "%s: a row stride (%zu, %zu) below vocab %zu", fn, p_row, q_row, vocab);
     if (bv.n_seqs == 0) return UQ_OK;
