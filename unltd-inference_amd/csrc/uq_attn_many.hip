@@ -461,7 +461,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
             // by way of LDS, 128 values of the 32 queries at a time, to store them row by row
             const int idx = done ? at_q
                             : whole ? (int)rec_whole(A, seq >= 0, 0, 0) + at_q
-                                    : (int)rec_part(A.part[seq >= 0], (int)blockIdx.x, starts, mine);
+                                    : (int)rec_part(A.part[seq >= 0], X.me, starts, mine);
             const float mul = !done ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             if (!done && in && h == 0) A.rec_al[idx] = make_float2(a, l);
             float *const dst = done ? A.a.out : A.rec_o;
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
         if (starts && tid < nq) {  // a block has half as many queries as the workgroup threads
             const int num = rb * RB + tid;
             put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
-                    done ? kDone : whole ? kWhole : (int)blockIdx.x,
+                    done ? kDone : whole ? kWhole : X.me,
                     done || whole ? 0 : X.last(), tid);
         }
     }

@@ -81,20 +81,17 @@ struct Work {
 };
 
 template <int U>
-__device__ __forceinline__ Work work_of(const AttnArgs &A, int s) {
-    Work w;
+__device__ __forceinline__ Work work_of(const AttnArgs &A, int s, const SeqRows &r, int len) {
     const int cap = A.b.max_pages << A.kv.map.log2_page;
-    if (s < 0) {
-        const SeqRows r = seq_rows(0, A.b.row_start[A.b.n_seqs], A.b.n_rows);
-        w = Work{r.lo, r.n, 0, 0, A.a.shared_len, 0, 0};
-    } else {
-        const SeqRows r = seq_rows(A.b.row_start[s], A.b.row_start[s + 1], A.b.n_rows);
-        const int len = A.b.len[s];
-        w = Work{r.lo, r.n, len, A.a.shared_len, seq_len(len, cap), 0, 0};
-    }
+    Work w = s < 0 ? Work{r.lo, r.n, 0, 0, A.a.shared_len, 0, 0} : Work{r.lo, r.n, len, A.a.shared_len, seq_len(len, cap), 0, 0};
     w.units = w.end > w.base ? (w.end - w.base + U - 1) / U : 0;
     w.blocks = blocks_of(w.n, A.group, A.part[s >= 0].rows);
     return w;
+}
+template <int U>
+__device__ __forceinline__ Work work_of(const AttnArgs &A, int s) {
+    if (s < 0) return work_of<U>(A, s, seq_rows(0, A.b.row_start[A.b.n_seqs], A.b.n_rows), 0);
+    return work_of<U>(A, s, seq_rows(A.b.row_start[s], A.b.row_start[s + 1], A.b.n_rows), A.b.len[s]);
 }
 
 // The units of a block of a sequence's own positions up to the last one that
@@ -135,7 +132,15 @@ __device__ __forceinline__ long long uniform(long long v) {
 // of a KV head counts OVER units beside its units of U positions: what its
 // start and end cost, so that a run with two of them has less else to do.
 // They lie before the units; a run that ends among them leaves the block to
-// the next one. What find reads are all row starts and lengths, by every
+// the next one.
+//
+// The shared positions by themselves are `blocks` alike, and where the
+// workgroups divide well among them every run lies in one block of one KV
+// head, and the runs of all blocks over the same positions go to one XCD at a
+// time (workgroup i runs on XCD i % 8), whose L2 then reads each tile once:
+// XXX
+//
+// What find reads are all row starts and lengths, by every
 // workgroup: one round trip to the L2, where another kernel for a plan would
 // cost a launch.
 struct WalkLds {
@@ -144,7 +149,8 @@ struct WalkLds {
 };
 template <int TPB, int U, int OVER>
 struct Walk {
-    int runs, seq, rb, units;  // runs of all workgroups; where the next block is looked for
+    int runs, me, over;        // runs of all workgroups, this one's; units counted for a block's start and end
+    int seq, rb, units;        // where the next block is looked for
     long long T, u, u1, off;   // all units, the rest of this run, the next unit's place among its block's (all KV heads)
     Work w;
     // the block at hand
@@ -155,8 +161,8 @@ struct Walk {
     __device__ __forceinline__ int units_of(const AttnArgs &A, int b) const {
         return seq < 0 ? w.units : seen_units<U>(A, w, b);
     }
-    __device__ __forceinline__ static long long cost(const AttnArgs &A, int n) {
-        return n > 0 ? (long long)A.kv.n_head_kv * (n + OVER) : 0;
+    __device__ __forceinline__ static long long cost(const AttnArgs &A, int n, int over) {
+        return n > 0 ? (long long)A.kv.n_head_kv * (n + over) : 0;
     }
     // Units before item c + tid and its own (of items c .. c + TPB - 1 with value(i) each); returns those up to c + TPB
     template <class Value>
@@ -188,22 +194,38 @@ struct Walk {
             if (i > 0 ? A.last == 0 : A.first == 1) return 0LL;
             mine_w = work_of<U>(A, i - 1);
             if (mine_w.units == 0) return 0LL;
-            return i == 0 ? cost(A, mine_w.units) * mine_w.blocks : A.kv.n_head_kv * seen_sum<U>(A, mine_w, OVER);
+            return i == 0 ? cost(A, mine_w.units, OVER) * mine_w.blocks : A.kv.n_head_kv * seen_sum<U>(A, mine_w, OVER);
         };
         long long mine = 0, before = 0, run = 0;
         T = 0;
         for (int c = 0; c < parts; c += TPB) T = scan(lds, c, parts, T, mine, before, value);
         T = uniform(T);
         runs = (int)min((long long)A.part[A.first].G, T);  // no empty runs between others
-        if ((int)blockIdx.x >= runs) return false;
-        u = run_start(T, runs, (int)blockIdx.x);
-        u1 = run_start(T, runs, (int)blockIdx.x + 1);
+        me = (int)blockIdx.x;
+        over = OVER;
+        if (A.last == 0) {
+            const Work all = work_of<U>(A, -1);
+            const int nkv = A.kv.n_head_kv, of = 8 / min(8, nkv & -nkv);  // J * nkv is a multiple of 8
+            const int J = all.blocks == 0 || all.blocks > runs / nkv ? 0 : min(all.units, runs / (nkv * all.blocks)) / of * of;
+            if (J > 0 && all.units / J <= T / runs + OVER) {
+                over = 0;
+                T = (long long)all.blocks * nkv * all.units;
+                runs = J * nkv * all.blocks;
+                const int i = me >> 3, at = i / all.blocks * 8 + (me & 7);  // the positions' run among all KV heads'
+                me = me < runs ? i % all.blocks * nkv * J + at : runs;
+                run = 0;
+                mine = threadIdx.x == 0 ? T : 0, before = 0, mine_w = all;
+            }
+        }
+        if (me >= runs) return false;
+        u = run_start(T, runs, me);
+        u1 = run_start(T, runs, me + 1);
         auto keep = [&](int i) {
             lds.index = i - 1, lds.off = u - before;
             lds.work[0] = mine_w.lo, lds.work[1] = mine_w.n, lds.work[2] = mine_w.len, lds.work[3] = mine_w.base;
             lds.work[4] = mine_w.end, lds.work[5] = mine_w.units, lds.work[6] = mine_w.blocks;
         };
-        if (parts <= TPB) {
+        if (parts <= TPB || over == 0) {
             if (mine > 0 && before <= u && u < before + mine) keep(tid);
         } else {
             for (int c = 0; c < parts; c += TPB) {
@@ -220,7 +242,7 @@ struct Walk {
         if (w.blocks > 1) {  // the block, likewise
             run = 0;
             for (int c = 0; c < w.blocks; c += TPB) {
-                run = scan(lds, c, w.blocks, run, mine, before, [&](int b) { return cost(A, units_of(A, b)); });
+                run = scan(lds, c, w.blocks, run, mine, before, [&](int b) { return cost(A, units_of(A, b), over); });
                 if (mine > 0 && before <= off && off < before + mine) lds.index = c + tid, lds.off = off - before;
                 if (off < run) break;  // the same for every thread
             }
@@ -234,7 +256,7 @@ struct Walk {
     // The next block with units of this run; false: none.
     __device__ __forceinline__ bool next(const AttnArgs &A) {
         while (u < u1) {
-            const int each = units > 0 ? units + OVER : 0;
+            const int each = units > 0 ? units + over : 0;
             if (off >= (long long)A.kv.n_head_kv * each) {
                 off -= (long long)A.kv.n_head_kv * each;
                 if (++rb >= w.blocks) {
@@ -249,8 +271,8 @@ struct Walk {
             }
             kvh = off >> 31 ? (int)(off / each) : (int)off / each;
             const int at = (int)(off - (long long)kvh * each), upto = (int)min((long long)each, at + (u1 - u));
-            un = max(0, at - OVER);
-            count = max(0, upto - OVER) - un;
+            un = max(0, at - over);
+            count = max(0, upto - over) - un;
             starts = un == 0, ends = upto == each;
             end = u + each - at - 1;
             u += upto - at;

@@ -477,7 +477,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                 }
                 *(f4u *)(A.a.out + ((size_t)row * A.a.n_head + head) * HD + d) = y;
             } else {
-                const size_t rec = whole ? rec_whole(A, seq >= 0, row, head) : rec_part(A.part[seq >= 0], (int)blockIdx.x, starts, r);
+                const size_t rec = whole ? rec_whole(A, seq >= 0, row, head) : rec_part(A.part[seq >= 0], X.me, starts, r);
                 *(f4 *)(A.rec_o + rec * HD + d) = o;
                 if (d == 0) A.rec_al[rec] = make_float2(ar, lr);
             }
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
         if (starts && tid < nq) {
             const int num = rb * ROWS + tid;
             put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
-                    done ? kDone : whole ? kWhole : (int)blockIdx.x, done || whole ? 0 : X.last(), tid);
+                    done ? kDone : whole ? kWhole : X.me, done || whole ? 0 : X.last(), tid);
         }
     }
 }
@@ -509,16 +509,23 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
     int2 sg[2];
 #pragma unroll
     for (int c = 0; c < 2; c++) sg[c] = A.seg[((size_t)c * A.b.n_rows + row) * A.a.n_head + head];
-    int seq = -1;
+    int seq = -1, len = 0;
+    SeqRows its{0, 0};
     for (int i0 = 0; i0 < A.b.n_seqs && seq < 0; i0 += 64) {
         const int i = i0 + lane;
-        bool mine = false;
+        SeqRows r{0, 0};
+        int l = 0;
         if (i < A.b.n_seqs) {
-            const SeqRows r = seq_rows(A.b.row_start[i], A.b.row_start[i + 1], A.b.n_rows);
-            mine = row >= r.lo && row < r.lo + r.n;
+            r = seq_rows(A.b.row_start[i], A.b.row_start[i + 1], A.b.n_rows);
+            l = A.b.len[i];
         }
-        const unsigned long long any = __ballot(mine);
-        if (any) seq = i0 + __builtin_ctzll(any);
+        const unsigned long long any = __ballot(row >= r.lo && row < r.lo + r.n);
+        if (any) {
+            const int at = __builtin_ctzll(any);
+            seq = i0 + at;
+            its = SeqRows{__builtin_amdgcn_readlane(r.lo, at), __builtin_amdgcn_readlane(r.n, at)};
+            len = __builtin_amdgcn_readlane(l, at);
+        }
     }
     if (seq < 0) return;
     // the two parts: records first .. first + count - 1 of workgroups, or one whole record
@@ -527,7 +534,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
     for (int c = 0; c < 2; c++) {
         if (c == 0 && A.a.shared_len == 0) continue;
         if (c == 1) {
-            const Work w = work_of<1>(A, seq);
+            const Work w = work_of<1>(A, seq, its, len);
             const int num = (row - w.lo) * A.group + head % A.group;
             if (w.units == 0 || seen_units<1>(A, w, num / A.part[1].rows) == 0) continue;
         }
@@ -544,8 +551,10 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
     };
     const int begin = WAVES == 1 ? 0 : wave;
     // the references of 64 records of this wave at a time
-    float amin = INFINITY;
-    for (int i = begin + WAVES * lane; i < total; i += 64 * WAVES) amin = fminf(amin, A.rec_al[rec(i)].x);
+    const int at0 = begin + WAVES * lane;
+    const float2 al0 = at0 < total ? A.rec_al[rec(at0)] : make_float2(INFINITY, 0.0f);
+    float amin = al0.x;
+    for (int i = at0 + 64 * WAVES; i < total; i += 64 * WAVES) amin = fminf(amin, A.rec_al[rec(i)].x);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) amin = fminf(amin, __shfl_xor(amin, d));
     if constexpr (WAVES > 1) {
@@ -561,7 +570,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
         const int mine = i0 + WAVES * lane;
         float f = 0.0f;
         if (mine < total) {
-            const float2 al = A.rec_al[rec(mine)];
+            const float2 al = i0 == begin ? al0 : A.rec_al[rec(mine)];
             f = al.x == INFINITY ? 0.0f : exp2_hw(amin - al.x);
             l += f * al.y;
         }
@@ -622,7 +631,7 @@ struct Plan {
 //    positions: 23 | 37; 12000: 43 | 50; 20000: 65 | 61).
 int block_rows(const PagesView &kv, size_t R, int n_seqs, int shared) {
     if (R <= 16 || kv.head_dim == 512) return 16;
-    if (R > 32 && attn_many_ok(kv)) return (R + 127) / 128 * 128 == (R + 63) / 64 * 64 ? 128 : 64;
+    if (R > 32 && attn_many_ok(kv)) return R > 64 ? 128 : 64;
     if (!kv.f16 && kv.head_dim == 256 && n_seqs > 2) return 16;
     const size_t tiles = (R + 15) / 16 * kv.n_head_kv * ((size_t)shared / (kv.f16 ? 32 : 16));
     return shared && tiles < 32 * 2 * kCUs ? 16 : 32;

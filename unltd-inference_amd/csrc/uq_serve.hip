@@ -310,108 +310,108 @@ __global__ __launch_bounds__(kVerTPB) void verify_sum_kernel(VerifyArgs a) {
     }
 }
 
-// Inclusive sum of v over the workgroup's threads in thread order (wave scan,
-// then the waves before); total: the last thread's. Three barriers.
-__device__ __forceinline__ double block_scan_d(double v, double *red, double *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double up = __shfl_up(v, d);
-        if (lane >= d) v += up;
-    }
-    if (lane == 63) red[wave] = v;
-    __syncthreads();
-    double before = 0.0, t = 0.0;
-    for (int i = 0; i < kVerTPB / 64; i++) {
-        if (i == wave) before = t;
-        t += red[i];
-    }
-    __syncthreads();
-    *total = t;
-    return before + v;
+// Inclusive sum of v over the wave's lanes in their order (a fixed tree: rows of 16, then the rows before).
+__device__ __forceinline__ double wave_scan_d(double v) {
+    v += dpp_d<0x111>(v);       // row_shr:1
+    v += dpp_d<0x112>(v);       // row_shr:2
+    v += dpp_d<0x114>(v);       // row_shr:4
+    v += dpp_d<0x118>(v);       // row_shr:8
+    v += dpp_d<0x142, 0xA>(v);  // row_bcast:15 into rows 1, 3
+    v += dpp_d<0x143, 0xC>(v);  // row_bcast:31 into rows 2, 3
+    return v;
 }
 
-// One workgroup a sequence: the chunk that the threshold falls in, then the
-// token in it. Rounded running sums need not ascend where a weight is zero or
-// at the joints of the tree, so a token needs weight of its own to be drawn,
-// and where no sum exceeds the threshold the last one with weight is it.
-__global__ __launch_bounds__(kVerTPB) void verify_draw_kernel(VerifyArgs a) {
-    __shared__ int hit, last, chunk_s;
-    __shared__ double red[kVerTPB / 64];
-    __shared__ double base_s;
-    const int s = blockIdx.x, tid = threadIdx.x;
-    // every thread a run of chunks; loads before anything waits for one
+// Where a lane's run of weights passes the threshold: the first with weight whose sum exceeds it, or else the last
+// with weight.
+struct Passed {
+    int at;       // -1: no weight
+    double base;  // the sum before it
+    bool over;
+};
+__device__ __forceinline__ void pass(Passed &o, double &run, int i, double w, double thr) {
+    if (o.over || !(w > 0.0)) return;
+    o.at = i;
+    o.base = run;
+    run += w;
+    o.over = run > thr;
+}
+// The lane that holds the draw; -1: no weight in any.
+__device__ __forceinline__ int drawing_lane(const Passed &o) {
+    const unsigned long long over = __ballot(o.over), some = __ballot(o.at >= 0);
+    return over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
+}
+
+// One wave a sequence: the chunk that the threshold falls in, then the token
+// in it. Rounded running sums need not ascend where a weight is zero or at the
+// joints of the tree, so a token needs weight of its own to be drawn, and
+// where no sum exceeds the threshold the last one with weight is it. The
+// time is round trips (the chunks' sums; the refused token; its chunk of p and
+// q): a wave needs no barriers between them (five sequences of
+// 152064 tokens: XXX us; a workgroup of four waves: 10).
+constexpr int kKeep = 8;  // chunks' sums of a lane kept in registers: a vocabulary of 2^18
+__global__ __launch_bounds__(64) void verify_draw_kernel(VerifyArgs a) {
+    const int s = blockIdx.x, lane = threadIdx.x;
+    // every lane a run of chunks; loads before anything waits for one
     const double2 *sums = a.sums + (size_t)s * a.chunks;
-    const int per = (a.chunks + kVerTPB - 1) / kVerTPB, c0 = min(a.chunks, tid * per), c1 = min(a.chunks, c0 + per);
-    double2 t = make_double2(0.0, 0.0);
-    for (int c = c0; c < c1; c++) t.x += sums[c].x, t.y += sums[c].y;  // a sequence without rows: of anything, not used
+    const int per = (a.chunks + 63) / 64, c0 = min(a.chunks, lane * per), c1 = min(a.chunks, c0 + per);
+    double2 keep[kKeep], t = make_double2(0.0, 0.0);
+#pragma unroll
+    for (int i = 0; i < kKeep; i++) keep[i] = c0 + i < c1 ? sums[c0 + i] : make_double2(0.0, 0.0);
     const int4 head = a.heads[s];
+#pragma unroll
+    for (int i = 0; i < kKeep; i++) t.x += keep[i].x, t.y += keep[i].y;  // a sequence without rows: of anything, not used
+    for (int c = c0 + kKeep; c < c1; c++) t.x += sums[c].x, t.y += sums[c].y;
     const SeqRows r{head.x, head.y};
-    const int accepted = head.z;
-    if (tid == 0) a.accepted[s] = accepted;
+    if (lane == 0) a.accepted[s] = head.z;
     if (r.n == 0) {
-        if (tid == 0) a.next[s] = -1;
+        if (lane == 0) a.next[s] = -1;
         return;
     }
+    const Row o = row_at(a, r, head.z);
+    double inc = wave_scan_d(t.x), total = __shfl(inc, 63);
+    const bool plain = !(total > 0.0);  // no weight after the refusal: p itself
+    if (plain) inc = wave_scan_d(t.y), total = __shfl(inc, 63);
     double u = (double)__int_as_float(head.w);
-    if (tid == 0) hit = INT_MAX, last = -1;
-    double total;
-    double inc = block_scan_d(t.x, red, &total);  // its barriers publish hit and last
-    const bool plain = !(total > 0.0);            // no weight after the refusal: p itself
-    if (plain) inc = block_scan_d(t.y, red, &total);
-    const double mine = plain ? t.y : t.x;
     u = u >= 0.0 ? u : u < 0.0 ? 0.0 : 1.0;  // NaN as 1
     const double thr = u >= 1.0 ? (double)INFINITY : u * total;
-    if (mine > 0.0) {
-        atomicMax(&last, tid);
-        if (inc > thr) atomicMin(&hit, tid);
-    }
-    __syncthreads();
-    if (last < 0) {
-        if (tid == 0) a.next[s] = -1;
+    Passed chunk{-1, 0.0, false};
+    double run = inc - (plain ? t.y : t.x);
+#pragma unroll
+    for (int i = 0; i < kKeep; i++) pass(chunk, run, c0 + i, plain ? keep[i].y : keep[i].x, thr);
+    for (int c = c0 + kKeep; c < c1; c++) pass(chunk, run, c, plain ? sums[c].y : sums[c].x, thr);
+    int from = drawing_lane(chunk);
+    if (from < 0) {
+        if (lane == 0) a.next[s] = -1;
         return;
     }
-    const int owner = hit != INT_MAX ? hit : last;
-    __syncthreads();
-    if (tid == owner) {  // the chunk in the run
-        double run = inc - mine, base = run;
-        int found = c0;
-        for (int c = c0; c < c1; c++) {
-            const double v = plain ? sums[c].y : sums[c].x;
-            if (!(v > 0.0)) continue;
-            found = c;
-            base = run;
-            run += v;
-            if (run > thr) break;
-        }
-        base_s = base;
-        chunk_s = found;
-        hit = INT_MAX;
-        last = -1;
-    }
-    __syncthreads();
-    // the token in the chunk: two neighbours a thread
-    const Row o = row_at(a, r, accepted);
+    // the chunk's tokens: eight neighbours a lane
     const float *p = a.p + o.row * a.p_row, *q = a.q && !o.ended ? a.q + o.row * a.q_row : p;
-    const int x0 = chunk_s * kVerChunk + 2 * tid;
-    double w[2];
+    const int x0 = __shfl(chunk.at, from) * kVerChunk + 8 * lane;
+    float vp[8], vq[8];
+    if (x0 + 8 <= a.vocab) {
+        load_row<8>(vp, p + x0);
+        load_row<8>(vq, q + x0);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int x = x0 + j;
-        const double2 v = x < a.vocab ? weights(a, o, x, p[x], q[x]) : make_double2(0.0, 0.0);
-        w[j] = plain ? v.y : v.x;
+        for (int e = 0; e < 8; e++) {
+            vp[e] = x0 + e < a.vocab ? p[x0 + e] : 0.0f;
+            vq[e] = x0 + e < a.vocab ? q[x0 + e] : 0.0f;
+        }
     }
-    const double upto = base_s + block_scan_d(w[0] + w[1], red, &total);
-    if (w[1] > 0.0) {
-        atomicMax(&last, x0 + 1);
-        if (upto > thr) atomicMin(&hit, x0 + 1);
+    double w[8], mine = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const double2 v = weights(a, o, x0 + e, vp[e], vq[e]);
+        w[e] = plain ? v.y : v.x;
+        mine += w[e];
     }
-    if (w[0] > 0.0) {
-        atomicMax(&last, x0);
-        if (upto - w[1] > thr) atomicMin(&hit, x0);
-    }
-    __syncthreads();
-    if (tid == 0) a.next[s] = hit != INT_MAX ? hit : last;
+    Passed token{-1, 0.0, false};
+    run = __shfl(chunk.base, from) + (wave_scan_d(mine) - mine);
+#pragma unroll
+    for (int e = 0; e < 8; e++) pass(token, run, x0 + e, w[e], thr);
+    from = drawing_lane(token);
+    const int drawn = __shfl(token.at, max(from, 0));
+    if (lane == 0) a.next[s] = drawn;
 }
 
 }  // namespace
@@ -454,7 +454,7 @@ hipError_t launch_draft_verify(int32_t *accepted, int32_t *next, const float *p,
     const int per = kVerTPB / 64 * run;
     hipLaunchKernelGGL(verify_sum_kernel, dim3((unsigned)((chunks + per - 1) / per), (unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
     if (hipError_t e = hipGetLastError()) return e;
-    hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)b.n_seqs), dim3(kVerTPB), 0, s, a);
+    hipLaunchKernelGGL(verify_draw_kernel, dim3((unsigned)b.n_seqs), dim3(64), 0, s, a);
     return hipGetLastError();
 }
 
