@@ -17,23 +17,6 @@ __device__ __forceinline__ float half_max(float v) {  // over the lanes l, l ^ 3
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The largest of the bit patterns of LANES neighbouring lanes (16, 32 or 64), in all of them.
-template <int LANES>
-__device__ __forceinline__ uint32_t group_max(uint32_t v) {
-    v = max(v, dpp_u<0xB1>(v));   // quad_perm [1,0,3,2]
-    v = max(v, dpp_u<0x4E>(v));   // quad_perm [2,3,0,1]
-    v = max(v, dpp_u<0x141>(v));  // row_half_mirror
-    v = max(v, dpp_u<0x140>(v));  // row_mirror
-    if constexpr (LANES >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-        v = max(r[0], r[1]);
-    }
-    if constexpr (LANES == 64) {
-        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-        v = max(r[0], r[1]);
-    }
-    return v;
-}
 // What a wave wrote to LDS, it may read.
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -118,8 +101,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
         const bool in = mine < nq;
         const int lim = row_lim[mine];
         int lim_min = in ? lim : INT_MAX;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, d));
+        lim_min = lanes_min<32>(lim_min);
         if (lane == 0) red[wave] = lim_min;
 
         // ---- tiles t = 0 .. count - 1 of positions p0 + NP t
@@ -162,7 +144,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
                     uint32_t top = 0;
 #pragma unroll
                     for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
-                    top = group_max<LQ>(top);
+                    top = lanes_max<LQ>(top);
                     // |q| < 2^ex; not finite: left as it is, its terms are not finite either
                     const int ex = top > 0 && top < 0x7F800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 15;
                     const int ex_n = __shfl(ex, (n & (RL - 1)) * LQ);  // of query n, where it is of this load

@@ -128,6 +128,59 @@ __device__ __forceinline__ long long uniform(long long v) {
     return (long long)((unsigned long long)hi << 32 | lo);
 }
 
+// Inclusive sum over the wave's lanes, and a reduction over LANES neighbouring lanes (16, 32 or 64) in all of them,
+// without a round trip to the LDS.
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ long long dpp_l(long long v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROW_MASK, 0xF, true);
+    return (long long)hi << 32 | lo;
+}
+__device__ __forceinline__ long long wave_scan_l(long long v) {
+    v += dpp_l<0x111>(v);       // row_shr:1
+    v += dpp_l<0x112>(v);       // row_shr:2
+    v += dpp_l<0x114>(v);       // row_shr:4
+    v += dpp_l<0x118>(v);       // row_shr:8
+    v += dpp_l<0x142, 0xA>(v);  // row_bcast:15 into rows 1, 3
+    v += dpp_l<0x143, 0xC>(v);  // row_bcast:31 into rows 2, 3
+    return v;
+}
+template <int LANES, class Op>
+__device__ __forceinline__ uint32_t lanes_of(uint32_t v, Op op) {
+    v = op(v, dpp_u<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = op(v, dpp_u<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = op(v, dpp_u<0x141>(v));  // row_half_mirror
+    v = op(v, dpp_u<0x140>(v));  // row_mirror
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    if constexpr (LANES == 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = op(r[0], r[1]);
+    }
+    return v;
+}
+// The largest bit pattern; the least signed integer; the least float.
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    return lanes_of<LANES>(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+template <int LANES>
+__device__ __forceinline__ int lanes_min(int v) {
+    return (int)lanes_of<LANES>((uint32_t)v, [](uint32_t a, uint32_t b) { return (uint32_t)min((int)a, (int)b); });
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_min(float v) {
+    return __uint_as_float(lanes_of<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fminf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ long long lane_of(long long v, int lane) {
+    return (long long)lane_of((int)(v >> 32), lane) << 32 | (unsigned)lane_of((int)v, lane);
+}
+
 // The walk of a workgroup of TPB threads over its run of the work. Every block
 // of a KV head counts OVER units beside its units of U positions: what its
 // start and end cost, so that a run with two of them has less else to do.
@@ -170,12 +223,7 @@ struct Walk {
                                                      Value value) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         mine = c + tid < n ? value(c + tid) : 0;
-        long long inc = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const long long up = __shfl_up(inc, d);
-            if (lane >= d) inc += up;
-        }
+        const long long inc = wave_scan_l(mine);
         __syncthreads();
         if (lane == 63) lds.scan[wave] = inc;
         __syncthreads();
@@ -187,8 +235,10 @@ struct Walk {
         }
         return run;
     }
+    // Few sequences (and few blocks of one): every wave looks by itself, and there is no barrier.
     __device__ bool find(const AttnArgs &A, WalkLds &lds) {
-        const int tid = threadIdx.x, parts = A.b.n_seqs + 1;
+        const int tid = threadIdx.x, lane = tid & 63, parts = A.b.n_seqs + 1;
+        const bool few = parts <= 64;
         Work mine_w{};
         auto value = [&](int i) {
             if (i > 0 ? A.last == 0 : A.first == 1) return 0LL;
@@ -198,8 +248,15 @@ struct Walk {
         };
         long long mine = 0, before = 0, run = 0;
         T = 0;
-        for (int c = 0; c < parts; c += TPB) T = scan(lds, c, parts, T, mine, before, value);
-        T = uniform(T);
+        if (few) {
+            mine = lane < parts ? value(lane) : 0;
+            const long long inc = wave_scan_l(mine);
+            before = inc - mine;
+            T = lane_of(inc, 63);
+        } else {
+            for (int c = 0; c < parts; c += TPB) T = scan(lds, c, parts, T, mine, before, value);
+            T = uniform(T);
+        }
         runs = (int)min((long long)A.part[A.first].G, T);  // no empty runs between others
         me = (int)blockIdx.x;
         over = OVER;
@@ -213,42 +270,59 @@ struct Walk {
                 runs = J * nkv * all.blocks;
                 const int i = me >> 3, at = i / all.blocks * 8 + (me & 7);  // the positions' run among all KV heads'
                 me = me < runs ? i % all.blocks * nkv * J + at : runs;
-                run = 0;
-                mine = threadIdx.x == 0 ? T : 0, before = 0, mine_w = all;
             }
         }
         if (me >= runs) return false;
         u = run_start(T, runs, me);
         u1 = run_start(T, runs, me + 1);
-        auto keep = [&](int i) {
-            lds.index = i - 1, lds.off = u - before;
-            lds.work[0] = mine_w.lo, lds.work[1] = mine_w.n, lds.work[2] = mine_w.len, lds.work[3] = mine_w.base;
-            lds.work[4] = mine_w.end, lds.work[5] = mine_w.units, lds.work[6] = mine_w.blocks;
-        };
-        if (parts <= TPB || over == 0) {
-            if (mine > 0 && before <= u && u < before + mine) keep(tid);
+        if (A.last == 0) {
+            seq = -1;
+            off = u;
+            w = work_of<U>(A, -1);
+            w = Work{uniform(w.lo), uniform(w.n), uniform(w.len), uniform(w.base), uniform(w.end), uniform(w.units), uniform(w.blocks)};
+        } else if (few) {
+            const int at = __builtin_ctzll(__ballot(mine > 0 && before <= u && u < before + mine) | 1ull << 63);
+            seq = at - 1;
+            off = u - lane_of(before, at);
+            w = Work{lane_of(mine_w.lo, at), lane_of(mine_w.n, at), lane_of(mine_w.len, at), lane_of(mine_w.base, at),
+                     lane_of(mine_w.end, at), lane_of(mine_w.units, at), lane_of(mine_w.blocks, at)};
         } else {
-            for (int c = 0; c < parts; c += TPB) {
-                run = scan(lds, c, parts, run, mine, before, value);
-                if (mine > 0 && before <= u && u < before + mine) keep(c + tid);
+            auto keep = [&](int i) {
+                lds.index = i - 1, lds.off = u - before;
+                lds.work[0] = mine_w.lo, lds.work[1] = mine_w.n, lds.work[2] = mine_w.len, lds.work[3] = mine_w.base;
+                lds.work[4] = mine_w.end, lds.work[5] = mine_w.units, lds.work[6] = mine_w.blocks;
+            };
+            if (parts <= TPB) {
+                if (mine > 0 && before <= u && u < before + mine) keep(tid);
+            } else {
+                for (int c = 0; c < parts; c += TPB) {
+                    run = scan(lds, c, parts, run, mine, before, value);
+                    if (mine > 0 && before <= u && u < before + mine) keep(c + tid);
+                }
             }
+            __syncthreads();
+            seq = uniform(lds.index);
+            off = uniform(lds.off);
+            w = Work{uniform(lds.work[0]), uniform(lds.work[1]), uniform(lds.work[2]), uniform(lds.work[3]),
+                     uniform(lds.work[4]), uniform(lds.work[5]), uniform(lds.work[6])};
         }
-        __syncthreads();
-        seq = uniform(lds.index);
-        off = uniform(lds.off);
-        w = Work{uniform(lds.work[0]), uniform(lds.work[1]), uniform(lds.work[2]), uniform(lds.work[3]),
-                 uniform(lds.work[4]), uniform(lds.work[5]), uniform(lds.work[6])};
         rb = 0;
-        if (w.blocks > 1) {  // the block, likewise
+        auto block = [&](int b) { return cost(A, units_of(A, b), over); };
+        if (w.blocks > 64) {  // the block, likewise
             run = 0;
             for (int c = 0; c < w.blocks; c += TPB) {
-                run = scan(lds, c, w.blocks, run, mine, before, [&](int b) { return cost(A, units_of(A, b), over); });
+                run = scan(lds, c, w.blocks, run, mine, before, block);
                 if (mine > 0 && before <= off && off < before + mine) lds.index = c + tid, lds.off = off - before;
                 if (off < run) break;  // the same for every thread
             }
             __syncthreads();
             rb = uniform(lds.index);
             off = uniform(lds.off);
+        } else if (w.blocks > 1) {
+            mine = lane < w.blocks ? block(lane) : 0;
+            before = wave_scan_l(mine) - mine;
+            rb = __builtin_ctzll(__ballot(mine > 0 && before <= off && off < before + mine) | 1ull << 63);
+            off -= lane_of(before, rb);
         }
         units = units_of(A, rb);
         return true;

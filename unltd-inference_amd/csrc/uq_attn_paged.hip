@@ -33,13 +33,18 @@ struct Geo<false, HD> {
     static constexpr int NP = 16, PT = 1, KC = HD / 16, DL = 4, NH = HD / 64, VS = 4;
 };
 
-__device__ __forceinline__ float row16_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
-    v = fmaxf(v, __shfl_xor(v, 16));
-    return fmaxf(v, __shfl_xor(v, 32));
+// Over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+template <class Op>
+__device__ __forceinline__ float rows16(float v, Op op) {
+    auto two = [&](const auto &r) { return op(__uint_as_float(r[0]), __uint_as_float(r[1])); };
+    v = two(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return two(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
+__device__ __forceinline__ float row16_max(float v) {
+    return rows16(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float row16_sum(float v) {
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
+    return rows16(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
@@ -160,8 +165,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                         }
                     }
                 }
-#pragma unroll
-                for (int d = 1; d < 16; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+                top = lanes_max<16>(top);
                 // |q| < 2^ex; not finite: left as it is, its terms are not finite either
                 const int ex = top > 0 && top < 0x7F800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 15;
                 fac = ldexpf(fac, ex - 15);
@@ -208,9 +212,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
             fac[y] = row_c[n + 16 * y];
             if (n + 16 * y < nq) lim_min = min(lim_min, lim[y]);
         }
-#pragma unroll
-        for (int d = 1; d < 16; d <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, d));
-        lim_min = uniform(lim_min);
+        lim_min = uniform(lanes_min<16>(lim_min));
         W.reset();
         bool unfinite = false;  // values that are not finite were left out where some query may not see them
         // A tile's keys and values in registers. The next tile's keys are on their way while this one's values are
@@ -555,8 +557,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
     const float2 al0 = at0 < total ? A.rec_al[rec(at0)] : make_float2(INFINITY, 0.0f);
     float amin = al0.x;
     for (int i = at0 + 64 * WAVES; i < total; i += 64 * WAVES) amin = fminf(amin, A.rec_al[rec(i)].x);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) amin = fminf(amin, __shfl_xor(amin, d));
+    amin = lanes_min<64>(amin);
     if constexpr (WAVES > 1) {
         if (lane == 0) red[wave] = amin;
         __syncthreads();
@@ -578,7 +579,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
 #pragma unroll 8
         for (int k = 0; k < n; k++) {
             const float *src = A.rec_o + rec(i0 + WAVES * k) * HD + lane;
-            const float fk = __shfl(f, k);
+            const float fk = __int_as_float(lane_of(__float_as_int(f), k));
 #pragma unroll
             for (int e = 0; e < E; e++) o[e] += fk * src[64 * e];
         }
