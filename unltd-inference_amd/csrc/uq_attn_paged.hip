@@ -492,6 +492,16 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
     }
 }
 
+template <int E>
+struct Floats {
+    typedef float V __attribute__((ext_vector_type(E)));
+    typedef float At __attribute__((ext_vector_type(E), aligned(4)));  // from any float on
+};
+template <>
+struct Floats<1> {
+    typedef float V, At;
+};
+
 // Joins the records of a row and head (its part of the shared positions, then
 // its own) where the workgroups have not written the result themselves: the
 // least reference first, then the sums. What it takes is round trips (row
@@ -501,9 +511,11 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
 // with few records.
 template <int HD, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kernel(AttnArgs A, int pairs) {
-    constexpr int E = HD / 64, PER = WAVES == 1 ? 4 : 1;  // pairs of a workgroup
+    constexpr int E = HD / 64, PER = WAVES == 1 ? 4 : 1;  // values of a lane, pairs of a workgroup
+    using Values = typename Floats<E>::V;
+    using ValuesAt = typename Floats<E>::At;
     __shared__ float red[WAVES], redl[WAVES];
-    __shared__ float part[WAVES][WAVES == 1 ? 1 : HD];
+    __shared__ __align__(32) float part[WAVES][WAVES == 1 ? 1 : HD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int pair = (int)blockIdx.x * PER + (WAVES == 1 ? wave : 0);
     if (pair >= pairs) return;  // a wave by itself (WAVES 1), else none
@@ -564,9 +576,8 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
 #pragma unroll
         for (int i = 0; i < WAVES; i++) amin = fminf(amin, red[i]);
     }
-    float l = 0.0f, o[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    float l = 0.0f;
+    Values o = (Values)0.0f;
     for (int i0 = begin; i0 < total; i0 += 64 * WAVES) {
         const int mine = i0 + WAVES * lane;
         float f = 0.0f;
@@ -578,36 +589,40 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
         const int n = min(64, (total - i0 + WAVES - 1) / WAVES);
 #pragma unroll 8
         for (int k = 0; k < n; k++) {
-            const float *src = A.rec_o + rec(i0 + WAVES * k) * HD + lane;
+            const Values x = *(const Values *)(A.rec_o + rec(i0 + WAVES * k) * HD + E * lane);
             const float fk = __int_as_float(lane_of(__float_as_int(f), k));
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] += fk * src[64 * e];
+            o += fk * x;
         }
     }
     l = wave_sum(l);
     if constexpr (WAVES > 1) {
         if (lane == 0) redl[wave] = l;
-#pragma unroll
-        for (int e = 0; e < E; e++) part[wave][64 * e + lane] = o[e];
+        *(Values *)&part[wave][E * lane] = o;
         __syncthreads();
         l = 0.0f;
 #pragma unroll
         for (int i = 0; i < WAVES; i++) l += redl[i];
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int d = 64 * e + lane;
-        if (WAVES > 1 && e % WAVES != wave) continue;  // the waves share the values
-        float y = o[e];
-        if constexpr (WAVES > 1) {
-            y = 0.0f;
+        for (int d = threadIdx.x; d < HD; d += 64 * WAVES) {
+            float y = 0.0f;
 #pragma unroll
             for (int i = 0; i < WAVES; i++) y += part[i][d];
+            y = l == 0.0f ? 0.0f : y * (1.0f / l);
+            if (A.a.gate) y *= sigmoid1(A.a.gate[(size_t)row * A.a.gate_row + (size_t)head * A.a.gate_head + d]);
+            A.a.out[((size_t)row * A.a.n_head + head) * HD + d] = y;
         }
-        y = l == 0.0f ? 0.0f : y * inv;
-        if (A.a.gate) y *= sigmoid1(A.a.gate[(size_t)row * A.a.gate_row + (size_t)head * A.a.gate_head + d]);
-        A.a.out[((size_t)row * A.a.n_head + head) * HD + d] = y;
+    } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        Values y = l == 0.0f ? (Values)0.0f : o * inv;
+        if (A.a.gate) {
+            const ValuesAt z = *(const ValuesAt *)(A.a.gate + (size_t)row * A.a.gate_row + (size_t)head * A.a.gate_head + E * lane);
+            if constexpr (E == 1) {
+                y *= sigmoid1(z);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++) y[e] *= sigmoid1(z[e]);
+            }
+        }
+        *(ValuesAt *)(A.a.out + ((size_t)row * A.a.n_head + head) * HD + E * lane) = y;
     }
 }
 
