@@ -125,6 +125,16 @@ __global__ __launch_bounds__(kAppTPB) void kv_append_kernel(AppendArgs a) {
     __shared__ float rowv[NW][HD];
     const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uq_head_rows &h = a.h;
+    const int nq = h.d_q ? (int)h.n_head : 0, nk = h.d_k ? a.kv.n_head_kv : 0, step_u = NW * (int)gridDim.y;
+    auto load = [&](float (&v)[E], int u) {
+        const float *src = u < nq        ? h.d_q + (size_t)row * h.q_row + (size_t)u * h.q_head
+                           : u >= nq + nk ? h.d_v + (size_t)row * h.v_row + (size_t)(u - nq - nk) * HD
+                                          : h.d_k + (size_t)row * h.k_row + (size_t)(u - nq) * HD;
+        load_row<E>(v, src + E * lane);
+    };
+    int u = wave + NW * (int)blockIdx.y;
+    float v[E], ahead[E];  // a head under way while the one before it is worked on, the first while the row is looked for
+    if (u < nq + 2 * nk) load(ahead, u);
     find_row(a.b, a.kv.map, row, &at);
     const int pos = at.pos, page = at.page;
     if (pos < 0) return;
@@ -141,17 +151,14 @@ __global__ __launch_bounds__(kAppTPB) void kv_append_kernel(AppendArgs a) {
         turn[t] = make_double2(sn, cs);
     }
     __syncthreads();
-    const int nq = h.d_q ? (int)h.n_head : 0, nk = h.d_k ? a.kv.n_head_kv : 0;
     const bool cached = page_ok(a.kv.map, page);
-    for (int u = wave + NW * (int)blockIdx.y; u < nq + 2 * nk; u += NW * (int)gridDim.y) {
+    for (; u < nq + 2 * nk; u += step_u) {
         const bool isq = u < nq, isv = u >= nq + nk;
         const int j = isq ? u : isv ? u - nq - nk : u - nq;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = ahead[e];
+        if (u + step_u < nq + 2 * nk) load(ahead, u + step_u);
         if (!isq && !cached) continue;  // the whole wave
-        const float *src = isq ? h.d_q + (size_t)row * h.q_row + (size_t)j * h.q_head
-                         : isv ? h.d_v + (size_t)row * h.v_row + (size_t)j * HD
-                               : h.d_k + (size_t)row * h.k_row + (size_t)j * HD;
-        float v[E];
-        load_row<E>(v, src + E * lane);
         if (!isv) {
             const float *w = isq ? h.d_q_norm : h.d_k_norm;
             if (w) {
