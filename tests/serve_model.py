@@ -12,13 +12,13 @@ DTYPE = {"f32": (uq.DType.F32, np.float32), "f16": (uq.DType.F16, np.float16)}
 class Cache:
     """Pools in pages, page tables and a batch's rows, on the host and (upload) on the device."""
 
-    def __init__(self, rng, dtype, kv, hd, page, rows, lens, pad=0, spare=2, shared=0, scale=1.0):
+    def __init__(self, rng, dtype, kv, hd, page, rows, lens, pad=0, spare=2, shared=0, scale=1.0, room=0):
         self.dtype, self.kv, self.hd, self.page, self.rows, self.lens = dtype, kv, hd, page, list(rows), list(lens)
         self.start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
         self.n_rows = int(self.start[-1]) + pad
         whole = shared // page
         need = [max(0, -(-x // page) - whole) for x in lens]
-        self.max_pages = whole + max(need + [1])
+        self.max_pages = max(whole + max(need + [1]), room // page)  # room: positions of a table that is longer than it need be
         self.n_pages = whole + sum(need) + spare
         order = rng.permutation(self.n_pages).astype(np.int32)
         self.table = np.full((len(rows), self.max_pages), -1, np.int32)

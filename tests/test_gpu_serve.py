@@ -210,6 +210,10 @@ def check(c, q, heads, scale, shared=0, gate=None, what=""):
           flush=True)
 
 
+# Positions of the page tables: no more than the batch needs (short ones: a workgroup takes a block by itself), and many
+# (blocks are divided, and joined; more than 32 queries of a KV head are another kernel's).
+ROOM = [0, 1 << 16]
+
 SHAPES = [
     # heads, kv, hd, page, rows, lens, shared, pad
     (16, 4, 256, 64, [1], [700], 0, 0),
@@ -241,41 +245,47 @@ SHAPES = [
     (24, 1, 256, 16, [1, 1], [40, 700], 0, 1),
     (32, 1, 64, 8, [1, 0, 1], [1, 5, 64], 0, 0),
     (8, 1, 128, 16, [3] * 4, [64, 90, 61, 150], 60, 0),
-    (16, 8, 64, 16, [1] * 100, [2601 + i % 7 for i in range(100)], 2600, 2)]  # f32: shared on 32, own on 16
+    (16, 8, 64, 16, [1] * 100, [2601 + i % 7 for i in range(100)], 2600, 2),  # f32: shared on 32, own on 16
+    # shared positions enough for the blocks of many queries
+    (16, 4, 256, 64, [1] * 25, [9300 + i % 3 for i in range(25)], 9290, 0),
+    (32, 2, 128, 16, [3] * 10, [3910 + 7 * i for i in range(10)], 3900, 1)]
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("case", range(len(SHAPES)))
-def test_attention_against_64_bits(dtype, case):
+def test_attention_against_64_bits(dtype, case, room):
     heads, kv, hd, page, rows, lens, shared, pad = SHAPES[case]
     rng = np.random.default_rng(100 + case)
-    c = M.Cache(rng, dtype, kv, hd, page, rows, lens, pad=pad, shared=shared)
+    c = M.Cache(rng, dtype, kv, hd, page, rows, lens, pad=pad, shared=shared, room=room)
     q = (2 * rng.standard_normal((c.n_rows, heads, hd))).astype(np.float32)
     gate = rng.standard_normal(q.shape).astype(np.float32) if case % 2 else None
     check(c, q, heads, 1 / np.sqrt(hd), shared, gate, f"{dtype} {SHAPES[case]}")
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype,seqs", [("f16", 300), ("f32", 600)])
-def test_attention_of_many_sequences(dtype, seqs):
+def test_attention_of_many_sequences(dtype, seqs, room):
     """More sequences than a workgroup's threads, some without rows or positions."""
     rng = np.random.default_rng(seqs)
     rows = rng.integers(0, 3, seqs)
     lens = np.where(rng.random(seqs) < 0.1, rows, rows + rng.integers(0, 60, seqs))
-    c = M.Cache(rng, dtype, 1, 64, 16, rows, lens, pad=1)
+    c = M.Cache(rng, dtype, 1, 64, 16, rows, lens, pad=1, room=room)
     q = rng.standard_normal((c.n_rows, 2, 64)).astype(np.float32)
     check(c, q, 2, 0.125, what=f"{dtype} {seqs} sequences")
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("shared", [0, 24])
-def test_attention_passes_over_what_no_row_sees(dtype, shared):
+def test_attention_passes_over_what_no_row_sees(dtype, shared, room):
     """Slots behind the lengths, unused pages, later rows' positions and pages that are none hold NaN, infinities
     and the type's lowest value: the results are those without them. A row without any position is zero."""
     rng = np.random.default_rng(21)
     rows, lens = [6, 3, 4, 2, 3], [70, 33, 2, 41, 60]
     if shared:
         lens[2] = 26
-    c = M.Cache(rng, dtype, 2, 128, 8, rows, lens, shared=shared)
+    c = M.Cache(rng, dtype, 2, 128, 8, rows, lens, shared=shared, room=room)
     lens = c.lens
     q = rng.standard_normal((c.n_rows, 4, 128)).astype(np.float32)
     used = np.zeros(c.k.shape[:3], bool)
@@ -308,12 +318,13 @@ def test_attention_passes_over_what_no_row_sees(dtype, shared):
         assert not np.isfinite(got[last[b]]).all(), "a row that sees them shows it"
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-def test_attention_with_a_value_not_finite_that_some_rows_see(dtype):
+def test_attention_with_a_value_not_finite_that_some_rows_see(dtype, room):
     """Position 40 of 45 holds values of NaN, infinity and numbers: rows before it are untouched, rows from it on
     are not finite in those columns alone."""
     rng = np.random.default_rng(22)
-    c = M.Cache(rng, dtype, 1, 64, 16, [9], [45])
+    c = M.Cache(rng, dtype, 1, 64, 16, [9], [45], room=room)
     q = rng.standard_normal((9, 2, 64)).astype(np.float32)
     clean, bound = M.attention(c, q, 2, 0.125)
     pg, sl, _ = c.slots(0, 45)
@@ -327,12 +338,13 @@ def test_attention_with_a_value_not_finite_that_some_rows_see(dtype):
     assert np.isnan(got[4:, :, 5]).all() and not np.isfinite(got[4:, :, 9]).any()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("rows,lens", [([1, 1], [1, 33]), ([50, 1], [50, 129])])
-def test_attention_keeps_a_nan_that_is_all_a_tile_shows(dtype, rows, lens):
+def test_attention_keeps_a_nan_that_is_all_a_tile_shows(dtype, rows, lens, room):
     """The only position that a row sees, or the only one in the last tile that it sees, has a key of NaN."""
     rng = np.random.default_rng(28)
-    c = M.Cache(rng, dtype, 1, 64, 16, rows, lens)
+    c = M.Cache(rng, dtype, 1, 64, 16, rows, lens, room=room)
     for b, pos in ((0, 0), (1, lens[1] - 1)):
         pg, sl, _ = c.slots(b, pos + 1)
         c.k[pg[-1], :, sl[-1]] = np.nan
@@ -340,11 +352,12 @@ def test_attention_keeps_a_nan_that_is_all_a_tile_shows(dtype, rows, lens):
     assert np.isnan(got).all()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-def test_attention_of_large_and_small_numbers(dtype):
+def test_attention_of_large_and_small_numbers(dtype, room):
     """Scores of thousands (one weight is all), queries of 1e-30 and 1e30, keys of zero, the largest f16."""
     rng = np.random.default_rng(23)
-    c = M.Cache(rng, dtype, 2, 64, 16, [1, 1, 1, 1], [100, 200, 300, 50])
+    c = M.Cache(rng, dtype, 2, 64, 16, [1, 1, 1, 1], [100, 200, 300, 50], room=room)
     q = rng.standard_normal((4, 4, 64)).astype(np.float32)
     q[0] *= 1000
     q[1] *= 1e-30
@@ -361,20 +374,22 @@ def test_attention_of_large_and_small_numbers(dtype):
     assert one.all()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-30])
-def test_attention_with_any_scale(dtype, scale):
+def test_attention_with_any_scale(dtype, scale, room):
     """Turned round, the mean of the values, nearly the mean: blocks of few and of many queries."""
     rng = np.random.default_rng(29)
-    c = M.Cache(rng, dtype, 2, 64, 16, [1, 30], [90, 200])
+    c = M.Cache(rng, dtype, 2, 64, 16, [1, 30], [90, 200], room=room)
     check(c, rng.standard_normal((31, 6, 64)).astype(np.float32), 6, scale, what=f"{dtype} scale {scale}")
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-def test_attention_of_many_queries_large_and_not_finite(dtype):
+def test_attention_of_many_queries_large_and_not_finite(dtype, room):
     """Queries of 1e30, 1e-30 and 0 among others, and of NaN and infinity, whose own results show it and no others."""
     rng = np.random.default_rng(30)
-    c = M.Cache(rng, dtype, 1, 128, 16, [40], [300])
+    c = M.Cache(rng, dtype, 1, 128, 16, [40], [300], room=room)
     q = rng.standard_normal((40, 4, 128)).astype(np.float32)
     clean = q.copy()
     q[3] *= 1e-30
@@ -419,8 +434,9 @@ def test_attention_without_pages_or_rows(dtype, rows):
             assert np.all(host(out, like) == want)
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
-def test_attention_in_a_pool_beyond_32_bits(dtype):
+def test_attention_in_a_pool_beyond_32_bits(dtype, room):
     """Pages whose values lie 2^32 and more bytes and elements into the arrays, appended to and read, by few queries
     and by many (a page number of them would be another page's in 32 bits)."""
     hd, page, heads = 128, 16, 4
@@ -429,7 +445,7 @@ def test_attention_in_a_pool_beyond_32_bits(dtype):
     n_pages = (1 << 32) // per + 64
     rows, lens = [40, 1], [200, 150]
     rng = np.random.default_rng(31)
-    c = M.Cache(rng, dtype, 1, hd, page, rows, lens, spare=0)
+    c = M.Cache(rng, dtype, 1, hd, page, rows, lens, spare=0, room=room)
     high = n_pages - 1 - np.arange(c.n_pages)  # page x of the small cache is this page of the large one
     d_k, d_v = uq.DeviceArray(n_pages * per * elem), uq.DeviceArray(n_pages * per * elem)
 
@@ -456,12 +472,13 @@ def test_attention_in_a_pool_beyond_32_bits(dtype):
         d.free()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("rows,lens,shared", [([3, 1], [70, 90], 48), ([50, 40], [90, 140], 40), ([70], [150], 0)])
-def test_attention_in_place_from_any_float(dtype, rows, lens, shared):
+def test_attention_in_place_from_any_float(dtype, rows, lens, shared, room):
     """d_out = d_q, four bytes off any alignment."""
     rng = np.random.default_rng(32)
-    c = M.Cache(rng, dtype, 2, 64, 16, rows, lens, shared=shared)
+    c = M.Cache(rng, dtype, 2, 64, 16, rows, lens, shared=shared, room=room)
     q = rng.standard_normal((c.n_rows, 4, 64)).astype(np.float32)
     want = attend(c, q, 4, 0.125, shared)
     pages, batch = c.upload()
@@ -502,7 +519,8 @@ def test_two_calls_at_once():
             assert np.array_equal(host(o, want).view(np.int32), want.view(np.int32))
 
 
-def test_two_graphs_share_a_workspace():
+@pytest.mark.parametrize("room", ROOM)
+def test_two_graphs_share_a_workspace(room):
     """Replayed in turn on one stream, with eager calls of the same workspace between: a call leaves nothing behind
     that another needs."""
     sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(__file__))))
@@ -512,7 +530,7 @@ def test_two_graphs_share_a_workspace():
     rng = np.random.default_rng(34)
     work = []
     for rows, lens, shared in [([1, 1, 1], [900, 33, 410], 0), ([40, 1], [300, 280], 256)]:
-        c = M.Cache(rng, "f16", 2, 128, 16, rows, lens, shared=shared)
+        c = M.Cache(rng, "f16", 2, 128, 16, rows, lens, shared=shared, room=room)
         q = rng.standard_normal((c.n_rows, 8, 128)).astype(np.float32)
         want = attend(c, q, 8, 0.1, shared)
         work.append((*c.upload(), dev(q), dev(np.zeros_like(q)), shared, want, c))
@@ -576,7 +594,8 @@ def test_attention_in_place_and_on_another_stream():
     assert np.array_equal(got.view(np.int32), want.view(np.int32))
 
 
-def test_attention_captured_follows_lengths_and_pages():
+@pytest.mark.parametrize("room", ROOM)
+def test_attention_captured_follows_lengths_and_pages(room):
     """One graph of append and attention; between the replays the lengths, pages and rows change on the device, and
     eager work with a workspace of its own runs."""
     sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(__file__))))
@@ -585,7 +604,7 @@ def test_attention_captured_follows_lengths_and_pages():
     s = hip.stream()
     heads, kv, hd, page = 8, 2, 128, 16
     rng = np.random.default_rng(27)
-    c = M.Cache(rng, "f16", kv, hd, page, [1, 2, 1], [200, 130, 9], pad=2, spare=20)
+    c = M.Cache(rng, "f16", kv, hd, page, [1, 2, 1], [200, 130, 9], pad=2, spare=20, room=room)
     pages, batch = c.upload()
     n = c.n_rows
     bufs = [uq.DeviceArray(4 * n * w * hd) for w in (heads, kv, kv, heads, heads)]

@@ -27,6 +27,8 @@ struct AttnArgs {
     PagesView kv;
     BatchView b;
     int group;
+    int common;       // positions that part 1 reads through the first sequence's pages (shared, but not a part)
+    bool alone;       // every block has a workgroup of its own: no records, no join
     int first, last;  // the launch's parts
     Part part[2];
     size_t whole;   // first of the rows' own records
@@ -114,11 +116,16 @@ __device__ __forceinline__ long long seen_sum(const AttnArgs &A, const Work &w, 
     long long t = 0;
     for (int rb = 0; rb < w.blocks; rb++) {
         const int units = seen_to<U>(w, rows);
-        t += units > 0 ? units + more : 0;
+        t += A.alone ? 1 : units > 0 ? units + more : 0;
         rows += step, left += rest;
         if (left >= A.group) rows++, left -= A.group;
     }
     return t;
+}
+
+// The page of a position of a sequence's own part, whose table's row is given.
+__device__ __forceinline__ int page_at(const AttnArgs &A, const int32_t *table, int pos) {
+    return (pos < A.common ? A.b.pages : table)[pos >> A.kv.map.log2_page];
 }
 
 // A value that is the same in every lane, in scalar registers.
@@ -214,8 +221,11 @@ struct Walk {
     __device__ __forceinline__ int units_of(const AttnArgs &A, int b) const {
         return seq < 0 ? w.units : seen_units<U>(A, w, b);
     }
+    __device__ __forceinline__ static int each_of(const AttnArgs &A, int n, int over) {  // of n units, for a KV head
+        return A.alone ? 1 : n > 0 ? n + over : 0;
+    }
     __device__ __forceinline__ static long long cost(const AttnArgs &A, int n, int over) {
-        return n > 0 ? (long long)A.kv.n_head_kv * (n + over) : 0;
+        return (long long)A.kv.n_head_kv * each_of(A, n, over);
     }
     // Units before item c + tid and its own (of items c .. c + TPB - 1 with value(i) each); returns those up to c + TPB
     template <class Value>
@@ -243,7 +253,7 @@ struct Walk {
         auto value = [&](int i) {
             if (i > 0 ? A.last == 0 : A.first == 1) return 0LL;
             mine_w = work_of<U>(A, i - 1);
-            if (mine_w.units == 0) return 0LL;
+            if (mine_w.units == 0 && !A.alone) return 0LL;
             return i == 0 ? cost(A, mine_w.units, OVER) * mine_w.blocks : A.kv.n_head_kv * seen_sum<U>(A, mine_w, OVER);
         };
         long long mine = 0, before = 0, run = 0;
@@ -330,7 +340,7 @@ struct Walk {
     // The next block with units of this run; false: none.
     __device__ __forceinline__ bool next(const AttnArgs &A) {
         while (u < u1) {
-            const int each = units > 0 ? units + over : 0;
+            const int each = each_of(A, units, over);
             if (off >= (long long)A.kv.n_head_kv * each) {
                 off -= (long long)A.kv.n_head_kv * each;
                 if (++rb >= w.blocks) {
@@ -351,6 +361,10 @@ struct Walk {
             end = u + each - at - 1;
             u += upto - at;
             off += upto - at;
+            if (A.alone) {
+                un = 0, count = units, starts = ends = true;
+                return true;
+            }
             if (count > 0) return true;
         }
         return false;

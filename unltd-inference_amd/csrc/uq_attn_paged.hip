@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
         const E *K = (const E *)A.kv.k, *V = (const E *)A.kv.v;
         auto page_of = [&](int it) {  // of position lane & (NP - 1) of tile it
             const int pos = w.base + (un + it) * NP + (lane & (NP - 1));
-            return it < count && pos < end ? table[pos >> map.log2_page] : -1;
+            return it < count && pos < end ? page_at(A, table, pos) : -1;
         };
         int page = page_of(wave), ahead = page_of(wave + kWaves);  // on their way while the queries are
 
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
               for (int it = wave; it < count; it += kWaves)
                   for (int x = 0; x < NP; x++) {
                       const int pos = w.base + (un + it) * NP + x;
-                      const int pg = pos < end ? table[pos >> map.log2_page] : -1;
+                      const int pg = pos < end ? page_at(A, table, pos) : -1;
                       if (!page_ok(map, pg)) continue;
                       const E *vp = V + (size_t)page_row(map, pg, kvh, pos) * HD;
 #pragma unroll
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                 if (d == 0) A.rec_al[rec] = make_float2(ar, lr);
             }
         }
-        if (starts && tid < nq) {
+        if (starts && !A.alone && tid < nq) {
             const int num = rb * ROWS + tid;
             put_seg(A, seq >= 0, w.lo + num / A.group, kvh * A.group + num % A.group,
                     done ? kDone : whole ? kWhole : X.me, done || whole ? 0 : X.last(), tid);
@@ -633,24 +633,27 @@ struct Plan {
     AttnArgs A;
 };
 
-// Queries of a block for R queries of a KV head (all rows' of the shared part,
-// a sequence's at the mean): 64 or 128 on attn_many_kernel for more than 32,
-// the least that wastes the least; else 16 or 32 on attn_paged_kernel. 32 read
-// the cache half as often (us, 16 | 32; f16, 32 sequences of 20 queries: 79 |
-// 68; f32, of 40: 117 | 106; 509 rows of one, f32: 500 | 370; 48 rows with
-// 16384 shared, f32: 300 | 180), but
+// Queries of a block for the R queries of a KV head of one of n_seqs sequences
+// (the mean) over at most `positions`: 64 or 128 on attn_many_kernel, else 16
+// or 32 on attn_paged_kernel. 32 read the cache half as often (us, 16 | 32;
+// f16, 32 sequences of 20 queries: 79 | 68; f32, of 40: 117 | 106; 509 rows of
+// one, f32: 500 | 370; 48 rows with 16384 shared, f32: 300 | 180), but
+//  - take longer over few tiles (`few` a CU), and so does attn_many_kernel: f16,
+//    chunks of 33 rows of 4 heads of 256 values over 1500 positions: 35 with
+//    16, 40; over 4096: 52, 42; of 128 values, 129 rows over 1500: 28, 30; 200:
+//    34, 31. The more where shared positions need a launch apart from own ones
+//    in blocks of 16: 25 rows of 16 heads of 128 values, 3000: 29, 43; 48 rows,
+//    4000: 43, 47; 20 rows of 32 heads, 16000: 89, 58. f32, 17 rows of 12
+//    heads, 12000: 43, 50; 20000: 65, 61;
 //  - leave a CU one workgroup for 256 f32 values, which reads too slowly from
 //    memory unless the blocks are of one or two sequences (32 sequences of 64
-//    queries: 220 | 274; 8 of 256: 345 | 382; 2 of 1024: 655 | 458);
-//  - of a shared part need a launch apart from own parts in blocks of 16,
-//    10 us that few tiles a wave do not bring in (17 rows' 12 heads over 2011
-//    positions: 23 | 37; 12000: 43 | 50; 20000: 65 | 61).
-int block_rows(const PagesView &kv, size_t R, int n_seqs, int shared) {
-    if (R <= 16 || kv.head_dim == 512) return 16;
+//    queries: 220 | 274; 8 of 256: 345 | 382; 2 of 1024: 655 | 458).
+int block_rows(const PagesView &kv, size_t R, int n_seqs, size_t positions, bool shared) {
+    const size_t tiles = n_seqs * ((R + 15) / 16) * kv.n_head_kv * (positions / (kv.f16 ? 32 : 16));  // of 16 queries
+    const size_t few = kv.f16 ? shared ? 28 : std::min(20, 2048 / kv.head_dim) : shared ? 64 : 28;
+    if (R <= 16 || kv.head_dim == 512 || tiles < few * kCUs) return 16;
     if (R > 32 && attn_many_ok(kv)) return R > 64 ? 128 : 64;
-    if (!kv.f16 && kv.head_dim == 256 && n_seqs > 2) return 16;
-    const size_t tiles = (R + 15) / 16 * kv.n_head_kv * ((size_t)shared / (kv.f16 ? 32 : 16));
-    return shared && tiles < 32 * 2 * kCUs ? 16 : 32;
+    return !kv.f16 && kv.head_dim == 256 && n_seqs > 2 ? 16 : 32;
 }
 int block_groups(const PagesView &kv, int rows) {
     if (rows <= 32) return kCUs * few_per_cu(kv.head_dim, rows / 16);
@@ -663,20 +666,29 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     Plan p{};
     AttnArgs &A = p.A;
     A.a = a, A.kv = kv, A.b = b, A.group = group;
-    A.part[1].rows = block_rows(kv, (queries + b.n_seqs - 1) / b.n_seqs, b.n_seqs, 0);
-    A.part[0].rows = a.shared_len ? block_rows(kv, queries, 1, a.shared_len) : A.part[1].rows;
-    if (A.part[0].rows == 16)  // no gain from a launch apart
-        A.part[0].rows = std::min(A.part[1].rows, 32);
+    const size_t own = (queries + b.n_seqs - 1) / b.n_seqs, cap = (size_t)b.max_pages << kv.map.log2_page;
+    // A block of few positions in a workgroup of its own, shared positions with it, saves the join: 9 us for 14 (13
+    // rows over 14 positions), 15 for 36 (15 rows, 83 positions shared, up to 512). What a workgroup reads alone takes
+    // as long as a join at 0.3 to 0.5 MB (f16, 256 values, up to 384 positions: 17.6 for 19.5; 736: 24 for 18).
+    const size_t most = (size_t)320 * 1024 / (2 * kv.head_dim * (kv.f16 ? 2 : 4));
+    A.alone = cap <= most && (b.n_seqs + queries / 16) * kv.n_head_kv <= 4 * kCUs;
+    if (A.alone) {
+        A.common = a.shared_len, A.a.shared_len = 0;
+        A.part[0].rows = A.part[1].rows = 16;
+    } else {
+        A.part[1].rows = block_rows(kv, own, b.n_seqs, cap, false);
+        A.part[0].rows = a.shared_len ? std::max(A.part[1].rows, block_rows(kv, queries, 1, a.shared_len, true)) : A.part[1].rows;
+    }
     for (Part &x : A.part) x.G = block_groups(kv, x.rows);
     auto groups_recs = [&](const Part &x) { return (size_t)2 * x.G * x.rows; };
-    size_t recs = groups_recs(A.part[1]);
+    size_t recs = A.alone ? 0 : groups_recs(A.part[1]);
     p.apart = A.part[0].rows != A.part[1].rows;
     if (p.apart) A.part[0].base = recs, recs += groups_recs(A.part[0]);
     A.whole = recs;
-    if (a.shared_len) recs += (size_t)2 * b.n_rows * a.n_head;
+    if (A.a.shared_len) recs += (size_t)2 * b.n_rows * a.n_head;
     p.al = recs * kv.head_dim * sizeof(float);
     p.seg = p.al + recs * sizeof(float2);
-    p.bytes = p.seg + (size_t)2 * b.n_rows * a.n_head * sizeof(int2);
+    p.bytes = A.alone ? 16 : p.seg + (size_t)2 * b.n_rows * a.n_head * sizeof(int2);
     return p;
 }
 
@@ -747,8 +759,8 @@ hipError_t launch_attn_paged(const PagesView &kv, const BatchView &b, const Attn
     };
     if (p.apart)
         if (hipError_t e = go(0, 0)) return e;
-    if (hipError_t e = go(a.shared_len && !p.apart ? 0 : 1, 1)) return e;
-    return launch_join(A, s);
+    if (hipError_t e = go(A.a.shared_len && !p.apart ? 0 : 1, 1)) return e;
+    return A.alone ? hipSuccess : launch_join(A, s);
 }
 
 }  // namespace uq
