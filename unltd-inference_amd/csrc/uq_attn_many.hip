@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 
-    Walk<NT, NP, M::kOver> X;
+    Walk<NT, NP, M::kOver, 1> X;
     if (!X.find(A, walk_lds)) return;
     while (X.next(A)) {
         const Work &w = X.w;

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
     const int nkv = A.kv.n_head_kv;
     const PageMap &map = A.kv.map;
 
-    Walk<kTPB, NP, kOver> X;
+    Walk<kTPB, NP, kOver, kWaves> X;
     if (!X.find(A, walk_lds)) return;
     Wave<F16, HD, RT> W;
     while (X.next(A)) {
