@@ -643,7 +643,7 @@ struct Plan {
 //    16, 40; over 4096: 52, 42; of 128 values, 129 rows over 1500: 28, 30; 200:
 //    34, 31. The more where shared positions need a launch apart from own ones
 //    in blocks of 16: 25 rows of 16 heads of 128 values, 3000: 29, 43; 48 rows,
-//    4000: 43, 47; 20 rows of 32 heads, 16000: 89, 58. f32, 17 rows of 12
+//    4000: 43, 47; 20 rows of 32 heads, 16000: 89, 58. f32, 14 rows of 12
 //    heads, 12000: 43, 50; 20000: 65, 61;
 //  - leave a CU one workgroup for 256 f32 values, which reads too slowly from
 //    memory unless the blocks are of one or two sequences (32 sequences of 64
