@@ -4,6 +4,7 @@ and rotations: types, head shapes, page sizes, lengths, padded batches, pages
 that are none, values that are not finite where a row may not see them, other
 streams, graphs, and the operators in a row."""
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -767,6 +768,12 @@ def test_verify_captured():
 
 
 # ------------------------------------------------------------------------- together
+
+def test_first_calls_of_a_process_captured():
+    child = os.path.join(os.path.dirname(os.path.abspath(__file__)), "serve_capture_child.py")
+    r = subprocess.run([sys.executable, child], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout + r.stderr
+
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_paged_attention_of_a_layer_equals_its_step(dtype):

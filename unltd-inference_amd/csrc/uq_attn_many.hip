@@ -112,7 +112,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
         auto look_up = [&]() {
             for (int x = tid; x < (M::CT + M::AHEAD) * NP; x += NT) {
                 const int pos = first + cb * NP + x;
-                const int page = cb + x / NP < count && pos < w.end ? page_at(A, table, pos) : -1;
+                const int page = cb + x / NP < count && pos < w.end ? table[pos >> map.log2_page] : -1;
                 const bool ok = page_ok(map, page);
                 rows[x] = ok ? page_row(map, page, kvh, pos) : 0;
                 const unsigned long long m = __ballot(ok);
@@ -417,7 +417,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
             for (int t = 0; t < count; t++) {
                 const int p0 = first + t * NP;
                 for (int y = 0; y < NP && p0 + y < w.end; y++) {
-                    const int page = page_at(A, table, p0 + y);
+                    const int page = table[(p0 + y) >> map.log2_page];
                     if (!page_ok(map, page)) continue;
                     const bool sees = p0 + y <= lim;
                     const _Float16 *vp = V + (size_t)page_row(map, page, kvh, p0 + y) * HD;

@@ -3,6 +3,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <exception>
 
 #include "uq_internal.h"
 #include "uq_serve_internal.h"
@@ -144,7 +145,11 @@ uq_status uq_attn_paged_d(float *d_out, const float *d_q, const uq_kv_pages *kv,
     const size_t need = uq::attn_paged_ws_bytes(pv, bv, (int)n_head, (int)shared_len);
     if (ws_bytes < need) return set_error(UQ_ERR_ARG, "%s: workspace of %zu bytes below %zu", fn, ws_bytes, need);
     const uq::AttnPagedArgs a{d_out, d_q, (int)n_head, (int)shared_len, kq_scale, d_gate, gate_row, gate_head};
-    return hip_st(uq::launch_attn_paged(pv, bv, a, d_ws, (hipStream_t)stream), fn);
+    try {
+        return hip_st(uq::launch_attn_paged(pv, bv, a, d_ws, (hipStream_t)stream), fn);
+    } catch (const std::exception &e) {  // the record of raised LDS limits is the one allocation
+        return set_error(UQ_ERR_HIP, "%s: %s", fn, e.what());
+    }
 }
 
 size_t uq_draft_verify_ws_bytes(const uq_seq_batch *batch, size_t vocab) {
