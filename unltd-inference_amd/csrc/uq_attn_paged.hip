@@ -246,7 +246,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                 for (int h = 0; h < G::NH; h++) T.v[i][h] = *(const VV *)(vp + 16 * G::DL * h);
             }
         };
-        if (map.n_pages > 0) {  // else there is nothing to load from
+        if (map.n_pages > 0 && wave < count) {  // else there is nothing to load from, or for
           Place cur, nxt;
           place(cur, wave, page);
           fetch_keys(cur);
