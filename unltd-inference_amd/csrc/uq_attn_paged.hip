@@ -259,12 +259,19 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
             const bool edge = have != ~0ull || p0 + NP - 1 > lim_min;
             const uint32_t hv = (uint32_t)have >> (4 * g);  // bit 16 t + i: position 16 t + 4 g + i
 
-            // scores
-            f4 s[RT][G::PT];
+            // scores; f32: the four values of a piece in sums of their own, which round a quarter of the terms each, half
+            // as large
+            f4 s[RT][G::PT], s3[RT][F16 ? 1 : 3];
 #pragma unroll
             for (int y = 0; y < RT; y++)
 #pragma unroll
                 for (int t = 0; t < G::PT; t++) s[y][t] = f4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (!F16) {
+#pragma unroll
+                for (int y = 0; y < RT; y++)
+#pragma unroll
+                    for (int e = 0; e < 3; e++) s3[y][e] = f4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
             for (int c = 0; c < G::KC; c++)
 #pragma unroll
@@ -280,9 +287,16 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                     } else {
                         const f4 q = ((const f4 *)lds)[y * HD * 4 + c * 64 + lane];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[y][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(T.k[0][c][e], q[e], s[y][0], 0, 0, 0);
+                        for (int e = 0; e < 4; e++) {
+                            f4 &to = e == 0 ? s[y][0] : s3[y][e - 1];
+                            to = __builtin_amdgcn_mfma_f32_16x16x4f32(T.k[0][c][e], q[e], to, 0, 0, 0);
+                        }
                     }
                 }
+            if constexpr (!F16) {
+#pragma unroll
+                for (int y = 0; y < RT; y++) s[y][0] = (s[y][0] + s3[y][0]) + (s3[y][1] + s3[y][2]);
+            }
 
             __builtin_amdgcn_sched_barrier(0);
             fetch_keys(nxt);
