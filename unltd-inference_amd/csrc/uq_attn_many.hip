@@ -136,11 +136,10 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
         // 16 at a time by way of the wave's part of LDS: rows are read whole, and by the lanes of a query from there
         const int at_q = (w.lo + (in ? num / A.group : rb * RB / A.group)) * A.a.n_head + kvh * A.group + (in ? num : rb * RB) % A.group;
         h8 qh[KC], ql[KC];
-        float fac = fabsf(A.a.scale) * kLog2e;
+        float fac = ldexpf(1.0f, A.scale_e);
         uint8_t *const own = lds + wave * 16384;
         {
             constexpr int LQ = HD / 4, RL = 64 / LQ, J = 16 / RL;  // lanes of a query, queries of a load, loads
-            const float sign = A.a.scale < 0.0f ? -1.0f : 1.0f;
             int exps = 15;
             f4 vs[2][J];
 #pragma unroll
@@ -163,7 +162,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
                     h4 hi, lo;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x = ldexpf(v[j][e] * sign, 15 - ex);
+                        const float x = product(ldexpf(v[j][e], 15 - ex), A.scale_m);
                         hi[e] = (_Float16)x;
                         lo[e] = (_Float16)(x - (float)hi[e]);
                     }
@@ -289,7 +288,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
             top = half_max(top) * fac;
             const bool move = top + a > kMove;  // not where both are infinite: nothing seen yet
             if (__any(move)) {
-                const float na = move ? kRef - top : a;
+                const float na = move ? reference(top, kRef) : a;
                 const float corr = move ? exp2_hw(na - a) : 1.0f;
                 a = na;
                 l *= corr;

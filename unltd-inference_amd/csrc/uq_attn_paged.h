@@ -7,6 +7,8 @@
 #include <climits>
 #include <type_traits>
 
+#include "uq_attn_ref.h"
+#include "uq_attn_ref.h"
 #include "uq_device.h"
 #include "uq_internal.h"
 #include "uq_serve_internal.h"
@@ -27,6 +29,8 @@ struct AttnArgs {
     PagesView kv;
     BatchView b;
     int group;
+    float scale_m;    // kq_scale log2 e = scale_m 2^scale_e: the queries take the mantissa (0.5 to 1, signed), the
+    int scale_e;      // exponent is a factor of their scores (uq_attn_ref.h)
     int common;       // positions that part 1 reads through the first sequence's pages (shared, but not a part)
     bool alone;       // every block has a workgroup of its own: no records, no join
     int first, last;  // the launch's parts
@@ -51,7 +55,6 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows star
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
-constexpr float kLog2e = 1.44269504088896340736f;
 
 // Where a block's units lie: in one workgroup that wrote the results itself,
 // in one whose record is the row's own, or in several workgroups' records.
@@ -375,6 +378,14 @@ struct Walk {
 };
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The f32 product, for every use of it: where the compiler sees it, a conversion to f16 is formed from the exact product
+// instead, and the two terms of a value are no longer those of one number.
+__device__ __forceinline__ float product(float a, float b) {
+    float v = a * b;
+    __asm__("" : "+v"(v));
+    return v;
+}
 
 }  // namespace
 }  // namespace uq

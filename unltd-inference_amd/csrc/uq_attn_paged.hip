@@ -12,6 +12,8 @@
 // KV heads of 256 f32 values: 5.1 TB/s with the start and end, 6.2 in the
 // loop); where there is little, its round trips do: lengths, page numbers,
 // tiles, the waves' sums (one tile a wave: 8 to 12 us).
+#include <cmath>
+
 #include "uq_attn_paged.h"
 
 namespace uq {
@@ -66,9 +68,10 @@ __device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) &
 // positions a lane: rows are loaded 16 bytes a lane and paired by v_perm, one
 // a register. No value crosses lanes but the maximum and row numbers.
 //
-// f16 cache: a query is scaled by a power of two to at most 2^15 and split
-// into two f16 terms, a weight (times 2^14) likewise; products are exact and
-// summed in f32. f32 cache: the f32 matrix products.
+// f16 cache: a query is scaled by a power of two to at most 2^15, times the
+// mantissa of the scale and log2 e, and split into two f16 terms, a weight
+// (times 2^14) likewise; products are exact and summed in f32. f32 cache: the
+// f32 matrix products.
 //
 // RT is 1 or 2: of 16 or 32 queries of a KV head, columns n and n + 16.
 template <bool F16, int HD, int RT>
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
     constexpr int NP = G::NP, MS = HD + 4, ROWS = 16 * RT;  // a unit is a wave's tile
     constexpr float kShift = F16 ? 14.0f : 0.0f;
     extern __shared__ __align__(1024) uint8_t lds[];  // the block's queries; the waves' sums at its end
-    __shared__ float row_c[ROWS];         // score factor of a query, times log2 e
+    __shared__ float row_c[ROWS];         // factor of a query's scores, a power of two (times log2 e)
     __shared__ int row_lim[ROWS];         // its last position, -1: none
     __shared__ float2 wave_al[kWaves][ROWS];
     __shared__ WalkLds walk_lds;
@@ -152,7 +155,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
             } else if (part == 0) {
                 row_lim[r] = in && w.len >= 0 ? max(-1, w.len - w.n + (row - w.lo)) : -1;
             }
-            float fac = A.a.scale * kLog2e;
+            float fac = ldexpf(1.0f, A.scale_e);
             if constexpr (F16) {
                 constexpr int C = (HD / 8 + 15) / 16;
                 float v[C][8];
@@ -174,14 +177,14 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                 top = lanes_max<16>(top);
                 // |q| < 2^ex; not finite: left as it is, its terms are not finite either
                 const int ex = top > 0 && top < 0x7F800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 15;
-                fac = ldexpf(fac, ex - 15);
+                fac = fmaxf(ldexpf(fac, ex - 15), 0x1p-126f);  // above zero: a masked score's -infinity stays one
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const int ch = part + 16 * c;
                     h8 hi, lo;
 #pragma unroll
                     for (int x = 0; x < 8; x++) {
-                        const float s = ldexpf(v[c][x], 15 - ex);
+                        const float s = product(ldexpf(v[c][x], 15 - ex), A.scale_m);
                         hi[x] = (_Float16)s;
                         lo[x] = (_Float16)(s - (float)hi[x]);
                     }
@@ -195,7 +198,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
 #pragma unroll
                 for (int c = 0; c < HD / 64; c++) {
                     const int ch = part + 16 * c;
-                    ((f4 *)lds)[y * HD * 4 + (ch >> 2) * 64 + (ch & 3) * 16 + (r & 15)] = in ? (f4) * (const f4u *)(q + 4 * ch) : f4{0.f, 0.f, 0.f, 0.f};
+                    ((f4 *)lds)[y * HD * 4 + (ch >> 2) * 64 + (ch & 3) * 16 + (r & 15)] = in ? (f4) * (const f4u *)(q + 4 * ch) * A.scale_m : f4{0.f, 0.f, 0.f, 0.f};
                 }
             }
             if (part == 0) row_c[r] = fac;
@@ -317,17 +320,20 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
 #pragma unroll
             for (int y = 0; y < RT; y++) {
                 const int room = lim[y] - p0 - 4 * g;
+                if (edge) {
+#pragma unroll
+                    for (int t = 0; t < G::PT; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            s[y][t][i] = ((hv >> (16 * t + i)) & 1) & (uint32_t)(16 * t + i <= room) ? s[y][t][i] : -INFINITY;
+                }
                 float top = -INFINITY;
-                bool sees[4 * G::PT];
 #pragma unroll
                 for (int t = 0; t < G::PT; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        sees[4 * t + i] = !edge || (((hv >> (16 * t + i)) & 1) && 16 * t + i <= room);
-                        top = fmaxf(top, sees[4 * t + i] ? s[y][t][i] * fac[y] : -INFINITY);
-                    }
-                top = row16_max(top);
-                const float na = fminf(W.a[y], kShift - top);
+                    for (int i = 0; i < 4; i++) top = fmaxf(top, s[y][t][i]);
+                top = row16_max(top) * fac[y];
+                const float na = fminf(W.a[y], kShift == 0.0f ? -top : reference(top, kShift));
                 const float corr = na == INFINITY ? 1.0f : exp2_hw(na - W.a[y]);
                 W.a[y] = na;
                 W.l[y] *= corr;
@@ -337,8 +343,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                     for (int i = 0; i < 4; i++) {
                         // no score above -infinity: no weight, but a NaN stays one
                         const float z = s[y][t][i];
-                        float v = na == INFINITY ? (z == z ? 0.0f : z) : exp2_hw(fmaf(z, fac[y], na));
-                        v = sees[4 * t + i] ? v : 0.0f;
+                        const float v = na == INFINITY ? (z == z ? 0.0f : z) : exp2_hw(fmaf(z, fac[y], na));
                         p[y][4 * t + i] = v;
                         W.l[y] += v;
                     }
@@ -691,6 +696,7 @@ Plan plan(const PagesView &kv, const BatchView &b, const AttnPagedArgs &a) {
     Plan p{};
     AttnArgs &A = p.A;
     A.a = a, A.kv = kv, A.b = b, A.group = group;
+    A.scale_m = (float)std::frexp((double)a.scale * M_LOG2E, &A.scale_e);
     const size_t own = (queries + b.n_seqs - 1) / b.n_seqs, cap = (size_t)b.max_pages << kv.map.log2_page;
     // A block of few positions in a workgroup of its own, shared positions with it, saves the join: 9 us for 14 (13
     // rows over 14 positions), 15 for 36 (15 rows, 83 positions shared, up to 512). What a workgroup reads alone takes

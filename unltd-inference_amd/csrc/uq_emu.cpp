@@ -12,6 +12,7 @@
 #include <cstring>
 #include <vector>
 
+#include "uq_attn_ref.h"
 #include "uq_policies.h"
 #include "uq_q8k_tiles.h"
 #include "uq_serve_index.h"
@@ -426,5 +427,31 @@ int uq_emu_page_row(int n_pages, int n_head_kv, int log2_page, int page, int j, 
 long long uq_emu_run_start(long long T, int G, int w) { return run_start(T, G, w); }
 int uq_emu_run_owner(long long T, int G, long long u) { return run_owner(T, G, u); }
 int uq_emu_blocks_of(int n, int group, int RB) { return blocks_of(n, group, RB); }
+
+// The paged attention's running reference over tiles of one query's scores z (times 2^exp: in powers of two): the sum of
+// the weights as it stands at the end, and the largest exponent that a weight was held with. move: the reference moves
+// where the largest would pass it (uq_attn_many.hip), else with every larger one (below 0).
+double uq_emu_softmax(const float *z, int n, int tile, int exp, float shift, float move, double *largest) {
+    const float fac = ldexpf(1.0f, exp);
+    float a = INFINITY;
+    double l = 0.0;
+    *largest = -INFINITY;
+    for (int t = 0; t < n; t += tile) {
+        const int end = t + tile < n ? t + tile : n;
+        float top = -INFINITY;
+        for (int i = t; i < end; i++) top = fmaxf(top, z[i]);
+        top *= fac;
+        const float to = reference(top, shift);
+        const float na = move < 0.0f ? fminf(a, to) : top + a > move ? to : a;
+        l *= na == INFINITY ? 1.0 : exp2((double)(na - a));
+        a = na;
+        for (int i = t; i < end && a < INFINITY; i++) {
+            const double e = fmaf(z[i], fac, a);
+            *largest = e > *largest ? e : *largest;
+            l += exp2(e);
+        }
+    }
+    return l;
+}
 
 }  // extern "C"
