@@ -98,3 +98,31 @@ def test_scores_far_and_near_in_one_row(dtype, kernel, order):
         least = (low @ v) / (high.sum())
         most = (high @ v) / (low.sum())
         assert np.all(got[r] >= 0.999 * least) and np.all(got[r] <= 1.001 * most)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+def test_scores_of_zero_under_any_scale(dtype, kernel):
+    """Keys of zero: the mean of the values, whatever the queries and the scale."""
+    heads, rows, room = KERNELS[kernel]
+    rng = np.random.default_rng(kernel + 5)
+    c, q = steps(rng, dtype, heads, rows, room, 0)
+    c.k[:] = 0
+    for size, scale in ((1e30, 1e30), (3e38, -1e38), (1e-38, 1.7e38), (1.0, -1.7e38), (1e-30, 1e-38)):
+        got = attend(c, (q * 0.2 * size).astype(np.float32), heads, scale)
+        want, bound = largest_of(c, np.ones_like(q), heads, 1.0)
+        assert np.all(np.abs(got - want) <= bound), (size, scale)
+
+
+@pytest.mark.parametrize("kernel", range(len(KERNELS)))
+def test_scales_that_meet_small_queries(kernel):
+    """A scale of 2^126 and queries of 2^-126 times ordinary ones are the ordinary attention, bit for bit; an f16
+    cache (an f32 cache's products would lie below the least normal number)."""
+    heads, rows, room = KERNELS[kernel]
+    rng = np.random.default_rng(kernel + 6)
+    c = M.Cache(rng, "f16", 1, 64, 16, rows, [300], room=room)
+    q = (8 * rng.integers(-2 ** 12, 2 ** 12, (c.n_rows, heads, 64)) * 2.0 ** -12).astype(np.float32)
+    want = attend(c, q, heads, 0.125)
+    for x in (40, 100, 120):
+        got = attend(c, (q * 2.0 ** -x).astype(np.float32), heads, 0.125 * 2.0 ** x)
+        assert np.array_equal(got.view(np.int32), want.view(np.int32)), x

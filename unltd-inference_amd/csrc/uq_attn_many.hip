@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
         // 16 at a time by way of the wave's part of LDS: rows are read whole, and by the lanes of a query from there
         const int at_q = (w.lo + (in ? num / A.group : rb * RB / A.group)) * A.a.n_head + kvh * A.group + (in ? num : rb * RB) % A.group;
         h8 qh[KC], ql[KC];
-        float fac = ldexpf(1.0f, A.scale_e);
+        float fac;
         uint8_t *const own = lds + wave * 16384;
         {
             constexpr int LQ = HD / 4, RL = 64 / LQ, J = 16 / RL;  // lanes of a query, queries of a load, loads
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
                 }
                 wave_fence();
             }
-            fac = fmaxf(ldexpf(fac, exps - 15), 0x1p-126f);  // above zero: a masked score's -infinity stays one
+            fac = score_factor(A.scale_e + exps - 15);
         }
 
         // Tile t into buffer b of the keys or values: LI loads a wave; what is no position brings any row. Their rows

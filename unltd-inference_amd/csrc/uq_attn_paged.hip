@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
             } else if (part == 0) {
                 row_lim[r] = in && w.len >= 0 ? max(-1, w.len - w.n + (row - w.lo)) : -1;
             }
-            float fac = ldexpf(1.0f, A.scale_e);
+            float fac = score_factor(A.scale_e);
             if constexpr (F16) {
                 constexpr int C = (HD / 8 + 15) / 16;
                 float v[C][8];
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                 top = lanes_max<16>(top);
                 // |q| < 2^ex; not finite: left as it is, its terms are not finite either
                 const int ex = top > 0 && top < 0x7F800000u ? __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 15;
-                fac = fmaxf(ldexpf(fac, ex - 15), 0x1p-126f);  // above zero: a masked score's -infinity stays one
+                fac = score_factor(A.scale_e + ex - 15);
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const int ch = part + 16 * c;
@@ -195,10 +195,11 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                     }
                 }
             } else {
+                const float m = ldexpf(A.scale_m, A.scale_e - min(127, max(-126, A.scale_e)));  // what the factor leaves
 #pragma unroll
                 for (int c = 0; c < HD / 64; c++) {
                     const int ch = part + 16 * c;
-                    ((f4 *)lds)[y * HD * 4 + (ch >> 2) * 64 + (ch & 3) * 16 + (r & 15)] = in ? (f4) * (const f4u *)(q + 4 * ch) * A.scale_m : f4{0.f, 0.f, 0.f, 0.f};
+                    ((f4 *)lds)[y * HD * 4 + (ch >> 2) * 64 + (ch & 3) * 16 + (r & 15)] = in ? (f4) * (const f4u *)(q + 4 * ch) * m : f4{0.f, 0.f, 0.f, 0.f};
                 }
             }
             if (part == 0) row_c[r] = fac;

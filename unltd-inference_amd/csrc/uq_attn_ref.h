@@ -17,6 +17,13 @@ namespace uq {
 
 constexpr float kFar = 0x1p22f;
 
+// The factor 2^e of a query's scores, a normal number: a score of zero stays
+// zero, a masked score's -infinity stays one. What the limits change are
+// scores of no size, or so far apart that one weight is all: sums of products
+// of f16 terms are zero or 2^-48 to 2^41 in size (an f32 cache's queries take
+// what the limits leave).
+UQ_HD float score_factor(int e) { return ldexpf(1.0f, e < -126 ? -126 : e > 127 ? 127 : e); }
+
 UQ_HD float reference(float top, float shift) { return (fabsf(top) < kFar ? shift : 0.0f) - top; }
 
 }  // namespace uq
