@@ -58,7 +58,7 @@ typedef struct uq_seq_batch {
     const int32_t *d_row_start; /* [n_seqs + 1] */
     const int32_t *d_len;       /* [n_seqs] */
     const int32_t *d_pages;     /* [n_seqs][max_pages] */
-    size_t max_pages;           /* max_pages * page_size below 2^31 */
+    size_t max_pages;           /* max_pages * page_size at most 2^31 - 2^16 */
 } uq_seq_batch;
 
 /* Position rotation of a head's first n_rot values, as the per-row entry

@@ -24,6 +24,8 @@ constexpr size_t kMaxRows = 1u << 23;  // of a call: a grid of 256 threads each 
 constexpr size_t kMaxSeqs = 65535;     // a grid dimension of the verification
 constexpr size_t kMaxPairs = 1u << 25; // rows times heads of the attention: a grid of 64 threads each, likewise
 constexpr size_t kMaxVocab = 1u << 24;
+// Positions of a table: the kernels' int counts run up to a block of tiles past the last one.
+constexpr size_t kMaxPositions = (size_t)INT_MAX + 1 - 65536;
 
 // need_len: the call reads lengths and pages as well as row starts.
 uq_status view_batch(const char *fn, const uq_seq_batch *b, bool need_len, uq::BatchView *v) {
@@ -54,9 +56,9 @@ uq_status view_pages(const char *fn, const uq_kv_pages *kv, const uq_seq_batch *
     if (((uintptr_t)kv->d_k | (uintptr_t)kv->d_v) % 16)
         return set_error(UQ_ERR_ARG, "%s: cache arrays are not 16-byte aligned", fn);
     UQ_TRY(view_batch(fn, b, true, bv));
-    if (b->max_pages > (size_t)INT_MAX / kv->page_size)
-        return set_error(UQ_ERR_ARG, "%s: a table of %zu pages of %zu reaches 2^31 positions", fn, b->max_pages,
-                         kv->page_size);
+    if (b->max_pages > kMaxPositions / kv->page_size)
+        return set_error(UQ_ERR_ARG, "%s: a table of %zu pages of %zu has more than 2^31 - 2^16 positions", fn,
+                         b->max_pages, kv->page_size);
     bv->max_pages = (int)b->max_pages;
     int lg = 0;
     while (((size_t)1 << lg) < kv->page_size) lg++;

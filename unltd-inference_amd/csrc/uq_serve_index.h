@@ -21,7 +21,7 @@ UQ_HD SeqRows seq_rows(int a, int b, int n_rows) {
 }
 
 // A sequence's length: lengths below 0 hold nothing, those beyond the table
-// end with it (cap = max_pages * page_size < 2^31).
+// end with it (cap = max_pages * page_size, at most 2^31 - 2^16).
 UQ_HD int seq_len(int len, int cap) { return len < 0 ? 0 : len > cap ? cap : len; }
 
 // Page geometry: the row of (page, kv head, slot) counts head_dim values.
