@@ -117,13 +117,20 @@ uq_status uq_kv_append_d(const uq_kv_pages *kv, const uq_seq_batch *batch, const
  * results are those of shared_len = 0 up to the order of the sums. Other
  * sequences' table entries of whole shared pages are not read.
  *
- * Numerics: f32 results of f32 sums over exact products of f32 queries and
- * weights (an f16 cache: each query and weight as two f16 terms, within 2^-22
- * of it), in a fixed order: a call repeated gives the same bits.
+ * Numerics: f32 results of f32 sums over exact products of f32 queries (times
+ * the mantissa of kq_scale log2 e, rounded) and weights, in a fixed order: a
+ * call repeated gives the same bits. Over an f16 cache each of them is two f16
+ * terms, within 2^-22 of it and, where it is small, a step of f16's least
+ * numbers: a value of a query within 2^-38 of the query's largest, a weight
+ * within 2^-33 of the row's largest (2^-25 for scores beyond 2^22). So values
+ * below 2^-16 of a query's largest, and weights below 2^-11 of the row's, have
+ * fewer bits than 22.
+ * Scores times log2 e beyond f32's range are infinite.
  * What a row does not see (later positions, slots behind the length, pages
  * that are none) does not enter, whatever it holds. A row that sees no
  * position, or only scores of -infinity, is zero. Queries, and keys or values
- * that a row sees, which are not finite make its results NaN or infinite.
+ * that a row sees, which are not finite make its results NaN or infinite,
+ * keys of a score of -infinity excepted.
  *
  * The workspace (uq_attn_paged_ws_bytes, 16-byte aligned) does not depend on
  * the lengths. uq_attn_paged_ws_bytes returns 0 for arguments that the call

@@ -20,7 +20,7 @@ namespace uq {
 
 namespace {
 
-constexpr float kRef = 8.0f;    // weights are held times 2^8 or a little more:
+constexpr float kRef = 8.0f;    // weights are held times 2^8 or more (small ones within 2^-25, half the least f16):
 constexpr float kMove = 15.0f;  // the reference moves where one would pass 2^15
 
 __device__ __forceinline__ float half_max(float v) {  // over the lanes l, l ^ 32

@@ -70,8 +70,10 @@ __device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) &
 //
 // f16 cache: a query is scaled by a power of two to at most 2^15, times the
 // mantissa of the scale and log2 e, and split into two f16 terms, a weight
-// (times 2^14) likewise; products are exact and summed in f32. f32 cache: the
-// f32 matrix products.
+// (times 2^14) likewise: within 2^-22 of the value and half a step of the least
+// f16, 2^-38 of a query's largest value (held at 2^13 or more) and 2^-39 of the
+// largest weight. Products are exact and summed in f32. f32 cache: the f32
+// matrix products.
 //
 // RT is 1 or 2: of 16 or 32 queries of a KV head, columns n and n + 16.
 template <bool F16, int HD, int RT>
