@@ -119,3 +119,25 @@ def one_sees_all(rng, hd, kernel, least=16):
     q = np.zeros((c.n_rows, heads, hd), np.float32)
     q[:, :, 0] = (least - np.log2(1.37)) * np.log(2)
     return c, q, heads, floor
+
+
+def every_position(rng, dtype, rows, heads, n, hd=64, shared=0):
+    """Queries of zero over n positions: every position weighs the same, and the values, small whole numbers, say which
+    were added how often: position p adds 1 + (t // 1024) % 3 to columns t % 32 and 32 + (t // 32) % 32 of its tile t of
+    32. Returns (cache, queries, exact results, tolerance). A sum takes at most 800 roundings of f32 in o and as many in
+    l (of its workgroup's tiles one after another, of the workgroups)."""
+    c = M.Cache(rng, dtype, 1, hd, 256, rows, [n - i for i in range(len(rows))], shared=shared)
+    p = np.arange(n)
+    t = p // 32
+    value = np.zeros((n, hd))
+    value[p, t % 32] = 1 + t // 1024 % 3
+    value[p, 32 + t // 32 % 32] = 1 + t // 1024 % 3
+    c.k[:], c.v[:] = 0, 0
+    total = np.cumsum(value, 0)
+    for b in range(len(rows)):
+        page, slot, ok = c.slots(b, c.lens[b])
+        assert ok.all()
+        c.v[page, 0, slot] = value[:c.lens[b]]
+        c.k[page, 0, slot] = rng.standard_normal((c.lens[b], hd))
+    want = np.stack([total[pos] / (pos + 1) for _, pos in c.row_positions()])
+    return c, np.zeros((c.n_rows, heads, hd), np.float32), value, np.repeat(want[:, None], heads, 1), 2 * 800 * U32 * want[:, None]

@@ -47,3 +47,13 @@ def test_keys_and_values_below_the_least_normal_f16(hd, kernel):
     assert 0 < np.abs(c.k[c.k != 0]).max() < 2.0 ** -14
     want, bound = B.attention(c, q, heads, 2.0 ** 18, roundings=8, floor=floor)
     inside(attend(c, q, heads, 2.0 ** 18), want, bound, f"{kernel} queries of {hd}")
+
+
+# ------------------------------------------------------------------------- every tile of a long cache
+
+@pytest.mark.parametrize("dtype,rows,heads,shared", [("f16", [2], 4, 0), ("f32", [2], 4, 0), ("f16", [40], 4, 0), ("f16", [10], 4, 0),
+                                                     ("f32", [40], 4, 0), ("f16", [1] * 3, 4, 69500), ("f32", [1] * 3, 4, 69500),
+                                                     ("f16", [2] * 20, 4, 69632)])
+def test_every_position_of_a_long_cache_counts_once(dtype, rows, heads, shared):
+    c, q, _, want, tolerance = B.every_position(np.random.default_rng(len(rows)), dtype, rows, heads, 70001, shared=shared)
+    inside(attend(c, q, heads, 0.125, shared), want, tolerance + 1e-30, f"{dtype} {rows} shared {shared}")

@@ -1,5 +1,5 @@
 """What the GPU tests of batched serving can see (serve_bounds.py), on the CPU: their bounds hold the two f16 terms of
-an f16 cache and do not hold one."""
+an f16 cache and do not hold one, and no tile of positions can be left out or taken twice within them."""
 import numpy as np
 import pytest
 
@@ -34,3 +34,16 @@ def test_small_terms_are_off_by_a_part_of_the_largest(kernel):
     off = abs(B.terms(np.array([w * 2.0 ** hold]), 2)[0] / 2.0 ** hold - w)
     assert off <= 2.0 ** -22 * w + floor
     assert (off > 2.0 ** -22 * w) == (hold == 8)
+
+
+@pytest.mark.parametrize("dtype,rows,heads", [("f16", [2], 4), ("f32", [2], 4), ("f16", [40], 4)])
+def test_no_tile_can_be_left_out_or_taken_twice(dtype, rows, heads):
+    """Every tile of 16 positions, and every position by itself, for the first row of the long cache."""
+    c, q, value, want, tolerance = B.every_position(np.random.default_rng(1), dtype, rows, heads, 70001)
+    n = c.row_positions()[0][1] + 1
+    whole = np.stack([value[t:min(t + 16, n)].sum(0) for t in range(0, n, 16)])
+    for part, size in ((whole, 16.0), (value[:n], 1.0)):
+        for sign in (-1, 1):
+            got = (value[:n].sum(0) + sign * part) / (n + sign * size)
+            outside = np.abs(got - want[0, 0]) > tolerance[0, 0]
+            assert outside.any(1).all()
