@@ -117,14 +117,14 @@ uq_status uq_kv_append_d(const uq_kv_pages *kv, const uq_seq_batch *batch, const
  * results are those of shared_len = 0 up to the order of the sums. Other
  * sequences' table entries of whole shared pages are not read.
  *
- * Numerics: f32 results of f32 sums over exact products of f32 queries (times
- * the mantissa of kq_scale log2 e, rounded) and weights, in a fixed order: a
- * call repeated gives the same bits. Over an f16 cache each of them is two f16
- * terms, within 2^-22 of it and, where it is small, a step of f16's least
- * numbers: a value of a query within 2^-38 of the query's largest, a weight
- * within 2^-33 of the row's largest (2^-25 for scores beyond 2^22). So values
- * below 2^-16 of a query's largest, and weights below 2^-11 of the row's, have
- * fewer bits than 22.
+ * Numerics: f32 results of f32 sums over exact products of weights and of
+ * queries times the mantissa of kq_scale log2 e (over an f32 cache rounded to
+ * f32), in a fixed order: a call repeated gives the same bits. Over an f16
+ * cache each of them is two f16 terms, within 2^-22 of it and, where it is
+ * small, a step of f16's least numbers: a value of a query within 2^-38 of the
+ * query's largest, a weight within 2^-33 of the row's largest (2^-25 for
+ * scores beyond 2^22). So values below 2^-16 of a query's largest, and weights
+ * below 2^-11 of the row's, have fewer bits than 22.
  * Scores times log2 e beyond f32's range are infinite.
  * What a row does not see (later positions, slots behind the length, pages
  * that are none) does not enter, whatever it holds. A row that sees no

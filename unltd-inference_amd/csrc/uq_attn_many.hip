@@ -162,9 +162,9 @@ __global__ __launch_bounds__(64 * QW, 1) void attn_many_kernel(AttnArgs A) {
                     h4 hi, lo;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float x = product(ldexpf(v[j][e], 15 - ex), A.scale_m);
-                        hi[e] = (_Float16)x;
-                        lo[e] = (_Float16)(x - (float)hi[e]);
+                        _Float16 a, b;
+                        product_terms(ldexpf(v[j][e], 15 - ex), A.scale_m, a, b);
+                        hi[e] = a, lo[e] = b;
                     }
                     uint8_t *to = own + q * HD * 2 + ((((lane % LQ) >> 1) ^ (q & 7)) << 4) + 8 * (lane & 1);
                     *(h4 *)to = hi;

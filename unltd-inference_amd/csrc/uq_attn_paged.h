@@ -379,12 +379,13 @@ struct Walk {
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The f32 product, for every use of it: where the compiler sees it, a conversion to f16 is formed from the exact product
-// instead, and the two terms of a value are no longer those of one number.
-__device__ __forceinline__ float product(float a, float b) {
+// The two f16 terms of a b, not rounded to f32 before. The first is taken from a register: where the compiler sees the
+// product, it converts it from f32 in one place and from the exact product in another, and the terms do not match.
+__device__ __forceinline__ void product_terms(float a, float b, _Float16 &hi, _Float16 &lo) {
     float v = a * b;
     __asm__("" : "+v"(v));
-    return v;
+    hi = (_Float16)v;
+    lo = (_Float16)fmaf(a, b, -(float)hi);
 }
 
 }  // namespace

@@ -186,9 +186,9 @@ __global__ __launch_bounds__(kTPB, few_per_cu(HD, RT)) void attn_paged_kernel(At
                     h8 hi, lo;
 #pragma unroll
                     for (int x = 0; x < 8; x++) {
-                        const float s = product(ldexpf(v[c][x], 15 - ex), A.scale_m);
-                        hi[x] = (_Float16)s;
-                        lo[x] = (_Float16)(s - (float)hi[x]);
+                        _Float16 a, b;
+                        product_terms(ldexpf(v[c][x], 15 - ex), A.scale_m, a, b);
+                        hi[x] = a, lo[x] = b;
                     }
                     if (ch < HD / 8) {
                         h8 *dst = (h8 *)lds + y * HD * 4 + (ch >> 2) * 128 + (ch & 3) * 16 + (r & 15);
