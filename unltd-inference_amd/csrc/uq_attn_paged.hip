@@ -537,10 +537,11 @@ struct Floats<1> {
 // Joins the records of a row and head (its part of the shared positions, then
 // its own) where the workgroups have not written the result themselves: the
 // least reference first, then the sums. What it takes is round trips (row
-// starts, lengths and seg; references; sums), so a row and head has a
-// workgroup of 16 or 4 waves that take every 16th or 4th record while there
-// are few of them, and one wave of a workgroup's four where there are many
-// with few records. 16 pairs of 6 records: 5 us, of 128: 12; 8144 pairs of 4
+// starts, lengths and seg; references; then a wave's records one after
+// another, two trips each: the part's base and rows from the arguments, and
+// the record), so a row and head has a workgroup of 16 or 4 waves that take
+// every 16th or 4th record while there are few of them, and one wave of a
+// workgroup's four where there are many with few records. 16 pairs of 6 records: 5 us, of 128: 12; 8144 pairs of 4
 // or 5: 14.5 us (37 MB read, 8 written).
 template <int HD, int WAVES>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kernel(AttnArgs A, int pairs) {
@@ -620,7 +621,6 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void attn_join_kerne
             l += f * al.y;
         }
         const int n = min(64, (total - i0 + WAVES - 1) / WAVES);
-#pragma unroll 8
         for (int k = 0; k < n; k++) {
             const Values x = *(const Values *)(A.rec_o + rec(i0 + WAVES * k) * HD + E * lane);
             const float fk = __int_as_float(lane_of(__float_as_int(f), k));

@@ -355,13 +355,14 @@ __device__ __forceinline__ int drawing_lane(const Passed &o) {
 // in it. Rounded running sums need not ascend where a weight is zero or at the
 // joints of the tree, so a token needs weight of its own to be drawn, and
 // where no sum exceeds the threshold the last one with weight is it. The
-// time is round trips (the chunks' sums; the refused token; its chunk of p and
-// q): a wave needs no barriers between them (64 sequences of 152064 tokens:
-// 4.5 us; a workgroup of four waves with its scans in LDS: 15).
-constexpr int kKeep = 8;  // chunks' sums of a lane kept in registers: a vocabulary of 2^18
+// time is round trips (a lane's chunks' sums, one after another; the refused
+// token; its chunk of p and q): a wave needs no barriers between them (64
+// sequences of 152064 tokens: 4.5 us; a workgroup of four waves with its scans
+// in LDS: 15).
+constexpr int kKeep = 8;  // chunks' sums of a lane read once, and kept (in scratch memory): a vocabulary of 2^18
 __global__ __launch_bounds__(64) void verify_draw_kernel(VerifyArgs a) {
     const int s = blockIdx.x, lane = threadIdx.x;
-    // every lane a run of chunks; loads before anything waits for one
+    // every lane a run of chunks
     const double2 *sums = a.sums + (size_t)s * a.chunks;
     const int per = (a.chunks + 63) / 64, c0 = min(a.chunks, lane * per), c1 = min(a.chunks, c0 + per);
     double2 keep[kKeep], t = make_double2(0.0, 0.0);
