@@ -11,8 +11,8 @@
 // the shadow of the products: the first product of tile t + 1 runs while tile
 // t's weights are formed, the second takes over while the other half is. A
 // tile then costs the LDS 160 KB of a CU's traffic in 4000 cycles. 509 rows of
-// 16 heads of 256 values over 4096 positions: 90 us; 48 rows of them over
-// 16384 shared positions: 52 us, in two blocks of 128 queries a KV head with
+// 16 heads of 256 values over 4096 positions: 92 us; 48 rows of them over
+// 16384 shared positions: 53 us, in two blocks of 128 queries a KV head with
 // the second half empty; 25 MB of records written at its end.
 #include "uq_attn_paged.h"
 #include "uq_mfma.h"
