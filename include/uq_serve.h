@@ -1,16 +1,22 @@
 /*
  * uq_serve.h -- batched serving over a paged KV cache: the new rows (tokens)
  * of several sequences of different lengths through the parts of an attention
- * layer that depend on their positions, and the verification of drafted
- * tokens. No counterpart in the reference, which runs one sequence over
- * contiguous caches (crates/unltd-generation/src/qwen35_forward.rs:585-671)
- * and decodes greedily (greedy.rs:18-65).
+ * layer that depend on their positions and of a GatedDeltaNet layer that
+ * depend on their states, the verification of drafted tokens and the log
+ * probabilities of given ones. No counterpart in the reference, which runs one
+ * sequence over contiguous caches and states
+ * (crates/unltd-generation/src/qwen35_forward.rs:333-543, :585-671) and
+ * decodes greedily (greedy.rs:18-65).
  *
  *   rows -> projections (uq_gemm / uq_gemm_q8k over all rows)
- *        -> uq_kv_append_d   (q / k norms, rotation, k and v into the pages)
- *        -> uq_attn_paged_d  (attention of the rows over the pages, gate)
- *        -> output projection, FFN, head, uq_softmax_d
- *        -> uq_draft_verify_d
+ *        -> an attention layer:
+ *             uq_kv_append_d   (q / k norms, rotation, k and v into the pages)
+ *             uq_attn_paged_d  (attention of the rows over the pages, gate)
+ *           a GatedDeltaNet layer:
+ *             uq_gdn_conv_d    (convolution, silu, q / k norms, gates)
+ *             uq_gdn_rule_d    (gated delta rule, gated norm)
+ *        -> output projection, FFN, head
+ *        -> uq_softmax_d, uq_draft_verify_d; uq_logprobs_d
  *
  * Every entry point takes device pointers of the current HIP device and a
  * stream of it (NULL: its null stream), is asynchronous on that stream,
@@ -168,6 +174,133 @@ size_t uq_draft_verify_ws_bytes(const uq_seq_batch *batch, size_t vocab);
 uq_status uq_draft_verify_d(int32_t *d_accepted, int32_t *d_next, const float *d_p, size_t p_row, const float *d_q,
                             size_t q_row, const int32_t *d_tokens, const float *d_u, const uq_seq_batch *batch,
                             size_t vocab, void *d_ws, size_t ws_bytes, void *stream);
+
+/* The states of one GatedDeltaNet layer, a slot for each sequence: what
+ * uq_gdn_layer_step_d carries from token to token, one after another.
+ * Sequence b begins with the state of slot d_from[b] (outside [0, n_slots):
+ * zeros, a new sequence) and leaves its last one in slot d_to[b] (outside:
+ * nowhere, as for drafts that are not verified yet: a second call with the
+ * accepted rows takes the state further). Several sequences may begin with one
+ * slot, as continuations of one prompt do. Two sequences that end in one slot
+ * leave there any part of either's state; one that begins with a slot that
+ * another of the call ends in gets unspecified results. A sequence without
+ * rows writes nothing. */
+typedef struct uq_gdn_states {
+    float *d_conv;  /* [n_slots][conv_kernel][channels], channels = (2 n_qk_heads + n_v_heads) head_dim:
+                       rows 0 .. conv_kernel - 2 are the last inputs; the last row is neither read nor written */
+    float *d_state; /* [n_slots][n_v_heads][head_dim][head_dim], 16-byte aligned */
+    size_t n_slots; /* n_slots * n_v_heads below 2^31 */
+    size_t n_qk_heads, n_v_heads; /* 1 .. 1024 each; value head h has query and key head h % n_qk_heads */
+    size_t head_dim;              /* 64 or 128 */
+    size_t conv_kernel;           /* 2 .. 9 */
+    const int32_t *d_from, *d_to; /* [n_seqs] */
+} uq_gdn_states;
+
+/* A batch's rows before the convolution, as the projections leave them.
+ * Strides are in floats. */
+typedef struct uq_gdn_rows {
+    const float *d_qkv; /* [n_rows][channels], rows qkv_row apart: query heads, key heads, value heads */
+    size_t qkv_row;
+    const float *d_conv1d; /* [channels][conv_kernel] */
+    float eps;             /* of the q / k norms */
+    float *d_out;          /* [n_rows][channels] */
+    const float *d_beta_raw, *d_alpha; /* [n_rows][n_v_heads], rows raw_row apart; both NULL: no gates */
+    size_t raw_row;                    /* 0: n_v_heads */
+    const float *d_dt_bias, *d_a; /* [n_v_heads] */
+    float *d_beta, *d_gate;       /* [n_rows][n_v_heads] */
+} uq_gdn_rows;
+
+/* The convolution of every row over its sequence's last conv_kernel inputs
+ * (those before its rows from the window), silu, and the query and key heads
+ * divided by max(their 2-norm, eps) (steps 4 and 5 of recr_layer,
+ * qwen35_forward.rs:427-464); the windows taken on; and the rows' gates
+ * (:405-419): beta = sigmoid(beta_raw), gate = softplus(alpha + dt_bias) a.
+ *
+ * Numerics: f32, the convolution's sum in the taps' order; silu, the norms and
+ * the gates add up to 16 roundings (2^-24) of their values. Norms' sums of
+ * squares beyond f32's range are infinite, as uq_l2_norm_rows'. A row's
+ * values that are not finite reach the rows that convolve them and, in query
+ * and key heads, the head.
+ * d_out may not overlap the rows or the windows. Only n_seqs, n_rows and
+ * d_row_start of the batch are read, and d_conv, not d_state.
+ * Errors: UQ_ERR_ARG (null pointers, shapes beyond the limits above),
+ * UQ_ERR_LEN (n_v_heads no multiple of n_qk_heads, a row stride below the
+ * row). */
+uq_status uq_gdn_conv_d(const uq_gdn_states *states, const uq_seq_batch *batch, const uq_gdn_rows *rows, void *stream);
+
+/* A batch's rows before the delta rule. Strides are in floats. */
+typedef struct uq_gdn_heads {
+    const float *d_q, *d_k; /* head h of row r at r * q_row (k_row) + h * head_dim, h < n_qk_heads */
+    const float *d_v;       /* likewise, h < n_v_heads */
+    size_t q_row, k_row, v_row;
+    const float *d_gate, *d_beta; /* [n_rows][n_v_heads] */
+    float scale;
+    const float *d_norm; /* rms norm weights [head_dim]; NULL: no norm */
+    float eps;
+    const float *d_z; /* head h of row r at r * z_row + h * head_dim; NULL: no gate */
+    size_t z_row;
+} uq_gdn_heads;
+
+/* The gated delta rule (uq_gdn_fused_step, uq_ops.h) of every row of a
+ * sequence in order, for each value head h with its query q, key k, value v,
+ * gate g and beta:
+ *   S <- exp(g) S;  S <- S + k (beta (v - S^T k))^T;  out = scale S^T q,
+ * then, where given, out <- rmsnorm(out) d_norm and out <- out silu(d_z), the
+ * gated norm of qwen35_forward.rs:495-511. d_out is [n_rows][n_v_heads]
+ * [head_dim] and may not overlap the inputs or the states.
+ *
+ * most_rows: the most rows of a sequence, where the caller knows it (0: it
+ * does not). It decides how the call is divided, never what it computes: a
+ * sequence may have more.
+ *
+ * Numerics: f32, within some 1e-6 of the largest result for keys of norm 1,
+ * gates at most 0 and betas of 0 to 1, however many rows. Gates above 0 and
+ * results beyond f32's range: unspecified for the sequence's head from the
+ * start of those 64 rows on. Values that are not finite make the results of
+ * their head from their row on, and its state, NaN, infinite or unspecified;
+ * earlier rows, other heads and other sequences do not see them.
+ *
+ * Only n_seqs, n_rows and d_row_start of the batch are read, and d_state, not
+ * d_conv. The workspace (uq_gdn_rule_ws_bytes, 16-byte aligned) does not
+ * depend on the row starts; uq_gdn_rule_ws_bytes returns 0 for arguments that
+ * the call refuses. Errors: UQ_ERR_ARG (null pointers, shapes beyond the limits
+ * above, a workspace too small, scale not finite), UQ_ERR_LEN (n_v_heads no
+ * multiple of n_qk_heads, a row stride below the row). */
+size_t uq_gdn_rule_ws_bytes(const uq_gdn_states *states, const uq_seq_batch *batch, size_t most_rows);
+uq_status uq_gdn_rule_d(float *d_out, const uq_gdn_states *states, const uq_seq_batch *batch,
+                        const uq_gdn_heads *heads, size_t most_rows, void *d_ws, size_t ws_bytes, void *stream);
+
+/* Results of uq_logprobs_d; any may be NULL. */
+typedef struct uq_logprobs {
+    float *d_logprob;     /* [n_rows]: the given token's */
+    int32_t *d_rank;      /* [n_rows]: tokens before it in the order below */
+    float *d_entropy;     /* [n_rows], in nats */
+    int32_t *d_top_id;    /* [n_rows][n_top]: the first tokens in that order */
+    float *d_top_logprob; /* [n_rows][n_top] */
+    size_t n_top;         /* 0 .. 64 */
+} uq_logprobs;
+
+/* Of every row of logits x (rows x_row floats apart) the logarithms of the
+ * probabilities softmax(scale x): those of the tokens d_tokens[r], the
+ * entropy -sum p log p (p log p = 0 where p is 0), and the n_top likeliest
+ * tokens. Tokens are ordered by their logits, the largest first, equal ones
+ * by their number. d_tokens may be NULL where neither d_logprob nor d_rank is
+ * wanted.
+ * A logit of -infinity is a token that cannot follow: its log probability is
+ * -infinity, and it is no alternative. Alternatives that there are not are
+ * -1 with -infinity. A row without any possible token has entropy 0. A token
+ * outside [0, vocab) has log probability -infinity and rank -1. A row with a
+ * logit that is NaN or +infinity has NaN for log probabilities and entropy, and
+ * -1 for ranks and alternatives.
+ * Numerics: f32; the sums over the vocabulary run in a fixed order, up to 2^20
+ * tokens none of more than 112 roundings. Ranks and alternatives are exact.
+ * Errors: UQ_ERR_ARG (null pointers, vocab 0 or above 2^24, n_rows above 2^23,
+ * n_rows * vocab above 2^39, n_top above 64, scale not positive or above
+ * 2^127, a workspace too small or not 16-byte aligned), UQ_ERR_LEN (x_row
+ * below vocab). */
+size_t uq_logprobs_ws_bytes(size_t n_rows, size_t vocab, size_t n_top);
+uq_status uq_logprobs_d(const uq_logprobs *out, const float *d_x, size_t x_row, const int32_t *d_tokens, size_t n_rows,
+                        size_t vocab, float scale, void *d_ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

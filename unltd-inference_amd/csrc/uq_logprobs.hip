@@ -1,0 +1,313 @@
+// Log probabilities of given tokens, their ranks, the entropy and the
+// likeliest alternatives of rows of logits (uq_logprobs_d).
+//
+// One pass over a row: with m the largest logit seen so far and c = scale
+// log2 e a lane keeps
+//     l = sum 2^(c (x - m)),   s = sum 2^(c (x - m)) c (x - m),
+// from which log p(t) = scale (x_t - m) - ln l and the entropy
+// ln l - ln 2 s / l; parts of a row join by 2^(c (m' - m)). The differences
+// are formed before the product, so that logits of any size, the type's lowest
+// value among them, neither overflow nor lose the small differences.
+//
+// Rows are cut into runs of tiles of 1024 values, a wave each, without
+// barriers or LDS. Memory bounds it where there is much of it.
+#include <algorithm>
+#include <cfloat>
+
+#include "uq_device.h"
+#include "uq_serve_internal.h"
+
+namespace uq {
+
+namespace {
+
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows start at any float
+
+constexpr int kTPB = 256, kTile = 1024, kVals = kTile / 64;
+constexpr float kLeast = -300.0f;  // 2^-300 is 0: exponents below it are taken as it, so that no 0 times infinity arises
+
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// What a wave leaves of its run.
+struct Part {
+    float m, l, s;
+    int before;  // tokens before the given one
+};
+
+struct Args {
+    uq_logprobs out;
+    const float *x;
+    size_t x_row;
+    const int32_t *tokens;
+    int n_rows, vocab, n_top, tiles, run, parts;  // tiles of a row, of a wave; waves of a row
+    float scale, c;
+    Part *part;      // [n_rows][parts]
+    uint64_t *keys;  // [n_rows][parts][n_top]
+};
+
+// Tokens in their order as integers: the larger the logit, then the smaller the number, the larger the key. 0 is none.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);  // -0 as +0
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t key_of(float x, int token) { return (uint64_t)ordered(x) << 32 | (uint32_t)~token; }
+
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+// The lane before's value, 0 in the first.
+__device__ __forceinline__ uint64_t from_before(uint64_t v) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), 0x138, 0xF, 0xF, true) << 32 |
+           (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x138, 0xF, 0xF, true);  // wave_shr:1
+}
+
+// The first n_top keys seen, in order over the lanes; `least` is the last of them.
+struct Best {
+    uint64_t mine = 0, least = 0;
+    int n_top;
+    __device__ __forceinline__ explicit Best(int n) : n_top(n) {}
+    // Takes up a key a lane, those that belong among the first, largest gain first or not: whatever the order, each
+    // that is taken was among the first of those seen.
+    __device__ __forceinline__ void take(uint64_t key) {
+        const int lane = threadIdx.x & 63;
+        for (;;) {
+            const unsigned long long over = __ballot(key > least);
+            if (!over) return;
+            const int from = __builtin_ctzll(over);
+            const uint64_t k = lane_of(key, from);
+            const int at = __builtin_popcountll(__ballot(mine > k));  // keys differ: a token is seen once
+            const uint64_t shifted = from_before(mine);
+            mine = lane < at ? mine : lane == at ? k : shifted;
+            least = lane_of(mine, n_top - 1);
+            if (lane == from) key = 0;
+        }
+    }
+};
+
+// A bound that at least n lanes' values reach (its upper 16 bits are those of the n-th largest, the rest 0).
+__device__ __forceinline__ uint32_t reached_by(uint32_t v, int n) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t more = t | 1u << bit;
+        if (__builtin_popcountll(__ballot(v >= more)) >= n) t = more;
+    }
+    return t;
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
+    const int lane = threadIdx.x & 63;
+    const int w = uniform((int)(blockIdx.x * (kTPB / 64) + (threadIdx.x >> 6)));
+    const int row = w / a.parts, part = w - row * a.parts;
+    if (row >= a.n_rows) return;
+    const float *x = a.x + (size_t)row * a.x_row;
+    const int t0 = part * a.run, t1 = min(a.tiles, t0 + a.run);
+    float v[kVals], next[kVals];
+    auto load = [&](float (&d)[kVals], int tile) {  // token 256 j + 4 lane + e of the tile in d[4 j + e]
+#pragma unroll
+        for (int j = 0; j < kVals / 4; j++) {
+            const int i = tile * kTile + 256 * j + 4 * lane;
+            if (i + 4 <= a.vocab) {
+                const f4u f = *(const f4u *)(x + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[4 * j + e] = f[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[4 * j + e] = i + e < a.vocab ? x[i + e] : -INFINITY;
+            }
+        }
+    };
+    load(v, t0);
+    const int token = a.tokens ? uniform(a.tokens[row]) : -1;
+    const bool ranked = (unsigned)token < (unsigned)a.vocab;
+    const float given = ranked ? x[token] : INFINITY;
+    float m = -FLT_MAX, l = 0.0f, s = 0.0f;
+    int before = 0;
+    Best best(a.n_top);
+    for (int t = t0; t < t1; t++) {
+        if (t + 1 < t1) load(next, t + 1);
+        float top = v[0];
+#pragma unroll
+        for (int i = 1; i < kVals; i++) top = fmaxf(top, v[i]);
+        if (__ballot(top > m)) {
+            const float to = fmaxf(m, top), d = fmaxf((m - to) * a.c, kLeast), f = exp2_hw(d);
+            s = f * fmaf(d, l, s);
+            l *= f;
+            m = to;
+        }
+        float tl[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ts[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kVals; i++) {
+            const float d = (v[i] - m) * a.c, e = exp2_hw(d);
+            tl[i % 4] += e;
+            ts[i % 4] = fmaf(e, fmaxf(d, kLeast), ts[i % 4]);
+        }
+        l += (tl[0] + tl[1]) + (tl[2] + tl[3]);
+        s += (ts[0] + ts[1]) + (ts[2] + ts[3]);
+        if (ranked) {
+            const int first = t * kTile;
+            if (token >= first + kTile) {
+#pragma unroll
+                for (int i = 0; i < kVals; i++) before += __builtin_popcountll(__ballot(v[i] >= given));
+            } else if (token < first) {
+#pragma unroll
+                for (int i = 0; i < kVals; i++) before += __builtin_popcountll(__ballot(v[i] > given));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVals; i++) {
+                    const int id = first + 256 * (i / 4) + 4 * lane + i % 4;
+                    before += __builtin_popcountll(__ballot(v[i] > given || (v[i] == given && id < token)));
+                }
+            }
+        }
+        if constexpr (TOP) {
+            // Later tokens of equal logits come after those held: only larger ones are looked at once the list is
+            // full. Where many lanes have some (a run's first tile), those below a bound that n_top lanes reach
+            // with their largest cannot be among the first.
+            uint32_t bound = (uint32_t)(best.least >> 32);
+            const uint32_t most = ordered(top);
+            const unsigned long long over = __ballot(top > -INFINITY && most > bound);
+            if (over) {
+                bound = bound ? bound + 1 : ordered(-INFINITY) + 1;
+                if (__builtin_popcountll(over) >= a.n_top) bound = max(bound, reached_by(most, a.n_top));
+#pragma unroll
+                for (int i = 0; i < kVals; i++) {
+                    const uint32_t o = ordered(v[i]);
+                    const bool in = o >= bound && v[i] == v[i];
+                    if (__ballot(in)) best.take(in ? (uint64_t)o << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4) : 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kVals; i++) v[i] = next[i];
+    }
+    // the lanes' sums
+    const float all = [&] {
+        float r = m;
+        for (int d = 1; d < 64; d *= 2) r = fmaxf(r, __shfl_xor(r, d));
+        return r;
+    }();
+    const float d = fmaxf((m - all) * a.c, kLeast), f = exp2_hw(d);
+    s = wave_sum(f * fmaf(d, l, s));
+    l = wave_sum(f * l);
+    const size_t o = (size_t)row * a.parts + part;
+    if (lane == 0) a.part[o] = Part{all, l, s, before};
+    if constexpr (TOP)
+        if (lane < a.n_top) a.keys[o * a.n_top + lane] = best.mine;
+}
+
+// A wave a row: joins its parts and writes the results.
+template <bool TOP>
+__global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
+    const int row = blockIdx.x, lane = threadIdx.x;
+    const Part *parts = a.part + (size_t)row * a.parts;
+    float m = -FLT_MAX, l = 0.0f, s = 0.0f;
+    int before = 0;
+    for (int i = lane; i < a.parts; i += 64) {
+        const Part p = parts[i];
+        const float to = fmaxf(m, p.m), d = fmaxf((m - to) * a.c, kLeast), dp = fmaxf((p.m - to) * a.c, kLeast);
+        const float f = exp2_hw(d), fp = exp2_hw(dp);
+        s = f * fmaf(d, l, s) + fp * fmaf(dp, p.l, p.s);
+        l = f * l + fp * p.l;
+        m = to;
+        before += p.before;
+    }
+    float all = m;
+    for (int d = 1; d < 64; d *= 2) all = fmaxf(all, __shfl_xor(all, d));
+    const float d = fmaxf((m - all) * a.c, kLeast), f = exp2_hw(d);
+    s = wave_sum(f * fmaf(d, l, s));
+    l = wave_sum(f * l);
+    for (int k = 1; k < 64; k *= 2) before += __shfl_xor(before, k);
+    const bool sound = l == l && l < INFINITY;  // no NaN and no infinite logit
+    const float ln_l = logf(l), nan = __uint_as_float(0x7FC00000u);
+    auto log_p = [&](float x) { return !sound ? nan : l > 0.0f ? fmaf(x - all, a.scale, -ln_l) : -INFINITY; };
+    if (lane == 0) {
+        const int token = a.tokens ? a.tokens[row] : -1;
+        const bool in = (unsigned)token < (unsigned)a.vocab;
+        if (a.out.d_logprob)
+            a.out.d_logprob[row] = in ? log_p(a.x[(size_t)row * a.x_row + token]) : sound ? -INFINITY : nan;
+        if (a.out.d_rank) a.out.d_rank[row] = in && sound ? before : -1;
+        // the terms are not positive but for their roundings
+        if (a.out.d_entropy) a.out.d_entropy[row] = !sound ? nan : l > 0.0f ? fmaxf(0.0f, ln_l - 0.693147182f * (s / l)) : 0.0f;
+    }
+    if constexpr (TOP) {
+        const uint64_t *keys = a.keys + (size_t)row * a.parts * a.n_top;
+        const int n = a.parts * a.n_top;
+        Best best(a.n_top);
+        constexpr int N = 16;  // keys of a lane at a time
+        for (int i0 = 0; i0 < n; i0 += 64 * N) {
+            uint64_t k[N], top = 0;
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const int i = i0 + 64 * j + lane;
+                k[j] = i < n ? keys[i] : 0;
+                top = k[j] > top ? k[j] : top;
+            }
+            const unsigned long long over = __ballot(top > best.least);
+            if (!over) continue;
+            uint64_t bound = best.least + 1;
+            if (__builtin_popcountll(over) >= a.n_top) {
+                const uint64_t r = (uint64_t)reached_by((uint32_t)(top >> 32), a.n_top) << 32;
+                bound = r > bound ? r : bound;
+            }
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (__ballot(k[j] >= bound)) best.take(k[j] >= bound ? k[j] : 0);
+        }
+        if (lane < a.n_top) {
+            const bool is = sound && best.mine != 0;
+            const uint32_t u = (uint32_t)(best.mine >> 32);
+            const float x = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+            const size_t o = (size_t)row * a.n_top + lane;
+            if (a.out.d_top_id) a.out.d_top_id[o] = is ? (int)~(uint32_t)best.mine : -1;
+            if (a.out.d_top_logprob) a.out.d_top_logprob[o] = !sound ? nan : is ? log_p(x) : -INFINITY;
+        }
+    }
+}
+
+// Tiles of a wave: one while the rows fill less than two rounds of 16 waves a CU, then more, up to 16.
+struct Shape {
+    int tiles, run, parts;
+};
+Shape shape_of(int n_rows, int vocab) {
+    Shape s;
+    s.tiles = (vocab + kTile - 1) / kTile;
+    const long long all = (long long)s.tiles * n_rows;
+    s.run = (int)std::min(16LL, std::max(1LL, all / (2 * 16 * 256)));
+    s.parts = (s.tiles + s.run - 1) / s.run;
+    return s;
+}
+
+}  // namespace
+
+size_t logprobs_ws_bytes(int n_rows, int vocab, int n_top) {
+    const Shape s = shape_of(n_rows, vocab);
+    return (size_t)n_rows * s.parts * (sizeof(Part) + (size_t)n_top * sizeof(uint64_t));
+}
+
+hipError_t launch_logprobs(const uq_logprobs &out, const float *x, size_t x_row, const int32_t *tokens, int n_rows,
+                           int vocab, float scale, void *ws, hipStream_t s) {
+    if (n_rows == 0) return hipSuccess;
+    const Shape h = shape_of(n_rows, vocab);
+    const bool top = out.n_top && (out.d_top_id || out.d_top_logprob);
+    Part *part = (Part *)ws;
+    const Args a{out,     x,     x_row, tokens,  n_rows,           vocab, top ? (int)out.n_top : 0,
+                 h.tiles, h.run, h.parts, scale, (float)(scale * 1.4426950408889634), part, (uint64_t *)(part + (size_t)n_rows * h.parts)};
+    const long long waves = (long long)n_rows * h.parts, per = kTPB / 64;
+    const dim3 grid((unsigned)((waves + per - 1) / per));
+    if (top)
+        hipLaunchKernelGGL(logprobs_kernel<true>, grid, dim3(kTPB), 0, s, a);
+    else
+        hipLaunchKernelGGL(logprobs_kernel<false>, grid, dim3(kTPB), 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (top)
+        hipLaunchKernelGGL(logprobs_join_kernel<true>, dim3((unsigned)n_rows), dim3(64), 0, s, a);
+    else
+        hipLaunchKernelGGL(logprobs_join_kernel<false>, dim3((unsigned)n_rows), dim3(64), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace uq

@@ -1,5 +1,5 @@
 // C ABI of batched serving (include/uq_serve.h): argument checks, then the
-// launches of uq_serve.hip and uq_attn_paged.hip.
+// launches of uq_serve.hip, uq_attn_paged.hip, uq_gdn.hip and uq_logprobs.hip.
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -84,6 +84,43 @@ uq_status view_attn(const char *fn, const uq_kv_pages *kv, const uq_seq_batch *b
     if (shared_len > b->max_pages * kv->page_size)
         return set_error(UQ_ERR_ARG, "%s: shared_len %zu beyond a table of %zu positions", fn, shared_len,
                          b->max_pages * kv->page_size);
+    return UQ_OK;
+}
+
+// The states and the batch of a GatedDeltaNet call; conv, state: which of the arrays it uses.
+uq_status view_states(const char *fn, const uq_gdn_states *st, const uq_seq_batch *b, bool conv, bool state,
+                      uq::StatesView *v, uq::BatchView *bv) {
+    if (!st) return set_error(UQ_ERR_ARG, "%s: null states", fn);
+    UQ_TRY(view_batch(fn, b, false, bv));
+    if (st->n_qk_heads == 0 || st->n_qk_heads > 1024 || st->n_v_heads == 0 || st->n_v_heads > 1024)
+        return set_error(UQ_ERR_ARG, "%s: %zu query/key and %zu value heads outside 1 .. 1024", fn, st->n_qk_heads,
+                         st->n_v_heads);
+    if (st->n_v_heads % st->n_qk_heads)
+        return set_error(UQ_ERR_LEN, "%s: n_v_heads %zu is not a multiple of n_qk_heads %zu", fn, st->n_v_heads,
+                         st->n_qk_heads);
+    if (st->head_dim != 64 && st->head_dim != 128)
+        return set_error(UQ_ERR_ARG, "%s: head_dim %zu is not 64 or 128", fn, st->head_dim);
+    if (st->conv_kernel < 2 || st->conv_kernel > 9)
+        return set_error(UQ_ERR_ARG, "%s: conv_kernel %zu outside 2 .. 9", fn, st->conv_kernel);
+    if (st->n_slots > (size_t)INT_MAX / st->n_v_heads)
+        return set_error(UQ_ERR_ARG, "%s: %zu slots of %zu heads reach 2^31", fn, st->n_slots, st->n_v_heads);
+    if (st->n_slots && ((conv && !st->d_conv) || (state && !st->d_state)))
+        return set_error(UQ_ERR_ARG, "%s: null states array", fn);
+    if (state && (uintptr_t)st->d_state % 16)
+        return set_error(UQ_ERR_ARG, "%s: the states are not 16-byte aligned", fn);
+    if (b->n_seqs && (!st->d_from || !st->d_to)) return set_error(UQ_ERR_ARG, "%s: null slots", fn);
+    *v = uq::StatesView{(int)st->n_slots,  (int)st->n_qk_heads,  (int)st->n_v_heads,
+                        (int)st->head_dim, (int)st->conv_kernel, (int)((2 * st->n_qk_heads + st->n_v_heads) * st->head_dim),
+                        st->d_conv,        st->d_state,          st->d_from,
+                        st->d_to};
+    return UQ_OK;
+}
+
+uq_status check_logprobs(const char *fn, size_t n_rows, size_t vocab, size_t n_top) {
+    if (vocab == 0 || vocab > kMaxVocab) return set_error(UQ_ERR_ARG, "%s: vocab %zu outside 1 .. 2^24", fn, vocab);
+    if (n_rows > kMaxRows) return set_error(UQ_ERR_ARG, "%s: %zu rows above %zu", fn, n_rows, kMaxRows);
+    if (n_rows * vocab > (size_t)1 << 39) return set_error(UQ_ERR_ARG, "%s: more than 2^39 logits", fn);  // a grid
+    if (n_top > 64) return set_error(UQ_ERR_ARG, "%s: %zu alternatives above 64", fn, n_top);
     return UQ_OK;
 }
 
@@ -177,6 +214,81 @@ uq_status uq_draft_verify_d(int32_t *d_accepted, int32_t *d_next, const float *d
     if (ws_bytes < need) return set_error(UQ_ERR_ARG, "%s: workspace of %zu bytes below %zu", fn, ws_bytes, need);
     return hip_st(uq::launch_draft_verify(d_accepted, d_next, d_p, p_row, d_q, q_row, d_tokens, d_u, bv, (int)vocab,
                                           d_ws, (hipStream_t)stream),
+                  fn);
+}
+
+uq_status uq_gdn_conv_d(const uq_gdn_states *states, const uq_seq_batch *batch, const uq_gdn_rows *rows, void *stream) {
+    const char *fn = "gdn_conv_d";
+    uq::StatesView sv;
+    uq::BatchView bv;
+    UQ_TRY(view_states(fn, states, batch, true, false, &sv, &bv));
+    if (!rows) return set_error(UQ_ERR_ARG, "%s: null rows", fn);
+    uq_gdn_rows r = *rows;
+    if (r.raw_row == 0) r.raw_row = states->n_v_heads;
+    if (batch->n_rows > 1 && r.qkv_row < (size_t)sv.channels)
+        return set_error(UQ_ERR_LEN, "%s: qkv_row %zu below %d channels", fn, r.qkv_row, sv.channels);
+    if ((r.d_beta_raw == nullptr) != (r.d_alpha == nullptr))
+        return set_error(UQ_ERR_ARG, "%s: one of d_beta_raw and d_alpha", fn);
+    if (r.d_alpha && (!r.d_dt_bias || !r.d_a || !r.d_beta || !r.d_gate))
+        return set_error(UQ_ERR_ARG, "%s: gates without d_dt_bias, d_a, d_beta or d_gate", fn);
+    if (r.d_alpha && batch->n_rows > 1 && r.raw_row < states->n_v_heads)
+        return set_error(UQ_ERR_LEN, "%s: raw_row %zu below %zu heads", fn, r.raw_row, states->n_v_heads);
+    if (bv.n_rows == 0 || bv.n_seqs == 0) return UQ_OK;
+    if (!r.d_qkv || !r.d_conv1d || !r.d_out) return set_error(UQ_ERR_ARG, "%s: null device pointer", fn);
+    if (r.d_out == r.d_qkv) return set_error(UQ_ERR_ARG, "%s: d_out is d_qkv", fn);
+    return hip_st(uq::launch_gdn_conv(sv, bv, r, (hipStream_t)stream), fn);
+}
+
+size_t uq_gdn_rule_ws_bytes(const uq_gdn_states *states, const uq_seq_batch *batch, size_t most_rows) {
+    uq::StatesView sv;
+    uq::BatchView bv;
+    if (view_states("gdn_rule_ws_bytes", states, batch, false, true, &sv, &bv)) return 0;
+    return uq::gdn_rule_ws_bytes(sv, bv, most_rows);
+}
+
+uq_status uq_gdn_rule_d(float *d_out, const uq_gdn_states *states, const uq_seq_batch *batch,
+                        const uq_gdn_heads *heads, size_t most_rows, void *d_ws, size_t ws_bytes, void *stream) {
+    const char *fn = "gdn_rule_d";
+    uq::StatesView sv;
+    uq::BatchView bv;
+    UQ_TRY(view_states(fn, states, batch, false, true, &sv, &bv));
+    if (!heads) return set_error(UQ_ERR_ARG, "%s: null heads", fn);
+    const size_t qk = states->n_qk_heads * states->head_dim, v = states->n_v_heads * states->head_dim;
+    if (batch->n_rows > 1 && (heads->q_row < qk || heads->k_row < qk || heads->v_row < v))
+        return set_error(UQ_ERR_LEN, "%s: q_row %zu, k_row %zu or v_row %zu below the heads of a row", fn, heads->q_row,
+                         heads->k_row, heads->v_row);
+    if (heads->d_z && batch->n_rows > 1 && heads->z_row < v)
+        return set_error(UQ_ERR_LEN, "%s: z_row %zu below %zu", fn, heads->z_row, v);
+    if (!std::isfinite(heads->scale)) return set_error(UQ_ERR_ARG, "%s: scale is not finite", fn);
+    if (bv.n_rows == 0 || bv.n_seqs == 0) return UQ_OK;
+    if (!d_out || !heads->d_q || !heads->d_k || !heads->d_v || !heads->d_gate || !heads->d_beta || !d_ws)
+        return set_error(UQ_ERR_ARG, "%s: null device pointer", fn);
+    if ((uintptr_t)d_ws % 16) return set_error(UQ_ERR_ARG, "%s: the workspace is not 16-byte aligned", fn);
+    const size_t need = uq::gdn_rule_ws_bytes(sv, bv, most_rows);
+    if (ws_bytes < need) return set_error(UQ_ERR_ARG, "%s: workspace of %zu bytes below %zu", fn, ws_bytes, need);
+    return hip_st(uq::launch_gdn_rule(d_out, sv, bv, *heads, most_rows, d_ws, (hipStream_t)stream), fn);
+}
+
+size_t uq_logprobs_ws_bytes(size_t n_rows, size_t vocab, size_t n_top) {
+    if (check_logprobs("logprobs_ws_bytes", n_rows, vocab, n_top)) return 0;
+    return uq::logprobs_ws_bytes((int)n_rows, (int)vocab, (int)n_top);
+}
+
+uq_status uq_logprobs_d(const uq_logprobs *out, const float *d_x, size_t x_row, const int32_t *d_tokens, size_t n_rows,
+                        size_t vocab, float scale, void *d_ws, size_t ws_bytes, void *stream) {
+    const char *fn = "logprobs_d";
+    if (!out) return set_error(UQ_ERR_ARG, "%s: null results", fn);
+    UQ_TRY(check_logprobs(fn, n_rows, vocab, out->n_top));
+    if (n_rows > 1 && x_row < vocab) return set_error(UQ_ERR_LEN, "%s: x_row %zu below vocab %zu", fn, x_row, vocab);
+    if (!(scale > 0.0f && scale <= 0x1p127f)) return set_error(UQ_ERR_ARG, "%s: scale is outside (0, 2^127]", fn);
+    if ((out->d_logprob || out->d_rank) && n_rows && !d_tokens) return set_error(UQ_ERR_ARG, "%s: null tokens", fn);
+    if (n_rows == 0) return UQ_OK;
+    if (!d_x || !d_ws) return set_error(UQ_ERR_ARG, "%s: null device pointer", fn);
+    if ((uintptr_t)d_ws % 16) return set_error(UQ_ERR_ARG, "%s: the workspace is not 16-byte aligned", fn);
+    const size_t need = uq::logprobs_ws_bytes((int)n_rows, (int)vocab, (int)out->n_top);
+    if (ws_bytes < need) return set_error(UQ_ERR_ARG, "%s: workspace of %zu bytes below %zu", fn, ws_bytes, need);
+    return hip_st(uq::launch_logprobs(*out, d_x, x_row, d_tokens, (int)n_rows, (int)vocab, scale, d_ws,
+                                      (hipStream_t)stream),
                   fn);
 }
 

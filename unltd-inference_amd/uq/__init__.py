@@ -148,6 +148,11 @@ SIGNATURES = {
     "uq_attn_paged_d": ([_P, _P, _P, _P, _S, _S, C.c_float, _P, _S, _S, _P, _S, _P], _I),
     "uq_draft_verify_ws_bytes": ([_P, _S], _S),
     "uq_draft_verify_d": ([_P, _P, _P, _S, _P, _S, _P, _P, _P, _S, _P, _S, _P], _I),
+    "uq_gdn_conv_d": ([_P, _P, _P, _P], _I),
+    "uq_gdn_rule_ws_bytes": ([_P, _P, _S], _S),
+    "uq_gdn_rule_d": ([_P, _P, _P, _P, _S, _P, _S, _P], _I),
+    "uq_logprobs_ws_bytes": ([_S, _S, _S], _S),
+    "uq_logprobs_d": ([_P, _P, _S, _P, _S, _S, C.c_float, _P, _S, _P], _I),
 }
 
 
