@@ -251,7 +251,13 @@ typedef struct uq_gdn_heads {
  *
  * most_rows: the most rows of a sequence, where the caller knows it (0: it
  * does not). It decides how the call is divided, never what it computes: a
- * sequence may have more.
+ * sequence may have more. Sequences of few rows take them one by one, those
+ * of many in chunks of 64 whose products run on the matrix cores:
+ *   (I + A) U = diag(beta) (V - diag(e^G) K S),  A[i][j] = beta_i e^(G_i - G_j) k_i.k_j  (j < i),
+ *   out = scale (diag(e^G) Q S + P U),           P[i][j] = e^(G_i - G_j) q_i.k_j         (j <= i),
+ *   S <- e^G_63 S + (diag(e^(G_63 - G)) K)^T U,  G the running sum of the gates.
+ * Both are deterministic; they differ by the order of f32 sums. The gates'
+ * sums are held in 64 bits, exponentials are of differences.
  *
  * Numerics: f32, within some 1e-6 of the largest result for keys of norm 1,
  * gates at most 0 and betas of 0 to 1, however many rows. Gates above 0 and

@@ -221,6 +221,30 @@ def test_rule_of_few_rows(nqk, nv, hd, rows, pad):
     r.check()
 
 
+@pytest.mark.parametrize("nqk,nv,hd,rows,pad", [
+    (1, 1, 64, [64], 0), (2, 4, 128, [65, 31, 32, 33, 1], 5), (1, 3, 64, [300, 0, 40, 7, 128, 63], 1), (3, 3, 128, [129, 100], 0),
+    (2, 2, 64, [40] * 40 + [1] * 300 + [70], 2), (16, 16, 64, [1, 200, 1], 0), (1, 2, 128, [1030], 3)])
+def test_rule_of_many_rows(nqk, nv, hd, rows, pad):
+    c = M.Case(nv + hd + len(rows), nqk, nv, hd, 4, rows, pad=pad)
+    for most in (0, max(rows)):
+        r = Rule(c, most, pad=pad)
+        r.run()
+        r.check()
+
+
+def test_rule_of_many_rows_without_norm_and_gate():
+    r = Rule(M.Case(41, 2, 4, 128, 4, [70, 3, 200]), 0, (False, False), 1)
+    r.run()
+    r.check(False)
+
+
+def test_rule_of_many_rows_hardly_forgetting():
+    """Decays near 1 and far from each other over many chunks: the state is as old as the sequence."""
+    r = Rule(M.Case(42, 1, 2, 64, 4, [700], decay=(-12, 0)), 0)
+    r.run()
+    r.check()
+
+
 @pytest.mark.parametrize("most", [0, 1, 10 ** 6])
 def test_rule_of_more_rows_than_it_was_told(most):
     r = Rule(M.Case(21, 2, 4, 64, 4, [1, 90, 3]), most)
@@ -228,9 +252,10 @@ def test_rule_of_more_rows_than_it_was_told(most):
     r.check()
 
 
-def test_rule_slots():
-    c = M.Case(22, 2, 4, 64, 4, [2, 3, 1, 20, 5], frm=[-1, 3, 3, 99, 0], to=[1, 2, 5, -7, 0])
-    r = Rule(c, 20)
+@pytest.mark.parametrize("rows", [[2, 3, 1, 20, 5], [70, 100, 33, 64, 130]])
+def test_rule_slots(rows):
+    c = M.Case(22, 2, 4, 64, 4, rows, frm=[-1, 3, 3, 99, 0], to=[1, 2, 5, -7, 0])
+    r = Rule(c, max(rows))
     r.run()
     r.check()
 

@@ -95,6 +95,52 @@ __device__ __forceinline__ Tile find_tile(const BatchView &b, int tile, int leas
     return Tile{-1, 0, 0, 0};
 }
 
+// Sequences of at least `least` rows that go by chunks, numbered through: l of
+// them lie before this one. Its chunks' slots in the workspace begin at
+// lo / 64 + l, so that none share one and none needs the others' counts.
+struct Long {
+    int seq, lo, n, slot;  // seq -1: there is none
+};
+constexpr int kChunk = 64;
+UQ_HD int chunk_slot(int lo, int l) { return lo / kChunk + l; }
+// SLOT: the sequence that holds slot `want`; else the one that `want` lie before.
+template <bool SLOT>
+__device__ __forceinline__ Long find_long(const BatchView &b, int want, int least) {
+    const int lane = threadIdx.x & 63;
+    int run = 0;
+    for (int c = 0; c < b.n_seqs; c += 256) {
+        const int i0 = c + 4 * lane;
+        int start[5], mine = 0;
+#pragma unroll
+        for (int e = 0; e < 5; e++) start[e] = b.row_start[min(i0 + e, b.n_seqs)];
+        SeqRows r[4];
+        bool is[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            r[e] = seq_rows(start[e], start[e + 1], b.n_rows);
+            is[e] = i0 + e < b.n_seqs && r[e].n >= least;
+            mine += is[e];
+        }
+        const int upto = wave_scan_i(mine);
+        int l = run + upto - mine;
+        Long t{-1, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int slot = chunk_slot(r[e].lo, l);
+            if (is[e] && t.seq < 0 && (SLOT ? want >= slot && want < slot + (r[e].n + kChunk - 1) / kChunk : l == want))
+                t = Long{i0 + e, r[e].lo, r[e].n, slot};
+            l += is[e];
+        }
+        const unsigned long long here = __ballot(t.seq >= 0);
+        if (here) {
+            const int from = __builtin_ctzll(here);
+            return Long{lane_of(t.seq, from), lane_of(t.lo, from), lane_of(t.n, from), lane_of(t.slot, from)};
+        }
+        run += lane_of(upto, 63);
+    }
+    return Long{-1, 0, 0, 0};
+}
+
 // ---- the convolution --------------------------------------------------------
 
 constexpr int kConvTPB = 256;
@@ -215,7 +261,9 @@ struct RuleArgs {
     StatesView st;
     BatchView b;
     uq_gdn_heads h;
-    int chunked;  // sequences of at least so many rows go by chunks
+    int chunked;      // sequences of at least so many rows go by chunks
+    int longs, slots; // of those at most, and of their chunks
+    float *ws;        // [slots][nv][kChunkFloats]
 };
 
 // The epilogue of a head's row: rms norm and gate, lane l its values
@@ -335,6 +383,354 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
     }
 }
 
+// ---- the delta rule by chunks ---------------------------------------------------
+//
+// Of 64 rows with the state S before them and G_i the gates' sum up to row i,
+// the corrections U solve
+//     (I + A) U = diag(beta) (V - diag(e^G) K S),  A[i][j] = beta_i e^(G_i - G_j) k_i.k_j  (j < i),
+// and  out = scale (diag(e^G) Q S + P U),          P[i][j] = e^(G_i - G_j) q_i.k_j         (j <= i),
+//      S <- e^G_63 S + K^T (diag(e^(G_63 - G)) U).
+// What does not depend on S, T = (I + A)^-1 diag(beta) and P, is formed for all
+// chunks at once (gdn_prep_kernel); gdn_chunks_kernel then takes a sequence's
+// chunks one after another, 16 columns of a head's state a workgroup, which
+// nothing of another column enters.
+//
+// Products run on the f32 matrix cores, 16x16x4, whose depth is a sum over k
+// = lane / 16: taken as 4 (lane / 16) + e in the e-th of four products, the left
+// operand is 4 neighbours of a row, one load, and a product's result (rows 4
+// (lane / 16) + e, column lane % 16) is a right operand as it is.
+//
+// A row with a key, beta or gate that is not finite leaves the products
+// (first: the first such row), and so do rows of a column from its first
+// correction on that is not: 0 times NaN would carry it to earlier rows.
+// Their results are set to NaN.
+
+struct ChunkWs {  // of a chunk and head, in floats
+    static constexpr int T = 0, P = kChunk * kChunk, ge = 2 * kChunk * kChunk, gl = ge + kChunk, first = gl + kChunk;
+};
+constexpr int kChunkFloats = ChunkWs::first + 4;
+constexpr float kLeastGate = -1000.0f;  // e^-1000 of any f32 is 0: gates below it are taken as it, so that differences are numbers
+
+__device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+__device__ __forceinline__ f4 mfma4(const f4 &a, const f4 &b, f4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+// T and P of a chunk and head. The 10 tiles on and below the diagonal of K K^T
+// and Q K^T are five for each wave: column w of the one and 3 - w of the
+// other. The triangle's inverse: a wave inverts a diagonal tile row after row,
+// a column a lane, then goes down its column of tiles,
+//     T_ij = -T_ii sum over j <= k < i of A_ik T_kj,
+// as substitution would, in whose order errors do not grow.
+constexpr int kPrepTPB = 256;
+template <int HD>
+__global__ __launch_bounds__(kPrepTPB) void gdn_prep_kernel(RuleArgs a) {
+    constexpr int KC = HD / 16, LD = kChunk + 4;
+    __shared__ __align__(16) float A[kChunk][LD], D[4][16][20];
+    __shared__ double G[kChunk];
+    __shared__ float beta[kChunk];
+    __shared__ unsigned bad_k[4];
+    __shared__ unsigned long long bad_g;
+    const int head = blockIdx.y, hq = head % a.st.nqk;
+    const Long s = find_long<true>(a.b, (int)blockIdx.x, a.chunked);
+    if (s.seq < 0) return;
+    const int c0 = ((int)blockIdx.x - s.slot) * kChunk, n = min(kChunk, s.n - c0);
+    const size_t row0 = (size_t)s.lo + c0;
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4;
+    float *ws = a.ws + ((size_t)blockIdx.x * a.st.nv + head) * kChunkFloats;
+    auto frag = [&](f4 (&f)[KC], const float *p, size_t stride, int tile) {
+        const float *r = p + (row0 + min(16 * tile + m, n - 1)) * stride + (size_t)hq * HD + 4 * g;
+#pragma unroll
+        for (int c = 0; c < KC; c++) f[c] = *(const f4u *)(r + 16 * c);
+    };
+    auto product = [&](const f4 (&x)[KC], const f4 (&y)[KC]) {
+        f4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+        for (int c = 0; c < KC; c += 2) s0 = mfma4(x[c], y[c], s0), s1 = mfma4(x[c + 1], y[c + 1], s1);
+        return s0 + s1;
+    };
+    f4 y[KC], x[KC];
+    frag(y, a.h.d_k, a.h.k_row, wave);
+    if (wave == 0) {
+        const bool in = lane < n;
+        float gt = in ? a.h.d_gate[(row0 + lane) * a.st.nv + head] : 0.0f, bt = in ? a.h.d_beta[(row0 + lane) * a.st.nv + head] : 0.0f;
+        if (gt < kLeastGate) gt = kLeastGate;
+        const bool ok = finite32(gt) && finite32(bt);
+        const unsigned long long no = __ballot(!ok);
+        double sum = ok ? (double)gt : 0.0;
+        sum += dpp_d<0x111>(sum);
+        sum += dpp_d<0x112>(sum);
+        sum += dpp_d<0x114>(sum);
+        sum += dpp_d<0x118>(sum);
+        sum += dpp_d<0x142, 0xA>(sum);
+        sum += dpp_d<0x143, 0xC>(sum);
+        G[lane] = sum;
+        beta[lane] = ok ? bt : 0.0f;
+        if (lane == 0) bad_g = no;
+        const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63), __builtin_amdgcn_readlane(__double2loint(sum), 63));
+        ws[ChunkWs::ge + lane] = expf((float)sum);
+        ws[ChunkWs::gl + lane] = expf((float)(last - sum));
+    }
+    {
+        bool ok = true;
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) ok = ok && finite32(y[c][e]);
+        const unsigned long long no = __ballot(!ok);
+        if (lane == 0) bad_k[wave] = (unsigned)((no | no >> 16 | no >> 32 | no >> 48) & 0xFFFF);
+    }
+    __syncthreads();
+    const unsigned long long bad = bad_g | bad_k[0] | (unsigned long long)bad_k[1] << 16 | (unsigned long long)bad_k[2] << 32 | (unsigned long long)bad_k[3] << 48;
+    const int first = bad ? __builtin_ctzll(bad) : kChunk;
+    if (threadIdx.x == 0) *(int *)(ws + ChunkWs::first) = first;
+    // A's tiles (r, wave), then P's (r, 3 - wave), r not above their column
+    auto decay = [&](int i, int j) { return expf((float)(G[i] - G[j])); };
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if (r < wave) continue;
+        frag(x, a.h.d_k, a.h.k_row, r);
+        const f4 d = product(x, y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = 16 * r + 4 * g + e, j = 16 * wave + m;
+            A[i][j] = j < i && i < first ? beta[i] * decay(i, j) * d[e] : 0.0f;
+        }
+    }
+    frag(y, a.h.d_k, a.h.k_row, 3 - wave);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if (r < 3 - wave) continue;
+        frag(x, a.h.d_q, a.h.q_row, r);
+        const f4 d = product(x, y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int i = 16 * r + 4 * g + e, j = 16 * (3 - wave) + m;
+            ws[ChunkWs::P + i * kChunk + j] = j <= i ? a.h.scale * decay(i, j) * d[e] : 0.0f;
+        }
+    }
+    __syncthreads();
+    // the diagonal tile's inverse, column m in every lane of it
+    {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float sum = i == m ? 1.0f : 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; j++) sum = fmaf(-A[16 * wave + i][16 * wave + j], v[j], sum);
+            v[i] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (g == i / 4) D[wave][i][m] = v[i];
+    }
+    __syncthreads();
+    f4 t[4];
+    const float bm = 16 * wave + m < first ? beta[16 * wave + m] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (i < wave) continue;
+        if (i == wave) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) t[i][e] = D[wave][4 * g + e][m];
+        } else {
+            f4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < i; k++)
+                if (k >= wave) sum = mfma4(*(const f4 *)&A[16 * i + m][16 * k + 4 * g], t[k], sum);
+            const f4 zero{0.f, 0.f, 0.f, 0.f};
+            t[i] = -mfma4(*(const f4 *)&D[i][m][4 * g], sum, zero);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) ws[ChunkWs::T + (16 * i + 4 * g + e) * kChunk + 16 * wave + m] = t[i][e] * bm;
+    }
+}
+
+// A sequence's chunks in order: four waves, wave w rows 16 w and on of the
+// chunk and HD / 4 rows of the state. Operands of the next chunk are loaded as
+// soon as this one's are used.
+constexpr int kColumns = 16;
+template <int HD>
+__global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
+    constexpr int KC = HD / 16, ST = HD / 64, NB = HD / kColumns;
+    __shared__ f4 lS[KC][64], lX[4][64], lU[4][64];
+    __shared__ int lBad[4];
+    // a head's column blocks on one XCD (workgroup i runs on XCD i % 8), whose L2 they share their operands in
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, pair = at / NB * 8 + xcd, head = pair % a.st.nv, hq = head % a.st.nqk;
+    if (pair >= a.longs * a.st.nv) return;
+    const Long s = find_long<false>(a.b, pair / a.st.nv, a.chunked);
+    if (s.seq < 0) return;
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4;
+    const int col = at % NB * kColumns + m;
+    const int chunks = (s.n + kChunk - 1) / kChunk;
+    f4 S[ST];
+    const int from = a.st.from[s.seq], to = a.st.to[s.seq];
+    auto state_row = [&](int t) { return HD / 4 * wave + 16 * t + 4 * g; };
+#pragma unroll
+    for (int t = 0; t < ST; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            S[t][e] = (unsigned)from < (unsigned)a.st.n_slots
+                          ? a.st.state[(((size_t)from * a.st.nv + head) * HD + state_row(t) + e) * HD + col]
+                          : 0.0f;
+    f4 k[KC], q[KC], T[4], P[4], kt[ST][4], v, ge, gl[4];
+    float whole;
+    int first;
+    // a chunk's row, the last one where there is none: what has no row has beta 0 and corrections of 0
+    auto row_of = [&](int c, int r) { return (size_t)s.lo + min(c * kChunk + r, s.n - 1); };
+    auto ws_of = [&](int c) { return a.ws + ((size_t)(s.slot + c) * a.st.nv + head) * kChunkFloats; };
+    auto load_k = [&](int c) {
+        const float *p = a.h.d_k + row_of(c, 16 * wave + m) * a.h.k_row + (size_t)hq * HD + 4 * g;
+#pragma unroll
+        for (int i = 0; i < KC; i++) k[i] = *(const f4u *)(p + 16 * i);
+    };
+    auto load_q = [&](int c) {
+        const float *p = a.h.d_q + row_of(c, 16 * wave + m) * a.h.q_row + (size_t)hq * HD + 4 * g;
+#pragma unroll
+        for (int i = 0; i < KC; i++) q[i] = *(const f4u *)(p + 16 * i);
+    };
+    auto load_v = [&](int c) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = a.h.d_v[row_of(c, 16 * wave + 4 * g + e) * a.h.v_row + (size_t)head * HD + col];
+        ge = *(const f4 *)(ws_of(c) + ChunkWs::ge + 16 * wave + 4 * g);
+        first = *(const int *)(ws_of(c) + ChunkWs::first);
+    };
+    auto load_t = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i <= wave) T[i] = *(const f4 *)(ws_of(c) + ChunkWs::T + (16 * wave + m) * kChunk + 16 * i + 4 * g);
+    };
+    auto load_p = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i <= wave) P[i] = *(const f4 *)(ws_of(c) + ChunkWs::P + (16 * wave + m) * kChunk + 16 * i + 4 * g);
+    };
+    auto load_kt = [&](int c) {  // K transposed: rows of the state, 4 neighbouring rows of the chunk
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            gl[i] = *(const f4 *)(ws_of(c) + ChunkWs::gl + 16 * i + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float *p = a.h.d_k + row_of(c, 16 * i + 4 * g + e) * a.h.k_row + (size_t)hq * HD + HD / 4 * wave + m;
+#pragma unroll
+                for (int t = 0; t < ST; t++) kt[t][i][e] = p[16 * t];
+            }
+        }
+        whole = ws_of(c)[ChunkWs::ge + kChunk - 1];
+    };
+    load_k(0), load_v(0), load_q(0), load_t(0), load_p(0), load_kt(0);
+    const f4 zero{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < chunks; c++) {
+        const int next = min(c + 1, chunks - 1);
+#pragma unroll
+        for (int t = 0; t < ST; t++) lS[ST * wave + t][lane] = S[t];
+        __syncthreads();
+        // X = V - diag(e^G) K S
+        f4 s0 = zero, s1 = zero;
+#pragma unroll
+        for (int i = 0; i < KC; i += 2) s0 = mfma4(k[i], lS[i][lane], s0), s1 = mfma4(k[i + 1], lS[i + 1][lane], s1);
+        load_k(next);
+        f4 x;
+        bool ok = true;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] = fmaf(-ge[e], s0[e] + s1[e], v[e]);
+            ok = ok && finite32(x[e]);
+        }
+        const int to_bad = first;
+        const f4 eg = ge;
+        load_v(next);
+        lX[wave][lane] = x;
+        const bool any = __ballot(!ok) != 0;
+        if (lane == 0) lBad[wave] = any;
+        s0 = zero, s1 = zero;
+#pragma unroll
+        for (int i = 0; i < KC; i += 2) s0 = mfma4(q[i], lS[i][lane], s0), s1 = mfma4(q[i + 1], lS[i + 1][lane], s1);
+        load_q(next);
+        __syncthreads();
+        // U = T X
+        const bool bad = uniform(lBad[0] | lBad[1] | lBad[2] | lBad[3]) || to_bad < kChunk;
+        int stop = to_bad;  // the column's rows from here on are not numbers
+        if (bad) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 3; e >= 0; e--)
+                    if (!finite32(lX[i][lane][e])) stop = min(stop, 16 * i + 4 * g + e);
+            stop = min(stop, __shfl_xor(stop, 16));
+            stop = min(stop, __shfl_xor(stop, 32));
+        }
+        f4 u = zero;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i > wave) continue;
+            f4 xi = lX[i][lane];
+            if (bad) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) xi[e] = 16 * i + 4 * g + e < stop ? xi[e] : 0.0f;
+            }
+            u = mfma4(T[i], xi, u);
+        }
+        load_t(next);
+        lU[wave][lane] = u;
+        f4 o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = eg[e] * a.h.scale * (s0[e] + s1[e]);
+        __syncthreads();
+        // out and the state
+        f4 ub[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            ub[i] = lU[i][lane];
+            if (i <= wave) o = mfma4(P[i], ub[i], o);
+        }
+        load_p(next);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int r = 16 * wave + 4 * g + e;
+            const float w = bad && r >= stop ? __uint_as_float(0x7FC00000u) : o[e];
+            if (c * kChunk + r < s.n) a.out[(((size_t)s.lo + c * kChunk + r) * a.st.nv + head) * HD + col] = w;
+        }
+#pragma unroll
+        for (int t = 0; t < ST; t++) S[t] *= whole;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f4 ug = ub[i] * gl[i];
+#pragma unroll
+            for (int t = 0; t < ST; t++) S[t] = mfma4(kt[t][i], ug, S[t]);
+        }
+        if (bad && stop < kChunk) {
+#pragma unroll
+            for (int t = 0; t < ST; t++) S[t] = f4{1.f, 1.f, 1.f, 1.f} * __uint_as_float(0x7FC00000u);
+        }
+        load_kt(next);
+    }
+    if ((unsigned)to < (unsigned)a.st.n_slots) {
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) a.st.state[(((size_t)to * a.st.nv + head) * HD + state_row(t) + e) * HD + col] = S[t][e];
+    }
+}
+
+// The epilogue of the rows that went by chunks: a workgroup a chunk and head.
+template <int HD>
+__global__ __launch_bounds__(256) void gdn_finish_kernel(RuleArgs a) {
+    const int head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const Long s = find_long<true>(a.b, (int)blockIdx.x, a.chunked);
+    if (s.seq < 0) return;
+    const int c0 = ((int)blockIdx.x - s.slot) * kChunk, n = min(kChunk, s.n - c0);
+    for (int r = wave; r < n; r += 4) {
+        const size_t row = (size_t)s.lo + c0 + r;
+        float v[HD / 64];
+#pragma unroll
+        for (int e = 0; e < HD / 64; e++) v[e] = a.out[(row * a.st.nv + head) * HD + HD / 64 * lane + e];
+        finish_row<HD>(a, row, head, v);
+    }
+}
+
 }  // namespace
 
 hipError_t launch_gdn_conv(const StatesView &st, const BatchView &b, const uq_gdn_rows &r, hipStream_t s) {
@@ -349,18 +745,52 @@ hipError_t launch_gdn_conv(const StatesView &st, const BatchView &b, const uq_gd
     return hipGetLastError();
 }
 
-size_t gdn_rule_ws_bytes(const StatesView &st, const BatchView &b, size_t most_rows) { return 16; }
+// Sequences of this many rows and more go by chunks.
+constexpr int kChunkLeast = 32;
+
+namespace {
+// How many sequences can go by chunks, and the slots of their chunks; 0 where none is expected to.
+struct Plan {
+    int longs, slots;
+};
+Plan plan_of(const BatchView &b, size_t most_rows) {
+    if (b.n_rows < kChunkLeast || (most_rows && most_rows < (size_t)kChunkLeast)) return Plan{0, 0};
+    const int longs = std::min(b.n_seqs, b.n_rows / kChunkLeast);
+    return Plan{longs, b.n_rows / kChunk + longs + 1};
+}
+}  // namespace
+
+size_t gdn_rule_ws_bytes(const StatesView &st, const BatchView &b, size_t most_rows) {
+    return 16 + (size_t)plan_of(b, most_rows).slots * st.nv * kChunkFloats * sizeof(float);
+}
+
+template <int HD>
+hipError_t launch_rule(RuleArgs a, bool some, hipStream_t s) {
+    if (a.longs) {
+        const dim3 chunks((unsigned)a.slots, (unsigned)a.st.nv);
+        hipLaunchKernelGGL(gdn_prep_kernel<HD>, chunks, dim3(kPrepTPB), 0, s, a);
+        if (hipError_t e = hipGetLastError()) return e;
+        const long long pairs = (long long)a.longs * a.st.nv, groups = (pairs + 7) / 8 * 8 * (HD / kColumns);
+        hipLaunchKernelGGL(gdn_chunks_kernel<HD>, dim3((unsigned)groups), dim3(256), 0, s, a);
+        if (hipError_t e = hipGetLastError()) return e;
+        if (a.h.d_norm || a.h.d_z) {
+            hipLaunchKernelGGL(gdn_finish_kernel<HD>, chunks, dim3(256), 0, s, a);
+            if (hipError_t e = hipGetLastError()) return e;
+        }
+    }
+    if (some) {
+        hipLaunchKernelGGL(gdn_rows_kernel<HD>, dim3((unsigned)a.st.nv, (unsigned)a.b.n_seqs), dim3(2 * HD), 0, s, a);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
+}
 
 hipError_t launch_gdn_rule(float *out, const StatesView &st, const BatchView &b, const uq_gdn_heads &h, size_t most_rows,
                            void *ws, hipStream_t s) {
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
-    const RuleArgs a{out, st, b, h, INT_MAX};
-    const dim3 grid((unsigned)st.nv, (unsigned)b.n_seqs);
-    if (st.hd == 128)
-        hipLaunchKernelGGL(gdn_rows_kernel<128>, grid, dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(gdn_rows_kernel<64>, grid, dim3(128), 0, s, a);
-    return hipGetLastError();
+    const Plan p = plan_of(b, most_rows);
+    const RuleArgs a{out, st, b, h, p.longs ? kChunkLeast : INT_MAX, p.longs, p.slots, (float *)ws};
+    return st.hd == 128 ? launch_rule<128>(a, true, s) : launch_rule<64>(a, true, s);
 }
 
 }  // namespace uq
