@@ -259,10 +259,13 @@ typedef struct uq_gdn_heads {
  * Both are deterministic; they differ by the order of f32 sums. The gates'
  * sums are held in 64 bits, exponentials are of differences.
  *
- * Numerics: f32, within some 1e-6 of the largest result for keys of norm 1,
- * gates at most 0 and betas of 0 to 1, however many rows. Gates above 0 and
- * results beyond f32's range: unspecified for the sequence's head from the
- * start of those 64 rows on. Values that are not finite make the results of
+ * Numerics: f32 sums. By chunks the products' operands are two f16 terms each,
+ * within 2^-22 of a value, or 2^-39 of the largest of its row (K, Q, T, P) or
+ * column (S, U and the values that U solves for) where it is below 2^-16 of
+ * that. For keys of norm 1, gates at most 0 and betas of 0 to 1 no error
+ * grows, however many rows; results are off by some 1e-6 of the largest.
+ * Gates above 0 and results beyond f32's range: unspecified for the sequence's
+ * head from the start of those 64 rows on. Values that are not finite make the results of
  * their head from their row on, and its state, NaN, infinite or unspecified;
  * earlier rows, other heads and other sequences do not see them.
  *
@@ -271,7 +274,7 @@ typedef struct uq_gdn_heads {
  * depend on the row starts; uq_gdn_rule_ws_bytes returns 0 for arguments that
  * the call refuses. Errors: UQ_ERR_ARG (null pointers, shapes beyond the limits
  * above, a workspace too small, scale not finite), UQ_ERR_LEN (n_v_heads no
- * multiple of n_qk_heads, a row stride below the row). */
+ * multiple of n_qk_heads, a row stride below the row, v_row above 2^24). */
 size_t uq_gdn_rule_ws_bytes(const uq_gdn_states *states, const uq_seq_batch *batch, size_t most_rows);
 uq_status uq_gdn_rule_d(float *d_out, const uq_gdn_states *states, const uq_seq_batch *batch,
                         const uq_gdn_heads *heads, size_t most_rows, void *d_ws, size_t ws_bytes, void *stream);

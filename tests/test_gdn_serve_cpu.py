@@ -66,7 +66,7 @@ def test_bad_rows_are_refused(kind, over):
 
 @pytest.mark.parametrize("kind,over", [
     ("ARG", dict(d_q=None)), ("ARG", dict(d_k=None)), ("ARG", dict(d_v=None)), ("ARG", dict(d_gate=None)), ("ARG", dict(d_beta=None)),
-    ("LEN", dict(q_row=127)), ("LEN", dict(k_row=127)), ("LEN", dict(v_row=255)), ("LEN", dict(z_row=255)), ("ARG", dict(scale=float("nan"))),
+    ("LEN", dict(q_row=127)), ("LEN", dict(k_row=127)), ("LEN", dict(v_row=255)), ("LEN", dict(v_row=(1 << 24) + 1)), ("LEN", dict(z_row=255)), ("ARG", dict(scale=float("nan"))),
     ("ARG", dict(scale=float("inf")))])
 def test_bad_heads_are_refused(kind, over):
     refused(kind, serve.gdn_rule_d, A, states(), batch(), heads(**over), A)

@@ -39,7 +39,7 @@ HIPCC_FLAGS = [
 # Matrix products with their sums in VGPRs, where one wave has a SIMD's registers to itself: the accumulation registers
 # then hold queries or tiles under way, and the vector units reach the sums without copies (attn_many_kernel with the
 # sums there: 25 registers spilled, 230 copies a tile).
-SOURCE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("uq_attn_many.hip", "uq_attn_paged.hip")}
+SOURCE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("uq_attn_many.hip", "uq_attn_paged.hip", "uq_gdn.hip")}
 
 
 def _run(cmd, verbose):

@@ -5,6 +5,8 @@
 #include <climits>
 
 #include "uq_device.h"
+#include "uq_internal.h"
+#include "uq_mfma.h"
 #include "uq_serve_internal.h"
 
 namespace uq {
@@ -263,7 +265,8 @@ struct RuleArgs {
     uq_gdn_heads h;
     int chunked;      // sequences of at least so many rows go by chunks
     int longs, slots; // of those at most, and of their chunks
-    float *ws;        // [slots][nv][kChunkFloats]
+    uint8_t *ws;      // [slots][nv] ChunkWs
+    uint8_t *kq;      // [slots][nqk] keys, then queries (KqWs)
 };
 
 // The epilogue of a head's row: rms norm and gate, lane l its values
@@ -392,342 +395,651 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
 //      S <- e^G_63 S + K^T (diag(e^(G_63 - G)) U).
 // What does not depend on S, T = (I + A)^-1 diag(beta) and P, is formed for all
 // chunks at once (gdn_prep_kernel); gdn_chunks_kernel then takes a sequence's
-// chunks one after another, 16 columns of a head's state a workgroup, which
+// chunks one after another, 16 columns of a head's state a wave, which
 // nothing of another column enters.
 //
-// Products run on the f32 matrix cores, 16x16x4, whose depth is a sum over k
-// = lane / 16: taken as 4 (lane / 16) + e in the e-th of four products, the left
-// operand is 4 neighbours of a row, one load, and a product's result (rows 4
-// (lane / 16) + e, column lane % 16) is a right operand as it is.
+// The second kernel's products run on the f16 matrix cores with two terms of
+// each operand, h + l = x 2^s within 2^-22 of it: s brings the largest value
+// of a row (left operands) or of a wave's column (right ones) to 2^13 .. 2^14,
+// so that values down to 2^-16 of it keep 22 bits and what is lost below is
+// 2^-39 of it. The products h h, h l and l h are exact and summed in f32; l l
+// is left out, 2^-22 of the product at most. The f32 matrix cores, eight times
+// slower for these three, took 7400 clocks a chunk of 16 columns and workgroup.
+//
+// A 16x16x32 product's depth is summed over lane / 16 and 8 values a lane, of
+// tiles 2 p and 2 p + 1: values 4 (lane / 16) .. + 3 of each. A result's rows
+// lie so over the lanes, so that a pair of results is a right operand as it is.
 //
 // A row with a key, beta or gate that is not finite leaves the products
 // (first: the first such row), and so do rows of a column from its first
 // correction on that is not: 0 times NaN would carry it to earlier rows.
 // Their results are set to NaN.
 
-struct ChunkWs {  // of a chunk and head, in floats
-    static constexpr int T = 0, P = kChunk * kChunk, ge = 2 * kChunk * kChunk, gl = ge + kChunk, first = gl + kChunk;
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+
+// Left operands in the workspace, pieces of 1 KB: [tile of 16 rows][pair of tiles in depth][h, l][64 lanes][8 f16].
+// The keys are read by columns as well (read_columns), 4 rows of 4 pieces of 4 columns at a time: those lie in
+// different banks when a piece's rows are turned by 4 for each group of columns.
+__device__ __forceinline__ int place(int m, int g) { return 16 * g + ((m + 4 * g) & 15); }
+struct ChunkWs {  // of a chunk and value head, in bytes
+    static constexpr int T = 0, P = 12 * 1024, vec = 24 * 1024;  // 6 pieces of h and l each: tile_piece
+    // vec, floats: factors of the rows of K S (e^G with the keys' scale), of U for the state (e^(G_63 - G) with it), of Q
+    // S, and of T's and P's rows; then e^G_63 and the first row that is left out
+    static constexpr int gx = 0, gg = 64, gq = 128, gt = 192, gp = 256, whole = 320, first = 321;
+    static constexpr int bytes = 28 * 1024;  // as many pieces for each of four waves
 };
-constexpr int kChunkFloats = ChunkWs::first + 4;
+__device__ __forceinline__ int tile_piece(int tile, int pair) { return tile < 2 ? tile : 2 * tile - 2 + pair; }
+constexpr int kq_bytes(int hd) { return kChunk * hd * 4; }  // of the keys or queries of a chunk
+
 constexpr float kLeastGate = -1000.0f;  // e^-1000 of any f32 is 0: gates below it are taken as it, so that differences are numbers
 
 __device__ __forceinline__ bool finite32(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }  // NaN above infinity
+template <int N>
+__device__ __forceinline__ uint32_t size_bits(const f4 (&v)[N]) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) r = max(r, size_bits(v[i][e]));
+    return r;
+}
+// Over the lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ uint32_t rows16_max(uint32_t v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(b[0], b[1]);
+}
+// The exponent ex that brings values of at most this size below 2^14: x 2^(14 - ex). Sizes below 2^-100 as it.
+__device__ __forceinline__ int scale_of(uint32_t bits) { return max(-100, __builtin_amdgcn_frexp_expf(__uint_as_float(bits))); }
+__device__ __forceinline__ float scale_up(int ex) { return ldexpf(1.0f, 14 - ex); }
+__device__ __forceinline__ float scale_down(int ex) { return ldexpf(1.0f, ex - 14); }
+// The two terms of a pair of tiles, each in one instruction that takes the product with s, a power of two, whole.
+__device__ __forceinline__ void two_terms(const f4 &a, const f4 &b, float s, h8 &h, h8 &l) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float v = e < 4 ? a[e & 3] : b[e & 3];
+        h[e] = (_Float16)fmaf(v, s, 0.0f);
+        l[e] = (_Float16)fmaf(v, s, -(float)h[e]);
+    }
+}
+// The largest size of N tiles' values but for NaN.
+template <int N>
+__device__ __forceinline__ float top_of(const f4 (&v)[N]) {
+    float r = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) r = fmaxf(fmaxf(fmaxf(r, fabsf(v[i][0])), fmaxf(fabsf(v[i][1]), fabsf(v[i][2]))), fabsf(v[i][3]));
+    return r;
+}
 __device__ __forceinline__ f4 mfma4(const f4 &a, const f4 &b, f4 c) {
 #pragma unroll
     for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
     return c;
 }
+__device__ __forceinline__ f4 mfma_h(const h8 &a, const h8 &b, const f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 
-// T and P of a chunk and head. The 10 tiles on and below the diagonal of K K^T
-// and Q K^T are five for each wave: column w of the one and 3 - w of the
-// other. The triangle's inverse: a wave inverts a diagonal tile row after row,
-// a column a lane, then goes down its column of tiles,
+// T and P of a chunk, and the keys and queries in two terms, a workgroup the
+// value heads of one query and key head. Keys and queries come to the LDS
+// once; of the 10 tiles on and below the diagonal of K K^T and of Q K^T five
+// are for each wave, column w of the one and 3 - w of the other, in f32, kept in registers
+// for the heads. The triangle's inverse: a wave inverts a diagonal tile, a
+// column a lane, its rows over the lanes' quarters, then goes down its column
+// of tiles,
 //     T_ij = -T_ii sum over j <= k < i of A_ik T_kj,
 // as substitution would, in whose order errors do not grow.
 constexpr int kPrepTPB = 256;
 template <int HD>
 __global__ __launch_bounds__(kPrepTPB) void gdn_prep_kernel(RuleArgs a) {
-    constexpr int KC = HD / 16, LD = kChunk + 4;
-    __shared__ __align__(16) float A[kChunk][LD], D[4][16][20];
+    constexpr int KC = HD / 16, LD = HD + 4, LA = kChunk + 4;
+    constexpr int kA = kChunk * LA, kRows = kChunk * LD > kA + 4 * 16 * 20 ? kChunk * LD : kA + 4 * 16 * 20, kTP = kChunk * LA + kChunk * kChunk;
+    __shared__ __align__(16) float rows0[kRows], rows1[kTP > kChunk * LD ? kTP : kChunk * LD];  // K, Q; then A and the diagonal's inverses, T and P
     __shared__ double G[kChunk];
     __shared__ float beta[kChunk];
-    __shared__ unsigned bad_k[4];
-    __shared__ unsigned long long bad_g;
-    const int head = blockIdx.y, hq = head % a.st.nqk;
+    __shared__ int ex_k[kChunk], ex_q[kChunk], first_bad;
+    float (*K)[LD] = (float (*)[LD])rows0, (*Q)[LD] = (float (*)[LD])rows1;
+    float (*A)[LA] = (float (*)[LA])rows0, (*D)[16][20] = (float (*)[16][20])(rows0 + kA);
+    float (*lT)[LA] = (float (*)[LA])rows1, (*lP)[kChunk] = (float (*)[kChunk])(rows1 + kA);
+    const int hq = blockIdx.y;
     const Long s = find_long<true>(a.b, (int)blockIdx.x, a.chunked);
     if (s.seq < 0) return;
     const int c0 = ((int)blockIdx.x - s.slot) * kChunk, n = min(kChunk, s.n - c0);
     const size_t row0 = (size_t)s.lo + c0;
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4;
-    float *ws = a.ws + ((size_t)blockIdx.x * a.st.nv + head) * kChunkFloats;
-    auto frag = [&](f4 (&f)[KC], const float *p, size_t stride, int tile) {
-        const float *r = p + (row0 + min(16 * tile + m, n - 1)) * stride + (size_t)hq * HD + 4 * g;
-#pragma unroll
-        for (int c = 0; c < KC; c++) f[c] = *(const f4u *)(r + 16 * c);
-    };
-    auto product = [&](const f4 (&x)[KC], const f4 (&y)[KC]) {
-        f4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0;
-#pragma unroll
-        for (int c = 0; c < KC; c += 2) s0 = mfma4(x[c], y[c], s0), s1 = mfma4(x[c + 1], y[c + 1], s1);
-        return s0 + s1;
-    };
-    f4 y[KC], x[KC];
-    frag(y, a.h.d_k, a.h.k_row, wave);
-    if (wave == 0) {
-        const bool in = lane < n;
-        float gt = in ? a.h.d_gate[(row0 + lane) * a.st.nv + head] : 0.0f, bt = in ? a.h.d_beta[(row0 + lane) * a.st.nv + head] : 0.0f;
-        if (gt < kLeastGate) gt = kLeastGate;
-        const bool ok = finite32(gt) && finite32(bt);
-        const unsigned long long no = __ballot(!ok);
-        double sum = ok ? (double)gt : 0.0;
-        sum += dpp_d<0x111>(sum);
-        sum += dpp_d<0x112>(sum);
-        sum += dpp_d<0x114>(sum);
-        sum += dpp_d<0x118>(sum);
-        sum += dpp_d<0x142, 0xA>(sum);
-        sum += dpp_d<0x143, 0xC>(sum);
-        G[lane] = sum;
-        beta[lane] = ok ? bt : 0.0f;
-        if (lane == 0) bad_g = no;
-        const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63), __builtin_amdgcn_readlane(__double2loint(sum), 63));
-        ws[ChunkWs::ge + lane] = expf((float)sum);
-        ws[ChunkWs::gl + lane] = expf((float)(last - sum));
-    }
     {
-        bool ok = true;
+        constexpr int PER = HD / 4, STEP = kPrepTPB / PER;  // threads of a row, rows at a time
+        const int r0 = threadIdx.x / PER, o = 4 * (threadIdx.x % PER);
+        const float *pk = a.h.d_k + row0 * a.h.k_row + (size_t)hq * HD + o, *pq = a.h.d_q + row0 * a.h.q_row + (size_t)hq * HD + o;
+        f4 k[kChunk / STEP], q[kChunk / STEP];
 #pragma unroll
-        for (int c = 0; c < KC; c++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) ok = ok && finite32(y[c][e]);
-        const unsigned long long no = __ballot(!ok);
-        if (lane == 0) bad_k[wave] = (unsigned)((no | no >> 16 | no >> 32 | no >> 48) & 0xFFFF);
-    }
-    __syncthreads();
-    const unsigned long long bad = bad_g | bad_k[0] | (unsigned long long)bad_k[1] << 16 | (unsigned long long)bad_k[2] << 32 | (unsigned long long)bad_k[3] << 48;
-    const int first = bad ? __builtin_ctzll(bad) : kChunk;
-    if (threadIdx.x == 0) *(int *)(ws + ChunkWs::first) = first;
-    // A's tiles (r, wave), then P's (r, 3 - wave), r not above their column
-    auto decay = [&](int i, int j) { return expf((float)(G[i] - G[j])); };
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-        if (r < wave) continue;
-        frag(x, a.h.d_k, a.h.k_row, r);
-        const f4 d = product(x, y);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int i = 16 * r + 4 * g + e, j = 16 * wave + m;
-            A[i][j] = j < i && i < first ? beta[i] * decay(i, j) * d[e] : 0.0f;
+        for (int i = 0; i < kChunk / STEP; i++) {
+            const size_t r = (size_t)min(r0 + STEP * i, n - 1);
+            k[i] = *(const f4u *)(pk + r * a.h.k_row);
+            q[i] = *(const f4u *)(pq + r * a.h.q_row);
         }
-    }
-    frag(y, a.h.d_k, a.h.k_row, 3 - wave);
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        if (r < 3 - wave) continue;
-        frag(x, a.h.d_q, a.h.q_row, r);
-        const f4 d = product(x, y);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int i = 16 * r + 4 * g + e, j = 16 * (3 - wave) + m;
-            ws[ChunkWs::P + i * kChunk + j] = j <= i ? a.h.scale * decay(i, j) * d[e] : 0.0f;
+        for (int i = 0; i < kChunk / STEP; i++) {
+            const int r = r0 + STEP * i;
+            *(f4 *)&K[r][o] = k[i];
+            *(f4 *)&Q[r][o] = q[i];
+            auto row_ex = [](const f4 &v) {
+                uint32_t b = max(max(size_bits(v[0]), size_bits(v[1])), max(size_bits(v[2]), size_bits(v[3])));
+                b = max(b, dpp_u<0xB1>(b));
+                b = max(b, dpp_u<0x4E>(b));
+                b = max(b, dpp_u<0x141>(b));
+                b = max(b, dpp_u<0x140>(b));
+                if constexpr (PER == 32) {
+                    const auto x = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+                    b = max(x[0], x[1]);
+                }
+                return scale_of(b);
+            };
+            const int ek = row_ex(k[i]), eq = row_ex(q[i]);
+            if (o == 0) ex_k[r] = ek, ex_q[r] = eq;
         }
     }
     __syncthreads();
-    // the diagonal tile's inverse, column m in every lane of it
     {
-        float v[16];
+        h8 *to = (h8 *)(a.kq + ((size_t)blockIdx.x * a.st.nqk + hq) * 2 * kq_bytes(HD)) + (size_t)wave * (HD / 32) * 128;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float sum = i == m ? 1.0f : 0.0f;
+        for (int x = 0; x < 2; x++) {
+            const float up = scale_up((x ? ex_q : ex_k)[16 * wave + m]);
+            const float *r = x ? Q[16 * wave + m] : K[16 * wave + m];
 #pragma unroll
-            for (int j = 0; j < i; j++) sum = fmaf(-A[16 * wave + i][16 * wave + j], v[j], sum);
-            v[i] = sum;
+            for (int p = 0; p < HD / 32; p++) {
+                h8 h, l;
+                two_terms(*(const f4 *)(r + 32 * p + 4 * g), *(const f4 *)(r + 32 * p + 16 + 4 * g), up, h, l);
+                to[(x * (kq_bytes(HD) / 16)) + p * 128 + place(m, g)] = h;
+                to[(x * (kq_bytes(HD) / 16)) + p * 128 + 64 + place(m, g)] = l;
+            }
+        }
+    }
+    f4 dk[4], dq[4];  // tiles (r, wave) of K K^T and (r, 3 - wave) of Q K^T
+    unsigned long long bad_k = 0;
+    {
+        f4 y[KC];
+        auto frag = [&](int tile) {
+#pragma unroll
+            for (int c = 0; c < KC; c++) y[c] = *(const f4 *)&K[16 * tile + m][16 * c + 4 * g];
+        };
+        auto product = [&](const float (*X)[LD], int r) {
+            f4 d[4] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const f4 x = *(const f4 *)&X[16 * r + m][16 * c + 4 * g];
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[c][e], d[e], 0, 0, 0);
+            }
+            return (d[0] + d[1]) + (d[2] + d[3]);
+        };
+        frag(wave);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r >= wave) dk[r] = product(K, r);
+        frag(3 - wave);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (r >= 3 - wave) dq[r] = product(Q, r);
+        if (wave == 0) {  // rows with a key that is not finite
+#pragma unroll
+            for (int tile = 0; tile < 4; tile++) {
+                frag(tile);
+                const unsigned long long no = __ballot(size_bits(y) >= 0x7F800000u);
+                bad_k |= ((no | no >> 16 | no >> 32 | no >> 48) & 0xFFFF) << 16 * tile;
+            }
+        }
+    }
+    for (int head = hq; head < a.st.nv; head += a.st.nqk) {
+        uint8_t *ws = a.ws + ((size_t)blockIdx.x * a.st.nv + head) * ChunkWs::bytes;
+        float *vec = (float *)(ws + ChunkWs::vec);
+        __syncthreads();  // the rows, or what the last head left there, are read
+        if (wave == 0) {
+            const bool in = lane < n;
+            float gt = in ? a.h.d_gate[(row0 + lane) * a.st.nv + head] : 0.0f, bt = in ? a.h.d_beta[(row0 + lane) * a.st.nv + head] : 0.0f;
+            if (gt < kLeastGate) gt = kLeastGate;
+            const bool ok = finite32(gt) && finite32(bt);
+            const unsigned long long bad = __ballot(!ok) | bad_k;
+            double sum = ok ? (double)gt : 0.0;
+            sum += dpp_d<0x111>(sum);
+            sum += dpp_d<0x112>(sum);
+            sum += dpp_d<0x114>(sum);
+            sum += dpp_d<0x118>(sum);
+            sum += dpp_d<0x142, 0xA>(sum);
+            sum += dpp_d<0x143, 0xC>(sum);
+            G[lane] = sum;
+            beta[lane] = ok ? bt : 0.0f;
+            const int first = bad ? __builtin_ctzll(bad) : kChunk;
+            if (lane == 0) first_bad = first, *(int *)(vec + ChunkWs::first) = first;
+            const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63), __builtin_amdgcn_readlane(__double2loint(sum), 63));
+            const float ge = expf((float)sum), gl = expf((float)(last - sum)), back = scale_down(ex_k[lane]);
+            vec[ChunkWs::gx + lane] = ge * back;
+            vec[ChunkWs::gg + lane] = gl * back;
+            vec[ChunkWs::gq + lane] = ge * a.h.scale * scale_down(ex_q[lane]);
+            if (lane == 63) vec[ChunkWs::whole] = ge;
+        }
+        __syncthreads();
+        const int first = uniform(first_bad);
+        auto decay = [&](int i, int j) { return expf((float)(G[i] - G[j])); };
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (r < wave) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = 16 * r + 4 * g + e, j = 16 * wave + m;
+                A[i][j] = j < i && i < first ? beta[i] * decay(i, j) * dk[r][e] : 0.0f;
+            }
+        }
+        const float bm = 16 * wave + m < first ? beta[16 * wave + m] : 0.0f;
+        __syncthreads();
+        // the diagonal tile's inverse: lane (m, g) has column m of rows 4 g and on; a row that is done goes to all
+        f4 t[4], v, lr[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = 4 * g + e == m ? 1.0f : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) lr[e][c] = *(const f4 *)&A[16 * wave + 4 * g + e][16 * wave + 4 * c];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[j % 4]), __float_as_uint(v[j % 4]), false, false);
+            const unsigned h = half[j / 8];
+            const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+            const float x = __uint_as_float(row[j / 4 % 2]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = fmaf(-lr[e][j / 4][j % 4], x, v[e]);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (g == i / 4) D[wave][i][m] = v[i];
-    }
-    __syncthreads();
-    f4 t[4];
-    const float bm = 16 * wave + m < first ? beta[16 * wave + m] : 0.0f;
+        for (int e = 0; e < 4; e++) D[wave][4 * g + e][m] = v[e];
+        // P meanwhile; above the diagonal, what lies in a pair with what does not
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (i < wave) continue;
-        if (i == wave) {
+        for (int r = 0; r < 4; r++) {
+            const int w = 3 - wave;
+            if (r < w && !((r == 0 && w == 1) || (r == 2 && w == 3))) continue;
 #pragma unroll
-            for (int e = 0; e < 4; e++) t[i][e] = D[wave][4 * g + e][m];
-        } else {
-            f4 sum{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; e++) {
+                const int i = 16 * r + 4 * g + e, j = 16 * w + m;
+                lP[i][j] = j <= i ? a.h.scale * decay(i, j) * dq[r][e] : 0.0f;
+            }
+        }
+        __syncthreads();
 #pragma unroll
-            for (int k = 0; k < i; k++)
-                if (k >= wave) sum = mfma4(*(const f4 *)&A[16 * i + m][16 * k + 4 * g], t[k], sum);
+        for (int i = 0; i < 4; i++) {
+            if (i < wave && !((i == 0 && wave == 1) || (i == 2 && wave == 3))) continue;
             const f4 zero{0.f, 0.f, 0.f, 0.f};
-            t[i] = -mfma4(*(const f4 *)&D[i][m][4 * g], sum, zero);
-        }
+            if (i < wave) {
+                t[i] = zero;
+            } else if (i == wave) {
+                t[i] = v;
+            } else {
+                f4 sum = zero;
 #pragma unroll
-        for (int e = 0; e < 4; e++) ws[ChunkWs::T + (16 * i + 4 * g + e) * kChunk + 16 * wave + m] = t[i][e] * bm;
+                for (int k = 0; k < i; k++)
+                    if (k >= wave) sum = mfma4(*(const f4 *)&A[16 * i + m][16 * k + 4 * g], t[k], sum);
+                t[i] = -mfma4(*(const f4 *)&D[i][m][4 * g], sum, zero);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) lT[16 * i + 4 * g + e][16 * wave + m] = t[i][e] * bm;
+        }
+        __syncthreads();
+        // rows of T and P in two terms
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int r = 16 * wave + m, pairs = wave < 2 ? 1 : 2;
+            f4 y[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                y[c] = f4{0.f, 0.f, 0.f, 0.f};
+                if (c < 2 * pairs) y[c] = x ? *(const f4 *)&lP[r][16 * c + 4 * g] : *(const f4 *)&lT[r][16 * c + 4 * g];
+            }
+            const int ex = scale_of(rows16_max(size_bits(y)));
+            h8 *to = (h8 *)(ws + (x ? ChunkWs::P : ChunkWs::T));
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                if (p >= pairs) continue;
+                h8 h, l;
+                two_terms(y[2 * p], y[2 * p + 1], scale_up(ex), h, l);
+                to[tile_piece(wave, p) * 128 + lane] = h;
+                to[tile_piece(wave, p) * 128 + 64 + lane] = l;
+            }
+            if (g == 0) vec[(x ? ChunkWs::gp : ChunkWs::gt) + r] = scale_down(ex);
+        }
     }
 }
 
-// A sequence's chunks in order: four waves, wave w rows 16 w and on of the
-// chunk and HD / 4 rows of the state. Operands of the next chunk are loaded as
-// soon as this one's are used.
-constexpr int kColumns = 16;
-template <int HD>
-__global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
-    constexpr int KC = HD / 16, ST = HD / 64, NB = HD / kColumns;
-    __shared__ f4 lS[KC][64], lX[4][64], lU[4][64];
-    __shared__ int lBad[4];
+// The transposing LDS read: of the 16 lanes' 16 x 4 values, lane i gets value i % 4 of lanes 4 j + i / 4, j < 4.
+__device__ __forceinline__ h4 read_columns(const uint8_t *p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)(uintptr_t)(
+                                      (__attribute__((address_space(3))) const uint8_t *)p)));
+}
+
+// A sequence's chunks in order, a wave 16 columns of a head, NW waves a
+// workgroup. All of a column's values are its wave's, in registers; left
+// operands come to the LDS, once for the waves: the next chunk's keys, T and P
+// while this one's are worked on, its queries when this one's are done with.
+// One wave a SIMD: products and the vector instructions between them are
+// ordered so that the latter run while the matrix cores work.
+constexpr int kChunkWaves = 4;
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void gdn_chunks_kernel(RuleArgs a) {
+    constexpr int KP = HD / 32, ST = HD / 16, COLS = 16 * NW, NB = HD / COLS, KB = kq_bytes(HD);
+    extern __shared__ __align__(1024) uint8_t lds[];  // keys twice, T, P and factors twice, queries
+    uint8_t *const lq = lds + 2 * KB + 2 * ChunkWs::bytes;
     // a head's column blocks on one XCD (workgroup i runs on XCD i % 8), whose L2 they share their operands in
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, pair = at / NB * 8 + xcd, head = pair % a.st.nv, hq = head % a.st.nqk;
     if (pair >= a.longs * a.st.nv) return;
     const Long s = find_long<false>(a.b, pair / a.st.nv, a.chunked);
     if (s.seq < 0) return;
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4;
-    const int col = at % NB * kColumns + m;
-    const int chunks = (s.n + kChunk - 1) / kChunk;
-    f4 S[ST];
+    const int col = at % NB * COLS + 16 * wave + m, chunks = (s.n + kChunk - 1) / kChunk;
     const int from = a.st.from[s.seq], to = a.st.to[s.seq];
-    auto state_row = [&](int t) { return HD / 4 * wave + 16 * t + 4 * g; };
-#pragma unroll
-    for (int t = 0; t < ST; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            S[t][e] = (unsigned)from < (unsigned)a.st.n_slots
-                          ? a.st.state[(((size_t)from * a.st.nv + head) * HD + state_row(t) + e) * HD + col]
-                          : 0.0f;
-    f4 k[KC], q[KC], T[4], P[4], kt[ST][4], v, ge, gl[4];
-    float whole;
-    int first;
-    // a chunk's row, the last one where there is none: what has no row has beta 0 and corrections of 0
-    auto row_of = [&](int c, int r) { return (size_t)s.lo + min(c * kChunk + r, s.n - 1); };
-    auto ws_of = [&](int c) { return a.ws + ((size_t)(s.slot + c) * a.st.nv + head) * kChunkFloats; };
-    auto load_k = [&](int c) {
-        const float *p = a.h.d_k + row_of(c, 16 * wave + m) * a.h.k_row + (size_t)hq * HD + 4 * g;
-#pragma unroll
-        for (int i = 0; i < KC; i++) k[i] = *(const f4u *)(p + 16 * i);
-    };
-    auto load_q = [&](int c) {
-        const float *p = a.h.d_q + row_of(c, 16 * wave + m) * a.h.q_row + (size_t)hq * HD + 4 * g;
-#pragma unroll
-        for (int i = 0; i < KC; i++) q[i] = *(const f4u *)(p + 16 * i);
-    };
-    auto load_v = [&](int c) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = a.h.d_v[row_of(c, 16 * wave + 4 * g + e) * a.h.v_row + (size_t)head * HD + col];
-        ge = *(const f4 *)(ws_of(c) + ChunkWs::ge + 16 * wave + 4 * g);
-        first = *(const int *)(ws_of(c) + ChunkWs::first);
-    };
-    auto load_t = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i <= wave) T[i] = *(const f4 *)(ws_of(c) + ChunkWs::T + (16 * wave + m) * kChunk + 16 * i + 4 * g);
-    };
-    auto load_p = [&](int c) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i <= wave) P[i] = *(const f4 *)(ws_of(c) + ChunkWs::P + (16 * wave + m) * kChunk + 16 * i + 4 * g);
-    };
-    auto load_kt = [&](int c) {  // K transposed: rows of the state, 4 neighbouring rows of the chunk
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            gl[i] = *(const f4 *)(ws_of(c) + ChunkWs::gl + 16 * i + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float *p = a.h.d_k + row_of(c, 16 * i + 4 * g + e) * a.h.k_row + (size_t)hq * HD + HD / 4 * wave + m;
-#pragma unroll
-                for (int t = 0; t < ST; t++) kt[t][i][e] = p[16 * t];
-            }
-        }
-        whole = ws_of(c)[ChunkWs::ge + kChunk - 1];
-    };
-    load_k(0), load_v(0), load_q(0), load_t(0), load_p(0), load_kt(0);
+    const size_t mine = (size_t)(4 * g) * HD + col;  // the lane's first value of a state
     const f4 zero{0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < chunks; c++) {
-        const int next = min(c + 1, chunks - 1);
+    f4 S[ST];
 #pragma unroll
-        for (int t = 0; t < ST; t++) lS[ST * wave + t][lane] = S[t];
-        __syncthreads();
-        // X = V - diag(e^G) K S
-        f4 s0 = zero, s1 = zero;
-#pragma unroll
-        for (int i = 0; i < KC; i += 2) s0 = mfma4(k[i], lS[i][lane], s0), s1 = mfma4(k[i + 1], lS[i + 1][lane], s1);
-        load_k(next);
-        f4 x;
-        bool ok = true;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[e] = fmaf(-ge[e], s0[e] + s1[e], v[e]);
-            ok = ok && finite32(x[e]);
-        }
-        const int to_bad = first;
-        const f4 eg = ge;
-        load_v(next);
-        lX[wave][lane] = x;
-        const bool any = __ballot(!ok) != 0;
-        if (lane == 0) lBad[wave] = any;
-        s0 = zero, s1 = zero;
-#pragma unroll
-        for (int i = 0; i < KC; i += 2) s0 = mfma4(q[i], lS[i][lane], s0), s1 = mfma4(q[i + 1], lS[i + 1][lane], s1);
-        load_q(next);
-        __syncthreads();
-        // U = T X
-        const bool bad = uniform(lBad[0] | lBad[1] | lBad[2] | lBad[3]) || to_bad < kChunk;
-        int stop = to_bad;  // the column's rows from here on are not numbers
-        if (bad) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int e = 3; e >= 0; e--)
-                    if (!finite32(lX[i][lane][e])) stop = min(stop, 16 * i + 4 * g + e);
-            stop = min(stop, __shfl_xor(stop, 16));
-            stop = min(stop, __shfl_xor(stop, 32));
-        }
-        f4 u = zero;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i > wave) continue;
-            f4 xi = lX[i][lane];
-            if (bad) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) xi[e] = 16 * i + 4 * g + e < stop ? xi[e] : 0.0f;
-            }
-            u = mfma4(T[i], xi, u);
-        }
-        load_t(next);
-        lU[wave][lane] = u;
-        f4 o;
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = eg[e] * a.h.scale * (s0[e] + s1[e]);
-        __syncthreads();
-        // out and the state
-        f4 ub[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            ub[i] = lU[i][lane];
-            if (i <= wave) o = mfma4(P[i], ub[i], o);
-        }
-        load_p(next);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int r = 16 * wave + 4 * g + e;
-            const float w = bad && r >= stop ? __uint_as_float(0x7FC00000u) : o[e];
-            if (c * kChunk + r < s.n) a.out[(((size_t)s.lo + c * kChunk + r) * a.st.nv + head) * HD + col] = w;
-        }
-#pragma unroll
-        for (int t = 0; t < ST; t++) S[t] *= whole;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const f4 ug = ub[i] * gl[i];
-#pragma unroll
-            for (int t = 0; t < ST; t++) S[t] = mfma4(kt[t][i], ug, S[t]);
-        }
-        if (bad && stop < kChunk) {
-#pragma unroll
-            for (int t = 0; t < ST; t++) S[t] = f4{1.f, 1.f, 1.f, 1.f} * __uint_as_float(0x7FC00000u);
-        }
-        load_kt(next);
-    }
-    if ((unsigned)to < (unsigned)a.st.n_slots) {
+    for (int t = 0; t < ST; t++) S[t] = zero;
+    if ((unsigned)from < (unsigned)a.st.n_slots) {
+        const float *p = a.st.state + ((size_t)from * a.st.nv + head) * HD * HD + mine;
 #pragma unroll
         for (int t = 0; t < ST; t++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) a.st.state[(((size_t)to * a.st.nv + head) * HD + state_row(t) + e) * HD + col] = S[t][e];
+            for (int e = 0; e < 4; e++) S[t][e] = p[(16 * t + e) * HD];
+    }
+    const uint8_t *ws = a.ws + ((size_t)s.slot * a.st.nv + head) * ChunkWs::bytes + 1024 * wave;
+    const uint8_t *kq = a.kq + ((size_t)s.slot * a.st.nqk + hq) * 2 * KB + 1024 * wave;
+    const size_t ws_step = (size_t)a.st.nv * ChunkWs::bytes, kq_step = (size_t)a.st.nqk * 2 * KB;
+    // The pieces of 1 KB that a wave brings of a chunk's keys or queries, and of T, P and the factors
+    constexpr int NK = KB / 1024 / NW, NT = ChunkWs::bytes / 1024 / NW, W = 1024 * NW;
+    static_assert(NK * W == KB && NT * W == ChunkWs::bytes, "as many pieces for each wave");
+    auto fetch_keys = [&](int c, int b, int i) { dma16(kq + (c * kq_step + W * i) + 16 * lane, lds + b * KB + 1024 * wave + W * i); };
+    auto fetch_queries = [&](int c, int i) { dma16(kq + (c * kq_step + KB + W * i) + 16 * lane, lq + 1024 * wave + W * i); };
+    auto fetch_tp = [&](int c, int b, int i) { dma16(ws + (c * ws_step + W * i) + 16 * lane, lds + 2 * KB + b * ChunkWs::bytes + 1024 * wave + W * i); };
+    // Values and results of a chunk's rows through a buffer that ends with the sequence: what lies behind is 0, and
+    // not written. A chunk's offsets stay below 2^32 (row strides below 2^24).
+    const uint32_t out_row = (uint32_t)(a.st.nv * HD), v_row = (uint32_t)a.h.v_row;
+    const float *V = a.h.d_v + (size_t)s.lo * a.h.v_row + (size_t)head * HD;
+    float *out = a.out + ((size_t)s.lo * a.st.nv + head) * HD;
+    const uint32_t v_at = 4 * (4 * g * v_row + col), o_at = 4 * (4 * g * out_row + col);
+    auto rows_of = [&](const float *p, uint32_t row, int c) {
+        return buf_rsrc(p + (size_t)c * kChunk * row, 4 * ((uint32_t)(min(kChunk, s.n - c * kChunk) - 1) * row + HD));
+    };
+    f4 v[4];
+    auto load_v = [&](int c) {
+        const auto b = rows_of(V, v_row, c);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[t][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, v_at + 4 * (16 * t + e) * v_row, 0, 0));
+    };
+#define STEP __builtin_amdgcn_sched_barrier(0)
+// N times a product and M vector instructions
+#define MIX(N, M)                                                \
+    _Pragma("unroll") for (int mix = 0; mix < (N); mix++) {      \
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
+        __builtin_amdgcn_sched_group_barrier(0x002, (M), 0);     \
+    }
+#pragma unroll
+    for (int i = 0; i < NK; i++) fetch_keys(0, 0, i), fetch_queries(0, i);
+#pragma unroll
+    for (int i = 0; i < NT; i++) fetch_tp(0, 0, i);
+    load_v(0);
+    float top_s = top_of(S);
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int c = 0; c < chunks; c++) {
+        const uint8_t *lk = lds + (c & 1) * KB, *tp = lds + 2 * KB + (c & 1) * ChunkWs::bytes;
+        const float *vec = (const float *)(tp + ChunkWs::vec);
+        const int next = min(c + 1, chunks - 1), into = (c + 1) & 1;  // the last chunk brings itself again, and waits for it at the end
+        auto factors = [&](f4 (&f)[4], int what) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) f[t] = *(const f4 *)(vec + what + 16 * t + 4 * g);
+        };
+        wait_vm_barrier<16>();  // all but the last chunk's results, which were stored last
+        // products of a pair of tiles' depth of four tiles of rows; an operand is read a step before it is used
+        struct Rows {
+            h8 h[4], l[4];
+        };
+        const uint8_t *row_at = lk + 16 * place(m, g), *query_at = lq + 16 * place(m, g);
+        auto read_rows = [&](Rows &x, const uint8_t *l, int p) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                x.h[t] = *(const h8 *)(l + (t * KP + p) * 2048);
+                x.l[t] = *(const h8 *)(l + (t * KP + p) * 2048 + 1024);
+            }
+        };
+        h8 sh[KP], sl[KP];
+        auto times = [&](const Rows &x, int p, f4 (&r)[4]) {
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) r[t] = mfma_h(k < 2 ? x.h[t] : x.l[t], k == 1 ? sl[p] : sh[p], r[t]);
+        };
+        Rows ra, rb;
+        read_rows(ra, row_at, 0);
+        STEP;
+        // K S; the state's terms a pair of tiles ahead
+        const int ex_s = scale_of(rows16_max(__float_as_uint(top_s)));
+        const float up_s = scale_up(ex_s), down_s = scale_down(ex_s);
+        two_terms(S[0], S[1], up_s, sh[0], sl[0]);
+        f4 x[4], o[4] = {zero, zero, zero, zero}, r[4] = {zero, zero, zero, zero}, fx[4], ft[4], fg[4];
+        STEP;
+#pragma unroll
+        for (int p = 0; p < KP; p++) {
+            Rows &now = p % 2 ? rb : ra, &then = p % 2 ? ra : rb;
+            read_rows(then, p + 1 < KP ? row_at : query_at, (p + 1) % KP);
+            times(now, p, r);
+            if (p + 1 < KP) two_terms(S[2 * p + 2], S[2 * p + 3], up_s, sh[p + 1], sl[p + 1]);
+            MIX(12, 2);
+            STEP;
+#pragma unroll
+            for (int i = p * NK / KP; i < (p + 1) * NK / KP; i++) fetch_keys(next, into, i);
+#pragma unroll
+            for (int i = p * NT / KP; i < (p + 1) * NT / KP; i++) fetch_tp(next, into, i);
+            STEP;
+        }
+        factors(fx, ChunkWs::gx);
+        const float whole = vec[ChunkWs::whole];
+        const int first_bad = *(const int *)(vec + ChunkWs::first);
+        read_rows(rb, query_at, 1);
+        STEP;
+        // X = V - diag(e^G) K S, and Q S, for which nothing waits
+        times(ra, 0, o);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[t][e] = fmaf(-(fx[t][e] * r[t][e]), down_s, v[t][e]);
+        int ex_x = scale_of(rows16_max(__float_as_uint(top_of(x))));
+        MIX(12, 5);
+        STEP;
+        // a triangle's product: pair 0 of all four tiles of rows, pair 1 of the last two
+        struct Tri {
+            h8 h[6], l[6];
+        };
+        auto read_tri = [&](Tri &y, int what) {
+#pragma unroll
+            for (int i = 0; i < 6; i++) {
+                y.h[i] = *(const h8 *)(tp + what + i * 2048 + 16 * lane);
+                y.l[i] = *(const h8 *)(tp + what + i * 2048 + 1024 + 16 * lane);
+            }
+        };
+        auto triangle = [&](const Tri &y, const h8 (&h)[2], const h8 (&l)[2], f4 (&d)[4]) {
+#pragma unroll
+            for (int t = 0; t < 4; t++) d[t] = zero;
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+#pragma unroll
+                    for (int t = 2 * p; t < 4; t++) d[t] = mfma_h(k < 2 ? y.h[tile_piece(t, p)] : y.l[tile_piece(t, p)], k == 1 ? l[p] : h[p], d[t]);
+        };
+        Tri tri;
+        h8 xh[2], xl[2], gh[2], gl[2];
+        read_tri(tri, ChunkWs::T);
+        factors(ft, ChunkWs::gt), factors(fg, ChunkWs::gg);
+        load_v(next);
+        STEP;
+        times(rb, 1, o);
+        if constexpr (KP > 2) read_rows(ra, query_at, 2), read_rows(rb, query_at, 3);
+#pragma unroll
+        for (int p = 0; p < 2; p++) two_terms(x[2 * p], x[2 * p + 1], scale_up(ex_x), xh[p], xl[p]);
+        MIX(12, 4);
+        STEP;
+        // U, in units of X's scale
+        f4 u[4], ug[4];
+        triangle(tri, xh, xl, u);
+        const int first = uniform(first_bad);
+        // A correction that is not finite makes what it is multiplied with in the last row NaN or infinite, by 0 too
+        const bool bad = first < kChunk || __ballot(!finite32(u[3][3])) != 0;
+        int stop = first;  // the column's rows from here on are not numbers
+        if (bad) {
+#pragma unroll
+            for (int t = 3; t >= 0; t--)
+#pragma unroll
+                for (int e = 3; e >= 0; e--)
+                    if (!finite32(x[t][e])) stop = min(stop, 16 * t + 4 * g + e);
+            stop = min(stop, __shfl_xor(stop, 16));
+            stop = min(stop, __shfl_xor(stop, 32));
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[t][e] = 16 * t + 4 * g + e < stop ? x[t][e] : 0.0f;
+            ex_x = scale_of(rows16_max(__float_as_uint(top_of(x))));
+#pragma unroll
+            for (int p = 0; p < 2; p++) two_terms(x[2 * p], x[2 * p + 1], scale_up(ex_x), xh[p], xl[p]);
+            triangle(tri, xh, xl, u);
+        }
+        STEP;
+        // the rest of Q S meanwhile
+        read_tri(tri, ChunkWs::P);
+        if constexpr (KP > 2) times(ra, 2, o), times(rb, 3, o);
+#pragma unroll
+        for (int t = 0; t < 4; t++) u[t] = u[t] * ft[t], ug[t] = u[t] * fg[t];
+        const int ex_g = scale_of(rows16_max(__float_as_uint(top_of(ug)))), ex_u = scale_of(rows16_max(__float_as_uint(top_of(u))));
+#pragma unroll
+        for (int p = 0; p < 2; p++) two_terms(ug[2 * p], ug[2 * p + 1], scale_up(ex_g), gh[p], gl[p]);
+        const float down_x = scale_down(ex_x), down_g = scale_down(ex_g) * down_x, down_u = scale_down(ex_u) * down_x;
+        if constexpr (KP > 2) {
+            MIX(24, 5);
+        }
+        STEP;
+        // S <- e^G_63 S + K^T (e^(G_63 - G) U), four tiles of the state at a time: the keys by columns, rows 4 g + m / 4
+        // of tile 2 p + (0, 1), columns 4 (m % 4) and on of state tile i
+        struct Cols {
+            h8 h[4], l[4];
+        };
+        const uint8_t *col_at = lk + 16 * place(4 * g + (m >> 2), m & 3);
+        auto read_tiles = [&](Cols &k, int i0, int p) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint8_t *y = col_at + (2 * p * KP + (i0 + j) / 2) * 2048 + 8 * ((i0 + j) & 1);
+                k.h[j] = __builtin_shufflevector(read_columns(y), read_columns(y + KP * 2048), 0, 1, 2, 3, 4, 5, 6, 7);
+                k.l[j] = __builtin_shufflevector(read_columns(y + 1024), read_columns(y + KP * 2048 + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        };
+        Cols ka, kb;
+        read_tiles(ka, 0, 0);
+        lds_barrier();  // the queries are read
+#pragma unroll
+        for (int i = 0; i < NK; i++) fetch_queries(next, i);
+        f4 fq[4], fp[4], d[ST];
+        STEP;
+#pragma unroll
+        for (int i = 0; i < ST; i++) d[i] = zero;
+        auto update = [&](int i0) {
+#pragma unroll
+            for (int i = i0; i < i0 + 4; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) S[i][e] = fmaf(d[i][e], down_g, S[i][e] * whole);
+        };
+#pragma unroll
+        for (int i = 0; i < ST; i += 4)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const Cols &k = p ? kb : ka;
+                if (p == 0)
+                    read_tiles(kb, i, 1);
+                else if (i + 4 < ST)
+                    read_tiles(ka, i + 4, 0);
+                else
+                    factors(fq, ChunkWs::gq), factors(fp, ChunkWs::gp);
+#pragma unroll
+                for (int y = 0; y < 3; y++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) d[i + t] = mfma_h(y < 2 ? k.h[t] : k.l[t], y == 1 ? gl[p] : gh[p], d[i + t]);
+                if (i == 0) two_terms(u[2 * p], u[2 * p + 1], scale_up(ex_u), xh[p], xl[p]);
+                if (i && p == 0) update(i - 4);
+                if (i + 4 >= ST && p == 1)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) o[t] = fq[t] * o[t] * down_s;
+                MIX(12, 3);
+                STEP;
+            }
+        // out
+        triangle(tri, xh, xl, r);
+        update(ST - 4);
+        top_s = top_of(S);
+        MIX(18, 3);
+        STEP;
+        const auto bo = rows_of(out, out_row, c);
+        if (bad && stop < kChunk) {
+            const float nan = __uint_as_float(0x7FC00000u);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) r[t][e] = 16 * t + 4 * g + e >= stop ? nan : r[t][e];
+#pragma unroll
+            for (int i = 0; i < ST; i++) S[i] = f4{nan, nan, nan, nan};
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(fp[t][e] * r[t][e], down_u, o[t][e])), bo, o_at + 4 * (16 * t + e) * out_row, 0, 0);
+    }
+#undef MIX
+#undef STEP
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what the last chunk brought lands before the wave leaves
+    if ((unsigned)to < (unsigned)a.st.n_slots) {
+        float *p = a.st.state + ((size_t)to * a.st.nv + head) * HD * HD + mine;
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[(16 * t + e) * HD] = S[t][e];
     }
 }
 
-// The epilogue of the rows that went by chunks: a workgroup a chunk and head.
+// The epilogue of the rows that went by chunks: a workgroup a chunk and head,
+// HD / 4 lanes a row, several rows of a lane under way.
 template <int HD>
 __global__ __launch_bounds__(256) void gdn_finish_kernel(RuleArgs a) {
-    const int head = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    constexpr int PER = HD / 4, STEP = 256 / PER, N = kChunk / STEP;  // threads of a row, rows at a time, rows of a thread
+    const int head = blockIdx.y, r0 = threadIdx.x / PER, o = 4 * (threadIdx.x % PER);
     const Long s = find_long<true>(a.b, (int)blockIdx.x, a.chunked);
     if (s.seq < 0) return;
     const int c0 = ((int)blockIdx.x - s.slot) * kChunk, n = min(kChunk, s.n - c0);
-    for (int r = wave; r < n; r += 4) {
-        const size_t row = (size_t)s.lo + c0 + r;
-        float v[HD / 64];
+    const size_t row0 = (size_t)s.lo + c0;
+    f4 v[N], z[N], w{1.f, 1.f, 1.f, 1.f};
+    if (a.h.d_norm) w = *(const f4u *)(a.h.d_norm + o);
 #pragma unroll
-        for (int e = 0; e < HD / 64; e++) v[e] = a.out[(row * a.st.nv + head) * HD + HD / 64 * lane + e];
-        finish_row<HD>(a, row, head, v);
+    for (int i = 0; i < N; i++) {
+        const size_t row = row0 + min(r0 + STEP * i, n - 1);
+        v[i] = *(const f4u *)(a.out + (row * a.st.nv + head) * HD + o);
+        if (a.h.d_z) z[i] = *(const f4u *)(a.h.d_z + row * a.h.z_row + (size_t)head * HD + o);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (a.h.d_norm) {
+            float sq = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) sq = fmaf(v[i][e], v[i][e], sq);
+            v[i] *= (1.0f / sqrtf(lanes_sum<PER>(sq) / (float)HD + a.h.eps)) * w;
+        }
+        if (a.h.d_z) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[i][e] *= silu(z[i][e]);
+        }
+        if (r0 + STEP * i < n) *(f4u *)(a.out + ((row0 + r0 + STEP * i) * a.st.nv + head) * HD + o) = v[i];
     }
 }
 
@@ -761,17 +1073,20 @@ Plan plan_of(const BatchView &b, size_t most_rows) {
 }  // namespace
 
 size_t gdn_rule_ws_bytes(const StatesView &st, const BatchView &b, size_t most_rows) {
-    return 16 + (size_t)plan_of(b, most_rows).slots * st.nv * kChunkFloats * sizeof(float);
+    return 16 + (size_t)plan_of(b, most_rows).slots * (st.nv * (size_t)ChunkWs::bytes + st.nqk * (size_t)(2 * kq_bytes(st.hd)));
 }
 
 template <int HD>
 hipError_t launch_rule(RuleArgs a, bool some, hipStream_t s) {
     if (a.longs) {
         const dim3 chunks((unsigned)a.slots, (unsigned)a.st.nv);
-        hipLaunchKernelGGL(gdn_prep_kernel<HD>, chunks, dim3(kPrepTPB), 0, s, a);
+        hipLaunchKernelGGL(gdn_prep_kernel<HD>, dim3((unsigned)a.slots, (unsigned)a.st.nqk), dim3(kPrepTPB), 0, s, a);
         if (hipError_t e = hipGetLastError()) return e;
-        const long long pairs = (long long)a.longs * a.st.nv, groups = (pairs + 7) / 8 * 8 * (HD / kColumns);
-        hipLaunchKernelGGL(gdn_chunks_kernel<HD>, dim3((unsigned)groups), dim3(256), 0, s, a);
+        constexpr size_t lds = 3 * kq_bytes(HD) + 2 * ChunkWs::bytes;
+        const long long pairs = (long long)a.longs * a.st.nv;
+        const auto kernel = gdn_chunks_kernel<HD, kChunkWaves>;
+        if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / (16 * kChunkWaves)))), dim3(64 * kChunkWaves), lds, s, a);
         if (hipError_t e = hipGetLastError()) return e;
         if (a.h.d_norm || a.h.d_z) {
             hipLaunchKernelGGL(gdn_finish_kernel<HD>, chunks, dim3(256), 0, s, a);
@@ -789,7 +1104,7 @@ hipError_t launch_gdn_rule(float *out, const StatesView &st, const BatchView &b,
                            void *ws, hipStream_t s) {
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
     const Plan p = plan_of(b, most_rows);
-    const RuleArgs a{out, st, b, h, p.longs ? kChunkLeast : INT_MAX, p.longs, p.slots, (float *)ws};
+    const RuleArgs a{out, st, b, h, p.longs ? kChunkLeast : INT_MAX, p.longs, p.slots, (uint8_t *)ws, (uint8_t *)ws + (size_t)p.slots * st.nv * ChunkWs::bytes};
     return st.hd == 128 ? launch_rule<128>(a, true, s) : launch_rule<64>(a, true, s);
 }
 

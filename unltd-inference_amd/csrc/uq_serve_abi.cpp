@@ -257,6 +257,8 @@ uq_status uq_gdn_rule_d(float *d_out, const uq_gdn_states *states, const uq_seq_
     if (batch->n_rows > 1 && (heads->q_row < qk || heads->k_row < qk || heads->v_row < v))
         return set_error(UQ_ERR_LEN, "%s: q_row %zu, k_row %zu or v_row %zu below the heads of a row", fn, heads->q_row,
                          heads->k_row, heads->v_row);
+    if (batch->n_rows > 1 && heads->v_row > (size_t)1 << 24)  // a chunk's offsets are 32-bit
+        return set_error(UQ_ERR_LEN, "%s: v_row %zu above 2^24", fn, heads->v_row);
     if (heads->d_z && batch->n_rows > 1 && heads->z_row < v)
         return set_error(UQ_ERR_LEN, "%s: z_row %zu below %zu", fn, heads->z_row, v);
     if (!std::isfinite(heads->scale)) return set_error(UQ_ERR_ARG, "%s: scale is not finite", fn);
@@ -266,7 +268,11 @@ uq_status uq_gdn_rule_d(float *d_out, const uq_gdn_states *states, const uq_seq_
     if ((uintptr_t)d_ws % 16) return set_error(UQ_ERR_ARG, "%s: the workspace is not 16-byte aligned", fn);
     const size_t need = uq::gdn_rule_ws_bytes(sv, bv, most_rows);
     if (ws_bytes < need) return set_error(UQ_ERR_ARG, "%s: workspace of %zu bytes below %zu", fn, ws_bytes, need);
-    return hip_st(uq::launch_gdn_rule(d_out, sv, bv, *heads, most_rows, d_ws, (hipStream_t)stream), fn);
+    try {
+        return hip_st(uq::launch_gdn_rule(d_out, sv, bv, *heads, most_rows, d_ws, (hipStream_t)stream), fn);
+    } catch (const std::exception &e) {  // the record of raised LDS limits is the one allocation
+        return set_error(UQ_ERR_HIP, "%s: %s", fn, e.what());
+    }
 }
 
 size_t uq_logprobs_ws_bytes(size_t n_rows, size_t vocab, size_t n_top) {
