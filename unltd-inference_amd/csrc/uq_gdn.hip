@@ -3,6 +3,8 @@
 // over its states (uq_gdn_rule_d).
 #include <algorithm>
 #include <climits>
+#include <type_traits>
+#include <utility>
 
 #include "uq_device.h"
 #include "uq_internal.h"
@@ -302,10 +304,9 @@ __device__ __forceinline__ void finish_row(const RuleArgs &a, size_t row, int he
 // bounds it for few rows.
 constexpr int kRowBuf = 16;  // rows whose results wait for the norm
 template <int HD>
-__global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
+__device__ __forceinline__ void rule_rows(const RuleArgs &a, int seq, int head, float (*buf)[HD]) {
     constexpr int R = HD / 8, NW = HD / 32;
-    __shared__ float buf[kRowBuf][HD];
-    const int head = blockIdx.x, seq = blockIdx.y, hq = head % a.st.nqk;
+    const int hq = head % a.st.nqk;
     const SeqRows rows = seq_rows(a.b.row_start[seq], a.b.row_start[seq + 1], a.b.n_rows);
     if (rows.n == 0 || rows.n >= a.chunked) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i0 = (lane >> 3) * R, j0 = 32 * wave + 4 * (lane & 7);
@@ -321,35 +322,43 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
         for (int r = 0; r < R; r++) S[r] = f4{0.f, 0.f, 0.f, 0.f};
     }
     struct Row {
-        f4 q[R / 4], k[R / 4], v;
+        f4 k[R / 4], v;
         float g, b;
+    };
+    f4 q[R / 4];
+    auto load_q = [&](int i) {
+        const float *p = a.h.d_q + ((size_t)rows.lo + i) * a.h.q_row + (size_t)hq * HD + i0;
+#pragma unroll
+        for (int u = 0; u < R / 4; u++) q[u] = *(const f4u *)(p + 4 * u);
     };
     auto load = [&](Row &x, int i) {
         const size_t row = (size_t)rows.lo + i;
-        const float *q = a.h.d_q + row * a.h.q_row + (size_t)hq * HD + i0, *k = a.h.d_k + row * a.h.k_row + (size_t)hq * HD + i0;
+        const float *k = a.h.d_k + row * a.h.k_row + (size_t)hq * HD + i0;
 #pragma unroll
-        for (int u = 0; u < R / 4; u++) x.q[u] = *(const f4u *)(q + 4 * u), x.k[u] = *(const f4u *)(k + 4 * u);
+        for (int u = 0; u < R / 4; u++) x.k[u] = *(const f4u *)(k + 4 * u);
         x.v = *(const f4u *)(a.h.d_v + row * a.h.v_row + (size_t)head * HD + j0);
         x.g = a.h.d_gate[row * a.st.nv + head];
         x.b = a.h.d_beta[row * a.st.nv + head];
     };
     Row x, next;
-    load(x, 0);
+    load(x, 0), load_q(0);
     for (int i = 0; i < rows.n; i++) {
-        load(next, min(i + 1, rows.n - 1));
+        const int then = min(i + 1, rows.n - 1);
+        load(next, then);
         const float eg = expf(x.g);
         f4 sk{0.f, 0.f, 0.f, 0.f}, sq = sk, d, o;
         float qk = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const float k = x.k[r / 4][r % 4], q = x.q[r / 4][r % 4];
-            qk = fmaf(q, k, qk);
+            const float k = x.k[r / 4][r % 4], qr = q[r / 4][r % 4];
+            qk = fmaf(qr, k, qk);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 sk[e] = fmaf(k, S[r][e], sk[e]);
-                sq[e] = fmaf(q, S[r][e], sq[e]);
+                sq[e] = fmaf(qr, S[r][e], sq[e]);
             }
         }
+        load_q(then);
         auto over_rows = [](float v) { return rows16_sum(v + dpp_f<0x128>(v)); };  // row_ror:8: lanes l, l ^ 8, l ^ 16, ..
         qk = over_rows(qk);
 #pragma unroll
@@ -384,6 +393,12 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
 #pragma unroll
         for (int r = 0; r < R; r++) *(f4 *)(s + (size_t)r * HD) = S[r];
     }
+}
+
+template <int HD>
+__global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
+    __shared__ __align__(16) float buf[kRowBuf][HD];
+    rule_rows<HD>(a, (int)blockIdx.y, (int)blockIdx.x, buf);
 }
 
 // ---- the delta rule by chunks ---------------------------------------------------
@@ -482,230 +497,221 @@ __device__ __forceinline__ f4 mfma_h(const h8 &a, const h8 &b, const f4 &c) {
 }
 
 // T and P of a chunk, and the keys and queries in two terms, a workgroup the
-// value heads of one query and key head. Keys and queries come to the LDS
-// once; of the 10 tiles on and below the diagonal of K K^T and of Q K^T five
-// are for each wave, column w of the one and 3 - w of the other, in f32, kept in registers
-// for the heads. The triangle's inverse: a wave inverts a diagonal tile, a
-// column a lane, its rows over the lanes' quarters, then goes down its column
-// of tiles,
-//     T_ij = -T_ii sum over j <= k < i of A_ik T_kj,
-// as substitution would, in whose order errors do not grow.
+// value heads of one query and key head. Wave w has rows 16 w .. + 15 of both;
+// all see the keys' pieces in the LDS. It takes tiles (r, w), r >= w, of K K^T
+// and (r, w), r <= w, of K Q^T, five for each wave, and keeps them for the
+// heads. Every result lies as the operand that it is next: lane (m, g) has
+// values 4 g .. + 3 of column m, which is a row's piece of the transposed. So
+// tile (i, j) of A is the left operand A_ij^T, K Q^T has P's rows, and T's row
+// of tiles i is formed from the diagonal back,
+//     T_ij^T = -T_jj^T sum over j < k <= i of A_kj^T T_ik^T,
+// by wave i from A and the diagonal's inverses alone.
 constexpr int kPrepTPB = 256;
 template <int HD>
-__global__ __launch_bounds__(kPrepTPB) void gdn_prep_kernel(RuleArgs a) {
-    constexpr int KC = HD / 16, LD = HD + 4, LA = kChunk + 4;
-    constexpr int kA = kChunk * LA, kRows = kChunk * LD > kA + 4 * 16 * 20 ? kChunk * LD : kA + 4 * 16 * 20, kTP = kChunk * LA + kChunk * kChunk;
-    __shared__ __align__(16) float rows0[kRows], rows1[kTP > kChunk * LD ? kTP : kChunk * LD];  // K, Q; then A and the diagonal's inverses, T and P
-    __shared__ double G[kChunk];
-    __shared__ float beta[kChunk];
-    __shared__ int ex_k[kChunk], ex_q[kChunk], first_bad;
-    float (*K)[LD] = (float (*)[LD])rows0, (*Q)[LD] = (float (*)[LD])rows1;
-    float (*A)[LA] = (float (*)[LA])rows0, (*D)[16][20] = (float (*)[16][20])(rows0 + kA);
-    float (*lT)[LA] = (float (*)[LA])rows1, (*lP)[kChunk] = (float (*)[kChunk])(rows1 + kA);
-    const int hq = blockIdx.y;
-    const Long s = find_long<true>(a.b, (int)blockIdx.x, a.chunked);
+struct PrepLds {
+    static constexpr int planes = kq_bytes(HD), tiles = 2 * 10 * 1024;  // the keys; A below the diagonal (6) and the inverses (4), twice
+    __align__(16) uint8_t space[planes > tiles ? planes : tiles];
+    double G[4][kChunk];  // of the wave
+    float beta[4][kChunk];
+    int ex_k[kChunk], ex_q[kChunk], bad[4];
+};
+template <int HD>
+__device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, PrepLds<HD> &l) {
+    constexpr int KP = HD / 32;
+    const Long s = find_long<true>(a.b, slot, a.chunked);
     if (s.seq < 0) return;
-    const int c0 = ((int)blockIdx.x - s.slot) * kChunk, n = min(kChunk, s.n - c0);
+    const int c0 = (slot - s.slot) * kChunk, n = min(kChunk, s.n - c0);
     const size_t row0 = (size_t)s.lo + c0;
-    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4, mine = 16 * wave + m;
+    const float *gates = a.h.d_gate + (row0 + min(lane, n - 1)) * a.st.nv, *betas = a.h.d_beta + (row0 + min(lane, n - 1)) * a.st.nv;
+    float gate = gates[hq], bt = betas[hq];
+    int exk, exq;  // of the wave's rows
+    h8 kh[KP], kl[KP], qh[KP], ql[KP];
     {
-        constexpr int PER = HD / 4, STEP = kPrepTPB / PER;  // threads of a row, rows at a time
-        const int r0 = threadIdx.x / PER, o = 4 * (threadIdx.x % PER);
-        const float *pk = a.h.d_k + row0 * a.h.k_row + (size_t)hq * HD + o, *pq = a.h.d_q + row0 * a.h.q_row + (size_t)hq * HD + o;
-        f4 k[kChunk / STEP], q[kChunk / STEP];
+        const size_t row = row0 + min(mine, n - 1);
+        const float *pk = a.h.d_k + row * a.h.k_row + (size_t)hq * HD + 4 * g, *pq = a.h.d_q + row * a.h.q_row + (size_t)hq * HD + 4 * g;
+        f4 k[2 * KP], q[2 * KP];
 #pragma unroll
-        for (int i = 0; i < kChunk / STEP; i++) {
-            const size_t r = (size_t)min(r0 + STEP * i, n - 1);
-            k[i] = *(const f4u *)(pk + r * a.h.k_row);
-            q[i] = *(const f4u *)(pq + r * a.h.q_row);
+        for (int c = 0; c < 2 * KP; c++) k[c] = *(const f4u *)(pk + 16 * c);
+#pragma unroll
+        for (int c = 0; c < 2 * KP; c++) q[c] = *(const f4u *)(pq + 16 * c);
+        const uint32_t top_k = rows16_max(size_bits(k)), top_q = rows16_max(size_bits(q));
+        __asm__ volatile("" : "+v"(gate), "+v"(bt));  // asked for before the stores below, behind which they would wait
+        const unsigned long long no = __ballot(top_k >= 0x7F800000u);  // rows with a key that is not finite
+        exk = scale_of(top_k), exq = scale_of(top_q);
+        if (g == 0) l.ex_k[mine] = exk, l.ex_q[mine] = exq;
+        if (lane == 0) l.bad[wave] = (int)(no & 0xFFFF);
+        h8 *to = (h8 *)(a.kq + ((size_t)slot * a.st.nqk + hq) * 2 * kq_bytes(HD)) + wave * KP * 128 + place(m, g);
+        h8 *lk = (h8 *)l.space + wave * KP * 128 + place(m, g);
+#pragma unroll
+        for (int p = 0; p < KP; p++) {
+            two_terms(k[2 * p], k[2 * p + 1], scale_up(exk), kh[p], kl[p]);
+            lk[p * 128] = to[p * 128] = kh[p];
+            lk[p * 128 + 64] = to[p * 128 + 64] = kl[p];
         }
 #pragma unroll
-        for (int i = 0; i < kChunk / STEP; i++) {
-            const int r = r0 + STEP * i;
-            *(f4 *)&K[r][o] = k[i];
-            *(f4 *)&Q[r][o] = q[i];
-            auto row_ex = [](const f4 &v) {
-                uint32_t b = max(max(size_bits(v[0]), size_bits(v[1])), max(size_bits(v[2]), size_bits(v[3])));
-                b = max(b, dpp_u<0xB1>(b));
-                b = max(b, dpp_u<0x4E>(b));
-                b = max(b, dpp_u<0x141>(b));
-                b = max(b, dpp_u<0x140>(b));
-                if constexpr (PER == 32) {
-                    const auto x = __builtin_amdgcn_permlane16_swap(b, b, false, false);
-                    b = max(x[0], x[1]);
-                }
-                return scale_of(b);
-            };
-            const int ek = row_ex(k[i]), eq = row_ex(q[i]);
-            if (o == 0) ex_k[r] = ek, ex_q[r] = eq;
+        for (int p = 0; p < KP; p++) {
+            two_terms(q[2 * p], q[2 * p + 1], scale_up(exq), qh[p], ql[p]);
+            to[kq_bytes(HD) / 16 + p * 128] = qh[p];
+            to[kq_bytes(HD) / 16 + p * 128 + 64] = ql[p];
         }
     }
     __syncthreads();
-    {
-        h8 *to = (h8 *)(a.kq + ((size_t)blockIdx.x * a.st.nqk + hq) * 2 * kq_bytes(HD)) + (size_t)wave * (HD / 32) * 128;
+    const f4 zero{0.f, 0.f, 0.f, 0.f};
+    f4 dk[4], dq[4];
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const float up = scale_up((x ? ex_q : ex_k)[16 * wave + m]);
-            const float *r = x ? Q[16 * wave + m] : K[16 * wave + m];
+    for (int r = 0; r < 4; r++) {
+        f4 k0 = zero, k1 = zero, q0 = zero, q1 = zero;
+        const h8 *x = (const h8 *)l.space + r * KP * 128 + place(m, g);
 #pragma unroll
-            for (int p = 0; p < HD / 32; p++) {
-                h8 h, l;
-                two_terms(*(const f4 *)(r + 32 * p + 4 * g), *(const f4 *)(r + 32 * p + 16 + 4 * g), up, h, l);
-                to[(x * (kq_bytes(HD) / 16)) + p * 128 + place(m, g)] = h;
-                to[(x * (kq_bytes(HD) / 16)) + p * 128 + 64 + place(m, g)] = l;
+        for (int p = 0; p < KP; p++) {
+            const h8 xh = x[p * 128], xl = x[p * 128 + 64];
+            if (r >= wave) {
+                k0 = mfma_h(xh, kh[p], k0);
+                k1 = mfma_h(xh, kl[p], k1);
+                k1 = mfma_h(xl, kh[p], k1);
+            }
+            if (r <= wave) {
+                q0 = mfma_h(xh, qh[p], q0);
+                q1 = mfma_h(xh, ql[p], q1);
+                q1 = mfma_h(xl, qh[p], q1);
             }
         }
-    }
-    f4 dk[4], dq[4];  // tiles (r, wave) of K K^T and (r, 3 - wave) of Q K^T
-    unsigned long long bad_k = 0;
-    {
-        f4 y[KC];
-        auto frag = [&](int tile) {
 #pragma unroll
-            for (int c = 0; c < KC; c++) y[c] = *(const f4 *)&K[16 * tile + m][16 * c + 4 * g];
-        };
-        auto product = [&](const float (*X)[LD], int r) {
-            f4 d[4] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int c = 0; c < KC; c++) {
-                const f4 x = *(const f4 *)&X[16 * r + m][16 * c + 4 * g];
-#pragma unroll
-                for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[c][e], d[e], 0, 0, 0);
-            }
-            return (d[0] + d[1]) + (d[2] + d[3]);
-        };
-        frag(wave);
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (r >= wave) dk[r] = product(K, r);
-        frag(3 - wave);
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (r >= 3 - wave) dq[r] = product(Q, r);
-        if (wave == 0) {  // rows with a key that is not finite
-#pragma unroll
-            for (int tile = 0; tile < 4; tile++) {
-                frag(tile);
-                const unsigned long long no = __ballot(size_bits(y) >= 0x7F800000u);
-                bad_k |= ((no | no >> 16 | no >> 32 | no >> 48) & 0xFFFF) << 16 * tile;
-            }
+        for (int e = 0; e < 4; e++) {
+            const int ex = l.ex_k[16 * r + 4 * g + e] - 28;
+            dk[r][e] = ldexpf(k0[e] + k1[e], ex + exk);
+            dq[r][e] = a.h.scale * ldexpf(q0[e] + q1[e], ex + exq);
         }
     }
-    for (int head = hq; head < a.st.nv; head += a.st.nqk) {
-        uint8_t *ws = a.ws + ((size_t)blockIdx.x * a.st.nv + head) * ChunkWs::bytes;
+    const unsigned long long bad_k = (unsigned long long)(uint32_t)(l.bad[0] | l.bad[1] << 16) | (unsigned long long)(uint32_t)(l.bad[2] | l.bad[3] << 16) << 32;
+    const float back_k = scale_down(l.ex_k[lane]), back_q = a.h.scale * scale_down(l.ex_q[lane]);
+    __syncthreads();  // the keys are read
+    double *const G = l.G[wave];
+    float *const beta = l.beta[wave];
+    f4 *tiles = (f4 *)l.space + lane;  // tile (i, j) of A at i (i - 1) / 2 + j, the inverse of (i, i) at 6 + i
+    for (int head = hq, turn = 0; head < a.st.nv; head += a.st.nqk, turn ^= 1) {
+        uint8_t *ws = a.ws + ((size_t)slot * a.st.nv + head) * ChunkWs::bytes;
         float *vec = (float *)(ws + ChunkWs::vec);
-        __syncthreads();  // the rows, or what the last head left there, are read
-        if (wave == 0) {
-            const bool in = lane < n;
-            float gt = in ? a.h.d_gate[(row0 + lane) * a.st.nv + head] : 0.0f, bt = in ? a.h.d_beta[(row0 + lane) * a.st.nv + head] : 0.0f;
-            if (gt < kLeastGate) gt = kLeastGate;
-            const bool ok = finite32(gt) && finite32(bt);
-            const unsigned long long bad = __ballot(!ok) | bad_k;
-            double sum = ok ? (double)gt : 0.0;
-            sum += dpp_d<0x111>(sum);
-            sum += dpp_d<0x112>(sum);
-            sum += dpp_d<0x114>(sum);
-            sum += dpp_d<0x118>(sum);
-            sum += dpp_d<0x142, 0xA>(sum);
-            sum += dpp_d<0x143, 0xC>(sum);
-            G[lane] = sum;
-            beta[lane] = ok ? bt : 0.0f;
-            const int first = bad ? __builtin_ctzll(bad) : kChunk;
-            if (lane == 0) first_bad = first, *(int *)(vec + ChunkWs::first) = first;
-            const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63), __builtin_amdgcn_readlane(__double2loint(sum), 63));
-            const float ge = expf((float)sum), gl = expf((float)(last - sum)), back = scale_down(ex_k[lane]);
-            vec[ChunkWs::gx + lane] = ge * back;
-            vec[ChunkWs::gg + lane] = gl * back;
-            vec[ChunkWs::gq + lane] = ge * a.h.scale * scale_down(ex_q[lane]);
-            if (lane == 63) vec[ChunkWs::whole] = ge;
-        }
-        __syncthreads();
-        const int first = uniform(first_bad);
-        auto decay = [&](int i, int j) { return expf((float)(G[i] - G[j])); };
+        f4 *at = tiles + turn * 10 * 64;
+        const bool in = lane < n;
+        float gt = in ? gate : 0.0f;
+        const float b = in ? bt : 0.0f;
+        if (gt < kLeastGate) gt = kLeastGate;
+        const int other = min(head + a.st.nqk, a.st.nv - 1);
+        gate = gates[other], bt = betas[other];
+        const bool ok = finite32(gt) && finite32(b);
+        const unsigned long long bad = __ballot(!ok) | bad_k;
+        const int first = bad ? __builtin_ctzll(bad) : kChunk;
+        double sum = ok ? (double)gt * 1.4426950408889634 : 0.0;  // by ln 2: powers of 2 are one instruction
+        sum += dpp_d<0x111>(sum);
+        sum += dpp_d<0x112>(sum);
+        sum += dpp_d<0x114>(sum);
+        sum += dpp_d<0x118>(sum);
+        sum += dpp_d<0x142, 0xA>(sum);
+        sum += dpp_d<0x143, 0xC>(sum);
+        __builtin_amdgcn_wave_barrier();
+        G[lane] = sum;
+        beta[lane] = lane < first ? b : 0.0f;
+        __builtin_amdgcn_wave_barrier();
+        auto power = [](double x) { return __builtin_amdgcn_exp2f((float)x); };
+        // P's tiles of the wave's row and A's of its column
+        const double Gm = G[mine];
+        f4 diag = zero, P[4], T[4], below[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            if (r < wave) continue;
+            const f4 be = *(const f4 *)&beta[16 * r + 4 * g];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int i = 16 * r + 4 * g + e, j = 16 * wave + m;
-                A[i][j] = j < i && i < first ? beta[i] * decay(i, j) * dk[r][e] : 0.0f;
+                const int i = 16 * r + 4 * g + e;
+                const float by = power(-fabs(G[i] - Gm));  // the gates' sums go down
+                P[r][e] = i <= mine ? by * dq[r][e] : 0.0f;
+                below[r][e] = i > mine && i < first ? be[e] * by * dk[r][e] : 0.0f;
+                if (r == wave) diag[e] = -below[r][e];
             }
+            T[r] = zero;
         }
-        const float bm = 16 * wave + m < first ? beta[16 * wave + m] : 0.0f;
-        __syncthreads();
-        // the diagonal tile's inverse: lane (m, g) has column m of rows 4 g and on; a row that is done goes to all
-        f4 t[4], v, lr[4][4];
+#pragma unroll
+        for (int r = 1; r < 4; r++)
+            if (r > wave) at[(r * (r - 1) / 2 + wave) * 64] = below[r];
+        // the diagonal tile's inverse, lane (m, g) column m of rows 4 g and on; a row that is done goes to all
+        f4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = 4 * g + e == m ? 1.0f : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) lr[e][c] = *(const f4 *)&A[16 * wave + 4 * g + e][16 * wave + 4 * c];
-#pragma unroll
-        for (int j = 0; j < 16; j++) {
+        auto eliminate = [&](auto J) {
+            constexpr int j = decltype(J)::value;
             const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[j % 4]), __float_as_uint(v[j % 4]), false, false);
             const unsigned h = half[j / 8];
             const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
             const float x = __uint_as_float(row[j / 4 % 2]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = fmaf(-lr[e][j / 4][j % 4], x, v[e]);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) D[wave][4 * g + e][m] = v[e];
-        // P meanwhile; above the diagonal, what lies in a pair with what does not
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int w = 3 - wave;
-            if (r < w && !((r == 0 && w == 1) || (r == 2 && w == 3))) continue;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int i = 16 * r + 4 * g + e, j = 16 * w + m;
-                lP[i][j] = j <= i ? a.h.scale * decay(i, j) * dq[r][e] : 0.0f;
-            }
-        }
+            for (int e = 0; e < 4; e++) v[e] = fmaf(dpp_f<0x150 + j>(diag[e]), x, v[e]);  // row_newbcast:j, column j of -A
+        };
+        [&]<int... J>(std::integer_sequence<int, J...>) { (eliminate(std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, 15>{});
+        at[(6 + wave) * 64] = v;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i < wave && !((i == 0 && wave == 1) || (i == 2 && wave == 3))) continue;
-            const f4 zero{0.f, 0.f, 0.f, 0.f};
-            if (i < wave) {
-                t[i] = zero;
-            } else if (i == wave) {
-                t[i] = v;
-            } else {
-                f4 sum = zero;
+        for (int e = 0; e < 4; e++) {
+            const float *d = (const float *)(at - lane + (6 + wave) * 64);
+            const float x = d[(16 * (m >> 2) + 4 * g + e) * 4 + (m & 3)];
 #pragma unroll
-                for (int k = 0; k < i; k++)
-                    if (k >= wave) sum = mfma4(*(const f4 *)&A[16 * i + m][16 * k + 4 * g], t[k], sum);
-                t[i] = -mfma4(*(const f4 *)&D[i][m][4 * g], sum, zero);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) lT[16 * i + 4 * g + e][16 * wave + m] = t[i][e] * bm;
+            for (int i = 0; i < 4; i++)
+                if (i == wave) T[i][e] = x;
         }
-        __syncthreads();
+#pragma unroll
+        for (int j = 2; j >= 0; j--) {
+            if (j >= wave) continue;
+            f4 sum2 = zero;
+#pragma unroll
+            for (int k = j + 1; k < 4; k++)
+                if (k <= wave) sum2 = mfma4(at[(k * (k - 1) / 2 + j) * 64], T[k], sum2);
+            T[j] = -mfma4(at[(6 + j) * 64], sum2, zero);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) T[r] *= *(const f4 *)&beta[16 * r + 4 * g];
+        __asm__ volatile("" : "+v"(gate), "+v"(bt));  // likewise
         // rows of T and P in two terms
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const int r = 16 * wave + m, pairs = wave < 2 ? 1 : 2;
-            f4 y[4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                y[c] = f4{0.f, 0.f, 0.f, 0.f};
-                if (c < 2 * pairs) y[c] = x ? *(const f4 *)&lP[r][16 * c + 4 * g] : *(const f4 *)&lT[r][16 * c + 4 * g];
-            }
+        const int pairs = wave < 2 ? 1 : 2;
+        auto store = [&](const f4 (&y)[4], int what, int factor) {
             const int ex = scale_of(rows16_max(size_bits(y)));
-            h8 *to = (h8 *)(ws + (x ? ChunkWs::P : ChunkWs::T));
+            h8 *to = (h8 *)(ws + what) + lane;
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 if (p >= pairs) continue;
-                h8 h, l;
-                two_terms(y[2 * p], y[2 * p + 1], scale_up(ex), h, l);
-                to[tile_piece(wave, p) * 128 + lane] = h;
-                to[tile_piece(wave, p) * 128 + 64 + lane] = l;
+                h8 h, lo;
+                two_terms(y[2 * p], y[2 * p + 1], scale_up(ex), h, lo);
+                to[tile_piece(wave, p) * 128] = h;
+                to[tile_piece(wave, p) * 128 + 64] = lo;
             }
-            if (g == 0) vec[(x ? ChunkWs::gp : ChunkWs::gt) + r] = scale_down(ex);
+            if (g == 0) vec[factor + mine] = scale_down(ex);
+        };
+        store(T, ChunkWs::T, ChunkWs::gt);
+        store(P, ChunkWs::P, ChunkWs::gp);
+        const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63), __builtin_amdgcn_readlane(__double2loint(sum), 63));
+        if (wave == 0) {
+            vec[ChunkWs::gx + lane] = power(sum) * back_k;
+        } else if (wave == 1) {
+            vec[ChunkWs::gg + lane] = power(last - sum) * back_k;
+        } else if (wave == 2) {
+            vec[ChunkWs::gq + lane] = power(sum) * back_q;
+        } else if (lane == 63) {
+            vec[ChunkWs::whole] = power(sum);
+            *(int *)(vec + ChunkWs::first) = first;
         }
     }
+}
+// The chunks' workgroups, which the next kernel waits for, then those of the sequences that go row by row.
+template <int HD>
+__global__ __launch_bounds__(kPrepTPB, 3) void gdn_prep_kernel(RuleArgs a) {
+    __shared__ union Lds {
+        PrepLds<HD> prep;
+        float buf[kRowBuf][HD];
+    } l;
+    const unsigned chunks = (unsigned)a.slots * a.st.nqk, i = blockIdx.y * gridDim.x + blockIdx.x;
+    if (i < chunks)
+        rule_prep<HD>(a, (int)(i / a.st.nqk), (int)(i % a.st.nqk), l.prep);
+    else if (threadIdx.x < 2 * HD && i - chunks < (unsigned)a.b.n_seqs * a.st.nv)  // whole waves
+        rule_rows<HD>(a, (int)((i - chunks) / a.st.nv), (int)((i - chunks) % a.st.nv), l.buf);
 }
 
 // The transposing LDS read: of the 16 lanes' 16 x 4 values, lane i gets value i % 4 of lanes 4 j + i / 4, j < 4.
@@ -1077,27 +1083,22 @@ size_t gdn_rule_ws_bytes(const StatesView &st, const BatchView &b, size_t most_r
 }
 
 template <int HD>
-hipError_t launch_rule(RuleArgs a, bool some, hipStream_t s) {
-    if (a.longs) {
-        const dim3 chunks((unsigned)a.slots, (unsigned)a.st.nv);
-        hipLaunchKernelGGL(gdn_prep_kernel<HD>, dim3((unsigned)a.slots, (unsigned)a.st.nqk), dim3(kPrepTPB), 0, s, a);
-        if (hipError_t e = hipGetLastError()) return e;
-        constexpr size_t lds = 3 * kq_bytes(HD) + 2 * ChunkWs::bytes;
-        const long long pairs = (long long)a.longs * a.st.nv;
-        const auto kernel = gdn_chunks_kernel<HD, kChunkWaves>;
-        if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / (16 * kChunkWaves)))), dim3(64 * kChunkWaves), lds, s, a);
-        if (hipError_t e = hipGetLastError()) return e;
-        if (a.h.d_norm || a.h.d_z) {
-            hipLaunchKernelGGL(gdn_finish_kernel<HD>, chunks, dim3(256), 0, s, a);
-            if (hipError_t e = hipGetLastError()) return e;
-        }
-    }
-    if (some) {
+hipError_t launch_rule(RuleArgs a, hipStream_t s) {
+    if (!a.longs) {
         hipLaunchKernelGGL(gdn_rows_kernel<HD>, dim3((unsigned)a.st.nv, (unsigned)a.b.n_seqs), dim3(2 * HD), 0, s, a);
-        if (hipError_t e = hipGetLastError()) return e;
+        return hipGetLastError();
     }
-    return hipSuccess;
+    const size_t first = (size_t)a.slots * a.st.nqk + (size_t)a.b.n_seqs * a.st.nv, across = std::min(first, (size_t)1 << 22);
+    hipLaunchKernelGGL(gdn_prep_kernel<HD>, dim3((unsigned)across, (unsigned)((first + across - 1) / across)), dim3(kPrepTPB), 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    constexpr size_t lds = 3 * kq_bytes(HD) + 2 * ChunkWs::bytes;
+    const long long pairs = (long long)a.longs * a.st.nv;
+    const auto kernel = gdn_chunks_kernel<HD, kChunkWaves>;
+    if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / (16 * kChunkWaves)))), dim3(64 * kChunkWaves), lds, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (a.h.d_norm || a.h.d_z) hipLaunchKernelGGL(gdn_finish_kernel<HD>, dim3((unsigned)a.slots, (unsigned)a.st.nv), dim3(256), 0, s, a);
+    return hipGetLastError();
 }
 
 hipError_t launch_gdn_rule(float *out, const StatesView &st, const BatchView &b, const uq_gdn_heads &h, size_t most_rows,
@@ -1105,7 +1106,7 @@ hipError_t launch_gdn_rule(float *out, const StatesView &st, const BatchView &b,
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
     const Plan p = plan_of(b, most_rows);
     const RuleArgs a{out, st, b, h, p.longs ? kChunkLeast : INT_MAX, p.longs, p.slots, (uint8_t *)ws, (uint8_t *)ws + (size_t)p.slots * st.nv * ChunkWs::bytes};
-    return st.hd == 128 ? launch_rule<128>(a, true, s) : launch_rule<64>(a, true, s);
+    return st.hd == 128 ? launch_rule<128>(a, s) : launch_rule<64>(a, s);
 }
 
 }  // namespace uq
