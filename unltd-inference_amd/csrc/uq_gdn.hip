@@ -4,7 +4,7 @@
 #include <algorithm>
 #include <climits>
 #include <type_traits>
-#include <utility>
+
 
 #include "uq_device.h"
 #include "uq_internal.h"
@@ -431,6 +431,7 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
 // Their results are set to NaN.
 
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4v __attribute__((vector_size(16)));
 
 // Left operands in the workspace, pieces of 1 KB: [tile of 16 rows][pair of tiles in depth][h, l][64 lanes][8 f16].
 // The keys are read by columns as well (read_columns), 4 rows of 4 pieces of 4 columns at a time: those lie in
@@ -438,10 +439,11 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ int place(int m, int g) { return 16 * g + ((m + 4 * g) & 15); }
 struct ChunkWs {  // of a chunk and value head, in bytes
     static constexpr int T = 0, P = 12 * 1024, vec = 24 * 1024;  // 6 pieces of h and l each: tile_piece
-    // vec, floats: factors of the rows of K S (e^G with the keys' scale), of U for the state (e^(G_63 - G) with it), of Q
-    // S, and of T's and P's rows; then e^G_63 and the first row that is left out
-    static constexpr int gx = 0, gg = 64, gq = 128, gt = 192, gp = 256, whole = 320, first = 321;
-    static constexpr int bytes = 28 * 1024;  // as many pieces for each of four waves
+    // vec, floats: factors of the rows of K S (e^G with the keys' scale), of T's product for the state (e^(G_63 - G) with
+    // the keys' scale and T's), of Q S, and of T's and P's rows; then e^G_63, the first row that is left out and the
+    // largest of gx
+    static constexpr int gx = 0, gg = 64, gq = 128, gt = 192, gp = 256, whole = 320, first = 321, top = 322;
+    static constexpr int bytes = 26 * 1024;
 };
 __device__ __forceinline__ int tile_piece(int tile, int pair) { return tile < 2 ? tile : 2 * tile - 2 + pair; }
 constexpr int kq_bytes(int hd) { return kChunk * hd * 4; }  // of the keys or queries of a chunk
@@ -466,26 +468,44 @@ __device__ __forceinline__ uint32_t rows16_max(uint32_t v) {
     const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return max(b[0], b[1]);
 }
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+    v = max(v, dpp_u<0xB1>(v));
+    v = max(v, dpp_u<0x4E>(v));
+    v = max(v, dpp_u<0x141>(v));
+    return rows16_max(max(v, dpp_u<0x140>(v)));
+}
 // The exponent ex that brings values of at most this size below 2^14: x 2^(14 - ex). Sizes below 2^-100 as it.
 __device__ __forceinline__ int scale_of(uint32_t bits) { return max(-100, __builtin_amdgcn_frexp_expf(__uint_as_float(bits))); }
 __device__ __forceinline__ float scale_up(int ex) { return ldexpf(1.0f, 14 - ex); }
 __device__ __forceinline__ float scale_down(int ex) { return ldexpf(1.0f, ex - 14); }
-// The two terms of a pair of tiles, each in one instruction that takes the product with s, a power of two, whole.
-__device__ __forceinline__ void two_terms(const f4 &a, const f4 &b, float s, h8 &h, h8 &l) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float v = e < 4 ? a[e & 3] : b[e & 3];
-        h[e] = (_Float16)fmaf(v, s, 0.0f);
-        l[e] = (_Float16)fmaf(v, s, -(float)h[e]);
-    }
+// The two terms of a pair of tiles, each rounded to the nearest. A pair of conversions, back, a difference: three
+// instructions a value of 4 clocks each, where a product and sum of mixed precision for each term takes 8 each.
+__device__ __forceinline__ void two_terms(const f4 &a, const f4 &b, h8 &h, h8 &l) {
+    typedef float f8 __attribute__((ext_vector_type(8)));
+    const f8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    h = __builtin_convertvector(v, h8);
+    l = __builtin_convertvector(v - __builtin_convertvector(h, f8), h8);
 }
-// The largest size of N tiles' values but for NaN.
+__device__ __forceinline__ void two_terms(const f4 &a, const f4 &b, float s, h8 &h, h8 &l) { two_terms(a * s, b * s, h, l); }
+// The largest size of N tiles' values, a NaN's above all. As floats' order is that of their bits, for those above zero as
+// signed, for those below as unsigned: an instruction a value, where floats, made canonical first, take one and a half.
 template <int N>
 __device__ __forceinline__ float top_of(const f4 (&v)[N]) {
-    float r = 0.0f;
+    int above[2] = {0, 0};
+    uint32_t below[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < N; i++) r = fmaxf(fmaxf(fmaxf(r, fabsf(v[i][0])), fmaxf(fabsf(v[i][1]), fabsf(v[i][2]))), fabsf(v[i][3]));
-    return r;
+    for (int i = 0; i < 2 * N; i++) {
+        const uint32_t x = __float_as_uint(v[i / 2][i % 2 * 2]), y = __float_as_uint(v[i / 2][i % 2 * 2 + 1]);
+        above[i % 2] = max(above[i % 2], max((int)x, (int)y));
+        below[i % 2] = max(below[i % 2], max(x, y));
+    }
+    return __uint_as_float(max((uint32_t)max(above[0], above[1]), max(below[0], below[1]) & 0x7FFFFFFFu));
+}
+// Nothing that depends on v moves up across this point.
+template <int N>
+__device__ __forceinline__ void hold(f4 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) __asm__ volatile("" : "+v"(v[i]));
 }
 __device__ __forceinline__ f4 mfma4(const f4 &a, const f4 &b, f4 c) {
 #pragma unroll
@@ -506,6 +526,17 @@ __device__ __forceinline__ f4 mfma_h(const h8 &a, const h8 &b, const f4 &c) {
 // of tiles i is formed from the diagonal back,
 //     T_ij^T = -T_jj^T sum over j < k <= i of A_kj^T T_ik^T,
 // by wave i from A and the diagonal's inverses alone.
+// Column J of -A, a lane's row of it in the quarter's lane J, times the inverse's row J.
+template <int J>
+__device__ __forceinline__ void eliminate(const f4 &a, f4 &v) {
+    const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[J % 4]), __float_as_uint(v[J % 4]), false, false);
+    const unsigned h = half[J / 8];
+    const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+    const float x = __uint_as_float(row[J / 4 % 2]);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = fmaf(dpp_f<0x150 + J>(a[e]), x, v[e]);  // row_newbcast:J
+    if constexpr (J < 14) eliminate<J + 1>(a, v);
+}
 constexpr int kPrepTPB = 256;
 template <int HD>
 struct PrepLds {
@@ -634,20 +665,11 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
 #pragma unroll
         for (int r = 1; r < 4; r++)
             if (r > wave) at[(r * (r - 1) / 2 + wave) * 64] = below[r];
-        // the diagonal tile's inverse, lane (m, g) column m of rows 4 g and on; a row that is done goes to all
+        // the diagonal tile's inverse, lane (m, g) column m of rows 4 g and on; a row that is done goes to all of them
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = 4 * g + e == m ? 1.0f : 0.0f;
-        auto eliminate = [&](auto J) {
-            constexpr int j = decltype(J)::value;
-            const auto half = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[j % 4]), __float_as_uint(v[j % 4]), false, false);
-            const unsigned h = half[j / 8];
-            const auto row = __builtin_amdgcn_permlane16_swap(h, h, false, false);
-            const float x = __uint_as_float(row[j / 4 % 2]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = fmaf(dpp_f<0x150 + j>(diag[e]), x, v[e]);  // row_newbcast:j, column j of -A
-        };
-        [&]<int... J>(std::integer_sequence<int, J...>) { (eliminate(std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, 15>{});
+        eliminate<0>(diag, v);
         at[(6 + wave) * 64] = v;
         __syncthreads();
 #pragma unroll
@@ -672,7 +694,7 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
         __asm__ volatile("" : "+v"(gate), "+v"(bt));  // likewise
         // rows of T and P in two terms
         const int pairs = wave < 2 ? 1 : 2;
-        auto store = [&](const f4 (&y)[4], int what, int factor) {
+        auto store = [&](const f4 (&y)[4], int what) {
             const int ex = scale_of(rows16_max(size_bits(y)));
             h8 *to = (h8 *)(ws + what) + lane;
 #pragma unroll
@@ -683,18 +705,23 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
                 to[tile_piece(wave, p) * 128] = h;
                 to[tile_piece(wave, p) * 128 + 64] = lo;
             }
-            if (g == 0) vec[factor + mine] = scale_down(ex);
+            return scale_down(ex);
         };
-        store(T, ChunkWs::T, ChunkWs::gt);
-        store(P, ChunkWs::P, ChunkWs::gp);
+        const float back_t = store(T, ChunkWs::T), back_p = store(P, ChunkWs::P);
         const double last = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(sum), 63), __builtin_amdgcn_readlane(__double2loint(sum), 63));
+        if (g == 0) {
+            vec[ChunkWs::gt + mine] = back_t;
+            vec[ChunkWs::gp + mine] = back_p;
+            vec[ChunkWs::gg + mine] = power(last - Gm) * scale_down(exk) * back_t;
+        }
         if (wave == 0) {
-            vec[ChunkWs::gx + lane] = power(sum) * back_k;
+            const float gx = power(sum) * back_k;
+            vec[ChunkWs::gx + lane] = gx;
+            const uint32_t top = wave_top(__float_as_uint(gx));
+            if (lane == 0) vec[ChunkWs::top] = __uint_as_float(top);
         } else if (wave == 1) {
-            vec[ChunkWs::gg + lane] = power(last - sum) * back_k;
-        } else if (wave == 2) {
             vec[ChunkWs::gq + lane] = power(sum) * back_q;
-        } else if (lane == 63) {
+        } else if (wave == 2 && lane == 63) {
             vec[ChunkWs::whole] = power(sum);
             *(int *)(vec + ChunkWs::first) = first;
         }
@@ -721,28 +748,217 @@ __device__ __forceinline__ h4 read_columns(const uint8_t *p) {
                                       (__attribute__((address_space(3))) const uint8_t *)p)));
 }
 
-// A sequence's chunks in order, a wave 16 columns of a head, NW waves a
-// workgroup. All of a column's values are its wave's, in registers; left
-// operands come to the LDS, once for the waves: the next chunk's keys, T and P
-// while this one's are worked on, its queries when this one's are done with.
-// One wave a SIMD: products and the vector instructions between them are
-// ordered so that the latter run while the matrix cores work.
-constexpr int kChunkWaves = 4;
-template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void gdn_chunks_kernel(RuleArgs a) {
-    constexpr int KP = HD / 32, ST = HD / 16, COLS = 16 * NW, NB = HD / COLS, KB = kq_bytes(HD);
-    extern __shared__ __align__(1024) uint8_t lds[];  // keys twice, T, P and factors twice, queries
-    uint8_t *const lq = lds + 2 * KB + 2 * ChunkWs::bytes;
+// A sequence's chunks in order, a workgroup 32 columns of a head. Two waves take
+// the state on, 16 columns each, all of a column's values in registers; two
+// more the results of the same columns, for which the former leave the state
+// before a chunk and the corrections, both as operands, in the LDS. Left
+// operands come to the LDS once for all, brought by the results' waves, whose
+// way is the shorter: between the chunk's two barriers P and the next chunk's
+// keys, then its queries, T and factors. One wave a SIMD: products and the
+// vector instructions between them are ordered so that the latter run while
+// the matrix cores work.
+constexpr int kChunkCols = 32;
+template <int HD>
+struct ChunkLds {
+    static constexpr int KB = kq_bytes(HD), Q = 2 * KB, T = 3 * KB, P = T + ChunkWs::P, vec = T + ChunkWs::vec, vec_bytes = ChunkWs::bytes - ChunkWs::vec;  // keys and factors twice
+    static constexpr int S = vec + 2 * vec_bytes, U = S + 2 * HD * 64, one = U + 2 * 4096, bytes = one + 2 * 256;  // of two waves
+};
+template <int HD>
+__global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
+    using L = ChunkLds<HD>;
+    constexpr int KP = HD / 32, ST = HD / 16, NB = HD / kChunkCols, KB = L::KB;
+    extern __shared__ __align__(1024) uint8_t lds[];
     // a head's column blocks on one XCD (workgroup i runs on XCD i % 8), whose L2 they share their operands in
     const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, pair = at / NB * 8 + xcd, head = pair % a.st.nv, hq = head % a.st.nqk;
     if (pair >= a.longs * a.st.nv) return;
     const Long s = find_long<false>(a.b, pair / a.st.nv, a.chunked);
     if (s.seq < 0) return;
-    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4;
-    const int col = at % NB * COLS + 16 * wave + m, chunks = (s.n + kChunk - 1) / kChunk;
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4, half = wave & 1;
+    const int col = at % NB * kChunkCols + 16 * half + m, chunks = (s.n + kChunk - 1) / kChunk;
+    const f4 zero{0.f, 0.f, 0.f, 0.f};
+    uint8_t *const ls = lds + L::S + half * HD * 64 + 16 * lane, *const lu = lds + L::U + half * 4096 + 16 * lane;
+    float *const one = (float *)(lds + L::one) + half * 64;  // of each column: the scales of its state and of U, its largest value, the row where U ends
+    // Values and results of a chunk's rows through a buffer that ends with the sequence: what lies behind is 0, and
+    // not written. A chunk's offsets stay below 2^32 (row strides below 2^24).
+    auto rows_of = [&](const float *p, uint32_t row, int c) {
+        return buf_rsrc(p + (size_t)c * kChunk * row, 4 * ((uint32_t)(min(kChunk, s.n - c * kChunk) - 1) * row + HD));
+    };
+    // Products of a pair of tiles' depth of four tiles of rows; an operand is read a step before it is used. Turned, a
+    // lane has a row's values 4 g and on, as they are stored, and not four rows' of a column.
+    struct Rows {
+        h8 h[4], l[4];
+    };
+    auto read_rows = [&](Rows &x, const uint8_t *l, int p) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) x.h[t] = *(const h8 *)(l + (t * KP + p) * 2048);
+#pragma unroll
+        for (int t = 0; t < 4; t++) x.l[t] = *(const h8 *)(l + (t * KP + p) * 2048 + 1024);
+    };
+    auto times = [&](const Rows &x, const h8 &h, const h8 &l, f4 (&r)[4], auto turned) {
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const h8 &y = k < 2 ? x.h[t] : x.l[t], &z = k == 1 ? l : h;
+                r[t] = decltype(turned)::value ? mfma_h(z, y, r[t]) : mfma_h(y, z, r[t]);
+            }
+    };
+    // a triangle's product: pair 0 of all four tiles of rows, pair 1 of the last two
+    struct Tri {
+        h8 h[6], l[6];
+    };
+    auto read_tri = [&](Tri &y, int what) {
+#pragma unroll
+        for (int i = 0; i < 6; i++) {
+            y.h[i] = *(const h8 *)(lds + what + i * 2048 + 16 * lane);
+            y.l[i] = *(const h8 *)(lds + what + i * 2048 + 1024 + 16 * lane);
+        }
+    };
+    auto triangle = [&](const Tri &y, const h8 (&h)[2], const h8 (&l)[2], f4 (&d)[4], auto turned) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) d[t] = zero;
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+#pragma unroll
+                for (int t = 2 * p; t < 4; t++) {
+                    const h8 &u = k < 2 ? y.h[tile_piece(t, p)] : y.l[tile_piece(t, p)], &z = k == 1 ? l[p] : h[p];
+                    d[t] = decltype(turned)::value ? mfma_h(z, u, d[t]) : mfma_h(u, z, d[t]);
+                }
+    };
+    auto factors = [&](f4 (&f)[4], int c, int what) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) f[t] = *(const f4 *)(lds + L::vec + (c & 1) * L::vec_bytes + 4 * (what + 16 * t + 4 * g));
+    };
+#define STEP __builtin_amdgcn_sched_barrier(0)
+// N times a product, R reads of the LDS and M vector instructions
+#define MIX(N, R, M)                                             \
+    _Pragma("unroll") for (int mix = 0; mix < (N); mix++) {      \
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
+        __builtin_amdgcn_sched_group_barrier(0x100, (R), 0);     \
+        __builtin_amdgcn_sched_group_barrier(0x002, (M), 0);     \
+    }
+    const uint8_t *ws = a.ws + ((size_t)s.slot * a.st.nv + head) * ChunkWs::bytes + 1024 * half + 16 * lane;
+    const uint8_t *kq = a.kq + ((size_t)s.slot * a.st.nqk + hq) * 2 * KB + 1024 * half + 16 * lane;
+    const size_t ws_step = (size_t)a.st.nv * ChunkWs::bytes, kq_step = (size_t)a.st.nqk * 2 * KB;
+    // the wave's half of a chunk's pieces of 1 KB
+    constexpr int NK = KB / 2048, NT = ChunkWs::P / 2048;
+    static_assert(L::vec_bytes == 2048, "a piece for each wave");
+    auto fetch = [&](const uint8_t *from, int to, int i) { dma16(from + 2048 * i, lds + to + 1024 * half + 2048 * i); };
+    // queries and T, part of n
+    auto fetch_after = [&](int c, int part, int n) {
+#pragma unroll
+        for (int i = part * NK / n; i < (part + 1) * NK / n; i++) fetch(kq + c * kq_step + KB, L::Q, i);
+#pragma unroll
+        for (int i = part * NT / n; i < (part + 1) * NT / n; i++) fetch(ws + c * ws_step, L::T, i);
+    };
+    if (wave >= 2) {  // the results
+        const uint32_t out_row = (uint32_t)(a.st.nv * HD), o_at = 4 * (m * out_row + col - m + 4 * g);
+        float *out = a.out + ((size_t)s.lo * a.st.nv + head) * HD;
+#pragma unroll
+        for (int i = 0; i < NK; i++) fetch(kq, 0, i), fetch(kq + KB, L::Q, i);
+#pragma unroll
+        for (int i = 0; i < NT; i++) fetch(ws, L::T, i);
+        fetch(ws + ChunkWs::vec, L::vec, 0);
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint8_t *query_at = lds + L::Q + 16 * place(m, g);
+        // the last chunk's products, and their columns' and rows' factors
+        f4 o[4], r[4], down_u, stop;
+        float fp[4];
+        auto store = [&](int c) {
+            const auto bo = rows_of(out, out_row, c);
+            int least = kChunk;
+#pragma unroll
+            for (int e = 0; e < 4; e++) least = min(least, __float_as_int(stop[e]));
+            const bool bad = __ballot(least < kChunk);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                f4 y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = fmaf(fp[t] * r[t][e], down_u[e], o[t][e]);
+                if (bad) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (16 * t + m >= __float_as_int(stop[e])) y[e] = __uint_as_float(0x7FC00000u);
+                }
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4v, y), bo, o_at + 64 * t * out_row, 0, 0);
+            }
+        };
+        for (int c = 0; c < chunks; c++) {
+            const int next = min(c + 1, chunks - 1), into = (c + 1) & 1;  // the last chunk brings itself again, and waits for it at the end
+            wait_vm_barrier<0>();
+            if (c > 0) store(c - 1);
+            h8 sh[KP], sl[KP];
+#pragma unroll
+            for (int p = 0; p < KP; p++) sh[p] = *(const h8 *)(ls + 2048 * p), sl[p] = *(const h8 *)(ls + 2048 * p + 1024);
+            Rows ra, rb;
+            read_rows(ra, query_at, 0);
+            const f4 down_s = *(const f4 *)(one + 4 * g);
+            float fq[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float *vec = (const float *)(lds + L::vec + (c & 1) * L::vec_bytes) + 16 * t + m;
+                fq[t] = vec[ChunkWs::gq], fp[t] = vec[ChunkWs::gp], o[t] = zero;
+            }
+            STEP;
+#pragma unroll
+            for (int i = 0; i < NT; i++) fetch(ws + c * ws_step + ChunkWs::P, L::P, i);
+#pragma unroll
+            for (int i = 0; i < NK; i++) fetch(kq + next * kq_step, into * KB, i);
+            fetch(ws + next * ws_step + ChunkWs::vec, L::vec + into * L::vec_bytes, 0);
+            STEP;
+#pragma unroll
+            for (int p = 0; p < KP; p++) {
+                Rows &now = p % 2 ? rb : ra, &then = p % 2 ? ra : rb;
+                if (p + 1 < KP) read_rows(then, query_at, p + 1);
+                times(now, sh[p], sl[p], o, std::true_type{});
+                MIX(8, 1, 1);
+                STEP;
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) o[t] *= fq[t] * down_s;
+            // the state's largest value, of its first terms, as whose scale's bound it serves
+            typedef unsigned short w8 __attribute__((ext_vector_type(8)));
+            w8 top = __builtin_bit_cast(w8, sh[0]) & (unsigned short)0x7FFF;
+#pragma unroll
+            for (int p = 1; p < KP; p++) top = __builtin_elementwise_max(top, (w8)(__builtin_bit_cast(w8, sh[p]) & (unsigned short)0x7FFF));
+            uint32_t largest = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) largest = max(largest, (uint32_t)top[e]);
+            one[16 + m] = (float)__builtin_bit_cast(_Float16, (unsigned short)rows16_max(largest));
+            STEP;
+            wait_vm_barrier<NK + 1>();  // P is there, the state and the queries are read; the corrections are there
+            f4 u[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) u[t] = *(const f4 *)(lu + 1024 * t);
+            Tri tri;
+            read_tri(tri, L::P);
+            f4 ft[4];
+            factors(ft, c, ChunkWs::gt);
+            down_u = *(const f4 *)(one + 32 + 4 * g), stop = *(const f4 *)(one + 48 + 4 * g);
+            STEP;
+            fetch_after(next, 1, 2);
+            STEP;
+#pragma unroll
+            for (int t = 0; t < 4; t++) u[t] *= ft[t];
+            const int ex_u = scale_of(rows16_max(__float_as_uint(top_of(u))));
+            h8 uh[2], ul[2];
+#pragma unroll
+            for (int p = 0; p < 2; p++) two_terms(u[2 * p], u[2 * p + 1], scale_up(ex_u), uh[p], ul[p]);
+            const float down = scale_down(ex_u);
+            f4 by;  // of the columns that the lane has of the products
+#pragma unroll
+            for (int e = 0; e < 4; e++) by[e] = __shfl(down, 4 * g + e);
+            triangle(tri, uh, ul, r, std::true_type{});
+            down_u *= by;
+        }
+        store(chunks - 1);
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what the last chunk brought lands before the wave leaves
+        return;
+    }
     const int from = a.st.from[s.seq], to = a.st.to[s.seq];
     const size_t mine = (size_t)(4 * g) * HD + col;  // the lane's first value of a state
-    const f4 zero{0.f, 0.f, 0.f, 0.f};
     f4 S[ST];
 #pragma unroll
     for (int t = 0; t < ST; t++) S[t] = zero;
@@ -753,24 +969,8 @@ __global__ __launch_bounds__(64 * NW, 1) void gdn_chunks_kernel(RuleArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) S[t][e] = p[(16 * t + e) * HD];
     }
-    const uint8_t *ws = a.ws + ((size_t)s.slot * a.st.nv + head) * ChunkWs::bytes + 1024 * wave;
-    const uint8_t *kq = a.kq + ((size_t)s.slot * a.st.nqk + hq) * 2 * KB + 1024 * wave;
-    const size_t ws_step = (size_t)a.st.nv * ChunkWs::bytes, kq_step = (size_t)a.st.nqk * 2 * KB;
-    // The pieces of 1 KB that a wave brings of a chunk's keys or queries, and of T, P and the factors
-    constexpr int NK = KB / 1024 / NW, NT = ChunkWs::bytes / 1024 / NW, W = 1024 * NW;
-    static_assert(NK * W == KB && NT * W == ChunkWs::bytes, "as many pieces for each wave");
-    auto fetch_keys = [&](int c, int b, int i) { dma16(kq + (c * kq_step + W * i) + 16 * lane, lds + b * KB + 1024 * wave + W * i); };
-    auto fetch_queries = [&](int c, int i) { dma16(kq + (c * kq_step + KB + W * i) + 16 * lane, lq + 1024 * wave + W * i); };
-    auto fetch_tp = [&](int c, int b, int i) { dma16(ws + (c * ws_step + W * i) + 16 * lane, lds + 2 * KB + b * ChunkWs::bytes + 1024 * wave + W * i); };
-    // Values and results of a chunk's rows through a buffer that ends with the sequence: what lies behind is 0, and
-    // not written. A chunk's offsets stay below 2^32 (row strides below 2^24).
-    const uint32_t out_row = (uint32_t)(a.st.nv * HD), v_row = (uint32_t)a.h.v_row;
+    const uint32_t v_row = (uint32_t)a.h.v_row, v_at = 4 * (4 * g * v_row + col);
     const float *V = a.h.d_v + (size_t)s.lo * a.h.v_row + (size_t)head * HD;
-    float *out = a.out + ((size_t)s.lo * a.st.nv + head) * HD;
-    const uint32_t v_at = 4 * (4 * g * v_row + col), o_at = 4 * (4 * g * out_row + col);
-    auto rows_of = [&](const float *p, uint32_t row, int c) {
-        return buf_rsrc(p + (size_t)c * kChunk * row, 4 * ((uint32_t)(min(kChunk, s.n - c * kChunk) - 1) * row + HD));
-    };
     f4 v[4];
     auto load_v = [&](int c) {
         const auto b = rows_of(V, v_row, c);
@@ -779,126 +979,80 @@ __global__ __launch_bounds__(64 * NW, 1) void gdn_chunks_kernel(RuleArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; e++) v[t][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, v_at + 4 * (16 * t + e) * v_row, 0, 0));
     };
-#define STEP __builtin_amdgcn_sched_barrier(0)
-// N times a product and M vector instructions
-#define MIX(N, M)                                                \
-    _Pragma("unroll") for (int mix = 0; mix < (N); mix++) {      \
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
-        __builtin_amdgcn_sched_group_barrier(0x002, (M), 0);     \
-    }
+    h8 sh[KP], sl[KP];
+    // A column's state is held in units of 2^(ex_s - 14). Its scale is set before the values are known, by a bound on the
+    // largest, as is that of X: of a sum's terms, of which f32's errors are parts of 2^-24. A bound 64 times too large
+    // costs 2^-33 of it.
+    int ex_s;
+    auto state_terms = [&](int p) {
+        two_terms(S[2 * p], S[2 * p + 1], sh[p], sl[p]);
+        *(h8 *)(ls + 2048 * p) = sh[p];
+        *(h8 *)(ls + 2048 * p + 1024) = sl[p];
+    };
+    auto column_top = [&](float v) { return rows16_max(__float_as_uint(v)); };
+    auto units = [&](int ex) {
 #pragma unroll
-    for (int i = 0; i < NK; i++) fetch_keys(0, 0, i), fetch_queries(0, i);
-#pragma unroll
-    for (int i = 0; i < NT; i++) fetch_tp(0, 0, i);
+        for (int t = 0; t < ST; t++) S[t] *= ldexpf(1.0f, ex);
+    };
     load_v(0);
-    float top_s = top_of(S);
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    ex_s = scale_of(column_top(top_of(S)));
+    units(14 - ex_s);
+#pragma unroll
+    for (int p = 0; p < KP; p++) state_terms(p);
+    one[m] = scale_down(ex_s);
     for (int c = 0; c < chunks; c++) {
-        const uint8_t *lk = lds + (c & 1) * KB, *tp = lds + 2 * KB + (c & 1) * ChunkWs::bytes;
-        const float *vec = (const float *)(tp + ChunkWs::vec);
-        const int next = min(c + 1, chunks - 1), into = (c + 1) & 1;  // the last chunk brings itself again, and waits for it at the end
-        auto factors = [&](f4 (&f)[4], int what) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) f[t] = *(const f4 *)(vec + what + 16 * t + 4 * g);
-        };
-        wait_vm_barrier<16>();  // all but the last chunk's results, which were stored last
-        // products of a pair of tiles' depth of four tiles of rows; an operand is read a step before it is used
-        struct Rows {
-            h8 h[4], l[4];
-        };
-        const uint8_t *row_at = lk + 16 * place(m, g), *query_at = lq + 16 * place(m, g);
-        auto read_rows = [&](Rows &x, const uint8_t *l, int p) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                x.h[t] = *(const h8 *)(l + (t * KP + p) * 2048);
-                x.l[t] = *(const h8 *)(l + (t * KP + p) * 2048 + 1024);
-            }
-        };
-        h8 sh[KP], sl[KP];
-        auto times = [&](const Rows &x, int p, f4 (&r)[4]) {
-#pragma unroll
-            for (int k = 0; k < 3; k++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) r[t] = mfma_h(k < 2 ? x.h[t] : x.l[t], k == 1 ? sl[p] : sh[p], r[t]);
-        };
+        const uint8_t *lk = lds + (c & 1) * KB, *row_at = lk + 16 * place(m, g);
+        const int next = min(c + 1, chunks - 1);
+        lds_barrier();  // the keys, T and the factors are there, and the state's terms
         Rows ra, rb;
+        f4 x[4], r[4] = {zero, zero, zero, zero}, fx[4], fg[4];
         read_rows(ra, row_at, 0);
+        const float *vec = (const float *)(lds + L::vec + (c & 1) * L::vec_bytes);
+        const float whole = vec[ChunkWs::whole], top_x = vec[ChunkWs::top];
+        const int first_bad = *(const int *)(vec + ChunkWs::first);
         STEP;
-        // K S; the state's terms a pair of tiles ahead
-        const int ex_s = scale_of(rows16_max(__float_as_uint(top_s)));
-        const float up_s = scale_up(ex_s), down_s = scale_down(ex_s);
-        two_terms(S[0], S[1], up_s, sh[0], sl[0]);
-        f4 x[4], o[4] = {zero, zero, zero, zero}, r[4] = {zero, zero, zero, zero}, fx[4], ft[4], fg[4];
+        // the scale of X while the keys come: at most |v| + |e^G k| |S|
+        hold(v);
+        int ex_x = scale_of(__float_as_uint(ldexpf(top_x * (HD * 16384.0f), ex_s) + __uint_as_float(column_top(top_of(v)))));
+        factors(fx, c, ChunkWs::gx);
         STEP;
+        Tri tri;
 #pragma unroll
         for (int p = 0; p < KP; p++) {
             Rows &now = p % 2 ? rb : ra, &then = p % 2 ? ra : rb;
-            read_rows(then, p + 1 < KP ? row_at : query_at, (p + 1) % KP);
-            times(now, p, r);
-            if (p + 1 < KP) two_terms(S[2 * p + 2], S[2 * p + 3], up_s, sh[p + 1], sl[p + 1]);
-            MIX(12, 2);
-            STEP;
+            if (p + 1 < KP)
+                read_rows(then, row_at, p + 1);
+            else
+                read_tri(tri, L::T), factors(fg, c, ChunkWs::gg);
+            times(now, sh[p], sl[p], r, std::false_type{});
+            if (p == KP - 1) {
+                hold(fx);
+                const float up = scale_up(ex_x), by = ldexpf(-1.0f, min(ex_s - ex_x, 127));  // beyond it all of fx is 0
 #pragma unroll
-            for (int i = p * NK / KP; i < (p + 1) * NK / KP; i++) fetch_keys(next, into, i);
-#pragma unroll
-            for (int i = p * NT / KP; i < (p + 1) * NT / KP; i++) fetch_tp(next, into, i);
+                for (int t = 0; t < 4; t++) fx[t] *= by, x[t] = v[t] * up;
+            }
+            MIX(12, 1, 3);
             STEP;
         }
-        factors(fx, ChunkWs::gx);
-        const float whole = vec[ChunkWs::whole];
-        const int first_bad = *(const int *)(vec + ChunkWs::first);
-        read_rows(rb, query_at, 1);
-        STEP;
-        // X = V - diag(e^G) K S, and Q S, for which nothing waits
-        times(ra, 0, o);
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[t][e] = fmaf(-(fx[t][e] * r[t][e]), down_s, v[t][e]);
-        int ex_x = scale_of(rows16_max(__float_as_uint(top_of(x))));
-        MIX(12, 5);
-        STEP;
-        // a triangle's product: pair 0 of all four tiles of rows, pair 1 of the last two
-        struct Tri {
-            h8 h[6], l[6];
-        };
-        auto read_tri = [&](Tri &y, int what) {
-#pragma unroll
-            for (int i = 0; i < 6; i++) {
-                y.h[i] = *(const h8 *)(tp + what + i * 2048 + 16 * lane);
-                y.l[i] = *(const h8 *)(tp + what + i * 2048 + 1024 + 16 * lane);
-            }
-        };
-        auto triangle = [&](const Tri &y, const h8 (&h)[2], const h8 (&l)[2], f4 (&d)[4]) {
-#pragma unroll
-            for (int t = 0; t < 4; t++) d[t] = zero;
-#pragma unroll
-            for (int p = 0; p < 2; p++)
-#pragma unroll
-                for (int k = 0; k < 3; k++)
-#pragma unroll
-                    for (int t = 2 * p; t < 4; t++) d[t] = mfma_h(k < 2 ? y.h[tile_piece(t, p)] : y.l[tile_piece(t, p)], k == 1 ? l[p] : h[p], d[t]);
-        };
-        Tri tri;
+        // X = V - diag(e^G) K S, in units of 2^(ex_x - 14)
         h8 xh[2], xl[2], gh[2], gl[2];
-        read_tri(tri, ChunkWs::T);
-        factors(ft, ChunkWs::gt), factors(fg, ChunkWs::gg);
-        load_v(next);
-        STEP;
-        times(rb, 1, o);
-        if constexpr (KP > 2) read_rows(ra, query_at, 2), read_rows(rb, query_at, 3);
 #pragma unroll
-        for (int p = 0; p < 2; p++) two_terms(x[2 * p], x[2 * p + 1], scale_up(ex_x), xh[p], xl[p]);
-        MIX(12, 4);
+        for (int p = 0; p < 2; p++) {
+#pragma unroll
+            for (int t = 2 * p; t < 2 * p + 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[t][e] = fmaf(fx[t][e], r[t][e], x[t][e]);
+            two_terms(x[2 * p], x[2 * p + 1], xh[p], xl[p]);
+        }
         STEP;
-        // U, in units of X's scale
-        f4 u[4], ug[4];
-        triangle(tri, xh, xl, u);
+        f4 u[4], ug[4];  // U, in X's units and of T's rows
+        triangle(tri, xh, xl, u, std::false_type{});
+        load_v(next);
         const int first = uniform(first_bad);
+        STEP;
         // A correction that is not finite makes what it is multiplied with in the last row NaN or infinite, by 0 too
-        const bool bad = first < kChunk || __ballot(!finite32(u[3][3])) != 0;
         int stop = first;  // the column's rows from here on are not numbers
-        if (bad) {
+        if (first < kChunk || __ballot(!finite32(u[3][3])) != 0) {
 #pragma unroll
             for (int t = 3; t >= 0; t--)
 #pragma unroll
@@ -910,102 +1064,93 @@ __global__ __launch_bounds__(64 * NW, 1) void gdn_chunks_kernel(RuleArgs a) {
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[t][e] = 16 * t + 4 * g + e < stop ? x[t][e] : 0.0f;
-            ex_x = scale_of(rows16_max(__float_as_uint(top_of(x))));
+            const int ex = scale_of(column_top(top_of(x)));
+            ex_x += ex - 14;
 #pragma unroll
-            for (int p = 0; p < 2; p++) two_terms(x[2 * p], x[2 * p + 1], scale_up(ex_x), xh[p], xl[p]);
-            triangle(tri, xh, xl, u);
+            for (int p = 0; p < 2; p++) two_terms(x[2 * p], x[2 * p + 1], scale_up(ex), xh[p], xl[p]);
+            triangle(tri, xh, xl, u, std::false_type{});
         }
-        STEP;
-        // the rest of Q S meanwhile
-        read_tri(tri, ChunkWs::P);
-        if constexpr (KP > 2) times(ra, 2, o), times(rb, 3, o);
-#pragma unroll
-        for (int t = 0; t < 4; t++) u[t] = u[t] * ft[t], ug[t] = u[t] * fg[t];
-        const int ex_g = scale_of(rows16_max(__float_as_uint(top_of(ug)))), ex_u = scale_of(rows16_max(__float_as_uint(top_of(u))));
-#pragma unroll
-        for (int p = 0; p < 2; p++) two_terms(ug[2 * p], ug[2 * p + 1], scale_up(ex_g), gh[p], gl[p]);
-        const float down_x = scale_down(ex_x), down_g = scale_down(ex_g) * down_x, down_u = scale_down(ex_u) * down_x;
-        if constexpr (KP > 2) {
-            MIX(24, 5);
-        }
-        STEP;
-        // S <- e^G_63 S + K^T (e^(G_63 - G) U), four tiles of the state at a time: the keys by columns, rows 4 g + m / 4
+        // S <- e^G_63 S + K^T (e^(G_63 - G) U), two tiles of the state at a time: the keys by columns, rows 4 g + m / 4
         // of tile 2 p + (0, 1), columns 4 (m % 4) and on of state tile i
         struct Cols {
-            h8 h[4], l[4];
+            h8 h[2][2], l[2][2];
         };
         const uint8_t *col_at = lk + 16 * place(4 * g + (m >> 2), m & 3);
-        auto read_tiles = [&](Cols &k, int i0, int p) {
+        auto read_tiles = [&](Cols &k, int i0) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint8_t *y = col_at + (2 * p * KP + (i0 + j) / 2) * 2048 + 8 * ((i0 + j) & 1);
-                k.h[j] = __builtin_shufflevector(read_columns(y), read_columns(y + KP * 2048), 0, 1, 2, 3, 4, 5, 6, 7);
-                k.l[j] = __builtin_shufflevector(read_columns(y + 1024), read_columns(y + KP * 2048 + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            for (int p = 0; p < 2; p++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint8_t *y = col_at + (2 * p * KP + i0 / 2) * 2048 + 8 * j;
+                    k.h[p][j] = __builtin_shufflevector(read_columns(y), read_columns(y + KP * 2048), 0, 1, 2, 3, 4, 5, 6, 7);
+                    k.l[p][j] = __builtin_shufflevector(read_columns(y + 1024), read_columns(y + KP * 2048 + 1024), 0, 1, 2, 3, 4, 5, 6, 7);
+                }
         };
-        Cols ka, kb;
-        read_tiles(ka, 0, 0);
-        lds_barrier();  // the queries are read
+        Cols cols[2];
+        read_tiles(cols[0], 0);
 #pragma unroll
-        for (int i = 0; i < NK; i++) fetch_queries(next, i);
-        f4 fq[4], fp[4], d[ST];
+        for (int t = 0; t < 4; t++) {
+            ug[t] = u[t] * fg[t];
+            *(f4 *)(lu + 1024 * t) = u[t];
+        }
+        one[32 + m] = scale_down(ex_x);
+        one[48 + m] = __int_as_float(stop);
+        const uint32_t top_g = column_top(top_of(ug));
+        const int ex_g = scale_of(top_g);
+        const float up_g = scale_up(ex_g);
+        two_terms(ug[0], ug[1], up_g, gh[0], gl[0]);
         STEP;
+        lds_barrier();  // the corrections are there
+        const float top_s = one[16 + m] + 0x1p-24f;  // f16 takes values to 0 below half of that
+        fetch_after(next, 0, 2);
+        STEP;
+        f4 d[2][2];
+        float keep = 0.0f, add = 0.0f;
+        auto update = [&](int q) {
 #pragma unroll
-        for (int i = 0; i < ST; i++) d[i] = zero;
-        auto update = [&](int i0) {
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int i = i0; i < i0 + 4; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) S[i][e] = fmaf(d[i][e], down_g, S[i][e] * whole);
+                for (int e = 0; e < 4; e++) S[2 * q + t][e] = fmaf(d[q % 2][t][e], add, S[2 * q + t][e] * keep);
+            state_terms(q);
         };
 #pragma unroll
-        for (int i = 0; i < ST; i += 4)
+        for (int q = 0; q < KP; q++) {
+            const Cols &k = cols[q % 2];
+            if (q + 1 < KP) read_tiles(cols[(q + 1) % 2], 2 * q + 2);
+            d[q % 2][0] = d[q % 2][1] = zero;
+            if (q == 0) two_terms(ug[2], ug[3], up_g, gh[1], gl[1]);
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                const Cols &k = p ? kb : ka;
-                if (p == 0)
-                    read_tiles(kb, i, 1);
-                else if (i + 4 < ST)
-                    read_tiles(ka, i + 4, 0);
-                else
-                    factors(fq, ChunkWs::gq), factors(fp, ChunkWs::gp);
+            for (int p = 0; p < 2; p++)
 #pragma unroll
                 for (int y = 0; y < 3; y++)
 #pragma unroll
-                    for (int t = 0; t < 4; t++) d[i + t] = mfma_h(y < 2 ? k.h[t] : k.l[t], y == 1 ? gl[p] : gh[p], d[i + t]);
-                if (i == 0) two_terms(u[2 * p], u[2 * p + 1], scale_up(ex_u), xh[p], xl[p]);
-                if (i && p == 0) update(i - 4);
-                if (i + 4 >= ST && p == 1)
-#pragma unroll
-                    for (int t = 0; t < 4; t++) o[t] = fq[t] * o[t] * down_s;
-                MIX(12, 3);
-                STEP;
+                    for (int t = 0; t < 2; t++) d[q % 2][t] = mfma_h(y < 2 ? k.h[p][t] : k.l[p][t], y == 1 ? gl[p] : gh[p], d[q % 2][t]);
+            if (q == 0) {
+                // what the sum's terms amount to at most; those of K^T U by the operands' scales and the depth
+                const int to = scale_of(__float_as_uint(ldexpf(top_s * whole, ex_s - 14) + ldexpf(__uint_as_float(top_g) * kChunk, ex_x)));
+                keep = ldexpf(whole, ex_s - to), add = ldexpf(1.0f, ex_g + ex_x - 14 - to);
+                ex_s = to;
+                one[m] = scale_down(ex_s);
+            } else {
+                update(q - 1);
             }
-        // out
-        triangle(tri, xh, xl, r);
-        update(ST - 4);
-        top_s = top_of(S);
-        MIX(18, 3);
-        STEP;
-        const auto bo = rows_of(out, out_row, c);
-        if (bad && stop < kChunk) {
-            const float nan = __uint_as_float(0x7FC00000u);
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) r[t][e] = 16 * t + 4 * g + e >= stop ? nan : r[t][e];
-#pragma unroll
-            for (int i = 0; i < ST; i++) S[i] = f4{nan, nan, nan, nan};
+            MIX(12, 2, 5);
+            STEP;
         }
+        update(KP - 1);
+        if (__ballot(stop < kChunk)) {
+            const float nan = __uint_as_float(0x7FC00000u);
+            if (stop < kChunk)
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+                for (int i = 0; i < ST; i++) S[i] = f4{nan, nan, nan, nan};
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(fmaf(fp[t][e] * r[t][e], down_u, o[t][e])), bo, o_at + 4 * (16 * t + e) * out_row, 0, 0);
+            for (int p = 0; p < KP; p++) state_terms(p);
+        }
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the queries and T; the values, too
     }
+    units(ex_s - 14);
 #undef MIX
 #undef STEP
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what the last chunk brought lands before the wave leaves
     if ((unsigned)to < (unsigned)a.st.n_slots) {
         float *p = a.st.state + ((size_t)to * a.st.nv + head) * HD * HD + mine;
 #pragma unroll
@@ -1091,11 +1236,11 @@ hipError_t launch_rule(RuleArgs a, hipStream_t s) {
     const size_t first = (size_t)a.slots * a.st.nqk + (size_t)a.b.n_seqs * a.st.nv, across = std::min(first, (size_t)1 << 22);
     hipLaunchKernelGGL(gdn_prep_kernel<HD>, dim3((unsigned)across, (unsigned)((first + across - 1) / across)), dim3(kPrepTPB), 0, s, a);
     if (hipError_t e = hipGetLastError()) return e;
-    constexpr size_t lds = 3 * kq_bytes(HD) + 2 * ChunkWs::bytes;
+    constexpr size_t lds = ChunkLds<HD>::bytes;
     const long long pairs = (long long)a.longs * a.st.nv;
-    const auto kernel = gdn_chunks_kernel<HD, kChunkWaves>;
+    const auto kernel = gdn_chunks_kernel<HD>;
     if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / (16 * kChunkWaves)))), dim3(64 * kChunkWaves), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / kChunkCols))), dim3(256), lds, s, a);
     if (hipError_t e = hipGetLastError()) return e;
     if (a.h.d_norm || a.h.d_z) hipLaunchKernelGGL(gdn_finish_kernel<HD>, dim3((unsigned)a.slots, (unsigned)a.st.nv), dim3(256), 0, s, a);
     return hipGetLastError();
