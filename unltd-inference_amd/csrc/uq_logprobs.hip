@@ -33,6 +33,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 struct Part {
     float m, l, s;
     int before;  // tokens before the given one
+    int kept, unused;  // keys
 };
 
 struct Args {
@@ -43,7 +44,7 @@ struct Args {
     int n_rows, vocab, n_top, tiles, run, parts;  // tiles of a row, of a wave; waves of a row
     float scale, c;
     Part *part;      // [n_rows][parts]
-    uint64_t *keys;  // [n_rows][parts][n_top]
+    uint64_t *keys;  // [n_rows][parts][64]
 };
 
 // Tokens in their order as integers: the larger the logit, then the smaller the number, the larger the key. 0 is none.
@@ -57,32 +58,48 @@ __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
            (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
-// The lane before's value, 0 in the first.
-__device__ __forceinline__ uint64_t from_before(uint64_t v) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), 0x138, 0xF, 0xF, true) << 32 |
-           (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x138, 0xF, 0xF, true);  // wave_shr:1
-}
+constexpr uint32_t kLowest = 0x00800000u;  // ordered(-infinity) + 1: neither it nor a NaN that is below it is kept
 
-// The first n_top keys seen, in order over the lanes; `least` is the last of them.
-struct Best {
-    uint64_t mine = 0, least = 0;
-    int n_top;
-    __device__ __forceinline__ explicit Best(int n) : n_top(n) {}
-    // Takes up a key a lane, those that belong among the first, largest gain first or not: whatever the order, each
-    // that is taken was among the first of those seen.
-    __device__ __forceinline__ void take(uint64_t key) {
+// Keys in the LDS, the first n_top (64 at most) of those offered among them. Only when they overflow are they put in
+// order, and the first n_top kept: a wave's run mostly ends before.
+constexpr int kPool = 128;  // 64 are free after that, as many as one call offers
+struct Pool {
+    uint64_t *at;
+    int n_top, count = 0;
+    uint32_t least = kLowest;  // logits below it are not among the first
+    bool full = false;         // n_top keys are kept, of which the last has the logit `least`
+    __device__ __forceinline__ Pool(uint64_t *p, int n) : at(p), n_top(n) {}
+    // Puts the keys in order and keeps the first n_top. A key's place is how many are larger: keys differ, as a token is seen once.
+    __device__ __forceinline__ void order() {
         const int lane = threadIdx.x & 63;
-        for (;;) {
-            const unsigned long long over = __ballot(key > least);
-            if (!over) return;
-            const int from = __builtin_ctzll(over);
-            const uint64_t k = lane_of(key, from);
-            const int at = __builtin_popcountll(__ballot(mine > k));  // keys differ: a token is seen once
-            const uint64_t shifted = from_before(mine);
-            mine = lane < at ? mine : lane == at ? k : shifted;
-            least = lane_of(mine, n_top - 1);
-            if (lane == from) key = 0;
+        const uint64_t k0 = lane < count ? at[lane] : 0, k1 = lane + 64 < count ? at[lane + 64] : 0;
+        int p0 = 0, p1 = 0;
+        for (int j = 0; j < min(count, 64); j++) p0 += lane_of(k0, j) > k0;
+        if (count > 64) {
+            for (int j = 0; j < 64; j++) p1 += lane_of(k0, j) > k1;
+            for (int j = 0; j < count - 64; j++) {
+                const uint64_t k = lane_of(k1, j);
+                p0 += k > k0;
+                p1 += k > k1;
+            }
         }
+        if (lane < count && p0 < n_top) at[p0] = k0;
+        if (lane + 64 < count && p1 < n_top) at[p1] = k1;
+        count = min(count, n_top);
+    }
+    __device__ __forceinline__ void take(uint64_t key, bool in) {
+        unsigned long long b = __ballot(in);
+        if (!b) return;
+        if (count + __builtin_popcountll(b) > kPool) {
+            order();
+            full = true;
+            least = max(least, (uint32_t)uniform((int)(at[n_top - 1] >> 32)));
+            in = in && (uint32_t)(key >> 32) >= least;
+            b = __ballot(in);
+        }
+        const int slot = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        if (in) at[count + slot] = key;
+        count += __builtin_popcountll(b);
     }
 };
 
@@ -126,7 +143,8 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
     const float given = ranked ? x[token] : INFINITY;
     float m = -FLT_MAX, l = 0.0f, s = 0.0f;
     int before = 0;
-    Best best(a.n_top);
+    __shared__ uint64_t pools[TOP ? kTPB / 64 : 1][kPool];
+    Pool pool(pools[TOP ? threadIdx.x >> 6 : 0], a.n_top);
     for (int t = t0; t < t1; t++) {
         if (t + 1 < t1) load(next, t + 1);
         float top = v[0];
@@ -164,20 +182,19 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
             }
         }
         if constexpr (TOP) {
-            // Later tokens of equal logits come after those held: only larger ones are looked at once the list is
-            // full. Where many lanes have some (a run's first tile), those below a bound that n_top lanes reach
-            // with their largest cannot be among the first.
-            uint32_t bound = (uint32_t)(best.least >> 32);
+            // Values below a bound that n_top lanes reach with their largest cannot be among the first.
             const uint32_t most = ordered(top);
-            const unsigned long long over = __ballot(top > -INFINITY && most > bound);
+            const unsigned long long over = __ballot(most >= pool.least);
             if (over) {
-                bound = bound ? bound + 1 : ordered(-INFINITY) + 1;
-                if (__builtin_popcountll(over) >= a.n_top) bound = max(bound, reached_by(most, a.n_top));
+                if (__builtin_popcountll(over) >= a.n_top) pool.least = max(pool.least, reached_by(most, a.n_top));
 #pragma unroll
                 for (int i = 0; i < kVals; i++) {
                     const uint32_t o = ordered(v[i]);
-                    const bool in = o >= bound && v[i] == v[i];
-                    if (__ballot(in)) best.take(in ? (uint64_t)o << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4) : 0);
+                    pool.take((uint64_t)o << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4), o >= pool.least && v[i] == v[i]);
+                }
+                if (pool.full) {  // later tokens of equal logits come after those kept
+                    pool.least += 1;
+                    pool.full = false;
                 }
             }
         }
@@ -194,9 +211,11 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
     s = wave_sum(f * fmaf(d, l, s));
     l = wave_sum(f * l);
     const size_t o = (size_t)row * a.parts + part;
-    if (lane == 0) a.part[o] = Part{all, l, s, before};
     if constexpr (TOP)
-        if (lane < a.n_top) a.keys[o * a.n_top + lane] = best.mine;
+        if (pool.count > 64) pool.order();
+    if (lane == 0) a.part[o] = Part{all, l, s, before, pool.count, 0};
+    if constexpr (TOP)
+        if (lane < pool.count) a.keys[o * 64 + lane] = pool.at[lane];
 }
 
 // A wave a row: joins its parts and writes the results.
@@ -206,14 +225,23 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
     const Part *parts = a.part + (size_t)row * a.parts;
     float m = -FLT_MAX, l = 0.0f, s = 0.0f;
     int before = 0;
-    for (int i = lane; i < a.parts; i += 64) {
-        const Part p = parts[i];
-        const float to = fmaxf(m, p.m), d = fmaxf((m - to) * a.c, kLeast), dp = fmaxf((p.m - to) * a.c, kLeast);
-        const float f = exp2_hw(d), fp = exp2_hw(dp);
-        s = f * fmaf(d, l, s) + fp * fmaf(dp, p.l, p.s);
-        l = f * l + fp * p.l;
-        m = to;
-        before += p.before;
+    uint32_t most = 0;
+    constexpr int P = 4;  // parts of a lane at a time
+    for (int i0 = 0; i0 < a.parts; i0 += 64 * P) {
+        Part p[P];
+#pragma unroll
+        for (int j = 0; j < P; j++) p[j] = parts[min(i0 + 64 * j + lane, a.parts - 1)];
+#pragma unroll
+        for (int j = 0; j < P; j++) {
+            if (i0 + 64 * j + lane >= a.parts) continue;
+            const float to = fmaxf(m, p[j].m), d = fmaxf((m - to) * a.c, kLeast), dp = fmaxf((p[j].m - to) * a.c, kLeast);
+            const float f = exp2_hw(d), fp = exp2_hw(dp);
+            s = f * fmaf(d, l, s) + fp * fmaf(dp, p[j].l, p[j].s);
+            l = f * l + fp * p[j].l;
+            m = to;
+            before += p[j].before;
+            most = max(most, ordered(p[j].m));
+        }
     }
     float all = m;
     for (int d = 1; d < 64; d *= 2) all = fmaxf(all, __shfl_xor(all, d));
@@ -234,35 +262,36 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
         if (a.out.d_entropy) a.out.d_entropy[row] = !sound ? nan : l > 0.0f ? fmaxf(0.0f, ln_l - 0.693147182f * (s / l)) : 0.0f;
     }
     if constexpr (TOP) {
-        const uint64_t *keys = a.keys + (size_t)row * a.parts * a.n_top;
-        const int n = a.parts * a.n_top;
-        Best best(a.n_top);
-        constexpr int N = 16;  // keys of a lane at a time
-        for (int i0 = 0; i0 < n; i0 += 64 * N) {
-            uint64_t k[N], top = 0;
+        // as within a wave's run: n_top parts reach the bound with their largest, and the others are not read
+        __shared__ uint64_t kept[kPool];
+        Pool pool(kept, a.n_top);
+        if (a.parts >= a.n_top) pool.least = max(pool.least, reached_by(most, a.n_top));
+        const uint64_t *keys = a.keys + (size_t)row * a.parts * 64;
+        for (int i0 = 0; i0 < a.parts; i0 += 64) {
+            const int i = min(i0 + lane, a.parts - 1);
+            const int count = parts[i].kept;
+            unsigned long long over = __ballot(i0 + lane < a.parts && ordered(parts[i].m) >= pool.least);
+            constexpr int N = 8;  // parts at a time
+            while (over) {
+                uint64_t k[N];
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const int i = i0 + 64 * j + lane;
-                k[j] = i < n ? keys[i] : 0;
-                top = k[j] > top ? k[j] : top;
-            }
-            const unsigned long long over = __ballot(top > best.least);
-            if (!over) continue;
-            uint64_t bound = best.least + 1;
-            if (__builtin_popcountll(over) >= a.n_top) {
-                const uint64_t r = (uint64_t)reached_by((uint32_t)(top >> 32), a.n_top) << 32;
-                bound = r > bound ? r : bound;
-            }
+                for (int j = 0; j < N; j++) {
+                    const int from = over ? __builtin_ctzll(over) : 0, n = over ? __builtin_amdgcn_readlane(count, from) : 0;
+                    k[j] = lane < n ? keys[(size_t)(i0 + from) * 64 + lane] : 0;
+                    over &= over - 1;
+                }
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (__ballot(k[j] >= bound)) best.take(k[j] >= bound ? k[j] : 0);
+                for (int j = 0; j < N; j++) pool.take(k[j], (uint32_t)(k[j] >> 32) >= pool.least);
+            }
         }
+        pool.order();
+        const uint64_t mine = lane < pool.count ? kept[lane] : 0;
         if (lane < a.n_top) {
-            const bool is = sound && best.mine != 0;
-            const uint32_t u = (uint32_t)(best.mine >> 32);
+            const bool is = sound && mine != 0;
+            const uint32_t u = (uint32_t)(mine >> 32);
             const float x = __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
             const size_t o = (size_t)row * a.n_top + lane;
-            if (a.out.d_top_id) a.out.d_top_id[o] = is ? (int)~(uint32_t)best.mine : -1;
+            if (a.out.d_top_id) a.out.d_top_id[o] = is ? (int)~(uint32_t)mine : -1;
             if (a.out.d_top_logprob) a.out.d_top_logprob[o] = !sound ? nan : is ? log_p(x) : -INFINITY;
         }
     }
@@ -285,7 +314,7 @@ Shape shape_of(int n_rows, int vocab) {
 
 size_t logprobs_ws_bytes(int n_rows, int vocab, int n_top) {
     const Shape s = shape_of(n_rows, vocab);
-    return (size_t)n_rows * s.parts * (sizeof(Part) + (size_t)n_top * sizeof(uint64_t));
+    return (size_t)n_rows * s.parts * (sizeof(Part) + (n_top ? 64 * sizeof(uint64_t) : 0));
 }
 
 hipError_t launch_logprobs(const uq_logprobs &out, const float *x, size_t x_row, const int32_t *tokens, int n_rows,
