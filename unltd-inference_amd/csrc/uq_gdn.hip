@@ -54,8 +54,9 @@ __device__ __forceinline__ int wave_scan_i(int v) {
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// x / (1 + e^-x). The quotient by the hardware's reciprocal (1 ulp).
-__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + expf(-x)); }
+// x / (1 + e^-x), by the hardware's power of 2 and reciprocal (1 ulp each). The exponent's rounding is |x| 2^-24 of e^-x,
+// of which at most x e^-x = 0.4 is left where it counts, and where it is large, below 0, so is x.
+__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x)); }
 
 // Sequences of at least `least` rows are cut into tiles of T rows, numbered
 // through; every wave finds its tile's by itself, 256 sequences at a time.
@@ -165,9 +166,10 @@ template <int CK>  // taps, 0: any up to 9
 __global__ __launch_bounds__(kConvTPB) void gdn_conv_kernel(ConvArgs a) {
     constexpr int MT = CK ? CK : 9, H = MT - 1, STEP = 4;
     const int taps = CK ? CK : a.st.taps, skip = MT - taps;  // places before the first tap
-    const int lane = threadIdx.x & 63, group = uniform((int)(blockIdx.y * (kConvTPB / 64) + (threadIdx.x >> 6)));
+    const unsigned per = (unsigned)(a.groups + kConvTPB / 64) / (kConvTPB / 64), i = blockIdx.y * gridDim.x + blockIdx.x, tile = i / per;
+    const int lane = threadIdx.x & 63, group = uniform((int)(i - tile * per) * (kConvTPB / 64) + (int)(threadIdx.x >> 6));
     if (group > a.groups) return;
-    const Tile t = find_tile<kConvRows>(a.b, (int)blockIdx.x, 1);
+    const Tile t = find_tile<kConvRows>(a.b, (int)tile, 1);
     if (t.seq < 0) return;
     const int nn = min(kConvRows, t.n - t.first);
     const size_t row0 = (size_t)t.lo + t.first;
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(kConvTPB) void gdn_conv_kernel(ConvArgs a) {
                 float s = 0.0f;
 #pragma unroll
                 for (int k = 0; k < MT; k++)
-                    if (k >= skip) s = __fadd_rn(s, __fmul_rn(x[u + k][e], tap[e][k]));
+                    if (k >= skip) s = fmaf(x[u + k][e], tap[e][k], s);
                 y[e] = silu(s);
             }
             float sq = 0.0f;
@@ -1165,10 +1167,12 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
 template <int HD>
 __global__ __launch_bounds__(256) void gdn_finish_kernel(RuleArgs a) {
     constexpr int PER = HD / 4, STEP = 256 / PER, N = kChunk / STEP;  // threads of a row, rows at a time, rows of a thread
-    const int head = blockIdx.y, r0 = threadIdx.x / PER, o = 4 * (threadIdx.x % PER);
-    const Long s = find_long<true>(a.b, (int)blockIdx.x, a.chunked);
+    const unsigned i = blockIdx.y * gridDim.x + blockIdx.x;
+    const int slot = (int)(i / a.st.nv), head = (int)(i % a.st.nv), r0 = threadIdx.x / PER, o = 4 * (threadIdx.x % PER);
+    if (slot >= a.slots) return;
+    const Long s = find_long<true>(a.b, slot, a.chunked);
     if (s.seq < 0) return;
-    const int c0 = ((int)blockIdx.x - s.slot) * kChunk, n = min(kChunk, s.n - c0);
+    const int c0 = (slot - s.slot) * kChunk, n = min(kChunk, s.n - c0);
     const size_t row0 = (size_t)s.lo + c0;
     f4 v[N], z[N], w{1.f, 1.f, 1.f, 1.f};
     if (a.h.d_norm) w = *(const f4u *)(a.h.d_norm + o);
@@ -1196,11 +1200,19 @@ __global__ __launch_bounds__(256) void gdn_finish_kernel(RuleArgs a) {
 
 }  // namespace
 
+// So many workgroups, of which a kernel numbers those across first.
+static dim3 grid_of(size_t n) {
+    const size_t across = std::min(n, (size_t)1 << 22);
+    return dim3((unsigned)across, (unsigned)((n + across - 1) / across));
+}
+
 hipError_t launch_gdn_conv(const StatesView &st, const BatchView &b, const uq_gdn_rows &r, hipStream_t s) {
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
     const ConvArgs a{st, b, r, (st.channels + 255) / 256};
     const unsigned per = kConvTPB / 64, tiles = (unsigned)(b.n_rows / kConvRows + std::min(b.n_seqs, b.n_rows));
-    const dim3 grid(tiles, ((unsigned)a.groups + per) / per);
+    // A tile's channels one after another: rows are often a power of 2 apart, and a column of tiles would meet in few of
+    // the memory's channels. Three prompts of 5000 rows of 8192 channels so take 82 us, and 99 the other way round.
+    const dim3 grid = grid_of((size_t)tiles * (((unsigned)a.groups + per) / per));
     if (st.taps == 4)
         hipLaunchKernelGGL(gdn_conv_kernel<4>, grid, dim3(kConvTPB), 0, s, a);
     else
@@ -1233,8 +1245,7 @@ hipError_t launch_rule(RuleArgs a, hipStream_t s) {
         hipLaunchKernelGGL(gdn_rows_kernel<HD>, dim3((unsigned)a.st.nv, (unsigned)a.b.n_seqs), dim3(2 * HD), 0, s, a);
         return hipGetLastError();
     }
-    const size_t first = (size_t)a.slots * a.st.nqk + (size_t)a.b.n_seqs * a.st.nv, across = std::min(first, (size_t)1 << 22);
-    hipLaunchKernelGGL(gdn_prep_kernel<HD>, dim3((unsigned)across, (unsigned)((first + across - 1) / across)), dim3(kPrepTPB), 0, s, a);
+    hipLaunchKernelGGL(gdn_prep_kernel<HD>, grid_of((size_t)a.slots * a.st.nqk + (size_t)a.b.n_seqs * a.st.nv), dim3(kPrepTPB), 0, s, a);
     if (hipError_t e = hipGetLastError()) return e;
     constexpr size_t lds = ChunkLds<HD>::bytes;
     const long long pairs = (long long)a.longs * a.st.nv;
@@ -1242,7 +1253,7 @@ hipError_t launch_rule(RuleArgs a, hipStream_t s) {
     if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / kChunkCols))), dim3(256), lds, s, a);
     if (hipError_t e = hipGetLastError()) return e;
-    if (a.h.d_norm || a.h.d_z) hipLaunchKernelGGL(gdn_finish_kernel<HD>, dim3((unsigned)a.slots, (unsigned)a.st.nv), dim3(256), 0, s, a);
+    if (a.h.d_norm || a.h.d_z) hipLaunchKernelGGL(gdn_finish_kernel<HD>, grid_of((size_t)a.slots * a.st.nv), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
