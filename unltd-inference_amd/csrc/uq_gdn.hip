@@ -269,6 +269,7 @@ struct RuleArgs {
     uq_gdn_heads h;
     int chunked;      // sequences of at least so many rows go by chunks
     int longs, slots; // of those at most, and of their chunks
+    int singles;      // workgroups of half the sequences that go row by row, a multiple of 8
     uint8_t *ws;      // [slots][nv] ChunkWs
     uint8_t *kq;      // [slots][nqk] keys, then queries (KqWs)
 };
@@ -397,6 +398,13 @@ __device__ __forceinline__ void rule_rows(const RuleArgs &a, int seq, int head, 
     }
 }
 
+// Workgroup i of the even (odd: 1) sequences' in a kernel of 256 threads. Both kernels of the chunks take half: each
+// leaves compute units free where chunks are few, and the states' way from memory and back is what these need.
+template <int HD>
+__device__ __forceinline__ void rule_rows_of(const RuleArgs &a, unsigned i, int odd, float (*buf)[HD]) {
+    const unsigned seq = 2 * (i / a.st.nv) + odd;
+    if (threadIdx.x < 2 * HD && seq < (unsigned)a.b.n_seqs) rule_rows<HD>(a, (int)seq, (int)(i % a.st.nv), buf);  // whole waves
+}
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
     __shared__ __align__(16) float buf[kRowBuf][HD];
@@ -729,7 +737,7 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
         }
     }
 }
-// The chunks' workgroups, which the next kernel waits for, then those of the sequences that go row by row.
+// The chunks' workgroups, which the next kernel waits for, then those of sequences that go row by row.
 template <int HD>
 __global__ __launch_bounds__(kPrepTPB, 3) void gdn_prep_kernel(RuleArgs a) {
     __shared__ union Lds {
@@ -739,8 +747,8 @@ __global__ __launch_bounds__(kPrepTPB, 3) void gdn_prep_kernel(RuleArgs a) {
     const unsigned chunks = (unsigned)a.slots * a.st.nqk, i = blockIdx.y * gridDim.x + blockIdx.x;
     if (i < chunks)
         rule_prep<HD>(a, (int)(i / a.st.nqk), (int)(i % a.st.nqk), l.prep);
-    else if (threadIdx.x < 2 * HD && i - chunks < (unsigned)a.b.n_seqs * a.st.nv)  // whole waves
-        rule_rows<HD>(a, (int)((i - chunks) / a.st.nv), (int)((i - chunks) % a.st.nv), l.buf);
+    else
+        rule_rows_of<HD>(a, i - chunks, 0, l.buf);
 }
 
 // The transposing LDS read: of the 16 lanes' 16 x 4 values, lane i gets value i % 4 of lanes 4 j + i / 4, j < 4.
@@ -760,6 +768,9 @@ __device__ __forceinline__ h4 read_columns(const uint8_t *p) {
 // vector instructions between them are ordered so that the latter run while
 // the matrix cores work.
 constexpr int kChunkCols = 32;
+// Workgroups of columns, one a compute unit, that go before the sequences that go row by row; most of the others, of
+// sequences that there may be, find none.
+constexpr int kFirstChains = 256;
 template <int HD>
 struct ChunkLds {
     static constexpr int KB = kq_bytes(HD), Q = 2 * KB, T = 3 * KB, P = T + ChunkWs::P, vec = T + ChunkWs::vec, vec_bytes = ChunkWs::bytes - ChunkWs::vec;  // keys and factors twice
@@ -771,7 +782,12 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
     constexpr int KP = HD / 32, ST = HD / 16, NB = HD / kChunkCols, KB = L::KB;
     extern __shared__ __align__(1024) uint8_t lds[];
     // a head's column blocks on one XCD (workgroup i runs on XCD i % 8), whose L2 they share their operands in
-    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, pair = at / NB * 8 + xcd, head = pair % a.st.nv, hq = head % a.st.nqk;
+    unsigned i = blockIdx.y * gridDim.x + blockIdx.x;
+    if (i >= (unsigned)kFirstChains) {
+        if (i - kFirstChains < (unsigned)a.singles) return rule_rows_of<HD>(a, i - kFirstChains, 1, (float (*)[HD])lds);
+        i -= a.singles;
+    }
+    const int xcd = i & 7, at = i >> 3, pair = at / NB * 8 + xcd, head = pair % a.st.nv, hq = head % a.st.nqk;
     if (pair >= a.longs * a.st.nv) return;
     const Long s = find_long<false>(a.b, pair / a.st.nv, a.chunked);
     if (s.seq < 0) return;
@@ -1220,23 +1236,28 @@ hipError_t launch_gdn_conv(const StatesView &st, const BatchView &b, const uq_gd
     return hipGetLastError();
 }
 
-// Sequences of this many rows and more go by chunks.
-constexpr int kChunkLeast = 32;
-
 namespace {
+// Sequences of this many rows and more go by chunks. One alone takes as long by chunks at 64 rows as at 20, and row by
+// row is quicker where many share the chip. Heads of 128, rows and us row by row / by chunks: 1 sequence of 32 heads,
+// 24: 30 / 23; 8, 32: 45 / 46; 64, 32: 203 / 275, 48: 288 / 286; 300, 64: 1586 / 1460.
+int chunk_least(const StatesView &st, const BatchView &b) {
+    const long long heads = (long long)b.n_seqs * st.nv;
+    return heads <= 64 ? 24 : heads <= 1024 ? 32 : 48;
+}
 // How many sequences can go by chunks, and the slots of their chunks; 0 where none is expected to.
 struct Plan {
-    int longs, slots;
+    int least, longs, slots;
 };
-Plan plan_of(const BatchView &b, size_t most_rows) {
-    if (b.n_rows < kChunkLeast || (most_rows && most_rows < (size_t)kChunkLeast)) return Plan{0, 0};
-    const int longs = std::min(b.n_seqs, b.n_rows / kChunkLeast);
-    return Plan{longs, b.n_rows / kChunk + longs + 1};
+Plan plan_of(const StatesView &st, const BatchView &b, size_t most_rows) {
+    const int least = chunk_least(st, b);
+    if (b.n_rows < least || (most_rows && most_rows < (size_t)least)) return Plan{INT_MAX, 0, 0};
+    const int longs = std::min(b.n_seqs, b.n_rows / least);
+    return Plan{least, longs, b.n_rows / kChunk + longs + 1};
 }
 }  // namespace
 
 size_t gdn_rule_ws_bytes(const StatesView &st, const BatchView &b, size_t most_rows) {
-    return 16 + (size_t)plan_of(b, most_rows).slots * (st.nv * (size_t)ChunkWs::bytes + st.nqk * (size_t)(2 * kq_bytes(st.hd)));
+    return 16 + (size_t)plan_of(st, b, most_rows).slots * (st.nv * (size_t)ChunkWs::bytes + st.nqk * (size_t)(2 * kq_bytes(st.hd)));
 }
 
 template <int HD>
@@ -1245,13 +1266,14 @@ hipError_t launch_rule(RuleArgs a, hipStream_t s) {
         hipLaunchKernelGGL(gdn_rows_kernel<HD>, dim3((unsigned)a.st.nv, (unsigned)a.b.n_seqs), dim3(2 * HD), 0, s, a);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(gdn_prep_kernel<HD>, grid_of((size_t)a.slots * a.st.nqk + (size_t)a.b.n_seqs * a.st.nv), dim3(kPrepTPB), 0, s, a);
-    if (hipError_t e = hipGetLastError()) return e;
     constexpr size_t lds = ChunkLds<HD>::bytes;
-    const long long pairs = (long long)a.longs * a.st.nv;
     const auto kernel = gdn_chunks_kernel<HD>;
     if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((pairs + 7) / 8 * 8 * (HD / kChunkCols))), dim3(256), lds, s, a);
+    const size_t pairs = (size_t)a.longs * a.st.nv, seqs = a.b.n_seqs, nv = a.st.nv;
+    a.singles = (int)((seqs / 2 * nv + 7) / 8 * 8);
+    hipLaunchKernelGGL(gdn_prep_kernel<HD>, grid_of((size_t)a.slots * a.st.nqk + (seqs + 1) / 2 * nv), dim3(kPrepTPB), 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    hipLaunchKernelGGL(kernel, grid_of(std::max((size_t)kFirstChains, (pairs + 7) / 8 * 8 * (HD / kChunkCols)) + a.singles), dim3(256), lds, s, a);
     if (hipError_t e = hipGetLastError()) return e;
     if (a.h.d_norm || a.h.d_z) hipLaunchKernelGGL(gdn_finish_kernel<HD>, grid_of((size_t)a.slots * a.st.nv), dim3(256), 0, s, a);
     return hipGetLastError();
@@ -1260,8 +1282,8 @@ hipError_t launch_rule(RuleArgs a, hipStream_t s) {
 hipError_t launch_gdn_rule(float *out, const StatesView &st, const BatchView &b, const uq_gdn_heads &h, size_t most_rows,
                            void *ws, hipStream_t s) {
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
-    const Plan p = plan_of(b, most_rows);
-    const RuleArgs a{out, st, b, h, p.longs ? kChunkLeast : INT_MAX, p.longs, p.slots, (uint8_t *)ws, (uint8_t *)ws + (size_t)p.slots * st.nv * ChunkWs::bytes};
+    const Plan p = plan_of(st, b, most_rows);
+    const RuleArgs a{out, st, b, h, p.least, p.longs, p.slots, 0, (uint8_t *)ws, (uint8_t *)ws + (size_t)p.slots * st.nv * ChunkWs::bytes};
     return st.hd == 128 ? launch_rule<128>(a, s) : launch_rule<64>(a, s);
 }
 
