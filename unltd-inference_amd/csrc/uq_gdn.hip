@@ -864,12 +864,12 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
     constexpr int NK = KB / 2048, NT = ChunkWs::P / 2048;
     static_assert(L::vec_bytes == 2048, "a piece for each wave");
     auto fetch = [&](const uint8_t *from, int to, int i) { dma16(from + 2048 * i, lds + to + 1024 * half + 2048 * i); };
-    // queries and T, part of n
-    auto fetch_after = [&](int c, int part, int n) {
+    // queries and T
+    auto fetch_after = [&](int c) {
 #pragma unroll
-        for (int i = part * NK / n; i < (part + 1) * NK / n; i++) fetch(kq + c * kq_step + KB, L::Q, i);
+        for (int i = 0; i < NK; i++) fetch(kq + c * kq_step + KB, L::Q, i);
 #pragma unroll
-        for (int i = part * NT / n; i < (part + 1) * NT / n; i++) fetch(ws + c * ws_step, L::T, i);
+        for (int i = 0; i < NT; i++) fetch(ws + c * ws_step, L::T, i);
     };
     if (wave >= 2) {  // the results
         const uint32_t out_row = (uint32_t)(a.st.nv * HD), o_at = 4 * (m * out_row + col - m + 4 * g);
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
             factors(ft, c, ChunkWs::gt);
             down_u = *(const f4 *)(one + 32 + 4 * g), stop = *(const f4 *)(one + 48 + 4 * g);
             STEP;
-            fetch_after(next, 1, 2);
+            fetch_after(next);
             STEP;
 #pragma unroll
             for (int t = 0; t < 4; t++) u[t] *= ft[t];
@@ -1120,8 +1120,6 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
         STEP;
         lds_barrier();  // the corrections are there
         const float top_s = one[16 + m] + 0x1p-24f;  // f16 takes values to 0 below half of that
-        fetch_after(next, 0, 2);
-        STEP;
         f4 d[2][2];
         float keep = 0.0f, add = 0.0f;
         auto update = [&](int q) {
@@ -1164,7 +1162,6 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
 #pragma unroll
             for (int p = 0; p < KP; p++) state_terms(p);
         }
-        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the queries and T; the values, too
     }
     units(ex_s - 14);
 #undef MIX
