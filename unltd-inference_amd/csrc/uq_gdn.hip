@@ -161,7 +161,7 @@ struct ConvArgs {
 // A wave takes 256 channels (four neighbours a lane) of a tile's rows, the
 // taps and the last inputs in registers; one more takes the tile's gates. The
 // wave of a sequence's first tile also takes the window on, whose old values
-// it alone reads.
+// it alone reads. Memory bounds it: 6010 rows of 8192 channels 82 us, 4.8 TB/s.
 template <int CK>  // taps, 0: any up to 9
 __global__ __launch_bounds__(kConvTPB) void gdn_conv_kernel(ConvArgs a) {
     constexpr int MT = CK ? CK : 9, H = MT - 1, STEP = 4;
@@ -271,7 +271,7 @@ struct RuleArgs {
     int longs, slots; // of those at most, and of their chunks
     int singles;      // workgroups of half the sequences that go row by row, a multiple of 8
     uint8_t *ws;      // [slots][nv] ChunkWs
-    uint8_t *kq;      // [slots][nqk] keys, then queries (KqWs)
+    uint8_t *kq;      // [slots][nqk] keys, then queries
 };
 
 // The epilogue of a head's row: rms norm and gate, lane l its values
@@ -304,7 +304,8 @@ __device__ __forceinline__ void finish_row(const RuleArgs &a, size_t row, int he
 //     S^T k = e^g (S_0^T k),   S^T q = e^g (S_0^T q) + (q.k) d,
 // so that their sums over the lanes run side by side, and no wave waits for
 // another but for the norm. The state passes through registers once, which
-// bounds it for few rows.
+// bounds it for few rows: 64 sequences of one row, 32 heads of 128, 58 us or
+// 4.7 TB/s. Each further row of one sequence takes 1.1 us.
 constexpr int kRowBuf = 16;  // rows whose results wait for the norm
 template <int HD>
 __device__ __forceinline__ void rule_rows(const RuleArgs &a, int seq, int head, float (*buf)[HD]) {
@@ -420,16 +421,18 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
 //      S <- e^G_63 S + K^T (diag(e^(G_63 - G)) U).
 // What does not depend on S, T = (I + A)^-1 diag(beta) and P, is formed for all
 // chunks at once (gdn_prep_kernel); gdn_chunks_kernel then takes a sequence's
-// chunks one after another, 16 columns of a head's state a wave, which
-// nothing of another column enters.
+// chunks one after another, by columns of a head's state, as nothing of
+// another column enters one; gdn_finish_kernel applies norm and gate. 509 rows
+// of 32 heads take 14, 24 and 7.5 us, three prompts of 5241 rows 60, 145 and 44.
 //
-// The second kernel's products run on the f16 matrix cores with two terms of
-// each operand, h + l = x 2^s within 2^-22 of it: s brings the largest value
-// of a row (left operands) or of a wave's column (right ones) to 2^13 .. 2^14,
-// so that values down to 2^-16 of it keep 22 bits and what is lost below is
-// 2^-39 of it. The products h h, h l and l h are exact and summed in f32; l l
-// is left out, 2^-22 of the product at most. The f32 matrix cores, eight times
-// slower for these three, took 7400 clocks a chunk of 16 columns and workgroup.
+// The products run on the f16 matrix cores with two terms of each operand,
+// h + l = x 2^s within 2^-22 of it: s brings the largest value of a row (left
+// operands) or column (right ones), or a bound on it, to 2^13 .. 2^14, so that
+// values down to 2^-16 of it keep 22 bits and what is lost below is 2^-39 of
+// it. The products h h, h l and l h are exact and summed in f32; l l is left
+// out, 2^-22 of the product at most. The three take 48 clocks for 16 x 16 x 32,
+// where the f32 matrix cores take 256: with those 509 rows of 32 heads took 81
+// us, and 70 when the second kernel was put on the others.
 //
 // A 16x16x32 product's depth is summed over lane / 16 and 8 values a lane, of
 // tiles 2 p and 2 p + 1: values 4 (lane / 16) .. + 3 of each. A result's rows
@@ -535,7 +538,8 @@ __device__ __forceinline__ f4 mfma_h(const h8 &a, const h8 &b, const f4 &c) {
 // tile (i, j) of A is the left operand A_ij^T, K Q^T has P's rows, and T's row
 // of tiles i is formed from the diagonal back,
 //     T_ij^T = -T_jj^T sum over j < k <= i of A_kj^T T_ik^T,
-// by wave i from A and the diagonal's inverses alone.
+// by wave i from A and the diagonal's inverses alone. What it reads and writes
+// bounds it for many chunks, at 4 TB/s.
 // Column J of -A, a lane's row of it in the quarter's lane J, times the inverse's row J.
 template <int J>
 __device__ __forceinline__ void eliminate(const f4 &a, f4 &v) {
@@ -764,9 +768,10 @@ __device__ __forceinline__ h4 read_columns(const uint8_t *p) {
 // before a chunk and the corrections, both as operands, in the LDS. Left
 // operands come to the LDS once for all, brought by the results' waves, whose
 // way is the shorter: between the chunk's two barriers P and the next chunk's
-// keys, then its queries, T and factors. One wave a SIMD: products and the
+// keys and factors, then its queries and T. One wave a SIMD: products and the
 // vector instructions between them are ordered so that the latter run while
-// the matrix cores work.
+// the matrix cores work. A chunk takes a state's wave 5300 clocks, 1800 of them
+// products; the operands' terms and what waits for one another are the rest.
 constexpr int kChunkCols = 32;
 // Workgroups of columns, one a compute unit, that go before the sequences that go row by row; most of the others, of
 // sequences that there may be, find none.
@@ -1176,7 +1181,8 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
 }
 
 // The epilogue of the rows that went by chunks: a workgroup a chunk and head,
-// HD / 4 lanes a row, several rows of a lane under way.
+// HD / 4 lanes a row, several rows of a lane under way. Memory bounds it: 5241
+// rows of 32 heads 44 us, 5.6 TB/s.
 template <int HD>
 __global__ __launch_bounds__(256) void gdn_finish_kernel(RuleArgs a) {
     constexpr int PER = HD / 4, STEP = 256 / PER, N = kChunk / STEP;  // threads of a row, rows at a time, rows of a thread
@@ -1224,7 +1230,7 @@ hipError_t launch_gdn_conv(const StatesView &st, const BatchView &b, const uq_gd
     const ConvArgs a{st, b, r, (st.channels + 255) / 256};
     const unsigned per = kConvTPB / 64, tiles = (unsigned)(b.n_rows / kConvRows + std::min(b.n_seqs, b.n_rows));
     // A tile's channels one after another: rows are often a power of 2 apart, and a column of tiles would meet in few of
-    // the memory's channels. Three prompts of 5000 rows of 8192 channels so take 82 us, and 99 the other way round.
+    // the memory's channels. 6010 rows of 8192 channels so take 82 us, and 94 the other way round.
     const dim3 grid = grid_of((size_t)tiles * (((unsigned)a.groups + per) / per));
     if (st.taps == 4)
         hipLaunchKernelGGL(gdn_conv_kernel<4>, grid, dim3(kConvTPB), 0, s, a);

