@@ -76,14 +76,15 @@ struct Pool {
         const int lane = threadIdx.x & 63;
         const uint64_t k0 = lane < count ? at[lane] : 0, k1 = lane + 64 < count ? at[lane + 64] : 0;
         int p0 = 0, p1 = 0;
-        for (int j = 0; j < min(count, 64); j++) p0 += lane_of(k0, j) > k0;
-        if (count > 64) {
-            for (int j = 0; j < 64; j++) p1 += lane_of(k0, j) > k1;
-            for (int j = 0; j < count - 64; j++) {
-                const uint64_t k = lane_of(k1, j);
-                p0 += k > k0;
-                p1 += k > k1;
-            }
+        for (int j = 0; j < min(count, 64); j++) {
+            const uint64_t k = lane_of(k0, j);
+            p0 += k > k0;
+            p1 += k > k1;
+        }
+        for (int j = 0; j < count - 64; j++) {
+            const uint64_t k = lane_of(k1, j);
+            p0 += k > k0;
+            p1 += k > k1;
         }
         if (lane < count && p0 < n_top) at[p0] = k0;
         if (lane + 64 < count && p1 < n_top) at[p1] = k1;
@@ -112,6 +113,27 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t v, int n) {
     for (int bit = 31; bit >= 16; bit--) {
         const uint32_t more = t | 1u << bit;
         if (__builtin_popcountll(__ballot(v >= more)) >= n) t = more;
+    }
+    return t;
+}
+
+// Above so many alternatives the bound by the lanes' largest lets too many pass: of 1024 values 43 for 32, 236 for 64.
+constexpr int kMany = 32;
+// How many of the lanes' values reach t, and the largest such t for n of them, but for its lower 16 bits, which are 0.
+template <int N>
+__device__ __forceinline__ int reaching(const uint32_t (&v)[N], uint32_t t) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) n += __builtin_popcountll(__ballot(v[i] >= t));
+    return n;
+}
+template <int N>
+__device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], int n) {
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t more = t | 1u << bit;
+        if (reaching(v, more) >= n) t = more;
     }
     return t;
 }
@@ -184,16 +206,19 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
             }
         }
         if constexpr (TOP) {
-            // Values below a bound that n_top lanes reach with their largest cannot be among the first.
+            // Values below a bound that n_top lanes reach with their largest cannot be among the first. Where that leaves
+            // more than fit, as it mostly does for n_top near 64, one that n_top values reach.
             const uint32_t most = ordered(top);
             const unsigned long long over = __ballot(most >= pool.least);
             if (over) {
                 if (__builtin_popcountll(over) >= a.n_top) pool.least = max(pool.least, reached_by(most, a.n_top));
+                uint32_t o[kVals];
 #pragma unroll
-                for (int i = 0; i < kVals; i++) {
-                    const uint32_t o = ordered(v[i]);
-                    pool.take((uint64_t)o << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4), o >= pool.least && v[i] == v[i]);
-                }
+                for (int i = 0; i < kVals; i++) o[i] = v[i] == v[i] ? ordered(v[i]) : 0;
+                if (a.n_top > kMany && pool.count + reaching(o, pool.least) > kPool) pool.least = max(pool.least, reached_by(o, a.n_top));
+#pragma unroll
+                for (int i = 0; i < kVals; i++)
+                    pool.take((uint64_t)o[i] << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4), o[i] >= pool.least);
                 if (pool.full) {  // later tokens of equal logits come after those kept
                     pool.least += 1;
                     pool.full = false;
@@ -227,8 +252,8 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
     const Part *parts = a.part + (size_t)row * a.parts;
     float m = -FLT_MAX, l = 0.0f, s = 0.0f;
     int before = 0;
-    uint32_t most = 0;
     constexpr int P = 4;  // parts of a lane at a time
+    uint32_t most[P] = {0, 0, 0, 0};
     for (int i0 = 0; i0 < a.parts; i0 += 64 * P) {
         Part p[P];
 #pragma unroll
@@ -242,7 +267,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
             l = f * l + fp * p[j].l;
             m = to;
             before += p[j].before;
-            most = max(most, ordered(p[j].m));
+            most[j] = max(most[j], ordered(p[j].m));
         }
     }
     float all = m;
@@ -273,7 +298,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
             const int i = min(i0 + lane, a.parts - 1);
             const int count = parts[i].kept;
             unsigned long long over = __ballot(i0 + lane < a.parts && ordered(parts[i].m) >= pool.least);
-            constexpr int N = 8;  // parts at a time
+            constexpr int N = 16;  // parts at a time
             while (over) {
                 uint64_t k[N];
 #pragma unroll
@@ -282,8 +307,12 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
                     k[j] = lane < n ? keys[(size_t)(i0 + from) * 64 + lane] : 0;
                     over &= over - 1;
                 }
+                uint32_t o[N];
 #pragma unroll
-                for (int j = 0; j < N; j++) pool.take(k[j], (uint32_t)(k[j] >> 32) >= pool.least);
+                for (int j = 0; j < N; j++) o[j] = (uint32_t)(k[j] >> 32);
+                if (a.n_top > kMany && pool.count + reaching(o, pool.least) > kPool) pool.least = max(pool.least, reached_by(o, a.n_top));
+#pragma unroll
+                for (int j = 0; j < N; j++) pool.take(k[j], o[j] >= pool.least);
             }
         }
         pool.order();
