@@ -180,3 +180,26 @@ def test_replays_and_streams():
         got = r.results()
         eager = Run(x, tokens, 1.1, r.n_top).run().results()
         assert all(np.array_equal(got[k].view(np.int32), eager[k].view(np.int32)) for k in eager), f"replay {i}"
+
+
+@pytest.mark.parametrize("n_top", [20, 33, 64])
+def test_more_candidates_than_are_kept(n_top):
+    """Rows whose tiles hold more that may be among the first than a wave keeps: the type's lowest value but for a few
+    tokens, one value but for larger and smaller ones among it, two values in turn, and tiles that end in ties."""
+    rng = np.random.default_rng(n_top)
+    vocab = 9 * 1024 + 77
+    low = np.float32(np.finfo(np.float32).min)
+    x = np.full((6, vocab), low, np.float32)
+    x[0, rng.permutation(vocab)[:11]] = rng.standard_normal(11)
+    x[1] = 1.0
+    x[1, rng.permutation(vocab)[:15]] = 2.0
+    x[1, rng.permutation(vocab)[:4000]] = -3.0
+    x[2] = np.where(np.arange(vocab) % 2, 5.0, 4.0)
+    x[3] = np.repeat(rng.permutation(vocab // 7 + 1), 7)[:vocab] // 9
+    x[4] = np.minimum(np.arange(vocab), 3000)
+    x[5] = rng.standard_normal(vocab)
+    x[5, 1024:2048] = 0.5
+    tokens = [5, 4000, 1, 77, 9000, 1500]
+    with np.errstate(over="ignore"):
+        check(x, tokens, 1.0, n_top)
+        check(np.repeat(x, 300, 0)[:, :6000], np.minimum(np.repeat(tokens, 300), 5999), 1.0, n_top)  # runs of several tiles

@@ -90,13 +90,15 @@ struct Pool {
         if (lane + 64 < count && p1 < n_top) at[p1] = k1;
         count = min(count, n_top);
     }
+    // LATER: tokens after all that were offered before, which go before them where logits are equal.
+    template <bool LATER>
     __device__ __forceinline__ void take(uint64_t key, bool in) {
         unsigned long long b = __ballot(in);
         if (!b) return;
         if (count + __builtin_popcountll(b) > kPool) {
             order();
             full = true;
-            least = max(least, (uint32_t)uniform((int)(at[n_top - 1] >> 32)));
+            least = max(least, (uint32_t)uniform((int)(at[n_top - 1] >> 32)) + (LATER ? 1 : 0));
             in = in && (uint32_t)(key >> 32) >= least;
             b = __ballot(in);
         }
@@ -117,9 +119,7 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t v, int n) {
     return t;
 }
 
-// Above so many alternatives the bound by the lanes' largest lets too many pass: of 1024 values 43 for 32, 236 for 64.
-constexpr int kMany = 32;
-// How many of the lanes' values reach t, and the largest such t for n of them, but for its lower 16 bits, which are 0.
+// How many of the lanes' values reach t, and the largest such t for n of them, but for its lowest bits, which are 0.
 template <int N>
 __device__ __forceinline__ int reaching(const uint32_t (&v)[N], uint32_t t) {
     int n = 0;
@@ -127,13 +127,38 @@ __device__ __forceinline__ int reaching(const uint32_t (&v)[N], uint32_t t) {
     for (int i = 0; i < N; i++) n += __builtin_popcountll(__ballot(v[i] >= t));
     return n;
 }
-template <int N>
+template <int LOWEST, int N>
 __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], int n) {
     uint32_t t = 0;
 #pragma unroll 1
-    for (int bit = 31; bit >= 16; bit--) {
+    for (int bit = 31; bit >= LOWEST; bit--) {
         const uint32_t more = t | 1u << bit;
         if (reaching(v, more) >= n) t = more;
+    }
+    return t;
+}
+// The first n of a tile's values (token 256 j + 4 lane + e in o[4 j + e]): others become 0. Returns the last one's size, 0
+// if n values are not as large as `least`: then all stay.
+__device__ __forceinline__ uint32_t first_of(uint32_t (&o)[kVals], int n, uint32_t least) {
+    const uint32_t t = reached_by<0>(o, n);
+    if (t < least) return 0;
+    int room = n - reaching(o, t + 1);
+#pragma unroll
+    for (int j = 0; j < kVals; j += 4) {
+        int rank = 0, all = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const unsigned long long b = __ballot(o[j + e] == t);
+            rank = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, rank));
+            all += __builtin_popcountll(b);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool tie = o[j + e] == t;
+            if (o[j + e] < t || (tie && rank >= room)) o[j + e] = 0;
+            rank += tie;
+        }
+        room -= all;
     }
     return t;
 }
@@ -207,7 +232,8 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
         }
         if constexpr (TOP) {
             // Values below a bound that n_top lanes reach with their largest cannot be among the first. Where that leaves
-            // more than fit, as it mostly does for n_top near 64, one that n_top values reach.
+            // more than fit, for n_top near 64 (of 1024 values 43 for 32, 236 for 64) or for equal logits, a bound that n_top
+            // values reach; then, for equal ones, the tile's first alone.
             const uint32_t most = ordered(top);
             const unsigned long long over = __ballot(most >= pool.least);
             if (over) {
@@ -215,10 +241,16 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
                 uint32_t o[kVals];
 #pragma unroll
                 for (int i = 0; i < kVals; i++) o[i] = v[i] == v[i] ? ordered(v[i]) : 0;
-                if (a.n_top > kMany && pool.count + reaching(o, pool.least) > kPool) pool.least = max(pool.least, reached_by(o, a.n_top));
+                if (__builtin_popcountll(__ballot(most >= pool.least)) > 32 && pool.count + reaching(o, pool.least) > kPool) {
+                    pool.least = max(pool.least, reached_by<16>(o, a.n_top));
+                    if (reaching(o, pool.least) > a.n_top + 32) {
+                        const uint32_t last = first_of(o, a.n_top, pool.least);
+                        if (last) pool.least = last, pool.full = true;
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < kVals; i++)
-                    pool.take((uint64_t)o[i] << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4), o[i] >= pool.least);
+                    pool.take<false>((uint64_t)o[i] << 32 | (uint32_t)~(t * kTile + 256 * (i / 4) + 4 * lane + i % 4), o[i] >= pool.least);
                 if (pool.full) {  // later tokens of equal logits come after those kept
                     pool.least += 1;
                     pool.full = false;
@@ -292,12 +324,13 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
         // as within a wave's run: n_top parts reach the bound with their largest, and the others are not read
         __shared__ uint64_t kept[kPool];
         Pool pool(kept, a.n_top);
-        if (a.parts >= a.n_top) pool.least = max(pool.least, reached_by(most, a.n_top));
+        if (a.parts >= a.n_top) pool.least = max(pool.least, reached_by<16>(most, a.n_top));
         const uint64_t *keys = a.keys + (size_t)row * a.parts * 64;
         for (int i0 = 0; i0 < a.parts; i0 += 64) {
             const int i = min(i0 + lane, a.parts - 1);
             const int count = parts[i].kept;
-            unsigned long long over = __ballot(i0 + lane < a.parts && ordered(parts[i].m) >= pool.least);
+            const uint32_t largest = i0 + lane < a.parts ? ordered(parts[i].m) : 0;
+            unsigned long long over = __ballot(largest >= pool.least);
             constexpr int N = 16;  // parts at a time
             while (over) {
                 uint64_t k[N];
@@ -310,9 +343,10 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
                 uint32_t o[N];
 #pragma unroll
                 for (int j = 0; j < N; j++) o[j] = (uint32_t)(k[j] >> 32);
-                if (a.n_top > kMany && pool.count + reaching(o, pool.least) > kPool) pool.least = max(pool.least, reached_by(o, a.n_top));
+                if (a.n_top > 32 && pool.count + reaching(o, pool.least) > kPool) pool.least = max(pool.least, reached_by<16>(o, a.n_top));
 #pragma unroll
-                for (int j = 0; j < N; j++) pool.take(k[j], o[j] >= pool.least);
+                for (int j = 0; j < N; j++) pool.take<true>(k[j], o[j] >= pool.least);
+                over &= __ballot(largest >= pool.least);
             }
         }
         pool.order();
