@@ -239,6 +239,14 @@ def test_rule_of_values_far_smaller_than_the_state():
     assert np.all(np.abs(st[0] - ws[0]) <= 2 * wt[0])
 
 
+@pytest.mark.parametrize("nqk,nv,hd,rows", [(4, 32, 64, [35] * 19 + [90]), (2, 34, 128, [70, 1, 33] * 6 + [40] * 7)])
+def test_rule_of_many_heads(nqk, nv, hd, rows):
+    """Many value heads of a key head in one workgroup, one after another; single rows between."""
+    r = Rule(M.Case(98, nqk, nv, hd, 4, rows), 0)
+    r.run()
+    r.check()
+
+
 def test_rows_of_no_sequence_between():
     """Row starts that leave rows out before, between and behind: as they were."""
     c = M.Case(97, 2, 2, 64, 4, [50, 3], pad=70)

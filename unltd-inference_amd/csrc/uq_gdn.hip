@@ -269,6 +269,7 @@ struct RuleArgs {
     uq_gdn_heads h;
     int chunked;      // sequences of at least so many rows go by chunks
     int longs, slots; // of those at most, and of their chunks
+    int parts;        // workgroups of a chunk and key head
     int singles;      // workgroups of half the sequences that go row by row, a multiple of 8
     uint8_t *ws;      // [slots][nv] ChunkWs
     uint8_t *kq;      // [slots][nqk] keys, then queries
@@ -423,7 +424,7 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
 // chunks at once (gdn_prep_kernel); gdn_chunks_kernel then takes a sequence's
 // chunks one after another, by columns of a head's state, as nothing of
 // another column enters one; gdn_finish_kernel applies norm and gate. 509 rows
-// of 32 heads take 14, 24 and 7.5 us, three prompts of 5241 rows 60, 145 and 44.
+// of 32 heads take 11.5, 23 and 7.5 us, three prompts of 5241 rows 60, 143 and 44.
 //
 // The products run on the f16 matrix cores with two terms of each operand,
 // h + l = x 2^s within 2^-22 of it: s brings the largest value of a row (left
@@ -561,7 +562,7 @@ struct PrepLds {
     int ex_k[kChunk], ex_q[kChunk], bad[4];
 };
 template <int HD>
-__device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, PrepLds<HD> &l) {
+__device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, int part, PrepLds<HD> &l) {
     constexpr int KP = HD / 32;
     const Long s = find_long<true>(a.b, slot, a.chunked);
     if (s.seq < 0) return;
@@ -569,7 +570,9 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
     const size_t row0 = (size_t)s.lo + c0;
     const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6)), m = lane & 15, g = lane >> 4, mine = 16 * wave + m;
     const float *gates = a.h.d_gate + (row0 + min(lane, n - 1)) * a.st.nv, *betas = a.h.d_beta + (row0 + min(lane, n - 1)) * a.st.nv;
-    float gate = gates[hq], bt = betas[hq];
+    const int step = a.parts * a.st.nqk;
+    int head = hq + part * a.st.nqk;
+    float gate = gates[head], bt = betas[head];
     int exk, exq;  // of the wave's rows
     h8 kh[KP], kl[KP], qh[KP], ql[KP];
     {
@@ -591,14 +594,18 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
 #pragma unroll
         for (int p = 0; p < KP; p++) {
             two_terms(k[2 * p], k[2 * p + 1], scale_up(exk), kh[p], kl[p]);
-            lk[p * 128] = to[p * 128] = kh[p];
-            lk[p * 128 + 64] = to[p * 128 + 64] = kl[p];
-        }
-#pragma unroll
-        for (int p = 0; p < KP; p++) {
             two_terms(q[2 * p], q[2 * p + 1], scale_up(exq), qh[p], ql[p]);
-            to[kq_bytes(HD) / 16 + p * 128] = qh[p];
-            to[kq_bytes(HD) / 16 + p * 128 + 64] = ql[p];
+            lk[p * 128] = kh[p];
+            lk[p * 128 + 64] = kl[p];
+        }
+        if (part == 0) {
+#pragma unroll
+            for (int p = 0; p < KP; p++) {
+                to[p * 128] = kh[p];
+                to[p * 128 + 64] = kl[p];
+                to[kq_bytes(HD) / 16 + p * 128] = qh[p];
+                to[kq_bytes(HD) / 16 + p * 128 + 64] = ql[p];
+            }
         }
     }
     __syncthreads();
@@ -635,7 +642,7 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
     double *const G = l.G[wave];
     float *const beta = l.beta[wave];
     f4 *tiles = (f4 *)l.space + lane;  // tile (i, j) of A at i (i - 1) / 2 + j, the inverse of (i, i) at 6 + i
-    for (int head = hq, turn = 0; head < a.st.nv; head += a.st.nqk, turn ^= 1) {
+    for (int turn = 0; head < a.st.nv; head += step, turn ^= 1) {
         uint8_t *ws = a.ws + ((size_t)slot * a.st.nv + head) * ChunkWs::bytes;
         float *vec = (float *)(ws + ChunkWs::vec);
         f4 *at = tiles + turn * 10 * 64;
@@ -643,7 +650,7 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, P
         float gt = in ? gate : 0.0f;
         const float b = in ? bt : 0.0f;
         if (gt < kLeastGate) gt = kLeastGate;
-        const int other = min(head + a.st.nqk, a.st.nv - 1);
+        const int other = min(head + step, a.st.nv - 1);
         gate = gates[other], bt = betas[other];
         const bool ok = finite32(gt) && finite32(b);
         const unsigned long long bad = __ballot(!ok) | bad_k;
@@ -748,9 +755,9 @@ __global__ __launch_bounds__(kPrepTPB, 3) void gdn_prep_kernel(RuleArgs a) {
         PrepLds<HD> prep;
         float buf[kRowBuf][HD];
     } l;
-    const unsigned chunks = (unsigned)a.slots * a.st.nqk, i = blockIdx.y * gridDim.x + blockIdx.x;
+    const unsigned per = (unsigned)a.parts * a.st.nqk, chunks = a.slots * per, i = blockIdx.y * gridDim.x + blockIdx.x, in = i % per;
     if (i < chunks)
-        rule_prep<HD>(a, (int)(i / a.st.nqk), (int)(i % a.st.nqk), l.prep);
+        rule_prep<HD>(a, (int)(i / per), (int)(in % a.st.nqk), (int)(in / a.st.nqk), l.prep);
     else
         rule_rows_of<HD>(a, i - chunks, 0, l.buf);
 }
@@ -1273,8 +1280,11 @@ hipError_t launch_rule(RuleArgs a, hipStream_t s) {
     const auto kernel = gdn_chunks_kernel<HD>;
     if (hipError_t e = allow_lds((const void *)kernel, lds)) return e;
     const size_t pairs = (size_t)a.longs * a.st.nv, seqs = a.b.n_seqs, nv = a.st.nv;
+    // The value heads of a key head one after another, or all at once where all find room on the chip: 509 rows 11.5 us
+    // against 14. More of them would keep sequences that go row by row from it: 34 against 31 for 1021 rows beside 40.
+    a.parts = a.slots * nv <= 3 * 256 ? a.st.nv / a.st.nqk : 1;
     a.singles = (int)((seqs / 2 * nv + 7) / 8 * 8);
-    hipLaunchKernelGGL(gdn_prep_kernel<HD>, grid_of((size_t)a.slots * a.st.nqk + (seqs + 1) / 2 * nv), dim3(kPrepTPB), 0, s, a);
+    hipLaunchKernelGGL(gdn_prep_kernel<HD>, grid_of((size_t)a.slots * a.parts * a.st.nqk + (seqs + 1) / 2 * nv), dim3(kPrepTPB), 0, s, a);
     if (hipError_t e = hipGetLastError()) return e;
     hipLaunchKernelGGL(kernel, grid_of(std::max((size_t)kFirstChains, (pairs + 7) / 8 * 8 * (HD / kChunkCols)) + a.singles), dim3(256), lds, s, a);
     if (hipError_t e = hipGetLastError()) return e;
@@ -1286,7 +1296,7 @@ hipError_t launch_gdn_rule(float *out, const StatesView &st, const BatchView &b,
                            void *ws, hipStream_t s) {
     if (b.n_rows == 0 || b.n_seqs == 0) return hipSuccess;
     const Plan p = plan_of(st, b, most_rows);
-    const RuleArgs a{out, st, b, h, p.least, p.longs, p.slots, 0, (uint8_t *)ws, (uint8_t *)ws + (size_t)p.slots * st.nv * ChunkWs::bytes};
+    const RuleArgs a{out, st, b, h, p.least, p.longs, p.slots, 1, 0, (uint8_t *)ws, (uint8_t *)ws + (size_t)p.slots * st.nv * ChunkWs::bytes};
     return st.hd == 128 ? launch_rule<128>(a, s) : launch_rule<64>(a, s);
 }
 
