@@ -10,7 +10,7 @@ import pytest
 
 import gdn_model as M
 import uq
-from test_gpu_gdn_serve import MARK, Conv, Rule, bits, dev, host
+from test_gpu_gdn_serve import MARK, Conv, Rule, bits, dev, hip_of_bench, host
 from test_gpu_layers import SMALL, Model, nodes_of
 from uq import layer as L
 from uq import serve
@@ -144,6 +144,33 @@ def test_drafts_scored_and_taken():
         assert np.array_equal(bits(later[[0, 2, 3]]), bits(after[[0, 2, 3]])) and not np.array_equal(later[1], after[1])
         start.upload(c.start)
         to.upload(c.to)
+
+
+def test_two_streams_at_once():
+    """Calls of two streams, each with states and a workspace of its own, under way at the same time."""
+    hip = hip_of_bench()
+    streams = [hip.stream(), hip.stream()]
+    cases = [M.Case(99, 2, 4, 128, 4, [200, 1, 70], frm=[0, 1, 2], to=[3, 4, 5], spare=3),
+             M.Case(100, 2, 6, 64, 4, [90, 5, 300], frm=[0, 1, 2], to=[3, 4, 5], spare=3)]
+    runs = [(Conv(c), Rule(c, 0)) for c in cases]
+    hip.sync()
+    want = []
+    for conv, rule in runs:
+        conv.run()
+        rule.run()
+        want.append((host(conv.out, conv.c.qkv), *rule.results()))
+        for d in (conv.out, rule.out):
+            d.upload(np.full(d.nbytes // 4, MARK, np.float32))
+    hip.sync()
+    for _ in range(6):
+        for (conv, rule), s in zip(runs, streams):
+            conv.run(s)
+            rule.run(s)
+    hip.sync()
+    for (conv, rule), (out, heads, st) in zip(runs, want):
+        got, gs = rule.results()
+        assert np.array_equal(bits(host(conv.out, conv.c.qkv)), bits(out))
+        assert np.array_equal(bits(got), bits(heads)) and np.array_equal(bits(gs), bits(st))
 
 
 # ------------------------------------------------------------------------- scales

@@ -662,10 +662,10 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, i
         sum += dpp_d<0x118>(sum);
         sum += dpp_d<0x142, 0xA>(sum);
         sum += dpp_d<0x143, 0xC>(sum);
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes alone read and write these
         G[lane] = sum;
         beta[lane] = lane < first ? b : 0.0f;
-        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's lanes alone read and write these
         auto power = [](double x) { return __builtin_amdgcn_exp2f((float)x); };
         // P's tiles of the wave's row and A's of its column
         const double Gm = G[mine];

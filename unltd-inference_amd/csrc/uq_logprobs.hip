@@ -49,18 +49,20 @@ struct Args {
     uint64_t *keys;  // [n_rows][parts][64]
 };
 
-// Tokens in their order as integers: the larger the logit, then the smaller the number, the larger the key. 0 is none.
+// A token's key is its logit as an integer in the order of its size, then the complement of its number. 0 is none.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);  // -0 as +0
     return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ uint64_t key_of(float x, int token) { return (uint64_t)ordered(x) << 32 | (uint32_t)~token; }
 
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
            (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 constexpr uint32_t kLowest = 0x00800000u;  // ordered(-infinity) + 1: neither it nor a NaN that is below it is kept
+
+// What the wave's lanes have written to the LDS is read by others behind this point.
+__device__ __forceinline__ void lanes_see() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // Keys in the LDS, the first n_top (64 at most) of those offered among them. Only when they overflow are they put in
 // order, and the first n_top kept: a wave's run mostly ends before.
@@ -74,6 +76,7 @@ struct Pool {
     // Puts the keys in order and keeps the first n_top. A key's place is how many are larger: keys differ, as a token is seen once.
     __device__ __forceinline__ void order() {
         const int lane = threadIdx.x & 63;
+        lanes_see();
         const uint64_t k0 = lane < count ? at[lane] : 0, k1 = lane + 64 < count ? at[lane + 64] : 0;
         int p0 = 0, p1 = 0;
         for (int j = 0; j < min(count, 64); j++) {
@@ -89,6 +92,7 @@ struct Pool {
         if (lane < count && p0 < n_top) at[p0] = k0;
         if (lane + 64 < count && p1 < n_top) at[p1] = k1;
         count = min(count, n_top);
+        lanes_see();
     }
     // LATER: tokens after all that were offered before, which go before them where logits are equal.
     template <bool LATER>
@@ -272,6 +276,7 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
     const size_t o = (size_t)row * a.parts + part;
     if constexpr (TOP)
         if (pool.count > 64) pool.order();
+    lanes_see();
     if (lane == 0) a.part[o] = Part{all, l, s, before, pool.count, 0};
     if constexpr (TOP)
         if (lane < pool.count) a.keys[o * 64 + lane] = pool.at[lane];
