@@ -301,11 +301,12 @@ typedef struct uq_logprobs {
  * by their number. d_tokens may be NULL where neither d_logprob nor d_rank is
  * wanted.
  * A logit of -infinity is a token that cannot follow: its log probability is
- * -infinity, and it is no alternative. Alternatives that there are not are
- * -1 with -infinity. A row without any possible token has entropy 0. A token
- * outside [0, vocab) has log probability -infinity and rank -1. A row with a
- * logit that is NaN or +infinity has NaN for log probabilities and entropy, and
- * -1 for ranks and alternatives.
+ * -infinity, and it is no alternative. Log probabilities below f32's range are
+ * -infinity, too. Alternatives that there are not are -1 with -infinity. A row
+ * without any possible token has entropy 0. A token outside [0, vocab) has log
+ * probability -infinity and rank -1. A row with a logit that is NaN or
+ * +infinity has NaN for log probabilities and entropy, and -1 for ranks and
+ * alternatives.
  * Numerics: f32; the sums over the vocabulary run in a fixed order, up to 2^20
  * tokens none of more than 112 roundings. Ranks and alternatives are exact.
  * Errors: UQ_ERR_ARG (null pointers, vocab 0 or above 2^24, n_rows above 2^23,

@@ -203,3 +203,32 @@ def test_more_candidates_than_are_kept(n_top):
     with np.errstate(over="ignore"):
         check(x, tokens, 1.0, n_top)
         check(np.repeat(x, 300, 0)[:, :6000], np.minimum(np.repeat(tokens, 300), 5999), 1.0, n_top)  # runs of several tiles
+
+
+@pytest.mark.parametrize("n_top", [0, 20, 64])
+def test_many_rows(n_top):
+    """So many rows that a wave takes more than one tile: ascending and descending ones, ties within and between tiles,
+    masks of the type's lowest value and of minus infinity, the same rows again and again."""
+    rng = np.random.default_rng(9)
+    vocab, n = 2100, 22001
+    x = rng.standard_normal((9, vocab)).astype(np.float32)
+    x[1], x[2] = np.sort(x[1]), np.sort(x[2])[::-1]
+    x[3] = 1.5
+    x[4] = np.arange(vocab) // 700
+    x[5], x[6] = np.finfo(np.float32).min, -np.inf
+    x[5, rng.permutation(vocab)[:9]] = 0.0
+    x[6, rng.permutation(vocab)[:30]] = rng.integers(0, 3, 30)
+    x[7, 1500:] = 7.0
+    tokens = np.array([3, 2000, 1, 1024, 700, 1999, 4, 1501, 1023])
+    which = np.arange(n) % 9
+    with np.errstate(over="ignore"):
+        want = M.logprobs(x, tokens, 1.25, n_top)
+        for k in ("logprob", "top_logprob"):  # 1.25 times the lowest value is nearest to -infinity among f32's
+            want[k] = np.where(want[k] < np.finfo(np.float32).min, -np.inf, want[k])
+    got = Run(x[which], tokens[which], 1.25, n_top).run().results()
+    close(got["logprob"], want["logprob"][which], want["tol_logprob"][which])
+    close(got["entropy"], want["entropy"][which], want["tol_entropy"][which])
+    assert np.array_equal(got["rank"], want["rank"][which])
+    if n_top:
+        assert np.array_equal(got["top_id"], want["top_id"][which])
+        close(got["top_logprob"], want["top_logprob"][which], want["tol_top"][which])
