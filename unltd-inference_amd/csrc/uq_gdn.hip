@@ -488,8 +488,12 @@ __device__ __forceinline__ uint32_t wave_top(uint32_t v) {
     v = max(v, dpp_u<0x141>(v));
     return rows16_max(max(v, dpp_u<0x140>(v)));
 }
-// The exponent ex that brings values of at most this size below 2^14: x 2^(14 - ex). Sizes below 2^-100 as it.
-__device__ __forceinline__ int scale_of(uint32_t bits) { return max(-100, __builtin_amdgcn_frexp_expf(__uint_as_float(bits))); }
+// The exponent ex that brings values of at most this size below 2^14: x 2^(14 - ex). Sizes below 2^-100 as it, 0 among
+// them, whose own exponent is 0, as if a column of zeros (a new sequence's state) held values near 1.
+__device__ __forceinline__ int scale_of(uint32_t bits) {
+    const int ex = __builtin_amdgcn_frexp_expf(__uint_as_float(bits));
+    return bits ? max(-100, ex) : -100;
+}
 __device__ __forceinline__ float scale_up(int ex) { return ldexpf(1.0f, 14 - ex); }
 __device__ __forceinline__ float scale_down(int ex) { return ldexpf(1.0f, ex - 14); }
 // The two terms of a pair of tiles, each rounded to the nearest. A pair of conversions, back, a difference: three
