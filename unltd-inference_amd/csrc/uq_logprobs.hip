@@ -7,7 +7,8 @@
 // from which log p(t) = scale (x_t - m) - ln l and the entropy
 // ln l - ln 2 s / l; parts of a row join by 2^(c (m' - m)). The differences
 // are formed before the product, so that logits of any size, the type's lowest
-// value among them, neither overflow nor lose the small differences.
+// value among them, do not lose the small ones. At scales below 1, which bring
+// differences beyond f32's range back into it, they are those of halves.
 //
 // Rows are cut into runs of tiles of 1024 values, a wave each, without
 // barriers. Memory bounds it where there is much of it: 1021 rows of 152064
@@ -44,9 +45,11 @@ struct Args {
     size_t x_row;
     const int32_t *tokens;
     int n_rows, vocab, n_top, tiles, run, parts;  // tiles of a row, of a wave; waves of a row
-    float scale, c;
+    // a logit's factor in a difference, 1 or 1/2, and by what the difference becomes an exponent of e, of 2
+    float pre, scale, c;
     Part *part;      // [n_rows][parts]
     uint64_t *keys;  // [n_rows][parts][64]
+    __device__ __forceinline__ float minus(float x, float y) const { return fmaf(x, pre, -(y * pre)); }
 };
 
 // A token's key is its logit as an integer in the order of its size, then the complement of its number. 0 is none.
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
 #pragma unroll
         for (int i = 1; i < kVals; i++) top = fmaxf(top, v[i]);
         if (__ballot(top > m)) {
-            const float to = fmaxf(m, top), d = fmaxf((m - to) * a.c, kLeast), f = exp2_hw(d);
+            const float to = fmaxf(m, top), d = fmaxf(a.minus(m, to) * a.c, kLeast), f = exp2_hw(d);
             s = f * fmaf(d, l, s);
             l *= f;
             m = to;
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
         float tl[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ts[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kVals; i++) {
-            const float d = (v[i] - m) * a.c, e = exp2_hw(d);
+            const float d = a.minus(v[i], m) * a.c, e = exp2_hw(d);
             tl[i % 4] += e;
             ts[i % 4] = fmaf(e, fmaxf(d, kLeast), ts[i % 4]);
         }
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(kTPB) void logprobs_kernel(Args a) {
         for (int d = 1; d < 64; d *= 2) r = fmaxf(r, __shfl_xor(r, d));
         return r;
     }();
-    const float d = fmaxf((m - all) * a.c, kLeast), f = exp2_hw(d);
+    const float d = fmaxf(a.minus(m, all) * a.c, kLeast), f = exp2_hw(d);
     s = wave_sum(f * fmaf(d, l, s));
     l = wave_sum(f * l);
     const size_t o = (size_t)row * a.parts + part;
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < P; j++) {
             if (i0 + 64 * j + lane >= a.parts) continue;
-            const float to = fmaxf(m, p[j].m), d = fmaxf((m - to) * a.c, kLeast), dp = fmaxf((p[j].m - to) * a.c, kLeast);
+            const float to = fmaxf(m, p[j].m), d = fmaxf(a.minus(m, to) * a.c, kLeast), dp = fmaxf(a.minus(p[j].m, to) * a.c, kLeast);
             const float f = exp2_hw(d), fp = exp2_hw(dp);
             s = f * fmaf(d, l, s) + fp * fmaf(dp, p[j].l, p[j].s);
             l = f * l + fp * p[j].l;
@@ -309,13 +312,13 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(Args a) {
     }
     float all = m;
     for (int d = 1; d < 64; d *= 2) all = fmaxf(all, __shfl_xor(all, d));
-    const float d = fmaxf((m - all) * a.c, kLeast), f = exp2_hw(d);
+    const float d = fmaxf(a.minus(m, all) * a.c, kLeast), f = exp2_hw(d);
     s = wave_sum(f * fmaf(d, l, s));
     l = wave_sum(f * l);
     for (int k = 1; k < 64; k *= 2) before += __shfl_xor(before, k);
     const bool sound = l == l && l < INFINITY;  // no NaN and no infinite logit
     const float ln_l = logf(l), nan = __uint_as_float(0x7FC00000u);
-    auto log_p = [&](float x) { return !sound ? nan : l > 0.0f ? fmaf(x - all, a.scale, -ln_l) : -INFINITY; };
+    auto log_p = [&](float x) { return !sound ? nan : l > 0.0f ? fmaf(a.minus(x, all), a.scale, -ln_l) : -INFINITY; };
     if (lane == 0) {
         const int token = a.tokens ? a.tokens[row] : -1;
         const bool in = (unsigned)token < (unsigned)a.vocab;
@@ -395,8 +398,9 @@ hipError_t launch_logprobs(const uq_logprobs &out, const float *x, size_t x_row,
     const Shape h = shape_of(n_rows, vocab);
     const bool top = out.n_top && (out.d_top_id || out.d_top_logprob);
     Part *part = (Part *)ws;
-    const Args a{out,     x,     x_row, tokens,  n_rows,           vocab, top ? (int)out.n_top : 0,
-                 h.tiles, h.run, h.parts, scale, (float)(scale * 1.4426950408889634), part, (uint64_t *)(part + (size_t)n_rows * h.parts)};
+    const float pre = scale < 1.0f ? 0.5f : 1.0f, by = scale / pre;
+    const Args a{out,     x,     x_row,   tokens, n_rows, vocab, top ? (int)out.n_top : 0,
+                 h.tiles, h.run, h.parts, pre,    by,     (float)(by * 1.4426950408889634), part, (uint64_t *)(part + (size_t)n_rows * h.parts)};
     const long long waves = (long long)n_rows * h.parts, per = kTPB / 64;
     const dim3 grid((unsigned)((waves + per - 1) / per));
     if (top)
