@@ -179,9 +179,10 @@ uq_status uq_draft_verify_d(int32_t *d_accepted, int32_t *d_next, const float *d
  * uq_gdn_layer_step_d carries from token to token, one after another.
  * Sequence b begins with the state of slot d_from[b] (outside [0, n_slots):
  * zeros, a new sequence) and leaves its last one in slot d_to[b] (outside:
- * nowhere, as for drafts that are not verified yet: a second call with the
- * accepted rows takes the state further). Several sequences may begin with one
- * slot, as continuations of one prompt do. Two sequences that end in one slot
+ * nowhere, as for drafts that are not verified yet: a second call over the
+ * same rows takes the state on, in which each sequence is its accepted rows
+ * and its refused ones a sequence behind it, from nothing to nowhere). Several
+ * sequences may begin with one slot, as continuations of one prompt do. Two sequences that end in one slot
  * leave there any part of either's state; one that begins with a slot that
  * another of the call ends in gets unspecified results. A sequence without
  * rows writes nothing. */
