@@ -496,6 +496,12 @@ __device__ __forceinline__ int scale_of(uint32_t bits) {
 }
 __device__ __forceinline__ float scale_up(int ex) { return ldexpf(1.0f, 14 - ex); }
 __device__ __forceinline__ float scale_down(int ex) { return ldexpf(1.0f, ex - 14); }
+// The same of a 2^i + b 2^j, a bound that may lie beyond f32's range where what it bounds does not, formed in 64 bits. At
+// 2^141 scale_down ends, far above what f32 holds.
+__device__ __forceinline__ int scale_of_sum(float a, int i, float b, int j) {
+    const double sum = ldexp((double)a, i) + ldexp((double)b, j) + 0x1p-200;
+    return min(141, max(-100, __builtin_amdgcn_frexp_exp(sum)));
+}
 // The two terms of a pair of tiles, each rounded to the nearest. A pair of conversions, back, a difference: three
 // instructions a value of 4 clocks each, where a product and sum of mixed precision for each term takes 8 each.
 __device__ __forceinline__ void two_terms(const f4 &a, const f4 &b, h8 &h, h8 &l) {
@@ -1047,7 +1053,7 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
         STEP;
         // the scale of X while the keys come: at most |v| + |e^G k| |S|
         hold(v);
-        int ex_x = scale_of(__float_as_uint(ldexpf(top_x * (HD * 16384.0f), ex_s) + __uint_as_float(column_top(top_of(v)))));
+        int ex_x = scale_of_sum(top_x, ex_s + 14 + (HD == 128 ? 7 : 6), __uint_as_float(column_top(top_of(v))), 0);
         factors(fx, c, ChunkWs::gx);
         STEP;
         Tri tri;
@@ -1159,7 +1165,7 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
                     for (int t = 0; t < 2; t++) d[q % 2][t] = mfma_h(y < 2 ? k.h[p][t] : k.l[p][t], y == 1 ? gl[p] : gh[p], d[q % 2][t]);
             if (q == 0) {
                 // what the sum's terms amount to at most; those of K^T U by the operands' scales and the depth
-                const int to = scale_of(__float_as_uint(ldexpf(top_s * whole, ex_s - 14) + ldexpf(__uint_as_float(top_g) * kChunk, ex_x)));
+                const int to = scale_of_sum(top_s * whole, ex_s - 14, __uint_as_float(top_g), ex_x + 6);
                 keep = ldexpf(whole, ex_s - to), add = ldexpf(1.0f, ex_g + ex_x - 14 - to);
                 ex_s = to;
                 one[m] = scale_down(ex_s);
