@@ -1053,7 +1053,16 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
         STEP;
         // the scale of X while the keys come: at most |v| + |e^G k| |S|
         hold(v);
-        int ex_x = scale_of_sum(top_x, ex_s + 14 + (HD == 128 ? 7 : 6), __uint_as_float(column_top(top_of(v))), 0);
+        uint32_t top_v = column_top(top_of(v));
+        if (__ballot(top_v >= 0x7F800000u)) {  // of the finite ones, whose rows may come before
+            f4 w[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[t][e] = finite32(v[t][e]) ? v[t][e] : 0.0f;
+            top_v = column_top(top_of(w));
+        }
+        int ex_x = scale_of_sum(top_x, ex_s + 14 + (HD == 128 ? 7 : 6), __uint_as_float(top_v), 0);
         factors(fx, c, ChunkWs::gx);
         STEP;
         Tri tri;
