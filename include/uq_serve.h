@@ -251,15 +251,16 @@ typedef struct uq_gdn_heads {
  * [head_dim] and may not overlap the inputs or the states.
  *
  * most_rows: the most rows of a sequence, where the caller knows it (0: it
- * does not). It decides how the call is divided, never what it computes: a
+ * does not). It decides how the call is divided, not what rows it takes: a
  * sequence may have more. Sequences of few rows take them one by one, those
  * of many (from 24 in a small batch, from 48 in a large one) in chunks of 64
  * whose products run on the matrix cores:
  *   (I + A) U = diag(beta) (V - diag(e^G) K S),  A[i][j] = beta_i e^(G_i - G_j) k_i.k_j  (j < i),
  *   out = scale (diag(e^G) Q S + P U),           P[i][j] = e^(G_i - G_j) q_i.k_j         (j <= i),
  *   S <- e^G_63 S + (diag(e^(G_63 - G)) K)^T U,  G the running sum of the gates.
- * Both are deterministic; they differ by the order of f32 sums. The gates'
- * sums are held in 64 bits, exponentials are of differences.
+ * Both are deterministic; they differ by the order of f32 sums and by the
+ * chunks' operands, as below. The gates' sums are held in 64 bits,
+ * exponentials are of differences.
  *
  * Numerics: f32 sums. By chunks the products' operands are two f16 terms each,
  * within 2^-22 of a value or 2^-39 of the largest of its row (K, Q, T, P) or
@@ -267,13 +268,14 @@ typedef struct uq_gdn_heads {
  * column: the sum of the terms' sizes, sums over products by their number
  * times the largest. For keys of norm 1, gates at most 0 and betas of 0 to 1
  * no error grows, however many rows; results are off by some 1e-6 of the
- * largest. Values 2^20 times smaller than others of their chunk and column,
- * as after a gate that has all forgotten, lose bits that row by row they keep.
- * Gates above 0 and results beyond f32's range: unspecified for the sequence's
- * head from the start of those 64 rows on. Values that are not finite make
- * the results of their head from their row on, and its state, NaN, infinite
- * or unspecified; earlier rows, other heads and other sequences do not see
- * them.
+ * largest; gates above 0 take an error on with the state. Values 2^20 times
+ * smaller than others of their chunk and column, as after a gate that has all
+ * forgotten, lose bits that row by row they keep.
+ * Results, and e to the sum of a chunk's gates up to a row, beyond f32's range:
+ * unspecified for the sequence's head from the start of those 64 rows on.
+ * Values that are not finite make the results of their head from their row on,
+ * and its state, NaN, infinite or unspecified; earlier rows, other heads and
+ * other sequences do not see them.
  *
  * Only n_seqs, n_rows and d_row_start of the batch are read, and d_state, not
  * d_conv. The workspace (uq_gdn_rule_ws_bytes, 16-byte aligned) does not

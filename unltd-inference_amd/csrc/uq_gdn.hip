@@ -498,8 +498,8 @@ __device__ __forceinline__ float scale_up(int ex) { return ldexpf(1.0f, 14 - ex)
 __device__ __forceinline__ float scale_down(int ex) { return ldexpf(1.0f, ex - 14); }
 // The same of a 2^i + b 2^j, a bound that may lie beyond f32's range where what it bounds does not, formed in 64 bits. At
 // 2^141 scale_down ends, far above what f32 holds.
-__device__ __forceinline__ int scale_of_sum(float a, int i, float b, int j) {
-    const double sum = ldexp((double)a, i) + ldexp((double)b, j) + 0x1p-200;
+__device__ __forceinline__ int scale_of_sum(double a, int i, float b, int j) {
+    const double sum = ldexp(a, i) + ldexp((double)b, j) + 0x1p-200;
     return min(141, max(-100, __builtin_amdgcn_frexp_exp(sum)));
 }
 // The two terms of a pair of tiles, each rounded to the nearest. A pair of conversions, back, a difference: three
@@ -686,7 +686,7 @@ __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, i
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int i = 16 * r + 4 * g + e;
-                const float by = power(-fabs(G[i] - Gm));  // the gates' sums go down
+                const float x = (float)(G[i] - Gm), by = __builtin_amdgcn_exp2f(i <= mine ? -x : x);  // from the earlier row to the later
                 P[r][e] = i <= mine ? by * dq[r][e] : 0.0f;
                 below[r][e] = i > mine && i < first ? be[e] * by * dk[r][e] : 0.0f;
                 if (r == wave) diag[e] = -below[r][e];
@@ -1174,7 +1174,7 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
                     for (int t = 0; t < 2; t++) d[q % 2][t] = mfma_h(y < 2 ? k.h[p][t] : k.l[p][t], y == 1 ? gl[p] : gh[p], d[q % 2][t]);
             if (q == 0) {
                 // what the sum's terms amount to at most; those of K^T U by the operands' scales and the depth
-                const int to = scale_of_sum(top_s * whole, ex_s - 14, __uint_as_float(top_g), ex_x + 6);
+                const int to = scale_of_sum((double)top_s * whole, ex_s - 14, __uint_as_float(top_g), ex_x + 6);
                 keep = ldexpf(whole, ex_s - to), add = ldexpf(1.0f, ex_g + ex_x - 14 - to);
                 ex_s = to;
                 one[m] = scale_down(ex_s);
