@@ -218,9 +218,9 @@ typedef struct uq_gdn_rows {
  * (:405-419): beta = sigmoid(beta_raw), gate = softplus(alpha + dt_bias) a.
  *
  * Numerics: f32, the convolution's sum in the taps' order; silu, the norms and
- * the gates add up to 16 roundings (2^-24) of their values, silu of an x below
- * 0 up to 2 |x| more. Norms' sums of squares beyond f32's range are infinite,
- * as uq_l2_norm_rows'. A row's values that are not finite reach the rows that
+ * the gates add up to 16 roundings (2^-24) of their values; silu below 2^-119
+ * may be 0. Norms' sums of squares beyond f32's range are infinite, as
+ * uq_l2_norm_rows'. A row's values that are not finite reach the rows that
  * convolve them and, in query and key heads, the head.
  * d_out may not overlap the rows or the windows. Only n_seqs, n_rows and
  * d_row_start of the batch are read, and d_conv, not d_state.

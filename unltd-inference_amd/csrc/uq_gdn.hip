@@ -54,9 +54,14 @@ __device__ __forceinline__ int wave_scan_i(int v) {
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// x / (1 + e^-x), by the hardware's power of 2 and reciprocal (1 ulp each). The exponent's rounding is |x| 2^-24 of e^-x,
-// of which at most x e^-x = 0.4 is left where it counts, and where it is large, below 0, so is x.
-__device__ __forceinline__ float silu(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x)); }
+// x / (1 + e^-x), by the hardware's power of 2 and reciprocal (1 ulp each). e^-x is 2^t (1 + c), t = -x log2 e rounded and c
+// what that and the constant's own rounding leave: far below 0, where t is large, 2^t alone would be off by |t| 2^-24. Where
+// the product overflows 2^t is 0 or infinite, and c need only be a number.
+__device__ __forceinline__ float silu(float x) {
+    const float t = -1.44269502f * x;
+    const float c = fminf(fmaf(fmaf(-1.44269502f, x, -t), 0.693147181f, fmaf(x, -1.33497589e-8f, 1.0f)), 2.0f);
+    return x * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_exp2f(t), c, 1.0f));
+}
 
 // Sequences of at least `least` rows are cut into tiles of T rows, numbered
 // through; every wave finds its tile's by itself, 256 sequences at a time.
