@@ -545,17 +545,6 @@ __device__ __forceinline__ f4 mfma_h(const h8 &a, const h8 &b, const f4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// T and P of a chunk, and the keys and queries in two terms, a workgroup the
-// value heads of one query and key head. Wave w has rows 16 w .. + 15 of both;
-// all see the keys' pieces in the LDS. It takes tiles (r, w), r >= w, of K K^T
-// and (r, w), r <= w, of K Q^T, five for each wave, and keeps them for the
-// heads. Every result lies as the operand that it is next: lane (m, g) has
-// values 4 g .. + 3 of column m, which is a row's piece of the transposed. So
-// tile (i, j) of A is the left operand A_ij^T, K Q^T has P's rows, and T's row
-// of tiles i is formed from the diagonal back,
-//     T_ij^T = -T_jj^T sum over j < k <= i of A_kj^T T_ik^T,
-// by wave i from A and the diagonal's inverses alone. What it reads and writes
-// bounds it for many chunks, at 4 TB/s.
 // Column J of -A, a lane's row of it in the quarter's lane J, times the inverse's row J.
 template <int J>
 __device__ __forceinline__ void eliminate(const f4 &a, f4 &v) {
@@ -576,6 +565,17 @@ struct PrepLds {
     float beta[4][kChunk];
     int ex_k[kChunk], ex_q[kChunk], bad[4];
 };
+// T and P of a chunk, and the keys and queries in two terms, a workgroup the
+// value heads of one query and key head. Wave w has rows 16 w .. + 15 of both;
+// all see the keys' pieces in the LDS. It takes tiles (r, w), r >= w, of K K^T
+// and (r, w), r <= w, of K Q^T, five for each wave, and keeps them for the
+// heads. Every result lies as the operand that it is next: lane (m, g) has
+// values 4 g .. + 3 of column m, which is a row's piece of the transposed. So
+// tile (i, j) of A is the left operand A_ij^T, K Q^T has P's rows, and T's row
+// of tiles i is formed from the diagonal back,
+//     T_ij^T = -T_jj^T sum over j < k <= i of A_kj^T T_ik^T,
+// by wave i from A and the diagonal's inverses alone. What it reads and writes
+// bounds it for many chunks, at 4 TB/s.
 template <int HD>
 __device__ __forceinline__ void rule_prep(const RuleArgs &a, int slot, int hq, int part, PrepLds<HD> &l) {
     constexpr int KP = HD / 32;
