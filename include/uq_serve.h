@@ -217,11 +217,12 @@ typedef struct uq_gdn_rows {
  * qwen35_forward.rs:427-464); the windows taken on; and the rows' gates
  * (:405-419): beta = sigmoid(beta_raw), gate = softplus(alpha + dt_bias) a.
  *
- * Numerics: f32, the convolution's sum in the taps' order; silu, the norms and
- * the gates add up to 16 roundings (2^-24) of their values; silu below 2^-119
- * may be 0. Norms' sums of squares beyond f32's range are infinite, as
- * uq_l2_norm_rows'. A row's values that are not finite reach the rows that
- * convolve them and, in query and key heads, the head.
+ * Numerics: f32, the convolution's sum in the taps' order and alpha + dt_bias
+ * rounded once; silu, the norms and the gates of these add up to 16 roundings
+ * (2^-24) of their values; silu below 2^-119 may be 0. Norms' sums of squares
+ * beyond f32's range are infinite, as uq_l2_norm_rows'. A row's values that are
+ * not finite reach the rows that convolve them and, in query and key heads, the
+ * head.
  * d_out may not overlap the rows or the windows. Only n_seqs, n_rows and
  * d_row_start of the batch are read, and d_conv, not d_state.
  * Errors: UQ_ERR_ARG (null pointers, shapes beyond the limits above),

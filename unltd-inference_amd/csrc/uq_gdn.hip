@@ -166,7 +166,8 @@ struct ConvArgs {
 // A wave takes 256 channels (four neighbours a lane) of a tile's rows, the
 // taps and the last inputs in registers; one more takes the tile's gates. The
 // wave of a sequence's first tile also takes the window on, whose old values
-// it alone reads. Memory bounds it: 6010 rows of 8192 channels 82 us, 4.8 TB/s.
+// it alone reads. Memory bounds it: 6010 rows of 8192 channels 84 us, 4.7 TB/s;
+// other taps than 4 hold nine in registers, three waves a SIMD and not five: 87 us with 3 of them, 150 with 8.
 template <int CK>  // taps, 0: any up to 9
 __global__ __launch_bounds__(kConvTPB) void gdn_conv_kernel(ConvArgs a) {
     constexpr int MT = CK ? CK : 9, H = MT - 1, STEP = 4;
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(2 * HD) void gdn_rows_kernel(RuleArgs a) {
 // chunks at once (gdn_prep_kernel); gdn_chunks_kernel then takes a sequence's
 // chunks one after another, by columns of a head's state, as nothing of
 // another column enters one; gdn_finish_kernel applies norm and gate. 509 rows
-// of 32 heads take 11.5, 23 and 7.5 us, three prompts of 5241 rows 60, 143 and 44.
+// of 32 heads take 11.5, 24 and 7.5 us, three prompts of 5241 rows 60, 146 and 45.
 //
 // The products run on the f16 matrix cores with two terms of each operand,
 // h + l = x 2^s within 2^-22 of it: s brings the largest value of a row (left
@@ -1213,7 +1214,7 @@ __global__ __launch_bounds__(256, 1) void gdn_chunks_kernel(RuleArgs a) {
 
 // The epilogue of the rows that went by chunks: a workgroup a chunk and head,
 // HD / 4 lanes a row, several rows of a lane under way. Memory bounds it: 5241
-// rows of 32 heads 44 us, 5.6 TB/s.
+// rows of 32 heads 45 us, 5.6 TB/s.
 template <int HD>
 __global__ __launch_bounds__(256) void gdn_finish_kernel(RuleArgs a) {
     constexpr int PER = HD / 4, STEP = 256 / PER, N = kChunk / STEP;  // threads of a row, rows at a time, rows of a thread
@@ -1261,7 +1262,7 @@ hipError_t launch_gdn_conv(const StatesView &st, const BatchView &b, const uq_gd
     const ConvArgs a{st, b, r, (st.channels + 255) / 256};
     const unsigned per = kConvTPB / 64, tiles = (unsigned)(b.n_rows / kConvRows + std::min(b.n_seqs, b.n_rows));
     // A tile's channels one after another: rows are often a power of 2 apart, and a column of tiles would meet in few of
-    // the memory's channels. 6010 rows of 8192 channels so take 82 us, and 94 the other way round.
+    // the memory's channels. 6010 rows of 8192 channels so took 82 us, and 94 the other way round.
     const dim3 grid = grid_of((size_t)tiles * (((unsigned)a.groups + per) / per));
     if (st.taps == 4)
         hipLaunchKernelGGL(gdn_conv_kernel<4>, grid, dim3(kConvTPB), 0, s, a);
