@@ -182,10 +182,10 @@ uq_status uq_draft_verify_d(int32_t *d_accepted, int32_t *d_next, const float *d
  * nowhere, as for drafts that are not verified yet: a second call over the
  * same rows takes the state on, in which each sequence is its accepted rows
  * and its refused ones a sequence behind it, from nothing to nowhere). Several
- * sequences may begin with one slot, as continuations of one prompt do. Two sequences that end in one slot
- * leave there any part of either's state; one that begins with a slot that
- * another of the call ends in gets unspecified results. A sequence without
- * rows writes nothing. */
+ * sequences may begin with one slot, as continuations of one prompt do. Two
+ * sequences that end in one slot leave there any part of either's state; one
+ * that begins with a slot that another of the call ends in gets unspecified
+ * results. A sequence without rows writes nothing. */
 typedef struct uq_gdn_states {
     float *d_conv;  /* [n_slots][conv_kernel][channels], channels = (2 n_qk_heads + n_v_heads) head_dim:
                        rows 0 .. conv_kernel - 2 are the last inputs; the last row is neither read nor written */

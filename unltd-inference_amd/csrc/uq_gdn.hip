@@ -54,7 +54,7 @@ __device__ __forceinline__ int wave_scan_i(int v) {
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// x / (1 + e^-x), by the hardware's power of 2 and reciprocal (1 ulp each). e^-x is 2^t (1 + c), t = -x log2 e rounded and c
+// x / (1 + e^-x), by the hardware's power of 2 and reciprocal (1 ulp each). e^-x is 2^t c, t = -x log2 e rounded and c
 // what that and the constant's own rounding leave: far below 0, where t is large, 2^t alone would be off by |t| 2^-24. Where
 // the product overflows 2^t is 0 or infinite, and c need only be a number.
 __device__ __forceinline__ float silu(float x) {
